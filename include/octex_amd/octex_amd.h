@@ -5,7 +5,8 @@
  *     C++-only detail::timed_batch / resident_search / memory_report, introspect.hpp:41-60);
  *   - the stage entry points: one HIP kernel each, on caller-provided device buffers, so that the
  *     parity tests call every kernel of the search path with controlled inputs (as the reference's
- *     cpp/tests/test_search.cu launches its kernels directly).
+ *     cpp/tests/test_search.cu launches its kernels directly);
+ *   - operators on rows of scores: products in 8-bit integers, log probabilities, distillation.
  * All return CUVS_SUCCESS / CUVS_ERROR with cuvsGetLastErrorText() set; `stream` is a hipStream_t
  * (NULL: the null stream); the stage calls wait for their kernel before returning.
  */
@@ -200,6 +201,80 @@ cuvsError_t octexStageKmeansUpdate(const float* ys, int64_t ns, int32_t w, const
  * Q [m, w] (fp32, by MFMA; ties by row), -1 for a row of NaN. */
 cuvsError_t octexStageNearest(const float* Q, int64_t m, const float* X, int32_t n, int32_t w, int32_t* nearest,
                               void* stream);
+
+/* ---- operators on rows of scores: what a model that makes the queries, or reads the neighbors, computes next to a search.
+ * None has a counterpart in the reference.  All take matrices in the memory of one GPU, launch on `stream` (a hipStream_t,
+ * NULL the null stream) and return without waiting; they allocate nothing and may be captured into a graph.  Outputs must
+ * not overlap inputs or each other.  Arrays outside the GPU's memory, types and shapes that do not fit, and sizes beyond
+ * the limits are errors; no rows at all is no work. ---- */
+
+typedef enum {
+  OCTEX_FLOAT32  = 0,
+  OCTEX_FLOAT16  = 1,
+  OCTEX_BFLOAT16 = 2,
+  OCTEX_INT8     = 3,
+  OCTEX_INT32    = 4,
+  OCTEX_INT64    = 5
+} octexType;
+
+/** rows x cols elements of `type` (an octexType); a row's elements lie side by side, rows start `stride` elements apart
+ * (at least cols).  A vector is a matrix of one column or one row. */
+typedef struct {
+  void* data;
+  int32_t type;
+  int64_t rows, cols, stride;
+} octexMatrix;
+
+/** codes [m, k] (int8) and scales [m] (float32, dense) of x [m, k] (float32, float16 or bfloat16): scale = max |x| / 127,
+ * code = the whole number nearest to x / scale, ties to even, the quotient rounded to float32 first.  A row of zeros has
+ * scale 0; one with a NaN or an infinity has scale NaN and codes 0. */
+cuvsError_t octexQuantizeRows(const octexMatrix* x, const octexMatrix* codes, float* scales, void* stream);
+
+/** out [m, n] (float32, float16 or bfloat16) of queries [m, k] and rows [n, k] (int8), k at most 131071:
+ * out[i][j] = query_scales[i] * row_scales[j] * sum_d queries[i][d] * rows[j][d] + bias[j], the sum exact, the products and
+ * the sum with bias in float32.  bias [n] may be NULL.  Queries of a float type (query_scales NULL) are quantized as
+ * octexQuantizeRows does, into `workspace`: *size (with size not NULL) receives its bytes, and nothing is launched. */
+cuvsError_t octexInt8Scores(const octexMatrix* queries, const float* query_scales, const octexMatrix* rows,
+                            const float* row_scales, const float* bias, const octexMatrix* out, void* workspace,
+                            int64_t bytes, int64_t* size, void* stream);
+
+/**
+ * Log probabilities of rows of logits x [m, n] (float32, float16 or bfloat16; n at most 2^30), p = softmax(x / temperature):
+ * log_probs [m, t] of ids [m, t] (int32 or int64; t at most 512), entropy [m], lse [m] = ln sum exp(x / temperature), and
+ * the `top` (at most 64) largest entries by (logit, lowest id) as top_log_probs, top_ids [m, top]; every output float32 and
+ * dense, ids int64.  An id outside [0, n) is padding and has log probability 0.  Logits of -inf have probability 0 and are
+ * no alternatives: top_ids is padded with -1, top_log_probs with -inf.  A row of nothing but -inf has lse and log
+ * probabilities -inf and entropy 0; a row with a NaN or +inf is NaN.  `workspace` and `size` as for octexInt8Scores.
+ */
+cuvsError_t octexLogProbs(const octexMatrix* logits, const octexMatrix* ids, float temperature, int32_t top,
+                          float* log_probs, float* entropy, float* lse, float* top_log_probs, int64_t* top_ids,
+                          void* workspace, int64_t bytes, int64_t* size, void* stream);
+
+/** grad [m, n] (the logits' type) of sum(grad_log_probs * log_probs) + sum(grad_entropy * entropy) by the logits;
+ * grad_log_probs [m, t] or grad_entropy [m] (float32, dense) may be NULL.  lse and entropy as octexLogProbs gave them. */
+cuvsError_t octexLogProbsBackward(const octexMatrix* logits, const octexMatrix* ids, float temperature,
+                                  const float* grad_log_probs, const float* grad_entropy, const float* lse,
+                                  const float* entropy, const octexMatrix* grad, void* stream);
+
+/**
+ * Distillation of rows of logits x [m, n] from a teacher's top logits [m, k] (float32, float16 or bfloat16; k at most 512) of
+ * the columns ids [m, k] (int32 or int64): q = softmax(teacher / temperature) over a row's listed ids, and
+ * loss[i] = sum_j q_j (ln q_j - log p of id_j), p = softmax(x / temperature); lse as octexLogProbs gives it.  Ids outside
+ * [0, n) are padding, as a search's -1; a row that lists nothing (or only teacher logits of -inf) has loss and gradient 0.
+ * An id listed twice has the sum of its entries.  `workspace` and `size` as for octexInt8Scores.
+ */
+cuvsError_t octexDistill(const octexMatrix* logits, const octexMatrix* ids, const octexMatrix* teacher, float temperature,
+                         float* loss, float* lse, void* workspace, int64_t bytes, int64_t* size, void* stream);
+
+/** grad [m, n] (the logits' type) of sum(grad_loss * loss) by the logits, lse as octexDistill gave it. */
+cuvsError_t octexDistillBackward(const octexMatrix* logits, const octexMatrix* ids, const octexMatrix* teacher,
+                                 float temperature, const float* grad_loss, const float* lse, const octexMatrix* grad,
+                                 void* stream);
+
+/** octexDistill and octexDistillBackward in one call: loss, lse and the gradient of sum(grad_loss * loss). */
+cuvsError_t octexDistillStep(const octexMatrix* logits, const octexMatrix* ids, const octexMatrix* teacher,
+                             float temperature, const float* grad_loss, float* loss, float* lse, const octexMatrix* grad,
+                             void* workspace, int64_t bytes, int64_t* size, void* stream);
 
 #ifdef __cplusplus
 }

@@ -122,6 +122,8 @@ EXPORTS = (
     "octexStageGather", "octexStageRerankKeep", "octexStageSketchKeep", "octexStagePickStarts",
     "octexStageFinalRerank", "octexStageTakeK", "octexStageMergeReverse", "octexStageKmeansUpdate",
     "octexStageNearest", "octexMeasureRowReads",
+    "octexQuantizeRows", "octexInt8Scores", "octexLogProbs", "octexLogProbsBackward", "octexDistill",
+    "octexDistillBackward", "octexDistillStep",
 )
 
 _lib = None

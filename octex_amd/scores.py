@@ -1,0 +1,314 @@
+"""Operators on rows of scores: what a model that makes the queries, or reads the neighbors, computes next to a search.
+
+    codes, scales = octex.quantize_rows(vectors)                     # once: 8 bits a value, a scale a row
+    logits = octex.int8_scores(queries, codes, scales)               # every query against every row
+    r = octex.log_probs(logits, ids, top=10)                         # log p of given ids, entropy, alternatives
+    distances, neighbors = index.search(queries, k=10)               # a teacher: its nearest rows ...
+    loss, grad = octex.distill_step(weights, logits, neighbors, -distances, temperature=2.0)   # ... and the lesson
+
+Every operator is a hand-written kernel and takes matrices whose rows may lie apart (a slice of a padded vocabulary's
+columns, say).  Operands in GPU memory are read in place: the work is ordered on their stream (torch's current stream, or
+the one their framework names) and not waited for.  Host operands are copied to the GPU and results come back as the
+first operand is.  Types that an operator does not take are converted, as for a search.
+"""
+
+import collections
+import contextlib
+import ctypes as ct
+import functools
+
+import numpy as np
+
+from . import _arrays, _lib
+
+FLOATS = ("float32", "float16", "bfloat16")
+INTS = ("int64", "int32")
+_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3, "int32": 4, "int64": 5}
+
+LogProbs = collections.namedtuple("LogProbs", "log_probs entropy lse top_log_probs top_ids")
+
+
+class _Matrix(ct.Structure):
+    """struct octexMatrix (octex_amd.h)."""
+
+    _fields_ = [("data", ct.c_void_p), ("type", ct.c_int32), ("rows", ct.c_int64), ("cols", ct.c_int64),
+                ("stride", ct.c_int64)]
+
+
+_P, _I32, _I64, _F = ct.c_void_p, ct.c_int32, ct.c_int64, ct.c_float
+_M = ct.POINTER(_Matrix)
+_SIZED = [_P, _I64, _P]  # workspace, bytes, size
+_ENTRIES = {
+    "octexQuantizeRows": [_M, _M, _P],
+    "octexInt8Scores": [_M, _P, _M, _P, _P, _M] + _SIZED,
+    "octexLogProbs": [_M, _M, _F, _I32, _P, _P, _P, _P, _P] + _SIZED,
+    "octexLogProbsBackward": [_M, _M, _F, _P, _P, _P, _P, _M],
+    "octexDistill": [_M, _M, _M, _F, _P, _P] + _SIZED,
+    "octexDistillBackward": [_M, _M, _M, _F, _P, _P, _M],
+    "octexDistillStep": [_M, _M, _M, _F, _P, _P, _P, _M] + _SIZED,
+}
+
+
+@functools.lru_cache(None)
+def _entry(name):
+    f = getattr(_lib.lib(), name)
+    f.argtypes = _ENTRIES[name] + [_P]  # the stream
+    return f
+
+
+@functools.lru_cache(None)
+def _torch():
+    import torch
+
+    names = {getattr(torch, n): n for n in _TYPES}
+    return torch, names
+
+
+class _Call:
+    """One call's operands and results, all on one GPU, and the stream they are ordered on."""
+
+    def __init__(self, first, name, types):
+        self.torch, self.names = _torch()
+        self.origin, self.device, self.stream, self.on_host = first, None, None, False
+        self.first = self.take(first, name, types)
+
+    def take(self, a, name, types, ndim=2, shape=None):
+        """The operand as a torch tensor on the call's GPU: of one of `types` (else converted to the first), the elements
+        of a row side by side.  A vector is one row unless ndim is 1."""
+        torch = self.torch
+        if isinstance(a, torch.Tensor):
+            t = a
+        elif _arrays.is_foreign_device(a):
+            if self.stream is None and self.device is None:
+                self.stream = _arrays._foreign_stream(a)
+            t = torch.from_dlpack(a) if hasattr(a, "__dlpack__") else torch.as_tensor(a, device="cuda")
+        else:
+            x = np.asarray(a)
+            t = torch.from_numpy(x if x.flags.writeable else x.copy())
+        if self.device is None:
+            self.on_host = not t.is_cuda
+            self.device = torch.device("cuda", torch.cuda.current_device()) if self.on_host else t.device
+            if self.stream is None:
+                self.stream = torch.cuda.current_stream(self.device).cuda_stream
+        if t.device != self.device:
+            if t.is_cuda:
+                raise ValueError(f"octex: {name} lies on {t.device}, the other operands on {self.device}")
+            if t.device.type != "cpu":
+                raise TypeError(f"octex: {name} must lie in host or GPU memory, not on {t.device}")
+            with self.context():
+                t = t.to(self.device)
+        if self.names.get(t.dtype) not in types:
+            if types == ("int8",) or (types is INTS and t.is_floating_point()):
+                raise TypeError(f"octex: {name} must be {' or '.join(types)}, not {str(t.dtype).replace('torch.', '')}")
+            with self.context():
+                t = t.to(getattr(torch, types[0]))
+        if ndim == 2 and t.ndim == 1:
+            t = t[None, :]
+        if t.ndim != ndim:
+            raise ValueError(f"octex: {name} must be a {'matrix' if ndim == 2 else 'vector'}, not of {t.ndim} dimensions")
+        if shape is not None and tuple(t.shape) != shape:
+            raise ValueError(f"octex: {name} has shape {tuple(t.shape)}, expected {shape}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1 or (ndim == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            with self.context():
+                t = t.contiguous()
+        return t
+
+    def dense(self, a, name, shape):
+        """A float32 operand without gaps between its rows."""
+        t = self.take(a, name, ("float32",), ndim=len(shape), shape=shape)
+        with self.context():
+            return t.contiguous()
+
+    def context(self):
+        """torch's own work (conversions, allocations) on the call's stream."""
+        torch = self.torch
+        if torch.cuda.current_stream(self.device).cuda_stream == self.stream:
+            return contextlib.nullcontext()
+        return torch.cuda.stream(torch.cuda.ExternalStream(self.stream, device=self.device))
+
+    def matrix(self, t):
+        return _Matrix(t.data_ptr(), _TYPES[self.names[t.dtype]], t.shape[0], t.shape[1], max(t.stride(0), t.shape[1]))
+
+    def new(self, shape, dtype="float32"):
+        return self.torch.empty(shape, dtype=getattr(self.torch, dtype), device=self.device)
+
+    def run(self, entry, *args):
+        if _entry(entry)(*args, self.stream) != _lib.CUVS_SUCCESS:
+            raise _lib.OctexError(_lib.lib().cuvsGetLastErrorText().decode())
+
+    def workspace(self, entry, *args):
+        """(address, bytes, no question) of the workspace that these arguments need; its tensor is kept with the call."""
+        size = _I64(0)
+        self.run(entry, *args, None, 0, ct.addressof(size))
+        if size.value == 0:
+            return None, 0, None
+        self.scratch = self.new((size.value,), "int8")
+        return self.scratch.data_ptr(), size.value, None
+
+    def give(self, t):
+        """A result in the framework, and the memory, of the first operand."""
+        if isinstance(self.origin, self.torch.Tensor):
+            return t.cpu() if self.on_host else t
+        if _arrays.is_foreign_device(self.origin):
+            conv = getattr(__import__("sys").modules.get(_arrays._module_of(self.origin)), "from_dlpack", None)
+            return conv(t) if conv is not None else t
+        return t.cpu().numpy()
+
+
+def quantize_rows(x):
+    """(codes, scales) of the rows of x [m, k] in 8 bits: scale = max |x| / 127, code = the whole number nearest to
+    x / scale (ties to even), so that x is about codes * scales[:, None].
+
+    A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN, which makes all its scores NaN.
+    """
+    c = _Call(x, "x", FLOATS)
+    x = c.first
+    with c.context():
+        codes, scales = c.new(tuple(x.shape), "int8"), c.new((x.shape[0],))
+    c.run("octexQuantizeRows", c.matrix(x), c.matrix(codes), scales.data_ptr())
+    return c.give(codes), c.give(scales)
+
+
+def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtype=None):
+    """The scores [m, n] of every query against every row, a product in 8-bit integers:
+    scores[i, j] = query_scales[i] * row_scales[j] * sum(queries[i] * rows[j]) + bias[j].
+
+    `rows` [n, k] and `row_scales` [n] are quantize_rows' of an index's vectors, a pool of candidates or a vocabulary's
+    embeddings.  `queries` [m, k] are codes with their `query_scales` [m], or floats, which the call quantizes the same way.
+    The integer sums are exact.  With bias = -|row|^2 / 2 a query's scores rank the rows as squared distances do.  `dtype`
+    ("float32", "float16" or "bfloat16") is that of the scores: the queries' own if they are floats, else float32.
+    """
+    coded = query_scales is not None
+    c = _Call(queries, "queries", ("int8",) if coded else FLOATS)
+    q = c.first
+    rows = c.take(rows, "rows", ("int8",))
+    (m, k), n = q.shape, rows.shape[0]
+    if rows.shape[1] != k:
+        raise ValueError(f"octex: queries have {k} values, rows {rows.shape[1]}")
+    row_scales = c.dense(row_scales, "row_scales", (n,))
+    if coded:
+        query_scales = c.dense(query_scales, "query_scales", (m,))
+    if bias is not None:
+        bias = c.dense(bias, "bias", (n,))
+    if dtype is None:
+        dtype = "float32" if coded else c.names[q.dtype]
+    dtype = str(dtype).replace("torch.", "") if not isinstance(dtype, type) else np.dtype(dtype).name
+    if dtype not in FLOATS:
+        raise ValueError(f"octex: scores are of type {', '.join(FLOATS)}, not {dtype}")
+    with c.context():
+        out = c.new((m, n), dtype)
+        args = (c.matrix(q), query_scales.data_ptr() if coded else None, c.matrix(rows), row_scales.data_ptr(),
+                None if bias is None else bias.data_ptr(), c.matrix(out))
+        c.run("octexInt8Scores", *args, *c.workspace("octexInt8Scores", *args))
+    return c.give(out)
+
+
+def _ids(c, ids, m):
+    """The ids of m rows as a matrix, and the shape their values come back in."""
+    shape = _arrays.shape_of(ids)
+    if len(shape) == 1:
+        ids = ids[:, None] if hasattr(ids, "ndim") else np.asarray(ids)[:, None]
+    t = c.take(ids, "ids", INTS)
+    if t.shape[0] != m:
+        raise ValueError(f"octex: ids of {t.shape[0]} rows, logits of {m}")
+    return t, shape
+
+
+def log_probs(logits, ids, *, top=0, temperature=1.0):
+    """Log probabilities under p = softmax(logits / temperature) of each row's given ids [m] or [m, t].
+
+    Returns LogProbs(log_probs, entropy, lse, top_log_probs, top_ids): the ids' log probabilities in their shape, each row's
+    entropy and log-sum-exp [m], and its `top` (at most 64) likeliest entries [m, top] by (logit, lowest id).  Everything is
+    float32, top_ids int64.
+
+    An id outside [0, n) is padding: its log probability is 0.  Logits of -inf (a masked vocabulary) have probability 0 and
+    are no alternatives: top_ids is padded with -1, as a search's neighbors are, and top_log_probs with -inf.  A row of
+    nothing but -inf has lse and log probabilities -inf and entropy 0; a row with a NaN or +inf is NaN.
+    """
+    c = _Call(logits, "logits", FLOATS)
+    x = c.first
+    m, top = x.shape[0], int(top)
+    if not 0 <= top <= 64:
+        raise ValueError(f"octex: 0 to 64 top entries, not {top}")
+    t, shape = _ids(c, ids, m)
+    with c.context():
+        logp, entropy, lse = c.new(shape), c.new((m,)), c.new((m,))
+        top_logp, top_ids = c.new((m, top)), c.new((m, top), "int64")
+        args = (c.matrix(x), c.matrix(t), temperature, top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+                top_logp.data_ptr(), top_ids.data_ptr())
+        c.run("octexLogProbs", *args, *c.workspace("octexLogProbs", *args))
+    return LogProbs(*(c.give(v) for v in (logp, entropy, lse, top_logp, top_ids)))
+
+
+def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, *, temperature=1.0):
+    """The gradient by the logits of sum(grad_log_probs * log_probs) + sum(grad_entropy * entropy), in the logits' type.
+
+    lse and entropy are log_probs' of the same logits and temperature; either gradient may be None.  An id given more than
+    once in a row gets the sum of its gradients.
+    """
+    c = _Call(logits, "logits", FLOATS)
+    x = c.first
+    m = x.shape[0]
+    t, shape = _ids(c, ids, m)
+    gl = None if grad_log_probs is None else c.dense(grad_log_probs, "grad_log_probs", shape)
+    gh = None if grad_entropy is None else c.dense(grad_entropy, "grad_entropy", (m,))
+    lse, entropy = c.dense(lse, "lse", (m,)), c.dense(entropy, "entropy", (m,))
+    with c.context():
+        grad = c.new(tuple(x.shape), c.names[x.dtype])
+    c.run("octexLogProbsBackward", c.matrix(x), c.matrix(t), temperature, None if gl is None else gl.data_ptr(),
+          None if gh is None else gh.data_ptr(), lse.data_ptr(), entropy.data_ptr(), c.matrix(grad))
+    return c.give(grad)
+
+
+def _teacher(logits, ids, teacher):
+    c = _Call(logits, "logits", FLOATS)
+    t, shape = _ids(c, ids, c.first.shape[0])
+    if len(shape) == 1:
+        teacher = teacher[:, None] if hasattr(teacher, "ndim") else np.asarray(teacher)[:, None]
+    return c, c.first, t, c.take(teacher, "teacher", FLOATS, shape=tuple(t.shape))
+
+
+def distill(logits, ids, teacher, *, temperature=1.0):
+    """(loss, lse) of a student's logits [m, n] against a teacher's top logits [m, k] of the columns ids [m, k]:
+    loss = sum q (ln q - ln p), q = softmax(teacher / temperature) over the listed ids, p = softmax(logits / temperature)
+    over all columns.
+
+    The teacher may be a search (its neighbors and -distances) or a larger model's top logits.  Ids outside [0, n), as a
+    search's -1, are padding; a row that lists nothing has loss 0.  A listed logit of -inf that the teacher gives a
+    probability makes its loss inf.  lse is the logits' log-sum-exp [m], for distill_backward.
+    """
+    c, x, t, teacher = _teacher(logits, ids, teacher)
+    m = x.shape[0]
+    with c.context():
+        loss, lse = c.new((m,)), c.new((m,))
+        args = (c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, loss.data_ptr(), lse.data_ptr())
+        c.run("octexDistill", *args, *c.workspace("octexDistill", *args))
+    return c.give(loss), c.give(lse)
+
+
+def distill_backward(grad_loss, logits, ids, teacher, lse, *, temperature=1.0):
+    """The gradient by the logits of sum(grad_loss * loss), in the logits' type: grad_loss (p - q) / temperature.
+
+    lse is distill's of the same logits and temperature.  A row that lists nothing has gradient 0.
+    """
+    c, x, t, teacher = _teacher(logits, ids, teacher)
+    m = x.shape[0]
+    g, lse = c.dense(grad_loss, "grad_loss", (m,)), c.dense(lse, "lse", (m,))
+    with c.context():
+        grad = c.new(tuple(x.shape), c.names[x.dtype])
+    c.run("octexDistillBackward", c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, g.data_ptr(), lse.data_ptr(),
+          c.matrix(grad))
+    return c.give(grad)
+
+
+def distill_step(grad_loss, logits, ids, teacher, *, temperature=1.0):
+    """(loss, grad): distill and distill_backward in one call, which reads the logits less often."""
+    c, x, t, teacher = _teacher(logits, ids, teacher)
+    m = x.shape[0]
+    g = c.dense(grad_loss, "grad_loss", (m,))
+    with c.context():
+        loss, lse, grad = c.new((m,)), c.new((m,)), c.new(tuple(x.shape), c.names[x.dtype])
+        args = (c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, g.data_ptr(), loss.data_ptr(), lse.data_ptr(),
+                c.matrix(grad))
+        c.run("octexDistillStep", *args, *c.workspace("octexDistillStep", *args))
+    return c.give(loss), c.give(grad)
