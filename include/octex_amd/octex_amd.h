@@ -233,7 +233,9 @@ cuvsError_t octexQuantizeRows(const octexMatrix* x, const octexMatrix* codes, fl
 /** out [m, n] (float32, float16 or bfloat16) of queries [m, k] and rows [n, k] (int8), k at most 131071:
  * out[i][j] = query_scales[i] * row_scales[j] * sum_d queries[i][d] * rows[j][d] + bias[j], the sum exact, the products and
  * the sum with bias in float32.  bias [n] may be NULL.  Queries of a float type (query_scales NULL) are quantized as
- * octexQuantizeRows does, into `workspace`: *size (with size not NULL) receives its bytes, and nothing is launched. */
+ * octexQuantizeRows does.  With size not NULL *size receives the bytes that `workspace` (at a multiple of 256) needs for
+ * these arguments, and nothing is launched.  Rows at multiples of 16 bytes are read in place; others are laid out anew in
+ * the workspace first, but for a few queries. */
 cuvsError_t octexInt8Scores(const octexMatrix* queries, const float* query_scales, const octexMatrix* rows,
                             const float* row_scales, const float* bias, const octexMatrix* out, void* workspace,
                             int64_t bytes, int64_t* size, void* stream);

@@ -66,6 +66,14 @@ __device__ inline void store16(T* p, uint4 raw)
   __builtin_memcpy(p, &raw, 16);
 }
 
+/** The same for results that no kernel reads soon: they pass by the caches. */
+template <typename T>
+__device__ inline void store16_nt(T* p, uint4 raw)
+{
+  using words = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  __builtin_nontemporal_store(words{raw.x, raw.y, raw.z, raw.w}, reinterpret_cast<words*>(p));
+}
+
 /** Elements [at, at + kPer16) of a row as they lie in memory, those from `end` on -inf. */
 template <typename T>
 __device__ inline auto load_row16(const T* row, int at, int end) -> uint4

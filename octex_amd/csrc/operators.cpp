@@ -133,9 +133,6 @@ auto asked_size(int64_t need, int64_t bytes, int64_t* size) -> bool
   return false;
 }
 
-constexpr int64_t kAlign = 256;
-auto align_up(int64_t v) -> int64_t { return (v + kAlign - 1) / kAlign * kAlign; }
-
 }  // namespace
 
 extern "C" cuvsError_t octexQuantizeRows(const octexMatrix* x, const octexMatrix* codes, float* scales, void* stream)
@@ -150,7 +147,8 @@ extern "C" cuvsError_t octexQuantizeRows(const octexMatrix* x, const octexMatrix
     if (x->rows == 0) return;
     on_gpu gpu;
     gpu.take(x->data, "x"), gpu.take(codes->data, "codes"), gpu.take(scales, "scales");
-    launch_quantize_rows(x->data, elem_of(*x), x->rows, static_cast<int>(x->cols), x->stride,
+    const int k = static_cast<int>(x->cols);
+    launch_quantize_rows(x->data, elem_of(*x), x->rows, k, k, x->stride,
                          static_cast<int8_t*>(codes->data), codes->stride, scales, static_cast<hipStream_t>(stream));
   });
 }
@@ -172,26 +170,20 @@ extern "C" cuvsError_t octexInt8Scores(const octexMatrix* queries, const float* 
     const int64_t n = rows->rows;
     shape(out, "out", m, n);
     float_type(*out, "out");
-    const int64_t pitch = (k + 15) / 16 * 16;  // of the quantized queries
-    if (asked_size(coded ? 0 : align_up(m * pitch) + align_up(m * 4), bytes, size)) return;
+    const int8_query q{queries->data, elem_of(*queries), queries->stride, query_scales};
+    const int8_rows r{static_cast<const int8_t*>(rows->data), rows->stride, row_scales};
+    const int64_t need = m == 0 || n == 0 ? 0 : int8_scores_workspace(q, m, r, n, static_cast<int>(k));
+    if (asked_size(need, bytes, size)) return;
     if (m == 0 || n == 0) return;
-    auto s = static_cast<hipStream_t>(stream);
     on_gpu gpu;
     gpu.take(queries->data, "queries"), gpu.take(rows->data, "rows"), gpu.take(row_scales, "row_scales");
     gpu.take(out->data, "out");
+    if (coded) gpu.take(query_scales, "query_scales");
     if (bias != nullptr) gpu.take(bias, "bias");
-    int8_rows q{static_cast<const int8_t*>(queries->data), queries->stride, query_scales};
-    if (coded) {
-      gpu.take(query_scales, "query_scales");
-    } else {
-      gpu.take(workspace, "workspace");
-      auto* codes  = static_cast<int8_t*>(workspace);
-      auto* scales = reinterpret_cast<float*>(codes + align_up(m * pitch));
-      launch_quantize_rows(queries->data, elem_of(*queries), m, static_cast<int>(k), queries->stride, codes, pitch, scales, s);
-      q = {codes, pitch, scales};
-    }
-    launch_int8_scores(q, m, {static_cast<const int8_t*>(rows->data), rows->stride, row_scales}, n, static_cast<int>(k), bias,
-                       out->data, elem_of(*out), out->stride, s);
+    if (need > 0) gpu.take(workspace, "workspace");
+    OCTEX_EXPECTS(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "octex: the workspace must lie at a multiple of 256 bytes");
+    launch_int8_scores(q, m, r, n, static_cast<int>(k), bias, out->data, elem_of(*out), out->stride, workspace,
+                       static_cast<hipStream_t>(stream));
   });
 }
 

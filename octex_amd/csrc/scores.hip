@@ -5,6 +5,8 @@
 #include "scores.hpp"
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 namespace cuvs::neighbors::octex::detail {
 
@@ -12,6 +14,8 @@ namespace {
 
 using i32x4  = int __attribute__((ext_vector_type(4)));
 using i32x16 = int __attribute__((ext_vector_type(16)));
+
+__device__ inline void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // ---- quantization of rows
 
@@ -22,36 +26,86 @@ __device__ inline auto code_of(float v, float scale) -> int
   return static_cast<int>(fminf(fmaxf(rintf(v / scale), -127.f), 127.f));
 }
 
-/** scale = max |x| / 127; code = the whole number nearest to x / scale (ties to even), the quotient rounded to fp32 first.
- * A row of zeros has scale 0 and codes 0; one with a NaN or an infinity has scale NaN and codes 0. */
-template <typename T>
-__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T* x, int64_t stride, int k, int8_t* codes,
-                                                                 int64_t cstride, float* scales, int64_t row0)
+/** A magnitude's bits, which order as it does, with infinity and NaN above every finite one. */
+__device__ inline auto magnitude(float v) -> unsigned { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ inline auto scale_of(unsigned top) -> float { return top < 0x7f800000u ? __uint_as_float(top) / 127.f : NAN; }
+
+template <int N>
+__device__ inline void codes_of(const float (&v)[N], float scale, int8_t (&c)[N])
 {
-  __shared__ unsigned tops[kQuantThreads / 64];
-  const int64_t r = row0 + blockIdx.x;
-  const T* row    = x + r * stride;
-  // a magnitude's bits order as it does, with infinity and NaN above every finite one
-  unsigned top = 0;
-  for (int i = threadIdx.x; i < k; i += kQuantThreads)
-    top = max(top, __float_as_uint(static_cast<float>(row[i])) & 0x7fffffffu);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    c[i] = scale > 0.f ? static_cast<int8_t>(code_of(v[i], scale)) : int8_t{0};
+}
+
+__device__ inline auto block_max(unsigned top, unsigned* parts) -> unsigned
+{
 #pragma unroll
   for (int mask = 32; mask > 0; mask >>= 1)
     top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), mask)));
-  if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+  if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = top;
   __syncthreads();
-  for (int w = 0; w < kQuantThreads / 64; ++w)
-    top = max(top, tops[w]);
-  const bool finite = top < 0x7f800000u;
-  const float scale = finite ? __uint_as_float(top) / 127.f : NAN;
-  if (threadIdx.x == 0) scales[r] = scale;
-  for (int i = threadIdx.x; i < k; i += kQuantThreads)
-    codes[r * cstride + i] = scale > 0.f ? static_cast<int8_t>(code_of(static_cast<float>(row[i]), scale)) : 0;
+  for (int w = 0; w < static_cast<int>(blockDim.x) / 64; ++w)
+    top = max(top, parts[w]);
+  return top;
 }
 
-// ---- the product: tiles of 64 x 64, 128 bytes of both operands in LDS at a time
-
-constexpr int kBK = 128;  // bytes of a row in LDS
+/**
+ * scale = max |x| / 127; code = the whole number nearest to x / scale (ties to even), the quotient rounded to fp32 first.
+ * A row of zeros has scale 0 and codes 0; one with a NaN or an infinity has scale NaN and codes 0.
+ *
+ * A workgroup holds a row of up to kHeld * 256 values in registers between the maximum and the codes, so that it is read
+ * once; longer rows are read again.  Columns k .. pad are written as 0.
+ */
+template <typename T, int kHeld>
+__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T* x, int64_t stride, int k, int pad, int8_t* codes,
+                                                                 int64_t cstride, float* scales, int64_t row0)
+{
+  constexpr int N = kPer16<T>, kStep = kQuantThreads * N;
+  __shared__ unsigned parts[kQuantThreads / 64];
+  const int64_t r = row0 + blockIdx.x;
+  const T* row    = x + r * stride;
+  int8_t* out     = codes + r * cstride;
+  const int mine  = threadIdx.x * N;
+  uint4 held[kHeld];
+  float v[N];
+  unsigned top = 0;
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (u * kStep + mine < k) held[u] = load_row16(row, u * kStep + mine, k);
+  const auto take = [&](uint4 raw, int at) {
+    unpack16<T>(raw, v);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at + i < k) top = max(top, magnitude(v[i]));
+  };
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (u * kStep + mine < k) take(held[u], u * kStep + mine);
+  for (int at = kHeld * kStep + mine; at < k; at += kStep)
+    take(load_row16(row, at, k), at);
+  const float scale = scale_of(block_max(top, parts));
+  if (threadIdx.x == 0) scales[r] = scale;
+  const auto give = [&](uint4 raw, int at) {
+    unpack16<T>(raw, v);
+    int8_t c[N];
+    codes_of(v, scale, c);
+    if (at + N <= k) {
+      __builtin_memcpy(out + at, c, N);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (at + i < k) out[at + i] = c[i];
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (u * kStep + mine < k) give(held[u], u * kStep + mine);
+  for (int at = kHeld * kStep + mine; at < k; at += kStep)
+    give(load_row16(row, at, k), at);
+  if (static_cast<int>(threadIdx.x) < pad - k) out[k + threadIdx.x] = 0;
+}
 
 struct product {
   int8_rows q, r;
@@ -61,6 +115,12 @@ struct product {
   void* out;
   int64_t ostride;
 };
+
+__device__ inline auto score_of(int sum, float qs, product const& p, int64_t j) -> float
+{
+  const float v = static_cast<float>(sum) * qs * p.r.scales[j];
+  return p.bias != nullptr ? v + p.bias[j] : v;
+}
 
 /** 16 values of a row at column at, those from k on 0. */
 __device__ inline auto load_codes(const int8_t* row, int at, int k) -> i32x4
@@ -78,48 +138,312 @@ __device__ inline auto load_codes(const int8_t* row, int at, int k) -> i32x4
   return v;
 }
 
-template <typename O>
-__global__ __launch_bounds__(256) void scores_kernel(product p, unsigned tiles_n)
+// ---- rows laid out anew: 16-byte chunks at aligned places, zeros after the last value
+
+constexpr int kPackThreads = 256;
+
+__global__ __launch_bounds__(kPackThreads) void pack_kernel(const int8_t* x, int64_t stride, int64_t n, int k, int8_t* out,
+                                                            int64_t pitch)
 {
-  // a row's eight 16-byte chunks, chunk c of row i at c ^ (i % 8): a fragment's 32 rows then fall on different banks
-  __shared__ i32x4 qa[64 * 8], ra[64 * 8];
-  const int64_t i0 = int64_t{blockIdx.x / tiles_n} * 64, j0 = int64_t{blockIdx.x % tiles_n} * 64;
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const int wi = wave / 2 * 32, wj = wave % 2 * 32;
-  i32x16 acc = {};
-  for (int k0 = 0; k0 < p.k; k0 += kBK) {
-    i32x4 a[2], b[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int e = threadIdx.x + 256 * u, i = e / 8, c = e % 8;
-      a[u] = i0 + i < p.m ? load_codes(p.q.x + (i0 + i) * p.q.stride, k0 + 16 * c, p.k) : i32x4{0, 0, 0, 0};
-      b[u] = j0 + i < p.n ? load_codes(p.r.x + (j0 + i) * p.r.stride, k0 + 16 * c, p.k) : i32x4{0, 0, 0, 0};
+  const int chunks    = (k + 15) / 16;
+  const int64_t total = n * chunks;
+  for (int64_t e = int64_t{blockIdx.x} * kPackThreads + threadIdx.x; e < total; e += int64_t{gridDim.x} * kPackThreads) {
+    const int64_t i = e / chunks;
+    const int c     = static_cast<int>(e - i * chunks);
+    *reinterpret_cast<i32x4*>(out + i * pitch + 16 * c) = load_codes(x + i * stride, 16 * c, k);
+  }
+}
+
+// ---- the product
+
+constexpr int64_t kMaxInt8Stride = int64_t{1} << 22;  // a tile's 256 rows within 32-bit offsets
+
+// ---- the product of few queries: every row's bytes are read once, by one wavefront
+
+constexpr int kPiece = 256;  // bytes of a row that a wavefront multiplies at a time
+
+/**
+ * A workgroup scores RT * 16 rows for up to 16 queries; its KW wavefronts share the columns out and their sums meet in
+ * LDS.  A matrix instruction takes 64 columns of 16 rows and 16 queries, so a lane loads 16 bytes of a row, and four such
+ * loads cover whole 128-byte lines.  With kFused the queries are floats: the workgroup quantizes them into LDS first.
+ */
+template <int RT, int KW, bool kFused, typename Q, typename O>
+__global__ __launch_bounds__(64 * KW) void few_scores_kernel(product p, const Q* floats, int64_t fstride, int pitch)
+{
+  extern __shared__ __align__(16) char few_lds[];
+  __shared__ float qscales[16];
+  __shared__ unsigned parts[KW];
+  constexpr int kThreadsHere = 64 * KW;
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, m = static_cast<int>(p.m);
+  const int64_t j0 = int64_t{blockIdx.x} * RT * 16;
+  if constexpr (kFused) {
+    for (int i = 0; i < m; ++i) {
+      const Q* row = floats + i * fstride;
+      unsigned top = 0;
+      for (int at = threadIdx.x; at < p.k; at += kThreadsHere)
+        top = max(top, magnitude(static_cast<float>(row[at])));
+      const float scale = scale_of(block_max(top, parts));
+      if (threadIdx.x == 0) qscales[i] = scale;
+      for (int at = threadIdx.x; at < pitch; at += kThreadsHere)
+        few_lds[i * pitch + at] =
+          at < p.k && scale > 0.f ? static_cast<char>(code_of(static_cast<float>(row[at]), scale)) : char{0};
+      __syncthreads();
     }
-    __syncthreads();
+  } else {
+    for (int i = threadIdx.x; i < m; i += kThreadsHere)
+      qscales[i] = p.q.scales[i];
+  }
+  i32x4 acc[RT] = {};
+  const int8_t* rows[RT];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int e = threadIdx.x + 256 * u, i = e / 8, c = e % 8;
-      qa[i * 8 + (c ^ (i & 7))] = a[u];
-      ra[i * 8 + (c ^ (i & 7))] = b[u];
+  for (int y = 0; y < RT; ++y)
+    rows[y] = p.r.x + min(j0 + 16 * y + lane % 16, p.n - 1) * p.r.stride;
+  const auto multiply = [&](int k0, auto load_row, auto load_query) {
+    i32x4 a[4], b[RT][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int at = k0 + 64 * s + 16 * (lane / 16);
+#pragma unroll
+      for (int y = 0; y < RT; ++y)
+        b[y][s] = load_row(rows[y], at);
+      a[s] = load_query(min(lane % 16, m - 1), at);
     }
-    __syncthreads();
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const int c = 2 * kk + lane / 32, i = lane % 32;
-      const i32x4 fa = qa[(wi + i) * 8 + (c ^ (i & 7))], fb = ra[(wj + i) * 8 + (c ^ (i & 7))];
-      acc            = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa, fb, acc, 0, 0, 0);
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int y = 0; y < RT; ++y)
+        acc[y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b[y][s], acc[y], 0, 0, 0);
+  };
+  const auto whole = [](const int8_t* row, int at) {
+    i32x4 v;
+    __builtin_memcpy(&v, row + at, 16);
+    return v;
+  };
+  const auto partial = [&](const int8_t* row, int at) { return load_codes(row, at, p.k); };
+  const auto coded   = [&](int i, int at) {  // the codes in LDS end with zeros
+    return at < pitch ? *reinterpret_cast<const i32x4*>(few_lds + i * pitch + at) : i32x4{0, 0, 0, 0};
+  };
+  for (int k0 = wave * kPiece; k0 < p.k; k0 += KW * kPiece) {
+    if (k0 + kPiece <= p.k) {
+      if constexpr (kFused)
+        multiply(k0, whole, coded);
+      else
+        multiply(k0, whole, [&](int i, int at) { return whole(p.q.x + i * p.q.stride, at); });
+    } else {
+      if constexpr (kFused)
+        multiply(k0, partial, coded);
+      else
+        multiply(k0, partial, [&](int i, int at) { return partial(p.q.x + i * p.q.stride, at); });
     }
   }
-  const int64_t j = j0 + wj + lane % 32;
-  if (j >= p.n) return;
-  const float rs = p.r.scales[j], b = p.bias != nullptr ? p.bias[j] : 0.f;
+  auto* sums = reinterpret_cast<int*>(few_lds);  // [KW][16][RT * 16]
+  constexpr int kWide = RT * 16, kAll = 16 * kWide;
+  __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int64_t i = i0 + wi + 8 * (e / 4) + 4 * (lane / 32) + e % 4;
-    if (i >= p.m) continue;
-    float v = static_cast<float>(acc[e]) * p.q.scales[i] * rs;
-    if (p.bias != nullptr) v += b;
-    static_cast<O*>(p.out)[i * p.ostride + j] = static_cast<O>(v);
+  for (int y = 0; y < RT; ++y)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      sums[wave * kAll + (4 * (lane / 16) + e) * kWide + 16 * y + lane % 16] = acc[y][e];
+  __syncthreads();
+  for (int e = threadIdx.x; e < m * kWide; e += kThreadsHere) {
+    const int i = e / kWide;
+    const int64_t j = j0 + e % kWide;
+    if (j >= p.n) continue;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+      sum += sums[w * kAll + e];
+    static_cast<O*>(p.out)[i * p.ostride + j] = static_cast<O>(score_of(sum, qscales[i], p, j));
+  }
+}
+
+// ---- the product of many rows: tiles of BM queries x BN rows, both operands' next 128 bytes loaded into LDS while the
+// matrix cores work on these
+
+constexpr unsigned kXcds = 8;
+
+/** A grid of tiles in the order its workgroups take them. */
+struct tile_order {
+  unsigned tm, tn;  // tiles of queries and of rows
+};
+
+/** The tile of a workgroup.  Workgroups go round the 8 XCDs in turn; each XCD takes a run of consecutive tiles, and a run
+ * goes through kBand tiles of queries before the next tile of rows, so that the tiles an XCD works on at a time share
+ * operands in its L2. */
+__device__ inline auto tile_of(unsigned b, tile_order o) -> uint2
+{
+  constexpr unsigned kBand = 4;
+  const unsigned tiles = o.tm * o.tn, xcd = b % kXcds, each = tiles / kXcds, more = tiles % kXcds;
+  const unsigned t     = xcd * each + min(xcd, more) + b / kXcds;
+  const unsigned band = t / (kBand * o.tn), in = t % (kBand * o.tn), high = min(kBand, o.tm - band * kBand);
+  return {band * kBand + in % high, in / high};
+}
+
+using rsrc_t = __amdgpu_buffer_rsrc_t;
+
+/** Waits until at most N of the wavefront's loads are in flight, and with kLds until its LDS reads are back. */
+template <int N, bool kLds = false>
+__device__ inline void wait_loads()
+{
+  static_assert(N < 64);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (kLds ? 0 : 15) << 8 | (N >> 4) << 14);
+  asm volatile("" ::: "memory");
+}
+
+template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
+__global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, tile_order order)
+{
+  constexpr int kWavesHere = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
+  constexpr int kChunks    = kStep / 16, kRows = 64 / kChunks;        // of a row; rows that a load of a wavefront covers
+  constexpr int kLoads     = (BM + BN) / kRows / kWavesHere;          // a wavefront's loads of a step
+  constexpr int kParts     = kStep / 32;                              // of a step, a matrix instruction deep
+  constexpr int kBuffer    = (BM + BN) * kStep;
+  static_assert((BM + BN) % (kRows * kWavesHere) == 0, "every wavefront loads as much, so that the waits count alike");
+  extern __shared__ __align__(1024) char lds[];  // kAhead + 1 buffers: queries, then rows
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const uint2 tile = tile_of(blockIdx.x, order);
+  const int64_t i0 = int64_t{tile.x} * BM, j0 = int64_t{tile.y} * BN;
+  const int mi = static_cast<int>(min(int64_t{BM}, p.m - i0)), nj = static_cast<int>(min(int64_t{BN}, p.n - j0));
+  // rows past the end lie past the buffer's: they load as 0
+  const auto qr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.q.x + i0 * p.q.stride), 0,
+                                                    static_cast<int>((mi - 1) * p.q.stride + p.k), 0x00020000);
+  const auto rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.r.x + j0 * p.r.stride), 0,
+                                                    static_cast<int>((nj - 1) * p.r.stride + p.k), 0x00020000);
+  // chunk c of row i lies at c ^ swizzle(i): any 16 rows' chunks c then cover all banks once
+  const auto swizzle = [](int i) { return i / (16 / kChunks) % kChunks; };
+  const int qrow = (lane / kChunks) * static_cast<int>(p.q.stride), rrow = (lane / kChunks) * static_cast<int>(p.r.stride);
+  const auto load = [&](int k0, int buffer, int u) {
+    const int g     = wave * kLoads + u;
+    const bool q    = g < BM / kRows;
+    const int chunk = 16 * ((lane % kChunks) ^ swizzle(g * kRows + lane / kChunks));
+    const int base  = (q ? g : g - BM / kRows) * kRows * static_cast<int>(q ? p.q.stride : p.r.stride);
+    // k is a multiple of 16; what lies past it loads as 0, and so do steps past the last, that the waits count alike
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(q ? qr : rr,
+                                             (__attribute__((address_space(3))) void*)(lds + buffer * kBuffer + g * 1024), 16,
+                                             k0 + chunk < p.k ? base + (q ? qrow : rrow) + chunk + k0 : 0x7fffff00, 0, 0, 0);
+  };
+  const int wi = wave / WN * TM * 32, wj = wave % WN * TN * 32;
+  i32x16 acc[TM][TN] = {};
+  i32x4 a[2][TM], b[2][TN];
+  const auto read = [&](int buffer, int part, i32x4(&fa)[TM], i32x4(&fb)[TN]) {
+    const char* qa = lds + buffer * kBuffer;
+    const int at   = ((2 * part + lane / 32) ^ swizzle(lane % 32)) * 16 + (lane % 32) * kStep;
+#pragma unroll
+    for (int y = 0; y < TN; ++y)
+      fb[y] = *reinterpret_cast<const i32x4*>(qa + (BM + wj + 32 * y) * kStep + at);
+#pragma unroll
+    for (int x = 0; x < TM; ++x)
+      fa[x] = *reinterpret_cast<const i32x4*>(qa + (wi + 32 * x) * kStep + at);
+  };
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t)
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+      load(t * kStep, t, u);
+  const int steps = (p.k + kStep - 1) / kStep;
+  wait_loads<(kAhead - 1) * kLoads>();
+  __builtin_amdgcn_s_barrier();
+  read(0, 0, a[0], b[0]);
+  int buffer = 0;
+  for (int t = 0; t < steps; ++t) {
+    const int before = buffer == 0 ? kAhead : buffer - 1, after = buffer == kAhead ? 0 : buffer + 1;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const int now = part & 1;
+      if (part + 1 < kParts) {
+        read(buffer, part + 1, a[1 - now], b[1 - now]);
+      } else {
+        // the next step's loads have landed in every wavefront, and this step's buffer has been read
+        wait_loads<(kAhead - 1) * kLoads, true>();
+        __builtin_amdgcn_s_barrier();
+        read(after, 0, a[1 - now], b[1 - now]);
+      }
+      constexpr int kMfma = TM * TN, kReads = TM + TN, kEach = (kLoads + kParts - 2) / (kParts - 1);  // the last part loads none
+      constexpr int kLoadsEach = (kEach + kMfma - 1) / kMfma, kReadsEach = (kReads + kMfma - 1) / kMfma;
+#pragma unroll
+      for (int x = 0; x < TM; ++x)
+#pragma unroll
+        for (int y = 0; y < TN; ++y) {
+          acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[now][y], a[now][x], acc[x][y], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < kLoadsEach; ++e) {
+            const int i = (x * TN + y) * kLoadsEach + e, u = part * kEach + i;
+            if (part + 1 < kParts && i < kEach && u < kLoads) load((t + kAhead) * kStep, before, u);
+          }
+        }
+      // a matrix instruction, then the LDS reads and the loads that go beside it
+#pragma unroll
+      for (int i = 0; i < kMfma; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReadsEach, 0);
+        if (part + 1 < kParts) __builtin_amdgcn_sched_group_barrier(0x020, kLoadsEach, 0);
+      }
+    }
+    buffer = after;
+  }
+  // a lane holds, of query lane % 32, rows 8 * (e / 4) + 4 * (lane / 32) + e % 4 of each 32 x 32 part: they go through LDS,
+  // 32 queries of the wavefront's at a time, so that a row of the output is stored in 16-byte pieces side by side
+  constexpr int kThreadsHere = 64 * kWavesHere, kWide = TN * 32, N = kPer16<O>;
+  constexpr int kPitch       = kWide * static_cast<int>(sizeof(O)) + 16;
+  auto* scales               = reinterpret_cast<float*>(lds);  // of the tile's rows, then their biases
+  auto* biases               = scales + BN;
+  // results of whole 64-byte pieces pass by the caches: the 200 MB of 1,000 x 960 x 100,000 in float16 then take 161 us in
+  // place of 177, where pieces at odd places lose (2048 x 512 x 50,000: 110 us against 86)
+  const bool by_cache = (reinterpret_cast<uintptr_t>(p.out) | p.ostride * sizeof(O)) % 64 != 0;
+  char* mine                 = lds + 2 * BN * sizeof(float) + wave * 32 * kPitch;
+  wait_loads<0, true>();  // the steps past the last, which load zeros
+  __syncthreads();
+  for (int j = threadIdx.x; j < BN; j += kThreadsHere) {
+    scales[j] = j < nj ? p.r.scales[j0 + j] : 0.f;
+    if (p.bias != nullptr) biases[j] = j < nj ? p.bias[j0 + j] : 0.f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < TM; ++x) {
+    const float qs = p.q.scales[i0 + min(wi + 32 * x + lane % 32, mi - 1)];
+#pragma unroll
+    for (int y = 0; y < TN; ++y)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int j     = 32 * y + 8 * e4 + 4 * (lane / 32);
+        const float4 rs = *reinterpret_cast<const float4*>(scales + wj + j);
+        float f[4]      = {static_cast<float>(acc[x][y][4 * e4]) * qs * rs.x, static_cast<float>(acc[x][y][4 * e4 + 1]) * qs * rs.y,
+                           static_cast<float>(acc[x][y][4 * e4 + 2]) * qs * rs.z,
+                           static_cast<float>(acc[x][y][4 * e4 + 3]) * qs * rs.w};
+        if (p.bias != nullptr) {
+          const float4 bs = *reinterpret_cast<const float4*>(biases + wj + j);
+          f[0] += bs.x, f[1] += bs.y, f[2] += bs.z, f[3] += bs.w;
+        }
+        O v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = static_cast<O>(f[e]);
+        __builtin_memcpy(__builtin_assume_aligned(mine + (lane % 32) * kPitch + j * static_cast<int>(sizeof(O)), 8), v, sizeof(v));
+      }
+    wave_fence();
+    constexpr int kPieces = kWide / N;  // of a row
+#pragma unroll 4
+    for (int u = 0; u < 32 * kPieces / 64; ++u) {
+      const int e = u * 64 + lane, row = e / kPieces, piece = e % kPieces;
+      const int io = wi + 32 * x + row, jo = wj + piece * N;
+      uint4 raw = *reinterpret_cast<const uint4*>(mine + row * kPitch + piece * 16);
+      if (io >= mi || jo >= nj) continue;
+      O* at = static_cast<O*>(p.out) + (i0 + io) * p.ostride + j0 + jo;
+      if (jo + N <= nj) {
+        if (by_cache)
+          store16(at, raw);
+        else
+          store16_nt(at, raw);
+      } else {
+        O part[N];
+        __builtin_memcpy(part, &raw, 16);
+#pragma unroll
+        for (int q = 0; q < N - 1; ++q)
+          if (q < nj - jo) at[q] = part[q];
+      }
+    }
+    wave_fence();
   }
 }
 
@@ -136,36 +460,204 @@ void with_float(elem type, F f)
 
 }  // namespace
 
-void launch_quantize_rows(const void* x, elem type, int64_t m, int k, int64_t stride, int8_t* codes, int64_t cstride,
-                          float* scales, hipStream_t s)
+void launch_quantize_rows(const void* x, elem type, int64_t m, int k, int pad, int64_t stride, int8_t* codes,
+                          int64_t cstride, float* scales, hipStream_t s)
 {
   constexpr int64_t kRows = (int64_t{1} << 32) / kQuantThreads - 1;  // less than 2^32 work-items a grid
   with_float(type, [&](auto e) {
     using T = decltype(e);
     for (int64_t row0 = 0; row0 < m; row0 += kRows) {
-      quantize_kernel<T><<<static_cast<unsigned>(std::min(kRows, m - row0)), kQuantThreads, 0, s>>>(
-        static_cast<const T*>(x), stride, k, codes, cstride, scales, row0);
+      const auto rows   = static_cast<unsigned>(std::min(kRows, m - row0));
+      constexpr int N   = kPer16<T>;
+      const auto launch = [&](auto kernel) {
+        kernel<<<rows, kQuantThreads, 0, s>>>(static_cast<const T*>(x), stride, k, pad, codes, cstride, scales, row0);
+      };
+      if (k <= kQuantThreads * N)
+        launch(quantize_kernel<T, 1>);
+      else if (k <= 2 * kQuantThreads * N)
+        launch(quantize_kernel<T, 2>);
+      else
+        launch(quantize_kernel<T, 8>);
       OCTEX_HIP(hipGetLastError());
     }
   });
 }
 
-void launch_int8_scores(int8_rows const& q, int64_t m, int8_rows const& r, int64_t n, int k, const float* bias, void* out,
-                        elem type, int64_t ostride, hipStream_t s)
+namespace {
+
+constexpr int64_t kMaxItems = (int64_t{1} << 32) - 1;  // work-items of a grid
+
+template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
+void launch_tiled(product const& p, hipStream_t s)
 {
-  constexpr int64_t kTiles = (int64_t{1} << 32) / 256 - 1;  // less than 2^32 work-items a grid
-  const int64_t tiles_n    = (n + 63) / 64;
-  OCTEX_EXPECTS(tiles_n <= kTiles, "octex: too many rows to score at once");
-  const int64_t step = kTiles / tiles_n * 64;  // queries of a grid
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, kThreadsHere = 64 * WM * WN;
+  constexpr int kOut   = 8 * BN + WM * WN * 32 * (TN * 32 * static_cast<int>(sizeof(O)) + 16);
+  constexpr size_t lds = std::max((kAhead + 1) * (BM + BN) * kStep, kOut);
+  const auto kernel    = tiled_scores_kernel<WM, WN, TM, TN, kStep, kAhead, O>;
+  allow_lds(reinterpret_cast<const void*>(kernel), lds);
+  const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
+  OCTEX_EXPECTS(tm * tn <= kMaxItems / kThreadsHere, "octex: too many scores at once");
+  const tile_order o{static_cast<unsigned>(tm), static_cast<unsigned>(tn)};
+  kernel<<<o.tm * o.tn, kThreadsHere, lds, s>>>(p, o);
+  OCTEX_HIP(hipGetLastError());
+}
+
+template <typename Q, bool kFused, typename O>
+void launch_few(product const& p, const Q* floats, int64_t fstride, hipStream_t s)
+{
+  const int pitch = (p.k + 15) / 16 * 16 + ((p.k + 15) / 16 % 2 == 0 ? 16 : 0);  // an odd number of chunks: rows on other banks
+  const auto launch = [&](auto rt, auto kw) {
+    constexpr int RT = decltype(rt)::value, KW = decltype(kw)::value;
+    const auto kernel = few_scores_kernel<RT, KW, kFused, Q, O>;
+    const size_t lds  = std::max<size_t>(KW * RT * 1024, kFused ? p.m * pitch : 0);
+    allow_lds(reinterpret_cast<const void*>(kernel), lds);
+    const int64_t blocks = (p.n + RT * 16 - 1) / (RT * 16);
+    OCTEX_EXPECTS(blocks * 64 * KW <= kMaxItems, "octex: too many rows to score at once");
+    kernel<<<static_cast<unsigned>(blocks), 64 * KW, lds, s>>>(p, floats, fstride, pitch);
+    OCTEX_HIP(hipGetLastError());
+  };
+  if (p.n >= 32768)
+    launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+  else if (p.n >= 8192)
+    launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+  else
+    launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+}
+
+/**
+ * The tilings, and what each was measured to take: `a` us a column and c us for one tile by itself; with all of its slots
+ * (workgroups on the GPU at a time) busy, `rate` operations a us and e us to store a round's results.  Larger tiles load
+ * each operand fewer times and smaller ones fill the GPU with less, so a product takes the tiling whose estimate is least
+ * (us, of 256 x 256, 256 x 128, 128 x 128 and 64 x 64):
+ *   1000 x 960 x 100,000: 161, 146, 180, 262;  4096 x 4096 x 4096: 66, 78, 90, 117;  2048 x 2048 x 2048: 27, 20, 16, 20;
+ *   333 x 1008 x 5003: 19, 12, 11, 8.5;  128 x 4096 x 8192: 50, 29, 22, 15.
+ */
+struct tiling {
+  int bm, bn, slots;
+  double c, a, rate, e;
+};
+constexpr tiling kTilings[] = {{256, 256, 256, 8.6, 0.0080, 2.40e9, 10.0},
+                               {256, 128, 512, 6.9, 0.0044, 1.92e9, 5.0},
+                               {128, 128, 512, 6.3, 0.0035, 1.75e9, 5.2},
+                               {64, 64, 768, 3.4, 0.0019, 1.65e9, 4.2}};
+
+auto estimate(tiling const& t, product const& p) -> double
+{
+  const double tiles  = static_cast<double>((p.m + t.bm - 1) / t.bm) * static_cast<double>((p.n + t.bn - 1) / t.bn);
+  const double rounds = std::ceil(tiles / t.slots), left = tiles - (rounds - 1) * t.slots;
+  const double tile   = 2.0 * t.bm * t.bn * p.k / t.rate;
+  return t.c + (rounds - 1) * (t.slots * tile + t.e) + std::max(t.a * p.k, left * tile);
+}
+
+template <typename O>
+void launch_best(product const& p, hipStream_t s)
+{
+  int best = 0;
+  for (int i = 1; i < 4; ++i)
+    if (estimate(kTilings[i], p) < estimate(kTilings[best], p)) best = i;
+  if (best == 0)
+    launch_tiled<2, 4, 4, 2, 128, 1, O>(p, s);
+  else if (best == 1)
+    launch_tiled<4, 2, 2, 2, 64, 2, O>(p, s);
+  else if (best == 2)
+    launch_tiled<2, 2, 2, 2, 64, 3, O>(p, s);
+  else
+    launch_tiled<2, 2, 1, 1, 128, 2, O>(p, s);
+}
+
+/** Whether whole 16-byte chunks reach all of an operand, a tile's rows within 32-bit offsets. */
+auto chunked(int8_rows const& r, int k) -> bool
+{
+  return k % 16 == 0 && r.stride % 16 == 0 && reinterpret_cast<uintptr_t>(r.x) % 16 == 0 && r.stride <= kMaxInt8Stride;
+}
+
+void launch_pack(const int8_t* x, int64_t stride, int64_t n, int k, int8_t* out, int64_t pitch, hipStream_t s)
+{
+  const int64_t blocks = (n * ((k + 15) / 16) + kPackThreads - 1) / kPackThreads;
+  pack_kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 20)), kPackThreads, 0, s>>>(x, stride, n, k, out, pitch);
+  OCTEX_HIP(hipGetLastError());
+}
+
+constexpr int kFewQueries      = 16;                  // a matrix instruction's
+constexpr int64_t kFewRows     = 8192;                // whose tiles would leave half of the GPU idle (1 x 4096 x 5000: 12.2 us, not 7.2)
+constexpr int kFewFused        = 8192;                // values up to which each workgroup quantizes all queries itself
+constexpr int64_t kPackedBytes = int64_t{128} << 20;  // of rows laid out anew at a time: they stay in the last-level cache
+
+/** How a product is made, and where its workspace lies. */
+struct scores_plan {
+  bool few;                          // by few_scores_kernel, from operands as they are (floats: quantized on the way)
+  bool pack_q, pack_r;               // operands laid out anew
+  int64_t pitch, part;               // of such rows; how many of them at a time
+  int64_t codes, scales, rows, end;  // offsets: the queries' codes and scales, the rows
+};
+
+auto plan_of(int8_query const& q, int64_t m, int8_rows const& r, int64_t n, int k) -> scores_plan
+{
+  constexpr int64_t kAlign = 256;
+  const auto up            = [](int64_t v) { return (v + kAlign - 1) / kAlign * kAlign; };
+  const bool floats = q.type != elem::i8, fused = floats && m <= kFewQueries && m * k <= kFewFused;
+  scores_plan p{};
+  // quantized queries end with zeros, so that their rows' chunks may be whole
+  const bool q_fits = floats || chunked({static_cast<const int8_t*>(q.x), q.stride, nullptr}, k), r_fits = chunked(r, k);
+  p.few    = fused || (m <= kFewQueries && (!r_fits || !q_fits || n < kFewRows));
+  p.pitch  = int8_pitch(k);
+  p.pack_q = !floats && !p.few && !(q_fits && r_fits);
+  p.pack_r = !p.few && !r_fits;
+  p.part   = p.pack_r ? std::min(n, std::max<int64_t>(kPackedBytes / p.pitch, 1)) : n;
+  if ((floats && !fused) || p.pack_q) p.scales = up(m * p.pitch);
+  if (floats && !fused) p.rows = p.scales + up(m * 4);
+  if (p.pack_q) p.rows = p.scales;
+  p.end = p.rows + (p.pack_r ? up(p.part * p.pitch) : 0);
+  return p;
+}
+
+}  // namespace
+
+auto int8_scores_workspace(int8_query const& q, int64_t m, int8_rows const& r, int64_t n, int k) -> int64_t
+{
+  return plan_of(q, m, r, n, k).end;
+}
+
+void launch_int8_scores(int8_query const& q, int64_t m, int8_rows const& r, int64_t n, int k, const float* bias, void* out,
+                        elem type, int64_t ostride, void* workspace, hipStream_t s)
+{
+  const auto plan   = plan_of(q, m, r, n, k);
+  auto* w           = static_cast<int8_t*>(workspace);
+  const bool floats = q.type != elem::i8;
+  product p{{static_cast<const int8_t*>(q.x), q.stride, q.scales}, r, m, n, k, bias, out, ostride};
   with_float(type, [&](auto e) {
     using O = decltype(e);
-    for (int64_t i0 = 0; i0 < m; i0 += step) {
-      product p{q, r, std::min(step, m - i0), n, k, bias, static_cast<O*>(out) + i0 * ostride, ostride};
-      p.q.x += i0 * q.stride;
-      p.q.scales += i0;
-      const int64_t tiles = (p.m + 63) / 64 * tiles_n;
-      scores_kernel<O><<<static_cast<unsigned>(tiles), 256, 0, s>>>(p, static_cast<unsigned>(tiles_n));
-      OCTEX_HIP(hipGetLastError());
+    if (floats && plan.end == 0) {
+      with_float(q.type, [&](auto f) {
+        using Q = decltype(f);
+        launch_few<Q, true, O>(p, static_cast<const Q*>(q.x), q.stride, s);
+      });
+      return;
+    }
+    const int chunks = (k + 15) / 16 * 16;
+    if (floats) {
+      auto* scales = reinterpret_cast<float*>(w + plan.scales);
+      launch_quantize_rows(q.x, q.type, m, k, chunks, q.stride, w, plan.pitch, scales, s);
+      p.q = {w, plan.pitch, scales};
+    } else if (plan.pack_q) {
+      launch_pack(p.q.x, p.q.stride, m, k, w, plan.pitch, s);
+      p.q = {w, plan.pitch, q.scales};
+    }
+    if (plan.few) {
+      launch_few<float, false, O>(p, nullptr, 0, s);
+      return;
+    }
+    p.k = chunks;
+    for (int64_t j0 = 0; j0 < n; j0 += plan.part) {
+      p.n = std::min(plan.part, n - j0);
+      p.r = {r.x + j0 * r.stride, r.stride, r.scales + j0};
+      if (plan.pack_r) {
+        launch_pack(p.r.x, r.stride, p.n, k, w + plan.rows, plan.pitch, s);
+        p.r.x = w + plan.rows, p.r.stride = plan.pitch;
+      }
+      p.bias = bias != nullptr ? bias + j0 : nullptr;
+      p.out  = static_cast<O*>(out) + j0;
+      launch_best<O>(p, s);
     }
   });
 }

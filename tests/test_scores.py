@@ -75,12 +75,14 @@ def test_sizes_are_answered(host):
     f = S._entry("octexLogProbs")
     assert f(*log_probs(host, size=at)[1:]) == _lib.CUVS_SUCCESS and size.value >= 0
     f = S._entry("octexInt8Scores")
-    x, codes, out = matrix(host["x"], FLOAT32), matrix(host["codes"], INT8), matrix(np.zeros((3, 3), np.float32), FLOAT32)
+    many = np.zeros((300, 40), np.float32)
+    x, codes, out = matrix(many, FLOAT32), matrix(host["codes"], INT8), matrix(np.zeros((300, 3), np.float32), FLOAT32)
     v = host["v"].ctypes.data
     assert f(x, None, codes, v, None, out, None, 0, at, None) == _lib.CUVS_SUCCESS
     need = size.value
-    assert need >= 3 * 40 + 3 * 4  # the quantized queries and their scales
-    assert f(codes, v, codes, v, None, out, None, 0, at, None) == _lib.CUVS_SUCCESS
+    assert need >= 300 * 40 + 300 * 4  # the quantized queries and their scales
+    own = matrix(np.zeros((300, 40), np.int8), INT8)
+    assert f(own, v, codes, v, None, out, None, 0, at, None) == _lib.CUVS_SUCCESS and size.value >= 0
     assert "workspace" in refused("octexInt8Scores", x, None, codes, v, None, out, v, need - 1, None, None)
 
 
