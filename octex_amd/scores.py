@@ -16,6 +16,7 @@ import collections
 import contextlib
 import ctypes as ct
 import functools
+import sys
 
 import numpy as np
 
@@ -58,38 +59,52 @@ def _entry(name):
 
 @functools.lru_cache(None)
 def _torch():
+    """torch, the names of its element types, and the raw handle of a GPU's current stream."""
     import torch
 
     names = {getattr(torch, n): n for n in _TYPES}
-    return torch, names
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the public call makes an object of 2 us
+    return torch, names, raw if raw is not None else lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
 
 
 class _Call:
     """One call's operands and results, all on one GPU, and the stream they are ordered on."""
 
+    __slots__ = ("torch", "names", "origin", "device", "stream", "on_host", "foreign", "first", "scratch")
+
     def __init__(self, first, name, types):
-        self.torch, self.names = _torch()
-        self.origin, self.device, self.stream, self.on_host = first, None, None, False
-        self.first = self.take(first, name, types)
+        self.torch, self.names, raw_stream = _torch()
+        self.origin, self.device, self.foreign = first, None, False
+        if isinstance(first, self.torch.Tensor):
+            t = first
+        elif _arrays.is_foreign_device(first):
+            self.foreign = True
+            t = self.view(first)
+        else:
+            t = self.view(first)
+        self.on_host = not t.is_cuda
+        if self.on_host:
+            self.device = self.torch.device("cuda", self.torch.cuda.current_device())
+        else:
+            self.device = t.device
+        self.stream = _arrays._foreign_stream(first) if self.foreign and t.is_cuda else raw_stream(self.device.index)
+        self.first = self.take(t, name, types)
+
+    def view(self, a):
+        """Any array as a torch tensor in the memory where it lies."""
+        if _arrays.is_foreign_device(a):
+            return self.torch.from_dlpack(a) if hasattr(a, "__dlpack__") else self.torch.as_tensor(a, device="cuda")
+        x = np.asarray(a)
+        return self.torch.from_numpy(x if x.flags.writeable else x.copy())
 
     def take(self, a, name, types, ndim=2, shape=None):
         """The operand as a torch tensor on the call's GPU: of one of `types` (else converted to the first), the elements
         of a row side by side.  A vector is one row unless ndim is 1."""
         torch = self.torch
-        if isinstance(a, torch.Tensor):
-            t = a
-        elif _arrays.is_foreign_device(a):
-            if self.stream is None and self.device is None:
-                self.stream = _arrays._foreign_stream(a)
-            t = torch.from_dlpack(a) if hasattr(a, "__dlpack__") else torch.as_tensor(a, device="cuda")
-        else:
-            x = np.asarray(a)
-            t = torch.from_numpy(x if x.flags.writeable else x.copy())
-        if self.device is None:
-            self.on_host = not t.is_cuda
-            self.device = torch.device("cuda", torch.cuda.current_device()) if self.on_host else t.device
-            if self.stream is None:
-                self.stream = torch.cuda.current_stream(self.device).cuda_stream
+        t = a if isinstance(a, torch.Tensor) else self.view(a)
         if t.device != self.device:
             if t.is_cuda:
                 raise ValueError(f"octex: {name} lies on {t.device}, the other operands on {self.device}")
@@ -102,55 +117,69 @@ class _Call:
                 raise TypeError(f"octex: {name} must be {' or '.join(types)}, not {str(t.dtype).replace('torch.', '')}")
             with self.context():
                 t = t.to(getattr(torch, types[0]))
-        if ndim == 2 and t.ndim == 1:
-            t = t[None, :]
         if t.ndim != ndim:
-            raise ValueError(f"octex: {name} must be a {'matrix' if ndim == 2 else 'vector'}, not of {t.ndim} dimensions")
-        if shape is not None and tuple(t.shape) != shape:
-            raise ValueError(f"octex: {name} has shape {tuple(t.shape)}, expected {shape}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1 or (ndim == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            if ndim == 2 and t.ndim == 1:
+                t = t[None, :]
+            else:
+                raise ValueError(f"octex: {name} must be a {'matrix' if ndim == 2 else 'vector'}, "
+                                 f"not of {t.ndim} dimensions")
+        s = t.shape
+        if shape is not None and s != shape:
+            raise ValueError(f"octex: {name} has shape {tuple(s)}, expected {tuple(shape)}")
+        if not t.is_contiguous() and (s[-1] > 1 and t.stride(-1) != 1 or (ndim == 2 and s[0] > 1 and t.stride(0) < s[1])):
             with self.context():
                 t = t.contiguous()
         return t
 
     def dense(self, a, name, shape):
         """A float32 operand without gaps between its rows."""
-        t = self.take(a, name, ("float32",), ndim=len(shape), shape=shape)
+        t = self.take(a, name, ("float32",), len(shape), shape)
+        if t.is_contiguous():
+            return t
         with self.context():
             return t.contiguous()
 
     def context(self):
-        """torch's own work (conversions, allocations) on the call's stream."""
-        torch = self.torch
-        if torch.cuda.current_stream(self.device).cuda_stream == self.stream:
-            return contextlib.nullcontext()
-        return torch.cuda.stream(torch.cuda.ExternalStream(self.stream, device=self.device))
+        """For torch's own work (conversions, allocations) on the call's stream."""
+        if not self.foreign:
+            return _HERE
+        return self.torch.cuda.stream(self.torch.cuda.ExternalStream(self.stream, device=self.device))
 
     def matrix(self, t):
-        return _Matrix(t.data_ptr(), _TYPES[self.names[t.dtype]], t.shape[0], t.shape[1], max(t.stride(0), t.shape[1]))
+        rows, cols = t.shape
+        return _Matrix(t.data_ptr(), _TYPES[self.names[t.dtype]], rows, cols, max(t.stride(0), cols))
 
-    def new(self, shape, dtype="float32"):
-        return self.torch.empty(shape, dtype=getattr(self.torch, dtype), device=self.device)
+    def new(self, *shapes, dtype=None):
+        """New results: float32, or of a torch type."""
+        empty, device, dtype = self.torch.empty, self.device, dtype or self.torch.float32
+        if self.foreign:
+            with self.context():
+                out = [empty(s, dtype=dtype, device=device) for s in shapes]
+        else:
+            out = [empty(s, dtype=dtype, device=device) for s in shapes]
+        return out if len(out) > 1 else out[0]
 
     def run(self, entry, *args):
         if _entry(entry)(*args, self.stream) != _lib.CUVS_SUCCESS:
             raise _lib.OctexError(_lib.lib().cuvsGetLastErrorText().decode())
 
-    def workspace(self, entry, *args):
-        """(address, bytes, no question) of the workspace that these arguments need; its tensor is kept with the call."""
+    def run_sized(self, entry, *args):
+        """run with the workspace that the arguments need; its tensor is kept with the call."""
         size = _I64(0)
         self.run(entry, *args, None, 0, ct.addressof(size))
         if size.value == 0:
-            return None, 0, None
-        self.scratch = self.new((size.value,), "int8")
-        return self.scratch.data_ptr(), size.value, None
+            return self.run(entry, *args, None, 0, None)
+        self.scratch = self.new((size.value,), dtype=self.torch.int8)
+        return self.run(entry, *args, self.scratch.data_ptr(), size.value, None)
 
     def give(self, t):
         """A result in the framework, and the memory, of the first operand."""
+        if not self.on_host and not self.foreign:
+            return t
         if isinstance(self.origin, self.torch.Tensor):
-            return t.cpu() if self.on_host else t
-        if _arrays.is_foreign_device(self.origin):
-            conv = getattr(__import__("sys").modules.get(_arrays._module_of(self.origin)), "from_dlpack", None)
+            return t.cpu()
+        if self.foreign:
+            conv = getattr(sys.modules.get(_arrays._module_of(self.origin)), "from_dlpack", None)
             return conv(t) if conv is not None else t
         return t.cpu().numpy()
 
@@ -163,8 +192,7 @@ def quantize_rows(x):
     """
     c = _Call(x, "x", FLOATS)
     x = c.first
-    with c.context():
-        codes, scales = c.new(tuple(x.shape), "int8"), c.new((x.shape[0],))
+    codes, scales = c.new(x.shape, dtype=c.torch.int8), c.new((x.shape[0],))
     c.run("octexQuantizeRows", c.matrix(x), c.matrix(codes), scales.data_ptr())
     return c.give(codes), c.give(scales)
 
@@ -192,26 +220,31 @@ def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtyp
         bias = c.dense(bias, "bias", (n,))
     if dtype is None:
         dtype = "float32" if coded else c.names[q.dtype]
-    dtype = str(dtype).replace("torch.", "") if not isinstance(dtype, type) else np.dtype(dtype).name
+    if dtype not in FLOATS:
+        dtype = np.dtype(dtype).name if isinstance(dtype, type) else str(dtype).replace("torch.", "")
     if dtype not in FLOATS:
         raise ValueError(f"octex: scores are of type {', '.join(FLOATS)}, not {dtype}")
-    with c.context():
-        out = c.new((m, n), dtype)
-        args = (c.matrix(q), query_scales.data_ptr() if coded else None, c.matrix(rows), row_scales.data_ptr(),
-                None if bias is None else bias.data_ptr(), c.matrix(out))
-        c.run("octexInt8Scores", *args, *c.workspace("octexInt8Scores", *args))
+    out = c.new((m, n), dtype=getattr(c.torch, dtype))
+    c.run_sized("octexInt8Scores", c.matrix(q), query_scales.data_ptr() if coded else None, c.matrix(rows),
+                row_scales.data_ptr(), None if bias is None else bias.data_ptr(), c.matrix(out))
     return c.give(out)
+
+
+def _columns(a):
+    """A vector, one entry a row, as a matrix of one column; and its shape."""
+    shape = a.shape if hasattr(a, "shape") else _arrays.shape_of(a)
+    if len(shape) != 1:
+        return a, shape
+    return (a if hasattr(a, "ndim") else np.asarray(a))[:, None], shape
 
 
 def _ids(c, ids, m):
     """The ids of m rows as a matrix, and the shape their values come back in."""
-    shape = _arrays.shape_of(ids)
-    if len(shape) == 1:
-        ids = ids[:, None] if hasattr(ids, "ndim") else np.asarray(ids)[:, None]
+    ids, shape = _columns(ids)
     t = c.take(ids, "ids", INTS)
     if t.shape[0] != m:
         raise ValueError(f"octex: ids of {t.shape[0]} rows, logits of {m}")
-    return t, shape
+    return t, tuple(shape)
 
 
 def log_probs(logits, ids, *, top=0, temperature=1.0):
@@ -231,13 +264,11 @@ def log_probs(logits, ids, *, top=0, temperature=1.0):
     if not 0 <= top <= 64:
         raise ValueError(f"octex: 0 to 64 top entries, not {top}")
     t, shape = _ids(c, ids, m)
-    with c.context():
-        logp, entropy, lse = c.new(shape), c.new((m,)), c.new((m,))
-        top_logp, top_ids = c.new((m, top)), c.new((m, top), "int64")
-        args = (c.matrix(x), c.matrix(t), temperature, top, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
-                top_logp.data_ptr(), top_ids.data_ptr())
-        c.run("octexLogProbs", *args, *c.workspace("octexLogProbs", *args))
-    return LogProbs(*(c.give(v) for v in (logp, entropy, lse, top_logp, top_ids)))
+    logp, entropy, lse, top_logp = c.new(shape, (m,), (m,), (m, top))
+    top_ids = c.new((m, top), dtype=c.torch.int64)
+    c.run_sized("octexLogProbs", c.matrix(x), c.matrix(t), temperature, top, logp.data_ptr(), entropy.data_ptr(),
+                lse.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
+    return LogProbs(c.give(logp), c.give(entropy), c.give(lse), c.give(top_logp), c.give(top_ids))
 
 
 def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, *, temperature=1.0):
@@ -253,8 +284,7 @@ def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, 
     gl = None if grad_log_probs is None else c.dense(grad_log_probs, "grad_log_probs", shape)
     gh = None if grad_entropy is None else c.dense(grad_entropy, "grad_entropy", (m,))
     lse, entropy = c.dense(lse, "lse", (m,)), c.dense(entropy, "entropy", (m,))
-    with c.context():
-        grad = c.new(tuple(x.shape), c.names[x.dtype])
+    grad = c.new(x.shape, dtype=x.dtype)
     c.run("octexLogProbsBackward", c.matrix(x), c.matrix(t), temperature, None if gl is None else gl.data_ptr(),
           None if gh is None else gh.data_ptr(), lse.data_ptr(), entropy.data_ptr(), c.matrix(grad))
     return c.give(grad)
@@ -262,10 +292,8 @@ def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, 
 
 def _teacher(logits, ids, teacher):
     c = _Call(logits, "logits", FLOATS)
-    t, shape = _ids(c, ids, c.first.shape[0])
-    if len(shape) == 1:
-        teacher = teacher[:, None] if hasattr(teacher, "ndim") else np.asarray(teacher)[:, None]
-    return c, c.first, t, c.take(teacher, "teacher", FLOATS, shape=tuple(t.shape))
+    t, _ = _ids(c, ids, c.first.shape[0])
+    return c, c.first, t, c.take(_columns(teacher)[0], "teacher", FLOATS, shape=t.shape)
 
 
 def distill(logits, ids, teacher, *, temperature=1.0):
@@ -279,10 +307,8 @@ def distill(logits, ids, teacher, *, temperature=1.0):
     """
     c, x, t, teacher = _teacher(logits, ids, teacher)
     m = x.shape[0]
-    with c.context():
-        loss, lse = c.new((m,)), c.new((m,))
-        args = (c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, loss.data_ptr(), lse.data_ptr())
-        c.run("octexDistill", *args, *c.workspace("octexDistill", *args))
+    loss, lse = c.new((m,), (m,))
+    c.run_sized("octexDistill", c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, loss.data_ptr(), lse.data_ptr())
     return c.give(loss), c.give(lse)
 
 
@@ -294,8 +320,7 @@ def distill_backward(grad_loss, logits, ids, teacher, lse, *, temperature=1.0):
     c, x, t, teacher = _teacher(logits, ids, teacher)
     m = x.shape[0]
     g, lse = c.dense(grad_loss, "grad_loss", (m,)), c.dense(lse, "lse", (m,))
-    with c.context():
-        grad = c.new(tuple(x.shape), c.names[x.dtype])
+    grad = c.new(x.shape, dtype=x.dtype)
     c.run("octexDistillBackward", c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, g.data_ptr(), lse.data_ptr(),
           c.matrix(grad))
     return c.give(grad)
@@ -306,9 +331,7 @@ def distill_step(grad_loss, logits, ids, teacher, *, temperature=1.0):
     c, x, t, teacher = _teacher(logits, ids, teacher)
     m = x.shape[0]
     g = c.dense(grad_loss, "grad_loss", (m,))
-    with c.context():
-        loss, lse, grad = c.new((m,)), c.new((m,)), c.new(tuple(x.shape), c.names[x.dtype])
-        args = (c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, g.data_ptr(), loss.data_ptr(), lse.data_ptr(),
-                c.matrix(grad))
-        c.run("octexDistillStep", *args, *c.workspace("octexDistillStep", *args))
+    (loss, lse), grad = c.new((m,), (m,)), c.new(x.shape, dtype=x.dtype)
+    c.run_sized("octexDistillStep", c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, g.data_ptr(), loss.data_ptr(),
+                lse.data_ptr(), c.matrix(grad))
     return c.give(loss), c.give(grad)
