@@ -133,6 +133,13 @@ auto asked_size(int64_t need, int64_t bytes, int64_t* size) -> bool
   return false;
 }
 
+void take_workspace(on_gpu& gpu, const void* workspace, int64_t need)
+{
+  if (need == 0) return;
+  gpu.take(workspace, "workspace");
+  OCTEX_EXPECTS(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "octex: the workspace must lie at a multiple of 256 bytes");
+}
+
 }  // namespace
 
 extern "C" cuvsError_t octexQuantizeRows(const octexMatrix* x, const octexMatrix* codes, float* scales, void* stream)
@@ -180,8 +187,7 @@ extern "C" cuvsError_t octexInt8Scores(const octexMatrix* queries, const float* 
     gpu.take(out->data, "out");
     if (coded) gpu.take(query_scales, "query_scales");
     if (bias != nullptr) gpu.take(bias, "bias");
-    if (need > 0) gpu.take(workspace, "workspace");
-    OCTEX_EXPECTS(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "octex: the workspace must lie at a multiple of 256 bytes");
+    take_workspace(gpu, workspace, need);
     launch_int8_scores(q, m, r, n, static_cast<int>(k), bias, out->data, elem_of(*out), out->stride, workspace,
                        static_cast<hipStream_t>(stream));
   });
@@ -195,14 +201,16 @@ extern "C" cuvsError_t octexLogProbs(const octexMatrix* logits, const octexMatri
     const auto in = logits_of(logits, temperature);
     const auto id = ids_of(ids, in.m);
     OCTEX_EXPECTS(top >= 0 && top <= kMaxTop, "octex: 0 to %d top entries, not %d", kMaxTop, top);
-    if (asked_size(0, bytes, size)) return;
-    (void)workspace;
+    const int64_t need = in.m == 0 ? 0 : log_probs_workspace(in.m, in.n, top);
+    if (asked_size(need, bytes, size)) return;
     if (in.m == 0) return;
     on_gpu gpu;
+    take_workspace(gpu, workspace, need);
     gpu.take(in.x, "logits"), gpu.take(entropy, "entropy"), gpu.take(lse, "lse");
     if (id.k > 0) gpu.take(id.ids, "ids"), gpu.take(log_probs, "log_probs");
     if (top > 0) gpu.take(top_log_probs, "top_log_probs"), gpu.take(top_ids, "top_ids");
-    launch_log_probs(in, id, {log_probs, entropy, lse, top_log_probs, top_ids, top}, static_cast<hipStream_t>(stream));
+    launch_log_probs(in, id, {log_probs, entropy, lse, top_log_probs, top_ids, top}, workspace,
+                     static_cast<hipStream_t>(stream));
   });
 }
 
@@ -233,13 +241,14 @@ extern "C" cuvsError_t octexDistill(const octexMatrix* logits, const octexMatrix
     const auto in = logits_of(logits, temperature);
     const auto id = ids_of(ids, in.m);
     const auto t  = teacher_of(teacher, id, in.m);
-    if (asked_size(0, bytes, size)) return;
-    (void)workspace;
+    const int64_t need = in.m == 0 ? 0 : distill_workspace(in.m, in.n);
+    if (asked_size(need, bytes, size)) return;
     if (in.m == 0) return;
     on_gpu gpu;
+    take_workspace(gpu, workspace, need);
     gpu.take(in.x, "logits"), gpu.take(loss, "loss"), gpu.take(lse, "lse");
     if (id.k > 0) gpu.take(id.ids, "ids"), gpu.take(t.x, "teacher");
-    launch_distill(in, id, t, loss, lse, static_cast<hipStream_t>(stream));
+    launch_distill(in, id, t, loss, lse, workspace, static_cast<hipStream_t>(stream));
   });
 }
 
@@ -269,15 +278,15 @@ extern "C" cuvsError_t octexDistillStep(const octexMatrix* logits, const octexMa
     const auto id = ids_of(ids, in.m);
     const auto t  = teacher_of(teacher, id, in.m);
     grad_of(grad, logits);
-    if (asked_size(0, bytes, size)) return;
-    (void)workspace;
+    const int64_t need = in.m == 0 || distill_step_held(in.n, in.type) ? 0 : distill_workspace(in.m, in.n);
+    if (asked_size(need, bytes, size)) return;
     if (in.m == 0) return;
     on_gpu gpu;
+    take_workspace(gpu, workspace, need);
     gpu.take(in.x, "logits"), gpu.take(grad_loss, "grad_loss"), gpu.take(loss, "loss"), gpu.take(lse, "lse");
     gpu.take(grad->data, "grad");
     if (id.k > 0) gpu.take(id.ids, "ids"), gpu.take(t.x, "teacher");
-    auto s = static_cast<hipStream_t>(stream);
-    launch_distill(in, id, t, loss, lse, s);
-    launch_distill_backward(in, id, t, grad_loss, lse, grad->data, grad->stride, s);
+    launch_distill_step(in, id, t, grad_loss, loss, lse, grad->data, grad->stride, workspace,
+                        static_cast<hipStream_t>(stream));
   });
 }

@@ -26,7 +26,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves   = kThreads / 64;
 constexpr int kUnroll  = 4;     // 16-byte loads a thread keeps in flight
 constexpr int kList    = 256;   // a wavefront's candidate keys: four a lane
-constexpr int kSlack   = 12;    // entries that a compaction may keep beyond the k best
+constexpr int kFull    = 128;   // keys from which a list is compacted
 
 __device__ inline auto exp2_fast(float v) -> float { return __builtin_amdgcn_exp2f(v); }
 
@@ -83,7 +83,8 @@ __device__ inline auto shuffle_xor(run const& a, int mask) -> run
   return r;
 }
 
-/** The whole workgroup's sums, the same in every thread; parts [kWaves] is LDS. */
+/** The whole workgroup's sums, the same in every thread; parts is LDS, one a wavefront. */
+template <int NT>
 __device__ inline auto join_block(run r, float c, run* parts) -> run
 {
 #pragma unroll
@@ -92,7 +93,7 @@ __device__ inline auto join_block(run r, float c, run* parts) -> run
   if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = r;
   __syncthreads();
   r = parts[0];
-  for (int w = 1; w < kWaves; ++w)
+  for (int w = 1; w < NT / 64; ++w)
     r = join(r, parts[w], c);
   return r;
 }
@@ -121,50 +122,63 @@ __device__ inline auto log_prob(float x, row_sums const& o, float temperature) -
 
 using key64 = unsigned long long;
 
-__device__ inline auto key_of(float v, int column) -> key64
+__device__ inline auto order_of(float v) -> unsigned
 {
   const unsigned b = __float_as_uint(v + 0.f);  // -0 and 0 are one value
-  const unsigned o = b >> 31 ? ~b : b | 0x80000000u;
-  return key64{o} << 32 | static_cast<unsigned>(~column);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+
+__device__ inline auto key_of(float v, int column) -> key64
+{
+  return key64{order_of(v)} << 32 | static_cast<unsigned>(~column);
 }
 
 __device__ inline auto value_of_order(unsigned o) -> float { return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
 __device__ inline auto value_of(key64 k) -> float { return value_of_order(static_cast<unsigned>(k >> 32)); }
 __device__ inline auto column_of(key64 k) -> int { return static_cast<int>(~static_cast<unsigned>(k)); }
 
-/** A floor such that at least k and at most k + slack of the wavefront's distinct keys (0: none) reach it; 0 if there are
- * not k. */
-__device__ inline auto floor_of(const key64 (&key)[4], int k, int slack) -> key64
+/** A floor that at least k and, unless equal values forbid it, at most `most` of the wavefront's values reach, as orders
+ * (0: none); 0 if there are not k. */
+template <int N>
+__device__ inline auto floor_of(const unsigned (&order)[N], int k, int most) -> unsigned
 {
-  key64 p = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const key64 q = p | key64{1} << bit;
-    int c         = 0;
+  unsigned p = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const unsigned q = p | 1u << bit;
+    int c            = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      c += __popcll(__ballot(key[j] >= q));
+    for (int j = 0; j < N; ++j)
+      c += __popcll(__ballot(order[j] >= q));
     if (c >= k) {
       p = q;
-      if (c <= k + slack) break;
+      if (c <= most) break;
     }
   }
   return p;
 }
 
-/** Writes the keys at or above floor to list, dense; returns their count. */
-__device__ inline auto keep_from(const key64 (&key)[4], key64 floor, key64* list) -> int
+/** The same for distinct keys, which leave at most `most`. */
+__device__ inline auto floor_of(const key64 (&key)[4], int k, int most) -> key64
 {
-  const int lane = threadIdx.x % 64;
-  int n          = 0;
+  unsigned order[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool in  = key[j] != 0 && key[j] >= floor;
-    const key64 at = __ballot(in);
-    if (in) list[n + __popcll(at & ((key64{1} << lane) - 1))] = key[j];
-    n += __popcll(at);
+  for (int j = 0; j < 4; ++j)
+    order[j] = static_cast<unsigned>(key[j] >> 32);
+  key64 p = key64{floor_of(order, k, most)} << 32;
+  if (p == 0) return 0;
+  int c = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    c += __popcll(__ballot(key[j] >= p));
+  for (int bit = 31; bit >= 0 && c > most; --bit) {  // equal values: by column
+    const key64 q = p | key64{1} << bit;
+    int d         = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      d += __popcll(__ballot(key[j] >= q));
+    if (d >= k) p = q, c = d;
   }
-  wave_fence();
-  return n;
+  return p;
 }
 
 struct top_list {
@@ -173,7 +187,8 @@ struct top_list {
   int n     = 0;
   float thr = -INFINITY;  // no later score at or below it is among the k best
 
-  __device__ void compact(int slack)
+  /** Keeps the k best and at most `most` keys, at `to`. */
+  __device__ void compact(int most, key64* to)
   {
     const int lane = threadIdx.x % 64;
     key64 key[4];
@@ -182,61 +197,86 @@ struct top_list {
     for (int j = 0; j < 4; ++j)
       key[j] = lane + 64 * j < n ? list[lane + 64 * j] : 0;
     wave_fence();
-    const key64 p    = floor_of(key, k, slack);
-    n                = keep_from(key, p, list);
-    const unsigned o = static_cast<unsigned>(p >> 32);
-    if (o >= 0x00800000u) thr = value_of_order(o);  // below: not a number's order
+    const key64 p = floor_of(key, k, most);
+    n             = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in  = key[j] != 0 && key[j] >= p;
+      const key64 at = __ballot(in);
+      if (in) to[n + __popcll(at & ((key64{1} << lane) - 1))] = key[j];
+      n += __popcll(at);
+    }
+    wave_fence();
+    raise(static_cast<unsigned>(p >> 32));
   }
 
-  /** Scores v of columns at + i, above every column of earlier calls; cm is their largest. */
+  __device__ void raise(unsigned order)
+  {
+    if (order >= 0x00800000u) thr = value_of_order(order);  // below: not a number's order
+  }
+
+  /** Scores v of columns at + i, above every column of earlier calls; cm is the lane's largest. */
   template <int N>
   __device__ void add(const float (&v)[N], float cm, int at)
   {
     const float before = thr;
     if (__ballot(cm > before) == 0) return;
     const int lane = threadIdx.x % 64;
+    if (before == -INFINITY) {
+      // the first floor: k lanes have a score that reaches it
+      const unsigned order[1] = {order_of(cm)};
+      raise(floor_of(order, k, k + 8));
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       // equal scores of lower columns may come in this very call, so a floor it raised lets them in
-      const bool in  = v[i] > before && v[i] >= thr;
+      const bool in        = v[i] > before && v[i] >= thr;
       const key64 at_lanes = __ballot(in);
       if (at_lanes == 0) continue;
       if (in) list[n + __popcll(at_lanes & ((key64{1} << lane) - 1))] = key_of(v[i], at + i);
       n += __popcll(at_lanes);
-      if (n > kList - 64) compact(kSlack);
+      if (n > kList - 64) compact(k + 32, list);
     }
+    if (n > kFull) compact(k + 32, list);
   }
 };
 
-/** The k best of `lists` lists of at most 64 keys each, lists[i * kList + ..] with counts n[i]; into list 0. */
-__device__ inline void merge_lists(key64* lists, int* n, int count, int k)
+/** Calls f(rank, key) for the k best of n distinct keys in LDS; a key's rank is the number of greater ones. */
+template <int NT, typename F>
+__device__ inline void rank_keys(const key64* keys, int n, int k, F f)
 {
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  while (count > 1) {
-    const int groups = (count + 3) / 4;
-    key64 key[4]     = {0, 0, 0, 0};
-    if (wave < groups) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int l = 4 * wave + j;
-        if (l < count && lane < n[l]) key[j] = lists[l * kList + lane];
-      }
-    }
-    __syncthreads();
-    if (wave < groups) {
-      const int kept = keep_from(key, floor_of(key, k, 0), lists + wave * kList);
-      if (lane == 0) n[wave] = kept;
-    }
-    __syncthreads();
-    count = groups;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const key64 mine = keys[i];
+    int rank         = 0;
+    for (int j = 0; j < n; ++j)
+      rank += keys[j] > mine;
+    if (rank < k) f(rank, mine);
   }
+}
+
+/** The lists' k best by rank: every wavefront's list to keys (LDS, [waves * 64]), dense.  Returns their number. */
+template <int NT>
+__device__ inline auto gather_lists(top_list& top, key64* keys, int* counts) -> int
+{
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  top.compact(64, top.list);
+  if (lane == 0) counts[wave] = top.n;
+  __syncthreads();
+  int from = 0, n = 0;
+  for (int w = 0; w < NT / 64; ++w) {
+    from += w < wave ? counts[w] : 0;
+    n += counts[w];
+  }
+  if (lane < top.n) keys[from + lane] = top.list[lane];
+  __syncthreads();
+  return n;
 }
 
 // ---- one pass over a row
 
 /** Calls f(v, at) for the scores of columns [c0, c1) that this thread takes, 16 bytes at a time in ascending order; a
  * score outside the range, or one that another thread takes, comes as -inf.  Every lane of a wavefront calls f alike. */
-template <typename T, typename F>
+template <typename T, int NT, typename F>
 __device__ inline void for_scores(const T* row, int c0, int c1, F f)
 {
   constexpr int N = kPer16<T>;
@@ -252,7 +292,7 @@ __device__ inline void for_scores(const T* row, int c0, int c1, F f)
   }
   const int last = c1 - N;  // a load that would pass the range's end is moved back to it
   const int wave = c0 + static_cast<int>(threadIdx.x / 64) * 64 * N, mine = static_cast<int>(threadIdx.x % 64) * N;
-  constexpr int kStep = kThreads * N;
+  constexpr int kStep = NT * N;
   uint4 next[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u)
@@ -291,52 +331,123 @@ __device__ inline auto id_at(listed_ids const& ids, int64_t row, int j) -> int64
   return ids.wide ? static_cast<const int64_t*>(ids.ids)[i] : static_cast<const int32_t*>(ids.ids)[i];
 }
 
-template <typename T, bool kTop>
-__global__ __launch_bounds__(kThreads) void log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
-                                                             int64_t row0)
+/** How rows are shared out: `parts` workgroups a row take `width` columns each. */
+struct row_split {
+  int parts, width;
+};
+
+/** What a workgroup found in its columns, for the row's last step. */
+struct part_sums {
+  float m, s, t;
+};
+
+__device__ inline auto as_run(part_sums const& p) -> run { return {p.m, p.m == -INFINITY ? 0.f : p.m, p.s, p.t}; }
+
+/** The outputs of row r but its alternatives. */
+template <typename T, int NT>
+__device__ inline void write_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out const& out, int64_t r,
+                                       row_sums const& o)
 {
-  __shared__ run parts[kWaves];
-  __shared__ key64 lists[kTop ? kWaves * kList : 1];
-  __shared__ int counts[kWaves];
-  const int64_t r = row0 + blockIdx.x;
-  const T* row    = static_cast<const T*>(in.x) + r * in.stride;
-  const float c   = kLog2e / in.temperature;
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  run sums        = nothing();
-  top_list top{lists + (kTop ? wave * kList : 0), out.top};
-  for_scores<T>(row, 0, in.n, [&](const auto& v, int at) {
-    const float cm = add_scores<true>(sums, v, c);
-    if constexpr (kTop) top.add(v, cm, at);
-  });
-  const auto o = finish(join_block(sums, c, parts), in.temperature);
   if (threadIdx.x == 0) {
     out.lse[r]     = o.lse;
     out.entropy[r] = o.entropy;
   }
-  for (int j = threadIdx.x; j < ids.k; j += kThreads) {
-    const int64_t id = id_at(ids, r, j);
-    out.logp[r * ids.k + j] =
-      id < 0 || id >= in.n ? 0.f : log_prob(static_cast<float>(row[id]), o, in.temperature);
+  const T* row = static_cast<const T*>(in.x) + r * in.stride;
+  for (int j = threadIdx.x; j < ids.k; j += NT) {
+    const int64_t id        = id_at(ids, r, j);
+    out.logp[r * ids.k + j] = id < 0 || id >= in.n ? 0.f : log_prob(static_cast<float>(row[id]), o, in.temperature);
   }
-  if constexpr (kTop) {
-    top.compact(0);
-    if (lane == 0) counts[wave] = top.n;
-    __syncthreads();
-    merge_lists(lists, counts, kWaves, out.top);
-    if (wave == 0 && lane < out.top) {
-      const bool bad  = isnan(o.lse);
-      const int n     = bad ? 0 : min(counts[0], out.top);
-      const key64 key = lane < n ? lists[lane] : 0;
-      int rank        = lane;
-      if (lane < n) {
-        rank = 0;
-        for (int j = 0; j < n; ++j)
-          rank += lists[j] > key;
-      }
-      const int64_t at    = r * out.top + rank;
-      out.top_logp[at] = lane < n ? log_prob(value_of(key), o, in.temperature) : (bad ? o.lse : -INFINITY);
-      out.top_ids[at]  = lane < n ? column_of(key) : -1;
+}
+
+/** The alternatives of row r: the best of n keys in LDS. */
+template <int NT>
+__device__ inline void write_top(score_rows const& in, log_probs_out const& out, int64_t r, row_sums const& o,
+                                 const key64* keys, int n)
+{
+  const bool bad = isnan(o.lse);
+  const int have = bad ? 0 : min(n, out.top);
+  rank_keys<NT>(keys, bad ? 0 : n, out.top, [&](int rank, key64 key) {
+    out.top_logp[r * out.top + rank] = log_prob(value_of(key), o, in.temperature);
+    out.top_ids[r * out.top + rank]  = column_of(key);
+  });
+  if (static_cast<int>(threadIdx.x) >= have && static_cast<int>(threadIdx.x) < out.top) {
+    out.top_logp[r * out.top + threadIdx.x] = bad ? o.lse : -INFINITY;
+    out.top_ids[r * out.top + threadIdx.x]  = -1;
+  }
+}
+
+/** A workgroup a row, or with kSplit a workgroup a part of a row, which leaves its sums and its best keys (0: none) to
+ * finish_log_probs_kernel. */
+template <typename T, bool kTop, bool kSplit>
+__global__ __launch_bounds__(kThreads) void log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
+                                                             row_split split, part_sums* part, key64* best, int64_t row0)
+{
+  __shared__ run parts[kWaves];
+  __shared__ key64 lists[kTop ? kWaves * kList : 1];
+  __shared__ key64 keys[kTop ? kWaves * 64 : 1];
+  __shared__ int counts[kWaves];
+  const int64_t b = row0 + blockIdx.x, r = kSplit ? b / split.parts : b;
+  const int c0 = kSplit ? static_cast<int>(b - r * split.parts) * split.width : 0;
+  const int c1 = kSplit ? min(c0 + split.width, in.n) : in.n;
+  const T* row = static_cast<const T*>(in.x) + r * in.stride;
+  const float c = kLog2e / in.temperature;
+  run sums      = nothing();
+  top_list top{lists + (kTop ? threadIdx.x / 64 * kList : 0), out.top};
+  for_scores<T, kThreads>(row, c0, c1, [&](const auto& v, int at) {
+    const float cm = add_scores<true>(sums, v, c);
+    if constexpr (kTop) top.add(v, cm, at);
+  });
+  sums  = join_block<kThreads>(sums, c, parts);
+  int n = 0;
+  if constexpr (kTop) n = gather_lists<kThreads>(top, keys, counts);
+  if constexpr (kSplit) {
+    if (threadIdx.x == 0) part[b] = {sums.m, sums.s, sums.t};
+    if constexpr (kTop) {
+      rank_keys<kThreads>(keys, n, out.top, [&](int rank, key64 key) { best[b * out.top + rank] = key; });
+      if (static_cast<int>(threadIdx.x) >= n && static_cast<int>(threadIdx.x) < out.top) best[b * out.top + threadIdx.x] = 0;
     }
+  } else {
+    const auto o = finish(sums, in.temperature);
+    write_log_probs<T, kThreads>(in, ids, out, r, o);
+    if constexpr (kTop) write_top<kThreads>(in, out, r, o, keys, n);
+  }
+}
+
+/** The sums of all parts of row r, the same in every lane of the calling wavefront; in the parts' order. */
+__device__ inline auto join_parts(const part_sums* part, int64_t r, int parts, float c) -> run
+{
+  const int lane = threadIdx.x % 64;
+  run sums       = nothing();
+  for (int p = lane; p < parts; p += 64)
+    sums = join(sums, as_run(part[r * parts + p]), c);
+#pragma unroll
+  for (int mask = 32; mask > 0; mask >>= 1)
+    sums = join(sums, shuffle_xor(sums, mask), c);
+  return sums;
+}
+
+constexpr int kMaxParts = 32;  // of a row
+
+template <typename T, bool kTop>
+__global__ __launch_bounds__(kThreads) void finish_log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
+                                                                    row_split split, const part_sums* part,
+                                                                    const key64* best, int64_t row0)
+{
+  __shared__ key64 keys[kTop ? kMaxParts * kMaxTop : 1];
+  __shared__ int found;
+  const int64_t r = row0 + blockIdx.x;
+  const auto o    = finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature);
+  write_log_probs<T, kThreads>(in, ids, out, r, o);
+  if constexpr (kTop) {
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    const int all = split.parts * out.top;
+    for (int i = threadIdx.x; i < all; i += kThreads) {
+      const key64 key = best[r * all + i];
+      if (key != 0) keys[atomicAdd(&found, 1)] = key;  // in any order: their ranks do not depend on it
+    }
+    __syncthreads();
+    write_top<kThreads>(in, out, r, o, keys, found);
   }
 }
 
@@ -372,7 +483,6 @@ __device__ inline auto read_teacher(score_rows const& in, listed_ids const& ids,
 {
   const int lane = threadIdx.x % 64;
   teacher_row t;
-  float top = -INFINITY, bad = 0.f;
 #pragma unroll
   for (int q = 0; q < kListed; ++q) {
     t.id[q] = -1;
@@ -380,18 +490,23 @@ __device__ inline auto read_teacher(score_rows const& in, listed_ids const& ids,
     const int j = lane + 64 * q;
     if (64 * q < ids.k && j < ids.k) {
       const int64_t id = id_at(ids, r, j);
+      const float x    = load_any(teacher.x, teacher.type, r * teacher.stride + j);
       if (id >= 0 && id < in.n) {
         t.id[q] = static_cast<int>(id);
-        t.z[q]  = load_any(teacher.x, teacher.type, r * teacher.stride + j) / in.temperature;
-        top     = fmaxf(top, t.z[q]);
-        if (isnan(t.z[q])) bad = t.z[q];
+        t.z[q]  = x / in.temperature;
       }
     }
+  }
+  float top = -INFINITY, bad = 0.f, w = 0.f;
+#pragma unroll
+  for (int q = 0; q < kListed; ++q) {
+    if (64 * q >= ids.k) continue;
+    top = fmaxf(top, t.z[q]);
+    if (isnan(t.z[q])) bad = t.z[q];
   }
   t.top  = wave_max(top);
   bad    = wave_sum(bad);
   t.some = t.top != -INFINITY || isnan(bad);
-  float w = 0.f;
 #pragma unroll
   for (int q = 0; q < kListed; ++q)
     if (64 * q < ids.k && t.id[q] >= 0 && t.z[q] != -INFINITY) w += expf(t.z[q] - t.top);
@@ -401,31 +516,77 @@ __device__ inline auto read_teacher(score_rows const& in, listed_ids const& ids,
 
 __device__ inline auto teacher_log_q(teacher_row const& t, int q) -> float { return t.z[q] - t.top - t.ln_w; }
 
+/** The scores of the listed ids of row r, 0 where none is listed: one wavefront's loads. */
 template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
-                                                           float* loss, float* lse, int64_t row0)
+__device__ inline void read_listed(const T* row, int k, teacher_row const& t, float (&x)[kListed])
 {
-  __shared__ run parts[kWaves];
-  const int64_t r = row0 + blockIdx.x;
-  const T* row    = static_cast<const T*>(in.x) + r * in.stride;
-  const float c   = kLog2e / in.temperature;
-  run sums        = nothing();
-  for_scores<T>(row, 0, in.n, [&](const auto& v, int) { add_scores<false>(sums, v, c); });
-  const auto o = finish(join_block(sums, c, parts), in.temperature);
-  if (threadIdx.x >= 64) return;
-  const auto t = read_teacher(in, ids, teacher, r);
-  float sum    = 0.f;
+#pragma unroll
+  for (int q = 0; q < kListed; ++q)
+    x[q] = 64 * q < k && t.id[q] >= 0 ? static_cast<float>(row[t.id[q]]) : 0.f;
+}
+
+/** The loss of a row from one wavefront's share of its list: the same in every lane. */
+__device__ inline auto loss_of(score_rows const& in, int k, teacher_row const& t, const float (&x)[kListed], row_sums const& o)
+  -> float
+{
+  float sum = 0.f;
 #pragma unroll
   for (int q = 0; q < kListed; ++q) {
-    if (64 * q >= ids.k || t.id[q] < 0 || t.z[q] == -INFINITY) continue;
+    if (64 * q >= k || t.id[q] < 0 || t.z[q] == -INFINITY) continue;
     const float lq = teacher_log_q(t, q), p = expf(lq);
-    if (p != 0.f) sum += p * (lq - log_prob(static_cast<float>(row[t.id[q]]), o, in.temperature));
+    if (p != 0.f) sum += p * (lq - log_prob(x[q], o, in.temperature));
   }
   sum = wave_sum(sum);
-  if (threadIdx.x == 0) {
-    loss[r] = t.some ? sum : 0.f;
+  return t.some ? sum : 0.f;
+}
+
+/** The last step of row r, for one wavefront. */
+template <typename T>
+__device__ inline void write_loss(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, float* loss,
+                                  float* lse, int64_t r, row_sums const& o)
+{
+  const auto t = read_teacher(in, ids, teacher, r);
+  float x[kListed];
+  read_listed(static_cast<const T*>(in.x) + r * in.stride, ids.k, t, x);
+  const float l = loss_of(in, ids.k, t, x, o);
+  if (threadIdx.x % 64 == 0) {
+    loss[r] = l;
     lse[r]  = o.lse;
   }
+}
+
+template <typename T, bool kSplit>
+__global__ __launch_bounds__(kThreads) void distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
+                                                           float* loss, float* lse, row_split split, part_sums* part,
+                                                           int64_t row0)
+{
+  __shared__ run parts[kWaves];
+  const int64_t b = row0 + blockIdx.x, r = kSplit ? b / split.parts : b;
+  const int c0  = kSplit ? static_cast<int>(b - r * split.parts) * split.width : 0;
+  const int c1  = kSplit ? min(c0 + split.width, in.n) : in.n;
+  const T* row  = static_cast<const T*>(in.x) + r * in.stride;
+  const float c = kLog2e / in.temperature;
+  run sums      = nothing();
+  for_scores<T, kThreads>(row, c0, c1, [&](const auto& v, int) { add_scores<false>(sums, v, c); });
+  sums = join_block<kThreads>(sums, c, parts);
+  if (threadIdx.x >= 64) return;
+  if constexpr (kSplit) {
+    if (threadIdx.x == 0) part[b] = {sums.m, sums.s, 0.f};
+  } else {
+    write_loss<T>(in, ids, teacher, loss, lse, r, finish(sums, in.temperature));
+  }
+}
+
+/** A wavefront a row. */
+template <typename T>
+__global__ __launch_bounds__(kThreads) void finish_distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
+                                                                  float* loss, float* lse, row_split split,
+                                                                  const part_sums* part, int64_t row0)
+{
+  const int64_t r = row0 + int64_t{blockIdx.x} * kWaves + threadIdx.x / 64;
+  if (r >= in.m) return;
+  write_loss<T>(in, ids, teacher, loss, lse, r,
+                finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature));
 }
 
 // ---- gradients
@@ -445,55 +606,76 @@ __device__ inline auto gradient(float x, gradient_row const& g) -> float
   return p * g.a;
 }
 
-/** Writes the gradient of columns [c0, c1), then that of the listed ids among them again with their shares w.  ids and w
- * are LDS; an id that is listed more than once gets the sum of its shares, in their order. */
-template <typename T, bool kEntropy>
-__device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, gradient_row const& g, const int* ids,
-                                      const float* w, int k)
+/** The listed ids of a row and their shares of its gradient, in LDS; an id that is listed more than once gets the sum of
+ * its shares, in their order. */
+struct listed_shares {
+  int id[kMaxListed];
+  float w[kMaxListed];
+};
+
+/** Writes the gradients of the listed ids in columns [c0, c1) again, with their shares, after everything else's. */
+template <typename T, bool kEntropy, int NT>
+__device__ inline void write_listed(const T* row, T* grad, int c0, int c1, gradient_row const& g, listed_shares const& l, int k)
 {
-  constexpr int N = kPer16<T>;
-  float v[N];
-  if (c1 - c0 < N) {
-    const int at = c0 + static_cast<int>(threadIdx.x);
-    if (at < c1) grad[at] = static_cast<T>(gradient<kEntropy>(static_cast<float>(row[at]), g));
-  } else {
-    const int last = c1 - N;
-    for (int at0 = c0 + static_cast<int>(threadIdx.x) * N; at0 < c1; at0 += kThreads * N) {
-      const int at = min(at0, last);  // the moved-back lane writes what its neighbor writes
-      unpack16<T>(load16(row + at), v);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        v[i] = gradient<kEntropy>(v[i], g);
-      store16(grad + at, pack16<T>(v));
-    }
-  }
   __syncthreads();
-  for (int j = threadIdx.x; j < k; j += kThreads) {
-    const int id = ids[j];
+  for (int j = threadIdx.x; j < k; j += NT) {
+    const int id = l.id[j];
     if (id < c0 || id >= c1) continue;
     bool first = true;
     for (int i = 0; i < j && first; ++i)
-      first = ids[i] != id;
+      first = l.id[i] != id;
     if (!first) continue;
     float sum = 0.f;
     for (int i = j; i < k; ++i)
-      if (ids[i] == id) sum += w[i];
+      if (l.id[i] == id) sum += l.w[i];
     grad[id] = static_cast<T>(gradient<kEntropy>(static_cast<float>(row[id]), g) + sum);
   }
 }
 
-/** A gradient of 0 in columns [c0, c1). */
-template <typename T>
-__device__ inline void write_zeros(T* grad, int c0, int c1)
+/** Writes the gradient of columns [c0, c1).  prepare() gives what a row needs, and false in `some` for a gradient of 0; it
+ * may hold barriers, and runs while the first scores are on their way. */
+template <typename T, bool kEntropy, typename P>
+__device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, listed_shares const& l, int k, P prepare)
 {
-  constexpr int N = kPer16<T>;
-  if (c1 - c0 < N) {
-    const int at = c0 + static_cast<int>(threadIdx.x);
-    if (at < c1) grad[at] = static_cast<T>(0.f);
-    return;
+  constexpr int N = kPer16<T>, kStep = kThreads * N;
+  const bool tiny = c1 - c0 < N;
+  const int last  = c1 - N;
+  uint4 next[kUnroll];
+  int at = c0 + static_cast<int>(threadIdx.x) * N;
+  if (!tiny) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      next[u] = load16(row + min(at + u * kStep, last));
   }
-  for (int at = c0 + static_cast<int>(threadIdx.x) * N; at < c1; at += kThreads * N)
-    store16(grad + min(at, c1 - N), uint4{0, 0, 0, 0});
+  bool some            = true;
+  const gradient_row g = prepare(some);
+  float v[N];
+  if (tiny) {
+    at = c0 + static_cast<int>(threadIdx.x);
+    if (at < c1) grad[at] = static_cast<T>(some ? gradient<kEntropy>(static_cast<float>(row[at]), g) : 0.f);
+  } else {
+    for (; at < c1; at += kUnroll * kStep) {
+      uint4 cur[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        cur[u] = next[u];
+      if (at + kUnroll * kStep < c1) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          next[u] = load16(row + min(at + (kUnroll + u) * kStep, last));
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (at + u * kStep >= c1) break;
+        unpack16<T>(cur[u], v);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          v[i] = some ? gradient<kEntropy>(v[i], g) : 0.f;
+        store16(grad + min(at + u * kStep, last), pack16<T>(v));  // a lane that was moved back writes what its neighbor does
+      }
+    }
+  }
+  if (some) write_listed<T, kEntropy, kThreads>(row, grad, c0, c1, g, l, k);
 }
 
 /**
@@ -509,8 +691,8 @@ __device__ inline auto gradient_base(const T* row, int n, float lse, float tempe
   g.l2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
   if (fabsf(lse) > kMaxLse && fabsf(lse) != INFINITY) {
     run sums = nothing();
-    for_scores<T>(row, 0, n, [&](const auto& v, int) { add_scores<false>(sums, v, g.c); });
-    sums  = join_block(sums, g.c, parts);
+    for_scores<T, kThreads>(row, 0, n, [&](const auto& v, int) { add_scores<false>(sums, v, g.c); });
+    sums  = join_block<kThreads>(sums, g.c, parts);
     g.ref = sums.ref;
     g.l2  = log2f(sums.s);
   }
@@ -521,67 +703,140 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void log_probs_backward_kernel(score_rows in, listed_ids ids, const float* grad_logp,
                                                                       const float* grad_entropy, const float* lse,
                                                                       const float* entropy, T* grad, int64_t gstride,
-                                                                      int64_t row0)
+                                                                      row_split split, int64_t row0)
 {
-  __shared__ int listed[kMaxListed];
-  __shared__ float w[kMaxListed];
+  __shared__ listed_shares listed;
   __shared__ float total;
   __shared__ run parts[kWaves];
-  const int64_t r = row0 + blockIdx.x;
-  if (threadIdx.x < 64) {
-    float sum = 0.f;
-    for (int j = threadIdx.x; j < ids.k; j += 64) {
-      const int64_t id = id_at(ids, r, j);
-      const bool in_row = id >= 0 && id < in.n;
-      const float gj    = in_row && grad_logp != nullptr ? grad_logp[r * ids.k + j] : 0.f;
-      listed[j]         = in_row ? static_cast<int>(id) : -1;
-      w[j]              = gj / in.temperature;
-      sum += gj;
+  const int64_t b = row0 + blockIdx.x, r = b / split.parts;
+  const int c0 = static_cast<int>(b - r * split.parts) * split.width, c1 = min(c0 + split.width, in.n);
+  const T* row = static_cast<const T*>(in.x) + r * in.stride;
+  write_gradient<T, true>(row, grad + r * gstride, c0, c1, listed, ids.k, [&](bool&) {
+    if (threadIdx.x < 64) {
+      float sum = 0.f;
+      for (int j = threadIdx.x; j < ids.k; j += 64) {
+        const int64_t id  = id_at(ids, r, j);
+        const bool in_row = id >= 0 && id < in.n;
+        const float gj    = in_row && grad_logp != nullptr ? grad_logp[r * ids.k + j] : 0.f;
+        listed.id[j]      = in_row ? static_cast<int>(id) : -1;
+        listed.w[j]       = gj / in.temperature;
+        sum += gj;
+      }
+      sum = wave_sum(sum);
+      if (threadIdx.x == 0) total = sum;
     }
-    sum = wave_sum(sum);
-    if (threadIdx.x == 0) total = sum;
+    __syncthreads();
+    const float h = grad_entropy != nullptr ? grad_entropy[r] : 0.f;
+    auto g        = gradient_base(row, in.n, lse[r], in.temperature, parts);
+    g.a           = -(total + (h != 0.f ? h * entropy[r] : 0.f)) / in.temperature;
+    g.b           = -h / in.temperature;
+    return g;
+  });
+}
+
+/** The shares -a q of a teacher's list, for one wavefront. */
+__device__ inline void write_shares(teacher_row const& t, int k, float a, listed_shares& l)
+{
+#pragma unroll
+  for (int q = 0; q < kListed; ++q) {
+    const int j = static_cast<int>(threadIdx.x % 64) + 64 * q;
+    if (64 * q >= k || j >= k) continue;
+    l.id[j] = t.id[q];
+    l.w[j]  = t.id[q] >= 0 && t.z[q] != -INFINITY ? -a * expf(teacher_log_q(t, q)) : 0.f;
   }
-  __syncthreads();
-  const float h = grad_entropy != nullptr ? grad_entropy[r] : 0.f;
-  const T* row  = static_cast<const T*>(in.x) + r * in.stride;
-  auto g        = gradient_base(row, in.n, lse[r], in.temperature, parts);
-  g.a           = -(total + (h != 0.f ? h * entropy[r] : 0.f)) / in.temperature;
-  g.b           = -h / in.temperature;
-  write_gradient<T, true>(row, grad + r * gstride, 0, in.n, g, listed, w, ids.k);
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                                     const float* grad_loss, const float* lse, T* grad,
-                                                                    int64_t gstride, int64_t row0)
+                                                                    int64_t gstride, row_split split, int64_t row0)
 {
-  __shared__ int listed[kMaxListed];
-  __shared__ float w[kMaxListed];
-  __shared__ int some;
+  __shared__ listed_shares listed;
+  __shared__ int any;
   __shared__ run parts[kWaves];
-  const int64_t r = row0 + blockIdx.x;
-  const float a   = grad_loss[r] / in.temperature;
-  if (threadIdx.x < 64) {
-    const auto t = read_teacher(in, ids, teacher, r);
-#pragma unroll
-    for (int q = 0; q < kListed; ++q) {
-      const int j = threadIdx.x + 64 * q;
-      if (64 * q >= ids.k || j >= ids.k) continue;
-      listed[j] = t.id[q];
-      w[j]      = t.id[q] >= 0 && t.z[q] != -INFINITY ? -a * expf(teacher_log_q(t, q)) : 0.f;
+  const int64_t b = row0 + blockIdx.x, r = b / split.parts;
+  const int c0 = static_cast<int>(b - r * split.parts) * split.width, c1 = min(c0 + split.width, in.n);
+  const T* row  = static_cast<const T*>(in.x) + r * in.stride;
+  const float a = grad_loss[r] / in.temperature;
+  write_gradient<T, false>(row, grad + r * gstride, c0, c1, listed, ids.k, [&](bool& some) {
+    if (threadIdx.x < 64) {
+      const auto t = read_teacher(in, ids, teacher, r);
+      write_shares(t, ids.k, a, listed);
+      if (threadIdx.x == 0) any = t.some;
     }
-    if (threadIdx.x == 0) some = t.some;
-  }
-  __syncthreads();
+    __syncthreads();
+    some   = any != 0;
+    auto g = gradient_base(row, in.n, lse[r], in.temperature, parts);
+    g.a    = a;
+    return g;
+  });
+}
+
+/**
+ * Both directions of a row whose scores a workgroup holds in registers, H pieces of 16 bytes a thread: it is read once and
+ * its gradient written once.  The first wavefront reads the teacher's list while the scores arrive.
+ */
+template <typename T, int NT, int H>
+__global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
+                                                          const float* grad_loss, float* loss, float* lse, T* grad,
+                                                          int64_t gstride, int64_t row0)
+{
+  constexpr int N = kPer16<T>, kStep = NT * N;
+  __shared__ listed_shares listed;
+  __shared__ int any;
+  __shared__ run parts[NT / 64];
+  const int64_t r = row0 + blockIdx.x;
+  const T* row    = static_cast<const T*>(in.x) + r * in.stride;
   grad += r * gstride;
-  if (!some) {  // nothing to learn from
-    write_zeros(grad, 0, in.n);
-    return;
+  const int last = in.n - N, mine = static_cast<int>(threadIdx.x) * N;
+  uint4 held[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+    if (h * kStep < in.n) held[h] = load16(row + min(h * kStep + mine, last));
+  const float a = grad_loss[r] / in.temperature, c = kLog2e / in.temperature;
+  teacher_row t;
+  float x[kListed];
+  if (threadIdx.x < 64) {
+    t = read_teacher(in, ids, teacher, r);
+    read_listed(row, ids.k, t, x);
+    write_shares(t, ids.k, a, listed);
+    if (threadIdx.x == 0) any = t.some;
   }
-  const T* row = static_cast<const T*>(in.x) + r * in.stride;
-  auto g       = gradient_base(row, in.n, lse[r], in.temperature, parts);
-  g.a          = a;
-  write_gradient<T, false>(row, grad, 0, in.n, g, listed, w, ids.k);
+  run sums = nothing();
+  float v[N];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    if (h * kStep >= in.n) break;
+    unpack16<T>(held[h], v);
+    if (h * kStep + kStep > in.n) {  // columns that another thread holds
+      const int at = h * kStep + mine, from = min(at, last);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (from + i < at) v[i] = -INFINITY;
+    }
+    add_scores<false>(sums, v, c);
+  }
+  sums = join_block<NT>(sums, c, parts);
+  if (threadIdx.x < 64) {
+    const auto o  = finish(sums, in.temperature);
+    const float l = loss_of(in, ids.k, t, x, o);
+    if (threadIdx.x == 0) {
+      loss[r] = l;
+      lse[r]  = o.lse;
+    }
+  }
+  const bool some = any != 0;
+  gradient_row g{sums.ref, c, sums.s > 0.f ? log2f(sums.s) : sums.s == 0.f ? INFINITY : sums.s, a, 0.f};
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    if (h * kStep + mine >= in.n) break;
+    unpack16<T>(held[h], v);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = some ? gradient<false>(v[i], g) : 0.f;
+    store16(grad + min(h * kStep + mine, last), pack16<T>(v));
+  }
+  if (some) write_listed<T, false, NT>(row, grad, 0, in.n, g, listed, ids.k);
 }
 
 /** Calls f with a value of the element type. */
@@ -596,28 +851,57 @@ void with_type(elem type, F f)
     f(bf16{});
 }
 
-/** Calls f(first row, rows) for parts of m rows whose grids of a workgroup a row have less than 2^32 work-items. */
+/** Calls f(first, count) for parts of `total` workgroups whose grids have less than 2^32 work-items. */
 template <typename F>
-void for_row_grids(int64_t m, F f)
+void for_grids(int64_t total, int threads, F f)
 {
-  constexpr int64_t kRows = (int64_t{1} << 32) / kThreads - 1;
-  for (int64_t r = 0; r < m; r += kRows)
-    f(r, static_cast<unsigned>(std::min(kRows, m - r)));
+  const int64_t most = (int64_t{1} << 32) / threads - 1;
+  for (int64_t first = 0; first < total; first += most)
+    f(first, static_cast<unsigned>(std::min(most, total - first)));
+}
+
+constexpr int kEnough   = 1024;  // workgroups of 256 threads that fill the GPU
+constexpr int kMinWidth = 4096;  // columns of a part
+
+/** Rows are split into parts of whole 16-byte pieces while they are fewer than the workgroups that fill the GPU. */
+auto split_of(int64_t m, int n) -> row_split
+{
+  const int64_t want = std::min<int64_t>({(kEnough + m - 1) / m, (n + kMinWidth - 1) / kMinWidth, kMaxParts});
+  if (want <= 1) return {1, n};
+  const int width = static_cast<int>((n + want - 1) / want + 63) / 64 * 64;
+  return {(n + width - 1) / width, width};
 }
 
 }  // namespace
 
-void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out const& out, hipStream_t s)
+auto log_probs_workspace(int64_t m, int n, int top) -> int64_t
 {
+  const auto split = split_of(m, n);
+  return split.parts == 1 ? 0 : m * split.parts * static_cast<int64_t>(sizeof(key64) * top + sizeof(part_sums));
+}
+
+auto distill_workspace(int64_t m, int n) -> int64_t { return log_probs_workspace(m, n, 0); }
+
+void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out const& out, void* workspace, hipStream_t s)
+{
+  const auto split = split_of(in.m, in.n);
+  auto* best       = static_cast<key64*>(workspace);
+  auto* part       = reinterpret_cast<part_sums*>(best + (split.parts > 1 ? in.m * split.parts * out.top : 0));
   with_type(in.type, [&](auto e) {
-    using T = decltype(e);
-    for_row_grids(in.m, [&](int64_t row0, unsigned rows) {
-      if (out.top > 0)
-        log_probs_kernel<T, true><<<rows, kThreads, 0, s>>>(in, ids, out, row0);
-      else
-        log_probs_kernel<T, false><<<rows, kThreads, 0, s>>>(in, ids, out, row0);
-      OCTEX_HIP(hipGetLastError());
-    });
+    using T          = decltype(e);
+    const auto launch = [&](auto kernel, int64_t total) {
+      for_grids(total, kThreads, [&](int64_t first, unsigned count) {
+        kernel<<<count, kThreads, 0, s>>>(in, ids, out, split, part, best, first);
+        OCTEX_HIP(hipGetLastError());
+      });
+    };
+    const bool top = out.top > 0;
+    if (split.parts == 1) {
+      launch(top ? log_probs_kernel<T, true, false> : log_probs_kernel<T, false, false>, in.m);
+      return;
+    }
+    launch(top ? log_probs_kernel<T, true, true> : log_probs_kernel<T, false, true>, in.m * split.parts);
+    launch(top ? finish_log_probs_kernel<T, true> : finish_log_probs_kernel<T, false>, in.m);
   });
 }
 
@@ -625,23 +909,32 @@ void launch_log_probs_backward(score_rows const& in, listed_ids const& ids, cons
                                const float* grad_entropy, const float* lse, const float* entropy, void* grad,
                                int64_t gstride, hipStream_t s)
 {
+  const auto split = split_of(in.m, in.n);
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
-    for_row_grids(in.m, [&](int64_t row0, unsigned rows) {
-      log_probs_backward_kernel<T><<<rows, kThreads, 0, s>>>(in, ids, grad_logp, grad_entropy, lse, entropy,
-                                                             static_cast<T*>(grad), gstride, row0);
+    for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
+      log_probs_backward_kernel<T><<<count, kThreads, 0, s>>>(in, ids, grad_logp, grad_entropy, lse, entropy,
+                                                              static_cast<T*>(grad), gstride, split, first);
       OCTEX_HIP(hipGetLastError());
     });
   });
 }
 
 void launch_distill(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, float* loss, float* lse,
-                    hipStream_t s)
+                    void* workspace, hipStream_t s)
 {
+  const auto split = split_of(in.m, in.n);
+  auto* part       = static_cast<part_sums*>(workspace);
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
-    for_row_grids(in.m, [&](int64_t row0, unsigned rows) {
-      distill_kernel<T><<<rows, kThreads, 0, s>>>(in, ids, teacher, loss, lse, row0);
+    for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
+      const auto kernel = split.parts == 1 ? distill_kernel<T, false> : distill_kernel<T, true>;
+      kernel<<<count, kThreads, 0, s>>>(in, ids, teacher, loss, lse, split, part, first);
+      OCTEX_HIP(hipGetLastError());
+    });
+    if (split.parts == 1) return;
+    for_grids((in.m + kWaves - 1) / kWaves, kThreads, [&](int64_t first, unsigned count) {
+      finish_distill_kernel<T><<<count, kThreads, 0, s>>>(in, ids, teacher, loss, lse, split, part, first * kWaves);
       OCTEX_HIP(hipGetLastError());
     });
   });
@@ -650,13 +943,52 @@ void launch_distill(score_rows const& in, listed_ids const& ids, teacher_logits 
 void launch_distill_backward(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher,
                              const float* grad_loss, const float* lse, void* grad, int64_t gstride, hipStream_t s)
 {
+  const auto split = split_of(in.m, in.n);
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
-    for_row_grids(in.m, [&](int64_t row0, unsigned rows) {
-      distill_backward_kernel<T><<<rows, kThreads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad),
-                                                           gstride, row0);
+    for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
+      distill_backward_kernel<T><<<count, kThreads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride,
+                                                            split, first);
       OCTEX_HIP(hipGetLastError());
     });
+  });
+}
+
+constexpr int kHeldThreads = 1024, kHeldPieces = 16;  // of the widest row that a workgroup holds
+
+auto distill_step_held(int n, elem type) -> bool
+{
+  const int per = 16 / elem_size(type);
+  return n >= per && n <= kHeldThreads * kHeldPieces * per;
+}
+
+void launch_distill_step(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, const float* grad_loss,
+                         float* loss, float* lse, void* grad, int64_t gstride, void* workspace, hipStream_t s)
+{
+  if (!distill_step_held(in.n, in.type)) {
+    launch_distill(in, ids, teacher, loss, lse, workspace, s);
+    launch_distill_backward(in, ids, teacher, grad_loss, lse, grad, gstride, s);
+    return;
+  }
+  with_type(in.type, [&](auto e) {
+    using T           = decltype(e);
+    const auto launch = [&](auto kernel, int threads) {
+      for_grids(in.m, threads, [&](int64_t first, unsigned count) {
+        kernel<<<count, threads, 0, s>>>(in, ids, teacher, grad_loss, loss, lse, static_cast<T*>(grad), gstride, first);
+        OCTEX_HIP(hipGetLastError());
+      });
+    };
+    const int pieces = (in.n + kPer16<T> - 1) / kPer16<T>;
+    if (pieces <= 1024)
+      launch(distill_step_kernel<T, 256, 4>, 256);
+    else if (pieces <= 4096 && in.m > 256)
+      launch(distill_step_kernel<T, 256, 16>, 256);
+    else if (pieces <= 4096)
+      launch(distill_step_kernel<T, 1024, 4>, 1024);
+    else if (pieces <= 8192)
+      launch(distill_step_kernel<T, 1024, 8>, 1024);
+    else
+      launch(distill_step_kernel<T, 1024, 16>, 1024);
   });
 }
 

@@ -53,7 +53,12 @@ struct teacher_logits {
   int64_t stride;
 };
 
-void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out const& out, hipStream_t s);
+/** The bytes of workspace (at a multiple of 256) that launch_log_probs and launch_distill need: rows that do not fill the
+ * GPU are split into parts, whose sums meet there. */
+auto log_probs_workspace(int64_t m, int n, int top) -> int64_t;
+auto distill_workspace(int64_t m, int n) -> int64_t;
+
+void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out const& out, void* workspace, hipStream_t s);
 
 /** grad [m, n] (in's type, rows gstride apart) of sum(grad_logp * logp) + sum(grad_entropy * entropy); either may be null. */
 void launch_log_probs_backward(score_rows const& in, listed_ids const& ids, const float* grad_logp,
@@ -61,9 +66,16 @@ void launch_log_probs_backward(score_rows const& in, listed_ids const& ids, cons
                                int64_t gstride, hipStream_t s);
 
 void launch_distill(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, float* loss, float* lse,
-                    hipStream_t s);
+                    void* workspace, hipStream_t s);
 
 void launch_distill_backward(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher,
                              const float* grad_loss, const float* lse, void* grad, int64_t gstride, hipStream_t s);
+
+/** Whether launch_distill_step holds a row in registers; else it needs launch_distill's workspace. */
+auto distill_step_held(int n, elem type) -> bool;
+
+/** Both directions; the logits are read once if a workgroup can hold a row. */
+void launch_distill_step(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, const float* grad_loss,
+                         float* loss, float* lse, void* grad, int64_t gstride, void* workspace, hipStream_t s);
 
 }  // namespace cuvs::neighbors::octex::detail
