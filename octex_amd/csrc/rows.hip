@@ -24,7 +24,6 @@ constexpr float kLn2   = 0.693147180559945309417f;
 constexpr float kFloor = -200.f;  // an exponent whose power of two is 0; keeps 0 * -inf out of the sums
 constexpr int kThreads = 256;
 constexpr int kWaves   = kThreads / 64;
-constexpr int kUnroll  = 4;     // 16-byte loads a thread keeps in flight
 constexpr int kList    = 256;   // a wavefront's candidate keys: four a lane
 constexpr int kFull    = 128;   // keys from which a list is compacted
 
@@ -181,32 +180,50 @@ __device__ inline auto floor_of(const key64 (&key)[4], int k, int most) -> key64
   return p;
 }
 
+/** A score and its column, as they come. */
+struct entry {
+  unsigned column;
+  float v;
+};
+
+__device__ inline auto lanes_below(key64 lanes) -> int
+{
+  return __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(lanes >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(lanes), 0));
+}
+
 struct top_list {
-  key64* list;  // [kList] in LDS, this wavefront's
+  entry* list;  // [kList] in LDS, this wavefront's
   int k;
   int n     = 0;
   float thr = -INFINITY;  // no later score at or below it is among the k best
 
-  /** Keeps the k best and at most `most` keys, at `to`. */
-  __device__ void compact(int most, key64* to)
+  /** The list's keys, 0 past its end. */
+  __device__ void read(key64 (&key)[4]) const
   {
     const int lane = threadIdx.x % 64;
-    key64 key[4];
     wave_fence();
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      key[j] = lane + 64 * j < n ? list[lane + 64 * j] : 0;
+    for (int j = 0; j < 4; ++j) {
+      const entry e = list[lane + 64 * j];
+      key[j]        = lane + 64 * j < n ? key_of(e.v, static_cast<int>(e.column)) : 0;
+    }
     wave_fence();
+  }
+
+  /** Keeps the k best and at most `most` entries. */
+  __device__ void compact(int most)
+  {
+    key64 key[4];
+    read(key);
     const key64 p = floor_of(key, k, most);
     n             = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const bool in  = key[j] != 0 && key[j] >= p;
       const key64 at = __ballot(in);
-      if (in) to[n + __popcll(at & ((key64{1} << lane) - 1))] = key[j];
+      if (in) list[n + lanes_below(at)] = {static_cast<unsigned>(column_of(key[j])), value_of(key[j])};
       n += __popcll(at);
     }
-    wave_fence();
     raise(static_cast<unsigned>(p >> 32));
   }
 
@@ -221,23 +238,29 @@ struct top_list {
   {
     const float before = thr;
     if (__ballot(cm > before) == 0) return;
-    const int lane = threadIdx.x % 64;
     if (before == -INFINITY) {
       // the first floor: k lanes have a score that reaches it
       const unsigned order[1] = {order_of(cm)};
       raise(floor_of(order, k, k + 8));
     }
+    unsigned left = 0;  // of this lane's scores
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < N; ++i)
+      left |= v[i] > before && v[i] >= thr ? 1u << i : 0u;
+    while (__ballot(left != 0) != 0) {  // every lane lists one
+      const int i = __ffs(static_cast<int>(left)) - 1;
+      float x     = v[0];
+#pragma unroll
+      for (int j = 1; j < N; ++j)
+        x = i == j ? v[j] : x;
       // equal scores of lower columns may come in this very call, so a floor it raised lets them in
-      const bool in        = v[i] > before && v[i] >= thr;
-      const key64 at_lanes = __ballot(in);
-      if (at_lanes == 0) continue;
-      if (in) list[n + __popcll(at_lanes & ((key64{1} << lane) - 1))] = key_of(v[i], at + i);
-      n += __popcll(at_lanes);
-      if (n > kList - 64) compact(k + 32, list);
+      const bool in     = left != 0 && x >= thr;
+      const key64 lanes = __ballot(in);
+      if (in) list[n + lanes_below(lanes)] = {static_cast<unsigned>(at + i), x};
+      n += __popcll(lanes);
+      left &= left - 1;
+      if (n > kFull) compact(k + 32);
     }
-    if (n > kFull) compact(k + 32, list);
   }
 };
 
@@ -248,38 +271,81 @@ __device__ inline void rank_keys(const key64* keys, int n, int k, F f)
   for (int i = threadIdx.x; i < n; i += NT) {
     const key64 mine = keys[i];
     int rank         = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j)
       rank += keys[j] > mine;
     if (rank < k) f(rank, mine);
   }
 }
 
-/** The lists' k best by rank: every wavefront's list to keys (LDS, [waves * 64]), dense.  Returns their number. */
+/** The k best of the wavefronts' keys (0: none) and few others to keys (LDS, [waves * 64]), dense.  Returns their number. */
 template <int NT>
-__device__ inline auto gather_lists(top_list& top, key64* keys, int* counts) -> int
+__device__ inline auto gather_keys(const key64 (&key)[4], int k, key64* keys, int* counts) -> int
 {
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  top.compact(64, top.list);
-  if (lane == 0) counts[wave] = top.n;
+  const int wave = threadIdx.x / 64;
+  const key64 p  = floor_of(key, k, 64);
+  key64 in[4];
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    in[j] = __ballot(key[j] != 0 && key[j] >= p);
+    mine += __popcll(in[j]);
+  }
+  if (threadIdx.x % 64 == 0) counts[wave] = mine;
   __syncthreads();
   int from = 0, n = 0;
   for (int w = 0; w < NT / 64; ++w) {
     from += w < wave ? counts[w] : 0;
     n += counts[w];
   }
-  if (lane < top.n) keys[from + lane] = top.list[lane];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (key[j] != 0 && key[j] >= p) keys[from + lanes_below(in[j])] = key[j];
+    from += __popcll(in[j]);
+  }
   __syncthreads();
   return n;
 }
 
 // ---- one pass over a row
 
-/** Calls f(v, at) for the scores of columns [c0, c1) that this thread takes, 16 bytes at a time in ascending order; a
- * score outside the range, or one that another thread takes, comes as -inf.  Every lane of a wavefront calls f alike. */
+constexpr int kRun    = 8;  // scores that a thread takes at a time: 16 bytes, of fp32 two times 16
+constexpr int kPieces = 4;  // of 16 bytes, that a thread has on their way
+
+template <typename T>
+struct run_bytes {
+  uint4 raw[kRun / kPer16<T>];
+};
+
+template <typename T>
+__device__ inline auto load_run(const T* p) -> run_bytes<T>
+{
+  run_bytes<T> r;
+#pragma unroll
+  for (int i = 0; i < kRun / kPer16<T>; ++i)
+    r.raw[i] = load16(p + i * kPer16<T>);
+  return r;
+}
+
+template <typename T>
+__device__ inline void unpack_run(run_bytes<T> const& r, float (&v)[kRun])
+{
+#pragma unroll
+  for (int i = 0; i < kRun / kPer16<T>; ++i) {
+    float e[kPer16<T>];
+    unpack16<T>(r.raw[i], e);
+#pragma unroll
+    for (int j = 0; j < kPer16<T>; ++j)
+      v[i * kPer16<T> + j] = e[j];
+  }
+}
+
+/** Calls f(v, at) for the scores of columns [c0, c1) that this thread takes, 8 at a time in ascending order; a score outside
+ * the range, or one that another thread takes, comes as -inf.  Every lane of a wavefront calls f alike. */
 template <typename T, int NT, typename F>
 __device__ inline void for_scores(const T* row, int c0, int c1, F f)
 {
-  constexpr int N = kPer16<T>;
+  constexpr int N = kRun, kAhead = kPieces * kPer16<T> / kRun;
   float v[N];
   if (c1 - c0 < N) {
     const int at = c0 + static_cast<int>(threadIdx.x);
@@ -291,27 +357,28 @@ __device__ inline void for_scores(const T* row, int c0, int c1, F f)
     return;
   }
   const int last = c1 - N;  // a load that would pass the range's end is moved back to it
-  const int wave = c0 + static_cast<int>(threadIdx.x / 64) * 64 * N, mine = static_cast<int>(threadIdx.x % 64) * N;
+  const int wave = c0 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 64 * N;
+  const int mine = static_cast<int>(threadIdx.x % 64) * N;
   constexpr int kStep = NT * N;
-  uint4 next[kUnroll];
+  run_bytes<T> next[kAhead];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    next[u] = load16(row + min(wave + u * kStep + mine, last));
-  for (int w = wave; w < c1; w += kUnroll * kStep) {
-    uint4 cur[kUnroll];
+  for (int u = 0; u < kAhead; ++u)
+    next[u] = load_run(row + min(wave + u * kStep + mine, last));
+  for (int w = wave; w < c1; w += kAhead * kStep) {
+    run_bytes<T> cur[kAhead];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kAhead; ++u)
       cur[u] = next[u];
-    if (w + kUnroll * kStep < c1) {
+    if (w + kAhead * kStep < c1) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        next[u] = load16(row + min(w + (kUnroll + u) * kStep + mine, last));
+      for (int u = 0; u < kAhead; ++u)
+        next[u] = load_run(row + min(w + (kAhead + u) * kStep + mine, last));
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < kAhead; ++u) {
       const int w0 = w + u * kStep;
       if (w0 >= c1) break;
-      unpack16<T>(cur[u], v);
+      unpack_run<T>(cur[u], v);
       int at = w0 + mine;
       if (w0 + 64 * N > c1) {
         const int from = min(at, last);
@@ -383,7 +450,7 @@ __global__ __launch_bounds__(kThreads) void log_probs_kernel(score_rows in, list
                                                              row_split split, part_sums* part, key64* best, int64_t row0)
 {
   __shared__ run parts[kWaves];
-  __shared__ key64 lists[kTop ? kWaves * kList : 1];
+  __shared__ entry lists[kTop ? kWaves * kList : 1];
   __shared__ key64 keys[kTop ? kWaves * 64 : 1];
   __shared__ int counts[kWaves];
   const int64_t b = row0 + blockIdx.x, r = kSplit ? b / split.parts : b;
@@ -399,7 +466,11 @@ __global__ __launch_bounds__(kThreads) void log_probs_kernel(score_rows in, list
   });
   sums  = join_block<kThreads>(sums, c, parts);
   int n = 0;
-  if constexpr (kTop) n = gather_lists<kThreads>(top, keys, counts);
+  if constexpr (kTop) {
+    key64 key[4];
+    top.read(key);
+    n = gather_keys<kThreads>(key, out.top, keys, counts);
+  }
   if constexpr (kSplit) {
     if (threadIdx.x == 0) part[b] = {sums.m, sums.s, sums.t};
     if constexpr (kTop) {
@@ -426,40 +497,43 @@ __device__ inline auto join_parts(const part_sums* part, int64_t r, int parts, f
   return sums;
 }
 
-constexpr int kMaxParts = 32;  // of a row
-
 template <typename T, bool kTop>
 __global__ __launch_bounds__(kThreads) void finish_log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
                                                                     row_split split, const part_sums* part,
                                                                     const key64* best, int64_t row0)
 {
-  __shared__ key64 keys[kTop ? kMaxParts * kMaxTop : 1];
-  __shared__ int found;
+  __shared__ key64 keys[kTop ? kWaves * 64 : 1];
+  __shared__ int counts[kWaves];
   const int64_t r = row0 + blockIdx.x;
-  const auto o    = finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature);
-  write_log_probs<T, kThreads>(in, ids, out, r, o);
+  key64 key[4];
   if constexpr (kTop) {
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
-    const int all = split.parts * out.top;
-    for (int i = threadIdx.x; i < all; i += kThreads) {
-      const key64 key = best[r * all + i];
-      if (key != 0) keys[atomicAdd(&found, 1)] = key;  // in any order: their ranks do not depend on it
+    const int all = split.parts * out.top;  // at most 4 * kThreads
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = static_cast<int>(threadIdx.x) + kThreads * j;
+      key[j]      = i < all ? best[r * all + i] : 0;
     }
-    __syncthreads();
-    write_top<kThreads>(in, out, r, o, keys, found);
   }
+  const auto o = finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature);
+  write_log_probs<T, kThreads>(in, ids, out, r, o);
+  if constexpr (kTop) write_top<kThreads>(in, out, r, o, keys, gather_keys<kThreads>(key, out.top, keys, counts));
 }
 
-// ---- the teacher's distribution: the first wavefront's work, kListed entries a lane
+// ---- the teacher's distribution: one wavefront's work, in LDS, a lane taking every 64th entry
 
-constexpr int kListed = kMaxListed / 64;
+/** A row's list: ids (-1: not listed), teacher / T (-inf where not listed), the student's scores, and shares of its
+ * gradient. */
+struct listed_row {
+  int id[kMaxListed];
+  float z[kMaxListed];
+  float x[kMaxListed];
+  float w[kMaxListed];
+};
 
-struct teacher_row {
-  int id[kListed];        // -1: not listed
-  float z[kListed];       // teacher / T, -inf where not listed
-  float top, ln_w;        // the largest z; ln sum exp(z - top)
-  bool some;              // whether an entry has a probability
+/** What a teacher's entries need: ln q = z - top - ln_w. */
+struct teacher_sums {
+  float top, ln_w;
+  bool some;  // whether an entry has a probability
 };
 
 __device__ inline auto wave_max(float v) -> float
@@ -478,79 +552,62 @@ __device__ inline auto wave_sum(float v) -> float
   return v;
 }
 
-__device__ inline auto read_teacher(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, int64_t r)
-  -> teacher_row
+template <typename T>
+__device__ inline auto read_teacher(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, int64_t r,
+                                    listed_row& l) -> teacher_sums
 {
   const int lane = threadIdx.x % 64;
-  teacher_row t;
-#pragma unroll
-  for (int q = 0; q < kListed; ++q) {
-    t.id[q] = -1;
-    t.z[q]  = -INFINITY;
-    const int j = lane + 64 * q;
-    if (64 * q < ids.k && j < ids.k) {
-      const int64_t id = id_at(ids, r, j);
-      const float x    = load_any(teacher.x, teacher.type, r * teacher.stride + j);
-      if (id >= 0 && id < in.n) {
-        t.id[q] = static_cast<int>(id);
-        t.z[q]  = x / in.temperature;
-      }
-    }
-  }
+  const T* row   = static_cast<const T*>(in.x) + r * in.stride;
   float top = -INFINITY, bad = 0.f, w = 0.f;
-#pragma unroll
-  for (int q = 0; q < kListed; ++q) {
-    if (64 * q >= ids.k) continue;
-    top = fmaxf(top, t.z[q]);
-    if (isnan(t.z[q])) bad = t.z[q];
+  for (int j = lane; j < ids.k; j += 64) {
+    const int64_t id   = id_at(ids, r, j);
+    const float z      = load_any(teacher.x, teacher.type, r * teacher.stride + j) / in.temperature;
+    const bool listed  = id >= 0 && id < in.n;
+    l.id[j]            = listed ? static_cast<int>(id) : -1;
+    l.z[j]             = listed ? z : -INFINITY;
+    l.x[j]             = listed ? static_cast<float>(row[id]) : 0.f;
+    top                = listed ? fmaxf(top, z) : top;
+    if (listed && isnan(z)) bad = z;
   }
+  teacher_sums t;
   t.top  = wave_max(top);
-  bad    = wave_sum(bad);
-  t.some = t.top != -INFINITY || isnan(bad);
-#pragma unroll
-  for (int q = 0; q < kListed; ++q)
-    if (64 * q < ids.k && t.id[q] >= 0 && t.z[q] != -INFINITY) w += expf(t.z[q] - t.top);
+  t.some = t.top != -INFINITY || __ballot(isnan(bad)) != 0;
+  for (int j = lane; j < ids.k; j += 64)
+    if (l.z[j] != -INFINITY) w += expf(l.z[j] - t.top);
   t.ln_w = logf(wave_sum(w));
   return t;
 }
 
-__device__ inline auto teacher_log_q(teacher_row const& t, int q) -> float { return t.z[q] - t.top - t.ln_w; }
-
-/** The scores of the listed ids of row r, 0 where none is listed: one wavefront's loads. */
-template <typename T>
-__device__ inline void read_listed(const T* row, int k, teacher_row const& t, float (&x)[kListed])
-{
-#pragma unroll
-  for (int q = 0; q < kListed; ++q)
-    x[q] = 64 * q < k && t.id[q] >= 0 ? static_cast<float>(row[t.id[q]]) : 0.f;
-}
-
-/** The loss of a row from one wavefront's share of its list: the same in every lane. */
-__device__ inline auto loss_of(score_rows const& in, int k, teacher_row const& t, const float (&x)[kListed], row_sums const& o)
+/** The loss of a row whose sums are o: the same in every lane of the wavefront that read its list. */
+__device__ inline auto loss_of(score_rows const& in, int k, teacher_sums const& t, listed_row const& l, row_sums const& o)
   -> float
 {
   float sum = 0.f;
-#pragma unroll
-  for (int q = 0; q < kListed; ++q) {
-    if (64 * q >= k || t.id[q] < 0 || t.z[q] == -INFINITY) continue;
-    const float lq = teacher_log_q(t, q), p = expf(lq);
-    if (p != 0.f) sum += p * (lq - log_prob(x[q], o, in.temperature));
+  for (int j = threadIdx.x % 64; j < k; j += 64) {
+    if (l.z[j] == -INFINITY) continue;
+    const float lq = l.z[j] - t.top - t.ln_w, p = expf(lq);
+    if (p != 0.f) sum += p * (lq - log_prob(l.x[j], o, in.temperature));
   }
   sum = wave_sum(sum);
   return t.some ? sum : 0.f;
 }
 
+/** The shares -a q of the list's entries, for the wavefront that read it. */
+__device__ inline void write_shares(teacher_sums const& t, int k, float a, listed_row& l)
+{
+  for (int j = threadIdx.x % 64; j < k; j += 64)
+    l.w[j] = l.z[j] != -INFINITY ? -a * expf(l.z[j] - t.top - t.ln_w) : 0.f;
+}
+
 /** The last step of row r, for one wavefront. */
 template <typename T>
 __device__ inline void write_loss(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, float* loss,
-                                  float* lse, int64_t r, row_sums const& o)
+                                  float* lse, int64_t r, listed_row& l, row_sums const& o)
 {
-  const auto t = read_teacher(in, ids, teacher, r);
-  float x[kListed];
-  read_listed(static_cast<const T*>(in.x) + r * in.stride, ids.k, t, x);
-  const float l = loss_of(in, ids.k, t, x, o);
+  const auto t      = read_teacher<T>(in, ids, teacher, r, l);
+  const float value = loss_of(in, ids.k, t, l, o);
   if (threadIdx.x % 64 == 0) {
-    loss[r] = l;
+    loss[r] = value;
     lse[r]  = o.lse;
   }
 }
@@ -561,6 +618,7 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(score_rows in, listed
                                                            int64_t row0)
 {
   __shared__ run parts[kWaves];
+  __shared__ listed_row listed;
   const int64_t b = row0 + blockIdx.x, r = kSplit ? b / split.parts : b;
   const int c0  = kSplit ? static_cast<int>(b - r * split.parts) * split.width : 0;
   const int c1  = kSplit ? min(c0 + split.width, in.n) : in.n;
@@ -573,19 +631,18 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(score_rows in, listed
   if constexpr (kSplit) {
     if (threadIdx.x == 0) part[b] = {sums.m, sums.s, 0.f};
   } else {
-    write_loss<T>(in, ids, teacher, loss, lse, r, finish(sums, in.temperature));
+    write_loss<T>(in, ids, teacher, loss, lse, r, listed, finish(sums, in.temperature));
   }
 }
 
-/** A wavefront a row. */
 template <typename T>
-__global__ __launch_bounds__(kThreads) void finish_distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
-                                                                  float* loss, float* lse, row_split split,
-                                                                  const part_sums* part, int64_t row0)
+__global__ __launch_bounds__(64) void finish_distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
+                                                            float* loss, float* lse, row_split split,
+                                                            const part_sums* part, int64_t row0)
 {
-  const int64_t r = row0 + int64_t{blockIdx.x} * kWaves + threadIdx.x / 64;
-  if (r >= in.m) return;
-  write_loss<T>(in, ids, teacher, loss, lse, r,
+  __shared__ listed_row listed;
+  const int64_t r = row0 + blockIdx.x;
+  write_loss<T>(in, ids, teacher, loss, lse, r, listed,
                 finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature));
 }
 
@@ -606,45 +663,40 @@ __device__ inline auto gradient(float x, gradient_row const& g) -> float
   return p * g.a;
 }
 
-/** The listed ids of a row and their shares of its gradient, in LDS; an id that is listed more than once gets the sum of
- * its shares, in their order. */
-struct listed_shares {
-  int id[kMaxListed];
-  float w[kMaxListed];
-};
-
-/** Writes the gradients of the listed ids in columns [c0, c1) again, with their shares, after everything else's. */
+/** Writes the gradients of the listed ids in columns [c0, c1) again, with their shares, after everything else's; an id that
+ * is listed more than once gets the sum of its shares, in their order. */
 template <typename T, bool kEntropy, int NT>
-__device__ inline void write_listed(const T* row, T* grad, int c0, int c1, gradient_row const& g, listed_shares const& l, int k)
+__device__ inline void write_listed(T* grad, int c0, int c1, gradient_row const& g, listed_row const& l, int k)
 {
   __syncthreads();
   for (int j = threadIdx.x; j < k; j += NT) {
     const int id = l.id[j];
     if (id < c0 || id >= c1) continue;
     bool first = true;
-    for (int i = 0; i < j && first; ++i)
-      first = l.id[i] != id;
-    if (!first) continue;
-    float sum = 0.f;
-    for (int i = j; i < k; ++i)
-      if (l.id[i] == id) sum += l.w[i];
-    grad[id] = static_cast<T>(gradient<kEntropy>(static_cast<float>(row[id]), g) + sum);
+    float sum  = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < k; ++i) {
+      const bool same = l.id[i] == id;
+      first           = first && (!same || i >= j);
+      sum += same ? l.w[i] : 0.f;
+    }
+    if (first) grad[id] = static_cast<T>(gradient<kEntropy>(l.x[j], g) + sum);
   }
 }
 
 /** Writes the gradient of columns [c0, c1).  prepare() gives what a row needs, and false in `some` for a gradient of 0; it
  * may hold barriers, and runs while the first scores are on their way. */
 template <typename T, bool kEntropy, typename P>
-__device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, listed_shares const& l, int k, P prepare)
+__device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, listed_row const& l, int k, P prepare)
 {
   constexpr int N = kPer16<T>, kStep = kThreads * N;
   const bool tiny = c1 - c0 < N;
   const int last  = c1 - N;
-  uint4 next[kUnroll];
+  uint4 next[kPieces];
   int at = c0 + static_cast<int>(threadIdx.x) * N;
   if (!tiny) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kPieces; ++u)
       next[u] = load16(row + min(at + u * kStep, last));
   }
   bool some            = true;
@@ -654,18 +706,18 @@ __device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, lis
     at = c0 + static_cast<int>(threadIdx.x);
     if (at < c1) grad[at] = static_cast<T>(some ? gradient<kEntropy>(static_cast<float>(row[at]), g) : 0.f);
   } else {
-    for (; at < c1; at += kUnroll * kStep) {
-      uint4 cur[kUnroll];
+    for (; at < c1; at += kPieces * kStep) {
+      uint4 cur[kPieces];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
+      for (int u = 0; u < kPieces; ++u)
         cur[u] = next[u];
-      if (at + kUnroll * kStep < c1) {
+      if (at + kPieces * kStep < c1) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          next[u] = load16(row + min(at + (kUnroll + u) * kStep, last));
+        for (int u = 0; u < kPieces; ++u)
+          next[u] = load16(row + min(at + (kPieces + u) * kStep, last));
       }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kPieces; ++u) {
         if (at + u * kStep >= c1) break;
         unpack16<T>(cur[u], v);
 #pragma unroll
@@ -675,7 +727,7 @@ __device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, lis
       }
     }
   }
-  if (some) write_listed<T, kEntropy, kThreads>(row, grad, c0, c1, g, l, k);
+  if (some) write_listed<T, kEntropy, kThreads>(grad, c0, c1, g, l, k);
 }
 
 /**
@@ -705,7 +757,7 @@ __global__ __launch_bounds__(kThreads) void log_probs_backward_kernel(score_rows
                                                                       const float* entropy, T* grad, int64_t gstride,
                                                                       row_split split, int64_t row0)
 {
-  __shared__ listed_shares listed;
+  __shared__ listed_row listed;
   __shared__ float total;
   __shared__ run parts[kWaves];
   const int64_t b = row0 + blockIdx.x, r = b / split.parts;
@@ -719,6 +771,7 @@ __global__ __launch_bounds__(kThreads) void log_probs_backward_kernel(score_rows
         const bool in_row = id >= 0 && id < in.n;
         const float gj    = in_row && grad_logp != nullptr ? grad_logp[r * ids.k + j] : 0.f;
         listed.id[j]      = in_row ? static_cast<int>(id) : -1;
+        listed.x[j]       = in_row ? static_cast<float>(row[id]) : 0.f;
         listed.w[j]       = gj / in.temperature;
         sum += gj;
       }
@@ -734,24 +787,12 @@ __global__ __launch_bounds__(kThreads) void log_probs_backward_kernel(score_rows
   });
 }
 
-/** The shares -a q of a teacher's list, for one wavefront. */
-__device__ inline void write_shares(teacher_row const& t, int k, float a, listed_shares& l)
-{
-#pragma unroll
-  for (int q = 0; q < kListed; ++q) {
-    const int j = static_cast<int>(threadIdx.x % 64) + 64 * q;
-    if (64 * q >= k || j >= k) continue;
-    l.id[j] = t.id[q];
-    l.w[j]  = t.id[q] >= 0 && t.z[q] != -INFINITY ? -a * expf(teacher_log_q(t, q)) : 0.f;
-  }
-}
-
 template <typename T>
 __global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                                     const float* grad_loss, const float* lse, T* grad,
                                                                     int64_t gstride, row_split split, int64_t row0)
 {
-  __shared__ listed_shares listed;
+  __shared__ listed_row listed;
   __shared__ int any;
   __shared__ run parts[kWaves];
   const int64_t b = row0 + blockIdx.x, r = b / split.parts;
@@ -760,7 +801,7 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows i
   const float a = grad_loss[r] / in.temperature;
   write_gradient<T, false>(row, grad + r * gstride, c0, c1, listed, ids.k, [&](bool& some) {
     if (threadIdx.x < 64) {
-      const auto t = read_teacher(in, ids, teacher, r);
+      const auto t = read_teacher<T>(in, ids, teacher, r, listed);
       write_shares(t, ids.k, a, listed);
       if (threadIdx.x == 0) any = t.some;
     }
@@ -773,70 +814,78 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows i
 }
 
 /**
- * Both directions of a row whose scores a workgroup holds in registers, H pieces of 16 bytes a thread: it is read once and
- * its gradient written once.  The first wavefront reads the teacher's list while the scores arrive.
+ * Both directions of rows that a workgroup holds in registers, H pieces of 16 bytes a thread: each is read once and its
+ * gradient written once.  A workgroup takes every gridDim-th row; as a piece of a row's gradient is stored, the same piece
+ * of its next row is loaded in its place, so that reads and writes go on side by side.  The first wavefront reads the
+ * teacher's list while the scores arrive.
  */
 template <typename T, int NT, int H>
 __global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                           const float* grad_loss, float* loss, float* lse, T* grad,
-                                                          int64_t gstride, int64_t row0)
+                                                          int64_t gstride)
 {
   constexpr int N = kPer16<T>, kStep = NT * N;
-  __shared__ listed_shares listed;
+  __shared__ listed_row listed;
   __shared__ int any;
   __shared__ run parts[NT / 64];
-  const int64_t r = row0 + blockIdx.x;
-  const T* row    = static_cast<const T*>(in.x) + r * in.stride;
-  grad += r * gstride;
-  const int last = in.n - N, mine = static_cast<int>(threadIdx.x) * N;
+  const int last = in.n - N;
+  int mine       = static_cast<int>(threadIdx.x) * N;
+  const float c  = kLog2e / in.temperature;
   uint4 held[H];
+  const auto load = [&](int64_t r, int h) {
+    held[h] = load16(static_cast<const T*>(in.x) + r * in.stride + min(h * kStep + mine, last));
+  };
 #pragma unroll
   for (int h = 0; h < H; ++h)
-    if (h * kStep < in.n) held[h] = load16(row + min(h * kStep + mine, last));
-  const float a = grad_loss[r] / in.temperature, c = kLog2e / in.temperature;
-  teacher_row t;
-  float x[kListed];
-  if (threadIdx.x < 64) {
-    t = read_teacher(in, ids, teacher, r);
-    read_listed(row, ids.k, t, x);
-    write_shares(t, ids.k, a, listed);
-    if (threadIdx.x == 0) any = t.some;
-  }
-  run sums = nothing();
-  float v[N];
+    if (h * kStep < in.n) load(blockIdx.x, h);
+  for (int64_t r = blockIdx.x; r < in.m; r += gridDim.x) {
+    asm volatile("" : "+v"(mine));  // the pieces' places are made again for every row: kept, they would take H registers
+    const float a = grad_loss[r] / in.temperature;
+    teacher_sums t;
+    if (threadIdx.x < 64) {
+      t = read_teacher<T>(in, ids, teacher, r, listed);
+      write_shares(t, ids.k, a, listed);
+      if (threadIdx.x == 0) any = t.some;
+    }
+    run sums = nothing();
+    float v[N];
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    if (h * kStep >= in.n) break;
-    unpack16<T>(held[h], v);
-    if (h * kStep + kStep > in.n) {  // columns that another thread holds
-      const int at = h * kStep + mine, from = min(at, last);
+    for (int h = 0; h < H; ++h) {
+      if (h * kStep >= in.n) break;
+      unpack16<T>(held[h], v);
+      if (h * kStep + kStep > in.n) {  // columns that another thread holds
+        const int at = h * kStep + mine, from = min(at, last);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (from + i < at) v[i] = -INFINITY;
+      }
+      add_scores<false>(sums, v, c);
+    }
+    sums = join_block<NT>(sums, c, parts);
+    if (threadIdx.x < 64) {
+      const auto o      = finish(sums, in.temperature);
+      const float value = loss_of(in, ids.k, t, listed, o);
+      if (threadIdx.x == 0) {
+        loss[r] = value;
+        lse[r]  = o.lse;
+      }
+    }
+    const bool some = any != 0, more = r + gridDim.x < in.m;
+    const gradient_row g{sums.ref, c, sums.s > 0.f ? log2f(sums.s) : sums.s == 0.f ? INFINITY : sums.s, a, 0.f};
+    T* out = grad + r * gstride;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      if (h * kStep >= in.n) break;
+      unpack16<T>(held[h], v);
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (from + i < at) v[i] = -INFINITY;
+        v[i] = some ? gradient<false>(v[i], g) : 0.f;
+      if (h * kStep + mine < in.n) store16(out + min(h * kStep + mine, last), pack16<T>(v));
+      if (more) load(r + gridDim.x, h);
     }
-    add_scores<false>(sums, v, c);
+    if (some) write_listed<T, false, NT>(out, 0, in.n, g, listed, ids.k);
+    __syncthreads();  // the list and the sums have been read
   }
-  sums = join_block<NT>(sums, c, parts);
-  if (threadIdx.x < 64) {
-    const auto o  = finish(sums, in.temperature);
-    const float l = loss_of(in, ids.k, t, x, o);
-    if (threadIdx.x == 0) {
-      loss[r] = l;
-      lse[r]  = o.lse;
-    }
-  }
-  const bool some = any != 0;
-  gradient_row g{sums.ref, c, sums.s > 0.f ? log2f(sums.s) : sums.s == 0.f ? INFINITY : sums.s, a, 0.f};
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    if (h * kStep + mine >= in.n) break;
-    unpack16<T>(held[h], v);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = some ? gradient<false>(v[i], g) : 0.f;
-    store16(grad + min(h * kStep + mine, last), pack16<T>(v));
-  }
-  if (some) write_listed<T, false, NT>(row, grad, 0, in.n, g, listed, ids.k);
 }
 
 /** Calls f with a value of the element type. */
@@ -860,23 +909,32 @@ void for_grids(int64_t total, int threads, F f)
     f(first, static_cast<unsigned>(std::min(most, total - first)));
 }
 
-constexpr int kEnough   = 1024;  // workgroups of 256 threads that fill the GPU
-constexpr int kMinWidth = 4096;  // columns of a part
+constexpr int kEnough    = 1024;  // workgroups of 256 threads that fill the GPU
+constexpr int kMinWidth  = 4096;  // columns of a part
+constexpr int kMaxParts  = 32;    // of a row
+constexpr int kFewRows   = 128;   // rows whose forward pass is split: more fill the GPU well enough to spare the second kernel
 
 /** Rows are split into parts of whole 16-byte pieces while they are fewer than the workgroups that fill the GPU. */
-auto split_of(int64_t m, int n) -> row_split
+auto split_of(int64_t m, int n, int64_t most = kMaxParts) -> row_split
 {
-  const int64_t want = std::min<int64_t>({(kEnough + m - 1) / m, (n + kMinWidth - 1) / kMinWidth, kMaxParts});
+  const int64_t want = std::min<int64_t>({kEnough / std::min<int64_t>(m, kEnough), (n + kMinWidth - 1) / kMinWidth, most});
   if (want <= 1) return {1, n};
   const int width = static_cast<int>((n + want - 1) / want + 63) / 64 * 64;
   return {(n + width - 1) / width, width};
+}
+
+/** Of a forward pass, whose parts' best entries are at most four a thread of the kernel that joins them. */
+auto forward_split_of(int64_t m, int n, int top) -> row_split
+{
+  if (m > kFewRows) return {1, n};
+  return split_of(m, n, std::min(kMaxParts, 4 * kThreads / std::max(top, 1)));
 }
 
 }  // namespace
 
 auto log_probs_workspace(int64_t m, int n, int top) -> int64_t
 {
-  const auto split = split_of(m, n);
+  const auto split = forward_split_of(m, n, top);
   return split.parts == 1 ? 0 : m * split.parts * static_cast<int64_t>(sizeof(key64) * top + sizeof(part_sums));
 }
 
@@ -884,7 +942,7 @@ auto distill_workspace(int64_t m, int n) -> int64_t { return log_probs_workspace
 
 void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out const& out, void* workspace, hipStream_t s)
 {
-  const auto split = split_of(in.m, in.n);
+  const auto split = forward_split_of(in.m, in.n, out.top);
   auto* best       = static_cast<key64*>(workspace);
   auto* part       = reinterpret_cast<part_sums*>(best + (split.parts > 1 ? in.m * split.parts * out.top : 0));
   with_type(in.type, [&](auto e) {
@@ -923,7 +981,7 @@ void launch_log_probs_backward(score_rows const& in, listed_ids const& ids, cons
 void launch_distill(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, float* loss, float* lse,
                     void* workspace, hipStream_t s)
 {
-  const auto split = split_of(in.m, in.n);
+  const auto split = forward_split_of(in.m, in.n, 0);
   auto* part       = static_cast<part_sums*>(workspace);
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
@@ -933,8 +991,8 @@ void launch_distill(score_rows const& in, listed_ids const& ids, teacher_logits 
       OCTEX_HIP(hipGetLastError());
     });
     if (split.parts == 1) return;
-    for_grids((in.m + kWaves - 1) / kWaves, kThreads, [&](int64_t first, unsigned count) {
-      finish_distill_kernel<T><<<count, kThreads, 0, s>>>(in, ids, teacher, loss, lse, split, part, first * kWaves);
+    for_grids(in.m, 64, [&](int64_t first, unsigned count) {
+      finish_distill_kernel<T><<<count, 64, 0, s>>>(in, ids, teacher, loss, lse, split, part, first);
       OCTEX_HIP(hipGetLastError());
     });
   });
@@ -972,23 +1030,22 @@ void launch_distill_step(score_rows const& in, listed_ids const& ids, teacher_lo
   }
   with_type(in.type, [&](auto e) {
     using T           = decltype(e);
-    const auto launch = [&](auto kernel, int threads) {
-      for_grids(in.m, threads, [&](int64_t first, unsigned count) {
-        kernel<<<count, threads, 0, s>>>(in, ids, teacher, grad_loss, loss, lse, static_cast<T*>(grad), gstride, first);
-        OCTEX_HIP(hipGetLastError());
-      });
+    const auto launch = [&](auto kernel, int threads, int64_t slots) {
+      kernel<<<static_cast<unsigned>(std::min(in.m, slots)), threads, 0, s>>>(in, ids, teacher, grad_loss, loss, lse,
+                                                                              static_cast<T*>(grad), gstride);
+      OCTEX_HIP(hipGetLastError());
     };
     const int pieces = (in.n + kPer16<T> - 1) / kPer16<T>;
     if (pieces <= 1024)
-      launch(distill_step_kernel<T, 256, 4>, 256);
+      launch(distill_step_kernel<T, 256, 4>, 256, 2048);
     else if (pieces <= 4096 && in.m > 256)
-      launch(distill_step_kernel<T, 256, 16>, 256);
+      launch(distill_step_kernel<T, 256, 16>, 256, 1024);
     else if (pieces <= 4096)
-      launch(distill_step_kernel<T, 1024, 4>, 1024);
+      launch(distill_step_kernel<T, 1024, 4>, 1024, 256);
     else if (pieces <= 8192)
-      launch(distill_step_kernel<T, 1024, 8>, 1024);
+      launch(distill_step_kernel<T, 1024, 8>, 1024, 256);
     else
-      launch(distill_step_kernel<T, 1024, 16>, 1024);
+      launch(distill_step_kernel<T, 1024, 16>, 1024, 256);
   });
 }
 
