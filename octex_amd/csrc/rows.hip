@@ -14,6 +14,7 @@
 #include "rows.hpp"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace cuvs::neighbors::octex::detail {
 
@@ -195,7 +196,22 @@ struct top_list {
   entry* list;  // [kList] in LDS, this wavefront's
   int k;
   int n     = 0;
-  float thr = -INFINITY;  // no later score at or below it is among the k best
+  float low = -FLT_MAX;  // no later score below it is among the k best
+
+  /** The first floor: at least k of the workgroup's threads have a score cm that reaches it, and few more.  orders is LDS,
+   * one a thread. */
+  template <int NT>
+  __device__ void start(float cm, unsigned* orders)
+  {
+    orders[threadIdx.x] = order_of(cm);
+    __syncthreads();
+    unsigned order[NT / 64];
+#pragma unroll
+    for (int j = 0; j < NT / 64; ++j)
+      order[j] = orders[threadIdx.x % 64 + 64 * j];
+    raise(floor_of(order, k, k + 8));
+    __syncthreads();
+  }
 
   /** The list's keys, 0 past its end. */
   __device__ void read(key64 (&key)[4]) const
@@ -210,12 +226,12 @@ struct top_list {
     wave_fence();
   }
 
-  /** Keeps the k best and at most `most` entries. */
-  __device__ void compact(int most)
+  /** Keeps the k best entries and at most 32 others.  Returns the order of a score that k of them reach (0: none). */
+  __device__ auto compact() -> unsigned
   {
     key64 key[4];
     read(key);
-    const key64 p = floor_of(key, k, most);
+    const key64 p = floor_of(key, k, k + 32);
     n             = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -224,29 +240,25 @@ struct top_list {
       if (in) list[n + lanes_below(at)] = {static_cast<unsigned>(column_of(key[j])), value_of(key[j])};
       n += __popcll(at);
     }
-    raise(static_cast<unsigned>(p >> 32));
+    return static_cast<unsigned>(p >> 32);
   }
 
   __device__ void raise(unsigned order)
   {
-    if (order >= 0x00800000u) thr = value_of_order(order);  // below: not a number's order
+    // below: not a number's order; above: infinity's, in a row that has no alternatives anyway
+    if (order >= 0x00800000u && order < 0xff800000u) low = fmaxf(low, value_of_order(order));
   }
 
   /** Scores v of columns at + i, above every column of earlier calls; cm is the lane's largest. */
   template <int N>
   __device__ void add(const float (&v)[N], float cm, int at)
   {
-    const float before = thr;
-    if (__ballot(cm > before) == 0) return;
-    if (before == -INFINITY) {
-      // the first floor: k lanes have a score that reaches it
-      const unsigned order[1] = {order_of(cm)};
-      raise(floor_of(order, k, k + 8));
-    }
+    if (__ballot(cm >= low) == 0) return;
     unsigned left = 0;  // of this lane's scores
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      left |= v[i] > before && v[i] >= thr ? 1u << i : 0u;
+      left |= v[i] >= low ? 1u << i : 0u;
+    unsigned floor = 0;
     while (__ballot(left != 0) != 0) {  // every lane lists one
       const int i = __ffs(static_cast<int>(left)) - 1;
       float x     = v[0];
@@ -254,38 +266,29 @@ struct top_list {
       for (int j = 1; j < N; ++j)
         x = i == j ? v[j] : x;
       // equal scores of lower columns may come in this very call, so a floor it raised lets them in
-      const bool in     = left != 0 && x >= thr;
+      const bool in     = left != 0 && x >= low;
       const key64 lanes = __ballot(in);
       if (in) list[n + lanes_below(lanes)] = {static_cast<unsigned>(at + i), x};
       n += __popcll(lanes);
       left &= left - 1;
-      if (n > kFull) compact(k + 32);
+      if (n > kFull) {
+        floor = compact();
+        raise(floor);
+      }
     }
+    if (floor != 0) raise(floor + 1);  // k scores of lower columns reach it: an equal one comes too late
   }
 };
 
-/** Calls f(rank, key) for the k best of n distinct keys in LDS; a key's rank is the number of greater ones. */
-template <int NT, typename F>
-__device__ inline void rank_keys(const key64* keys, int n, int k, F f)
-{
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const key64 mine = keys[i];
-    int rank         = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j)
-      rank += keys[j] > mine;
-    if (rank < k) f(rank, mine);
-  }
-}
-
-/** The k best of the wavefronts' keys (0: none) and few others to keys (LDS, [waves * 64]), dense.  Returns their number. */
+/** The wavefronts' keys (0: none; `mine` of them here) that may be among the k best to keys (LDS, [waves * 64]), dense.
+ * Returns their number. */
 template <int NT>
-__device__ inline auto gather_keys(const key64 (&key)[4], int k, key64* keys, int* counts) -> int
+__device__ inline auto gather_keys(const key64 (&key)[4], int mine, int k, key64* keys, int* counts) -> int
 {
   const int wave = threadIdx.x / 64;
-  const key64 p  = floor_of(key, k, 64);
+  const key64 p  = mine <= 64 ? 1 : floor_of(key, k, 64);
   key64 in[4];
-  int mine = 0;
+  mine = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     in[j] = __ballot(key[j] != 0 && key[j] >= p);
@@ -305,6 +308,37 @@ __device__ inline auto gather_keys(const key64 (&key)[4], int k, key64* keys, in
   }
   __syncthreads();
   return n;
+}
+
+/** Calls f(rank, key) for the k best of n (at most 256) distinct keys in LDS, which it leaves in another order; a key's rank
+ * is the number of greater ones.  One wavefront's work. */
+template <typename F>
+__device__ inline void rank_keys(key64* keys, int n, int k, F f)
+{
+  const int lane = threadIdx.x % 64;
+  if (n > 64) {
+    key64 key[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      key[j] = lane + 64 * j < n ? keys[lane + 64 * j] : 0;
+    wave_fence();
+    const key64 p = floor_of(key, k, 64);
+    n             = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in  = key[j] != 0 && key[j] >= p;
+      const key64 at = __ballot(in);
+      if (in) keys[n + lanes_below(at)] = key[j];
+      n += __popcll(at);
+    }
+    wave_fence();
+  }
+  const key64 mine = lane < n ? keys[lane] : 0;
+  int rank         = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j)
+    rank += keys[j] > mine;
+  if (lane < n && rank < k) f(rank, mine);
 }
 
 // ---- one pass over a row
@@ -341,9 +375,10 @@ __device__ inline void unpack_run(run_bytes<T> const& r, float (&v)[kRun])
 }
 
 /** Calls f(v, at) for the scores of columns [c0, c1) that this thread takes, 8 at a time in ascending order; a score outside
- * the range, or one that another thread takes, comes as -inf.  Every lane of a wavefront calls f alike. */
-template <typename T, int NT, typename F>
-__device__ inline void for_scores(const T* row, int c0, int c1, F f)
+ * the range, or one that another thread takes, comes as -inf.  Every lane of a wavefront calls f alike.  start(largest) is
+ * called before, by all threads, with the largest of some of the thread's scores (-inf: none), none of them another's too. */
+template <typename T, int NT, typename G, typename F>
+__device__ inline void for_scores(const T* row, int c0, int c1, G start, F f)
 {
   constexpr int N = kRun, kAhead = kPieces * kPer16<T> / kRun;
   float v[N];
@@ -353,6 +388,7 @@ __device__ inline void for_scores(const T* row, int c0, int c1, F f)
     for (int i = 0; i < N; ++i)
       v[i] = -INFINITY;
     if (at < c1) v[0] = static_cast<float>(row[at]);
+    start(v[0]);
     f(v, at);
     return;
   }
@@ -364,6 +400,16 @@ __device__ inline void for_scores(const T* row, int c0, int c1, F f)
 #pragma unroll
   for (int u = 0; u < kAhead; ++u)
     next[u] = load_run(row + min(wave + u * kStep + mine, last));
+  float largest = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    if (wave + u * kStep + 64 * N > c1) break;  // this run's scores would not be its own
+    unpack_run<T>(next[u], v);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      largest = fmaxf(largest, v[i]);
+  }
+  start(largest);
   for (int w = wave; w < c1; w += kAhead * kStep) {
     run_bytes<T> cur[kAhead];
 #pragma unroll
@@ -426,33 +472,35 @@ __device__ inline void write_log_probs(score_rows const& in, listed_ids const& i
   }
 }
 
-/** The alternatives of row r: the best of n keys in LDS. */
-template <int NT>
-__device__ inline void write_top(score_rows const& in, log_probs_out const& out, int64_t r, row_sums const& o,
-                                 const key64* keys, int n)
+/** The alternatives of row r: the best of n keys in LDS.  The first wavefront's work. */
+__device__ inline void write_top(score_rows const& in, log_probs_out const& out, int64_t r, row_sums const& o, key64* keys,
+                                 int n)
 {
+  const int lane = static_cast<int>(threadIdx.x);
+  if (lane >= 64) return;
   const bool bad = isnan(o.lse);
   const int have = bad ? 0 : min(n, out.top);
-  rank_keys<NT>(keys, bad ? 0 : n, out.top, [&](int rank, key64 key) {
+  rank_keys(keys, bad ? 0 : n, out.top, [&](int rank, key64 key) {
     out.top_logp[r * out.top + rank] = log_prob(value_of(key), o, in.temperature);
     out.top_ids[r * out.top + rank]  = column_of(key);
   });
-  if (static_cast<int>(threadIdx.x) >= have && static_cast<int>(threadIdx.x) < out.top) {
-    out.top_logp[r * out.top + threadIdx.x] = bad ? o.lse : -INFINITY;
-    out.top_ids[r * out.top + threadIdx.x]  = -1;
+  if (lane >= have && lane < out.top) {
+    out.top_logp[r * out.top + lane] = bad ? o.lse : -INFINITY;
+    out.top_ids[r * out.top + lane]  = -1;
   }
 }
 
 /** A workgroup a row, or with kSplit a workgroup a part of a row, which leaves its sums and its best keys (0: none) to
  * finish_log_probs_kernel. */
-template <typename T, bool kTop, bool kSplit>
-__global__ __launch_bounds__(kThreads) void log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
+template <typename T, int NT, bool kTop, bool kSplit>
+__global__ __launch_bounds__(NT) void log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
                                                              row_split split, part_sums* part, key64* best, int64_t row0)
 {
-  __shared__ run parts[kWaves];
-  __shared__ entry lists[kTop ? kWaves * kList : 1];
-  __shared__ key64 keys[kTop ? kWaves * 64 : 1];
-  __shared__ int counts[kWaves];
+  constexpr int kWavesHere = NT / 64;
+  __shared__ run parts[kWavesHere];
+  __shared__ entry lists[kTop ? kWavesHere * kList : 1];
+  __shared__ key64 keys[kTop ? kWavesHere * 64 : 1];
+  __shared__ int counts[kWavesHere];
   const int64_t b = row0 + blockIdx.x, r = kSplit ? b / split.parts : b;
   const int c0 = kSplit ? static_cast<int>(b - r * split.parts) * split.width : 0;
   const int c1 = kSplit ? min(c0 + split.width, in.n) : in.n;
@@ -460,27 +508,34 @@ __global__ __launch_bounds__(kThreads) void log_probs_kernel(score_rows in, list
   const float c = kLog2e / in.temperature;
   run sums      = nothing();
   top_list top{lists + (kTop ? threadIdx.x / 64 * kList : 0), out.top};
-  for_scores<T, kThreads>(row, c0, c1, [&](const auto& v, int at) {
-    const float cm = add_scores<true>(sums, v, c);
-    if constexpr (kTop) top.add(v, cm, at);
-  });
-  sums  = join_block<kThreads>(sums, c, parts);
+  for_scores<T, NT>(
+    row, c0, c1,
+    [&](float cm) {
+      if constexpr (kTop) top.start<NT>(cm, reinterpret_cast<unsigned*>(keys));
+    },
+    [&](const auto& v, int at) {
+      const float cm = add_scores<true>(sums, v, c);
+      if constexpr (kTop) top.add(v, cm, at);
+    });
+  sums  = join_block<NT>(sums, c, parts);
   int n = 0;
   if constexpr (kTop) {
     key64 key[4];
     top.read(key);
-    n = gather_keys<kThreads>(key, out.top, keys, counts);
+    n = gather_keys<NT>(key, top.n, out.top, keys, counts);
   }
   if constexpr (kSplit) {
     if (threadIdx.x == 0) part[b] = {sums.m, sums.s, sums.t};
     if constexpr (kTop) {
-      rank_keys<kThreads>(keys, n, out.top, [&](int rank, key64 key) { best[b * out.top + rank] = key; });
-      if (static_cast<int>(threadIdx.x) >= n && static_cast<int>(threadIdx.x) < out.top) best[b * out.top + threadIdx.x] = 0;
+      if (threadIdx.x < 64) {
+        rank_keys(keys, n, out.top, [&](int rank, key64 key) { best[b * out.top + rank] = key; });
+        if (static_cast<int>(threadIdx.x) >= n && static_cast<int>(threadIdx.x) < out.top) best[b * out.top + threadIdx.x] = 0;
+      }
     }
   } else {
     const auto o = finish(sums, in.temperature);
-    write_log_probs<T, kThreads>(in, ids, out, r, o);
-    if constexpr (kTop) write_top<kThreads>(in, out, r, o, keys, n);
+    write_log_probs<T, NT>(in, ids, out, r, o);
+    if constexpr (kTop) write_top(in, out, r, o, keys, n);
   }
 }
 
@@ -516,7 +571,7 @@ __global__ __launch_bounds__(kThreads) void finish_log_probs_kernel(score_rows i
   }
   const auto o = finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature);
   write_log_probs<T, kThreads>(in, ids, out, r, o);
-  if constexpr (kTop) write_top<kThreads>(in, out, r, o, keys, gather_keys<kThreads>(key, out.top, keys, counts));
+  if constexpr (kTop) write_top(in, out, r, o, keys, gather_keys<kThreads>(key, 256, out.top, keys, counts));
 }
 
 // ---- the teacher's distribution: one wavefront's work, in LDS, a lane taking every 64th entry
@@ -524,11 +579,19 @@ __global__ __launch_bounds__(kThreads) void finish_log_probs_kernel(score_rows i
 /** A row's list: ids (-1: not listed), teacher / T (-inf where not listed), the student's scores, and shares of its
  * gradient. */
 struct listed_row {
-  int id[kMaxListed];
-  float z[kMaxListed];
-  float x[kMaxListed];
-  float w[kMaxListed];
+  int* id;
+  float *z, *x, *w;
 };
+
+extern __shared__ __align__(16) char row_lds[];  // the kernel's `lists` of k entries
+
+__device__ inline auto listed_at(int k, int list) -> listed_row
+{
+  auto* p = reinterpret_cast<float*>(row_lds) + list * 4 * k;
+  return {reinterpret_cast<int*>(p), p + k, p + 2 * k, p + 3 * k};
+}
+
+constexpr auto listed_bytes(int k, int lists) -> size_t { return size_t{16} * lists * k; }
 
 /** What a teacher's entries need: ln q = z - top - ln_w. */
 struct teacher_sums {
@@ -554,7 +617,7 @@ __device__ inline auto wave_sum(float v) -> float
 
 template <typename T>
 __device__ inline auto read_teacher(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, int64_t r,
-                                    listed_row& l) -> teacher_sums
+                                    listed_row const& l) -> teacher_sums
 {
   const int lane = threadIdx.x % 64;
   const T* row   = static_cast<const T*>(in.x) + r * in.stride;
@@ -593,7 +656,7 @@ __device__ inline auto loss_of(score_rows const& in, int k, teacher_sums const& 
 }
 
 /** The shares -a q of the list's entries, for the wavefront that read it. */
-__device__ inline void write_shares(teacher_sums const& t, int k, float a, listed_row& l)
+__device__ inline void write_shares(teacher_sums const& t, int k, float a, listed_row const& l)
 {
   for (int j = threadIdx.x % 64; j < k; j += 64)
     l.w[j] = l.z[j] != -INFINITY ? -a * expf(l.z[j] - t.top - t.ln_w) : 0.f;
@@ -602,7 +665,7 @@ __device__ inline void write_shares(teacher_sums const& t, int k, float a, liste
 /** The last step of row r, for one wavefront. */
 template <typename T>
 __device__ inline void write_loss(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, float* loss,
-                                  float* lse, int64_t r, listed_row& l, row_sums const& o)
+                                  float* lse, int64_t r, listed_row const& l, row_sums const& o)
 {
   const auto t      = read_teacher<T>(in, ids, teacher, r, l);
   const float value = loss_of(in, ids.k, t, l, o);
@@ -612,21 +675,21 @@ __device__ inline void write_loss(score_rows const& in, listed_ids const& ids, t
   }
 }
 
-template <typename T, bool kSplit>
-__global__ __launch_bounds__(kThreads) void distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
+template <typename T, int NT, bool kSplit>
+__global__ __launch_bounds__(NT) void distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                            float* loss, float* lse, row_split split, part_sums* part,
                                                            int64_t row0)
 {
-  __shared__ run parts[kWaves];
-  __shared__ listed_row listed;
+  __shared__ run parts[NT / 64];
+  const auto listed = listed_at(ids.k, 0);
   const int64_t b = row0 + blockIdx.x, r = kSplit ? b / split.parts : b;
   const int c0  = kSplit ? static_cast<int>(b - r * split.parts) * split.width : 0;
   const int c1  = kSplit ? min(c0 + split.width, in.n) : in.n;
   const T* row  = static_cast<const T*>(in.x) + r * in.stride;
   const float c = kLog2e / in.temperature;
   run sums      = nothing();
-  for_scores<T, kThreads>(row, c0, c1, [&](const auto& v, int) { add_scores<false>(sums, v, c); });
-  sums = join_block<kThreads>(sums, c, parts);
+  for_scores<T, NT>(row, c0, c1, [](float) {}, [&](const auto& v, int) { add_scores<false>(sums, v, c); });
+  sums = join_block<NT>(sums, c, parts);
   if (threadIdx.x >= 64) return;
   if constexpr (kSplit) {
     if (threadIdx.x == 0) part[b] = {sums.m, sums.s, 0.f};
@@ -640,7 +703,7 @@ __global__ __launch_bounds__(64) void finish_distill_kernel(score_rows in, liste
                                                             float* loss, float* lse, row_split split,
                                                             const part_sums* part, int64_t row0)
 {
-  __shared__ listed_row listed;
+  const auto listed = listed_at(ids.k, 0);
   const int64_t r = row0 + blockIdx.x;
   write_loss<T>(in, ids, teacher, loss, lse, r, listed,
                 finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature));
@@ -663,12 +726,11 @@ __device__ inline auto gradient(float x, gradient_row const& g) -> float
   return p * g.a;
 }
 
-/** Writes the gradients of the listed ids in columns [c0, c1) again, with their shares, after everything else's; an id that
- * is listed more than once gets the sum of its shares, in their order. */
+/** Writes the gradients of the listed ids in columns [c0, c1) again, with their shares, after everything else's and a
+ * barrier; an id that is listed more than once gets the sum of its shares, in their order. */
 template <typename T, bool kEntropy, int NT>
 __device__ inline void write_listed(T* grad, int c0, int c1, gradient_row const& g, listed_row const& l, int k)
 {
-  __syncthreads();
   for (int j = threadIdx.x; j < k; j += NT) {
     const int id = l.id[j];
     if (id < c0 || id >= c1) continue;
@@ -727,6 +789,7 @@ __device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, lis
       }
     }
   }
+  __syncthreads();
   if (some) write_listed<T, kEntropy, kThreads>(grad, c0, c1, g, l, k);
 }
 
@@ -743,7 +806,7 @@ __device__ inline auto gradient_base(const T* row, int n, float lse, float tempe
   g.l2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
   if (fabsf(lse) > kMaxLse && fabsf(lse) != INFINITY) {
     run sums = nothing();
-    for_scores<T, kThreads>(row, 0, n, [&](const auto& v, int) { add_scores<false>(sums, v, g.c); });
+    for_scores<T, kThreads>(row, 0, n, [](float) {}, [&](const auto& v, int) { add_scores<false>(sums, v, g.c); });
     sums  = join_block<kThreads>(sums, g.c, parts);
     g.ref = sums.ref;
     g.l2  = log2f(sums.s);
@@ -757,7 +820,7 @@ __global__ __launch_bounds__(kThreads) void log_probs_backward_kernel(score_rows
                                                                       const float* entropy, T* grad, int64_t gstride,
                                                                       row_split split, int64_t row0)
 {
-  __shared__ listed_row listed;
+  const auto listed = listed_at(ids.k, 0);
   __shared__ float total;
   __shared__ run parts[kWaves];
   const int64_t b = row0 + blockIdx.x, r = b / split.parts;
@@ -792,7 +855,7 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows i
                                                                     const float* grad_loss, const float* lse, T* grad,
                                                                     int64_t gstride, row_split split, int64_t row0)
 {
-  __shared__ listed_row listed;
+  const auto listed = listed_at(ids.k, 0);
   __shared__ int any;
   __shared__ run parts[kWaves];
   const int64_t b = row0 + blockIdx.x, r = b / split.parts;
@@ -816,75 +879,87 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows i
 /**
  * Both directions of rows that a workgroup holds in registers, H pieces of 16 bytes a thread: each is read once and its
  * gradient written once.  A workgroup takes every gridDim-th row; as a piece of a row's gradient is stored, the same piece
- * of its next row is loaded in its place, so that reads and writes go on side by side.  The first wavefront reads the
- * teacher's list while the scores arrive.
+ * of its next row is loaded in its place, and pieces that have arrived enter that row's sums, so that reads, writes and
+ * arithmetic go on side by side.  The first wavefront reads the next row's list meanwhile.
  */
 template <typename T, int NT, int H>
 __global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                           const float* grad_loss, float* loss, float* lse, T* grad,
                                                           int64_t gstride)
 {
-  constexpr int N = kPer16<T>, kStep = NT * N;
-  __shared__ listed_row listed;
-  __shared__ int any;
+  constexpr int N = kPer16<T>, kStep = NT * N, kLag = H < 8 ? H : 4;  // pieces on their way
+  __shared__ int any[2];
   __shared__ run parts[NT / 64];
   const int last = in.n - N;
   int mine       = static_cast<int>(threadIdx.x) * N;
   const float c  = kLog2e / in.temperature;
   uint4 held[H];
+  run sums;
+  float v[N];
   const auto load = [&](int64_t r, int h) {
     held[h] = load16(static_cast<const T*>(in.x) + r * in.stride + min(h * kStep + mine, last));
+  };
+  const auto add = [&](int h) {
+    unpack16<T>(held[h], v);
+    if (h * kStep + kStep > in.n) {  // columns that another thread holds
+      const int at = h * kStep + mine, from = min(at, last);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (from + i < at) v[i] = -INFINITY;
+    }
+    add_scores<false>(sums, v, c);
+  };
+  teacher_sums t{};
+  const auto read_list = [&](int64_t r, int list) {
+    if (threadIdx.x >= 64) return;
+    const auto l = listed_at(ids.k, list);
+    t            = read_teacher<T>(in, ids, teacher, r, l);
+    write_shares(t, ids.k, grad_loss[r] / in.temperature, l);
+    if (threadIdx.x == 0) any[list] = t.some;
   };
 #pragma unroll
   for (int h = 0; h < H; ++h)
     if (h * kStep < in.n) load(blockIdx.x, h);
-  for (int64_t r = blockIdx.x; r < in.m; r += gridDim.x) {
+  read_list(blockIdx.x, 0);
+  sums = nothing();
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+    if (h * kStep < in.n) add(h);
+  int list = 0;
+  for (int64_t r = blockIdx.x; r < in.m; r += gridDim.x, list ^= 1) {
     asm volatile("" : "+v"(mine));  // the pieces' places are made again for every row: kept, they would take H registers
-    const float a = grad_loss[r] / in.temperature;
-    teacher_sums t;
+    const int64_t next = r + gridDim.x;
+    const bool more    = next < in.m;
+    const run all      = join_block<NT>(sums, c, parts);
+    const auto l       = listed_at(ids.k, list);
     if (threadIdx.x < 64) {
-      t = read_teacher<T>(in, ids, teacher, r, listed);
-      write_shares(t, ids.k, a, listed);
-      if (threadIdx.x == 0) any = t.some;
-    }
-    run sums = nothing();
-    float v[N];
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      if (h * kStep >= in.n) break;
-      unpack16<T>(held[h], v);
-      if (h * kStep + kStep > in.n) {  // columns that another thread holds
-        const int at = h * kStep + mine, from = min(at, last);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (from + i < at) v[i] = -INFINITY;
-      }
-      add_scores<false>(sums, v, c);
-    }
-    sums = join_block<NT>(sums, c, parts);
-    if (threadIdx.x < 64) {
-      const auto o      = finish(sums, in.temperature);
-      const float value = loss_of(in, ids.k, t, listed, o);
+      const auto o      = finish(all, in.temperature);
+      const float value = loss_of(in, ids.k, t, l, o);
       if (threadIdx.x == 0) {
         loss[r] = value;
         lse[r]  = o.lse;
       }
     }
-    const bool some = any != 0, more = r + gridDim.x < in.m;
-    const gradient_row g{sums.ref, c, sums.s > 0.f ? log2f(sums.s) : sums.s == 0.f ? INFINITY : sums.s, a, 0.f};
+    const bool some = any[list] != 0;
+    if (more) read_list(next, list ^ 1);
+    const gradient_row g{all.ref, c, all.s > 0.f ? log2f(all.s) : all.s == 0.f ? INFINITY : all.s,
+                         grad_loss[r] / in.temperature, 0.f};
     T* out = grad + r * gstride;
+    sums   = nothing();
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      if (h * kStep >= in.n) break;
-      unpack16<T>(held[h], v);
+    for (int h = 0; h < H + kLag; ++h) {
+      if (h < H && h * kStep < in.n) {
+        unpack16<T>(held[h], v);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        v[i] = some ? gradient<false>(v[i], g) : 0.f;
-      if (h * kStep + mine < in.n) store16(out + min(h * kStep + mine, last), pack16<T>(v));
-      if (more) load(r + gridDim.x, h);
+        for (int i = 0; i < N; ++i)
+          v[i] = some ? gradient<false>(v[i], g) : 0.f;
+        if (h * kStep + mine < in.n) store16(out + min(h * kStep + mine, last), pack16<T>(v));
+        if (more) load(next, h);
+      }
+      if (more && h >= kLag && (h - kLag) * kStep < in.n) add(h - kLag);
     }
-    if (some) write_listed<T, false, NT>(out, 0, in.n, g, listed, ids.k);
-    __syncthreads();  // the list and the sums have been read
+    __syncthreads();
+    if (some) write_listed<T, false, NT>(out, 0, in.n, g, l, ids.k);
   }
 }
 
@@ -930,6 +1005,9 @@ auto forward_split_of(int64_t m, int n, int top) -> row_split
   return split_of(m, n, std::min(kMaxParts, 4 * kThreads / std::max(top, 1)));
 }
 
+/** Rows of few columns take a wavefront each where there are enough of them. */
+auto by_wavefront(int64_t m, int n) -> bool { return m >= 2048 && n <= 4096; }
+
 }  // namespace
 
 auto log_probs_workspace(int64_t m, int n, int top) -> int64_t
@@ -947,19 +1025,22 @@ void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out
   auto* part       = reinterpret_cast<part_sums*>(best + (split.parts > 1 ? in.m * split.parts * out.top : 0));
   with_type(in.type, [&](auto e) {
     using T          = decltype(e);
-    const auto launch = [&](auto kernel, int64_t total) {
-      for_grids(total, kThreads, [&](int64_t first, unsigned count) {
-        kernel<<<count, kThreads, 0, s>>>(in, ids, out, split, part, best, first);
+    const auto launch = [&](auto kernel, int threads, int64_t total) {
+      for_grids(total, threads, [&](int64_t first, unsigned count) {
+        kernel<<<count, threads, 0, s>>>(in, ids, out, split, part, best, first);
         OCTEX_HIP(hipGetLastError());
       });
     };
     const bool top = out.top > 0;
-    if (split.parts == 1) {
-      launch(top ? log_probs_kernel<T, true, false> : log_probs_kernel<T, false, false>, in.m);
-      return;
+    if (split.parts > 1) {
+      launch(top ? log_probs_kernel<T, kThreads, true, true> : log_probs_kernel<T, kThreads, false, true>, kThreads,
+             in.m * split.parts);
+      launch(top ? finish_log_probs_kernel<T, true> : finish_log_probs_kernel<T, false>, kThreads, in.m);
+    } else if (by_wavefront(in.m, in.n)) {
+      launch(top ? log_probs_kernel<T, 64, true, false> : log_probs_kernel<T, 64, false, false>, 64, in.m);
+    } else {
+      launch(top ? log_probs_kernel<T, kThreads, true, false> : log_probs_kernel<T, kThreads, false, false>, kThreads, in.m);
     }
-    launch(top ? log_probs_kernel<T, true, true> : log_probs_kernel<T, false, true>, in.m * split.parts);
-    launch(top ? finish_log_probs_kernel<T, true> : finish_log_probs_kernel<T, false>, in.m);
   });
 }
 
@@ -971,7 +1052,7 @@ void launch_log_probs_backward(score_rows const& in, listed_ids const& ids, cons
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
     for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
-      log_probs_backward_kernel<T><<<count, kThreads, 0, s>>>(in, ids, grad_logp, grad_entropy, lse, entropy,
+      log_probs_backward_kernel<T><<<count, kThreads, listed_bytes(ids.k, 1), s>>>(in, ids, grad_logp, grad_entropy, lse, entropy,
                                                               static_cast<T*>(grad), gstride, split, first);
       OCTEX_HIP(hipGetLastError());
     });
@@ -985,16 +1066,21 @@ void launch_distill(score_rows const& in, listed_ids const& ids, teacher_logits 
   auto* part       = static_cast<part_sums*>(workspace);
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
-    for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
-      const auto kernel = split.parts == 1 ? distill_kernel<T, false> : distill_kernel<T, true>;
-      kernel<<<count, kThreads, 0, s>>>(in, ids, teacher, loss, lse, split, part, first);
-      OCTEX_HIP(hipGetLastError());
-    });
-    if (split.parts == 1) return;
-    for_grids(in.m, 64, [&](int64_t first, unsigned count) {
-      finish_distill_kernel<T><<<count, 64, 0, s>>>(in, ids, teacher, loss, lse, split, part, first);
-      OCTEX_HIP(hipGetLastError());
-    });
+    const size_t lds = listed_bytes(ids.k, 1);
+    const auto launch = [&](auto kernel, int threads, int64_t total, size_t bytes) {
+      for_grids(total, threads, [&](int64_t first, unsigned count) {
+        kernel<<<count, threads, bytes, s>>>(in, ids, teacher, loss, lse, split, part, first);
+        OCTEX_HIP(hipGetLastError());
+      });
+    };
+    if (split.parts > 1) {
+      launch(distill_kernel<T, kThreads, true>, kThreads, in.m * split.parts, 0);
+      launch(finish_distill_kernel<T>, 64, in.m, lds);
+    } else if (by_wavefront(in.m, in.n)) {
+      launch(distill_kernel<T, 64, false>, 64, in.m, lds);
+    } else {
+      launch(distill_kernel<T, kThreads, false>, kThreads, in.m, lds);
+    }
   });
 }
 
@@ -1005,7 +1091,7 @@ void launch_distill_backward(score_rows const& in, listed_ids const& ids, teache
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
     for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
-      distill_backward_kernel<T><<<count, kThreads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride,
+      distill_backward_kernel<T><<<count, kThreads, listed_bytes(ids.k, 1), s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride,
                                                             split, first);
       OCTEX_HIP(hipGetLastError());
     });
@@ -1031,12 +1117,16 @@ void launch_distill_step(score_rows const& in, listed_ids const& ids, teacher_lo
   with_type(in.type, [&](auto e) {
     using T           = decltype(e);
     const auto launch = [&](auto kernel, int threads, int64_t slots) {
-      kernel<<<static_cast<unsigned>(std::min(in.m, slots)), threads, 0, s>>>(in, ids, teacher, grad_loss, loss, lse,
-                                                                              static_cast<T*>(grad), gstride);
+      kernel<<<static_cast<unsigned>(std::min(in.m, slots)), threads, listed_bytes(ids.k, 2), s>>>(
+        in, ids, teacher, grad_loss, loss, lse, static_cast<T*>(grad), gstride);
       OCTEX_HIP(hipGetLastError());
     };
     const int pieces = (in.n + kPer16<T> - 1) / kPer16<T>;
-    if (pieces <= 1024)
+    if (pieces <= 256 && in.m >= 2048)
+      launch(distill_step_kernel<T, 64, 4>, 64, 8192);
+    else if (pieces <= 1024 && in.m >= 2048)
+      launch(distill_step_kernel<T, 64, 16>, 64, 4096);
+    else if (pieces <= 1024)
       launch(distill_step_kernel<T, 256, 4>, 256, 2048);
     else if (pieces <= 4096 && in.m > 256)
       launch(distill_step_kernel<T, 256, 16>, 256, 1024);
