@@ -278,7 +278,7 @@ extern "C" cuvsError_t octexDistillStep(const octexMatrix* logits, const octexMa
     const auto id = ids_of(ids, in.m);
     const auto t  = teacher_of(teacher, id, in.m);
     grad_of(grad, logits);
-    const int64_t need = in.m == 0 || distill_step_held(in.n, in.type) ? 0 : distill_workspace(in.m, in.n);
+    const int64_t need = in.m == 0 || distill_step_held(in.m, in.n, in.type) ? 0 : distill_workspace(in.m, in.n);
     if (asked_size(need, bytes, size)) return;
     if (in.m == 0) return;
     on_gpu gpu;

@@ -32,6 +32,14 @@ __device__ inline auto exp2_fast(float v) -> float { return __builtin_amdgcn_exp
 
 __device__ inline void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
+/** A barrier for what lies in LDS: the workgroup's loads and stores of other memory stay on their way. */
+__device__ inline void lds_barrier()
+{
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 /** The running sums of a part of a row; ref is m, or 0 while there is no finite score. */
 struct run {
   float m, ref, s, t;
@@ -91,7 +99,7 @@ __device__ inline auto join_block(run r, float c, run* parts) -> run
   for (int mask = 32; mask > 0; mask >>= 1)
     r = join(r, shuffle_xor(r, mask), c);
   if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = r;
-  __syncthreads();
+  lds_barrier();
   r = parts[0];
   for (int w = 1; w < NT / 64; ++w)
     r = join(r, parts[w], c);
@@ -204,13 +212,13 @@ struct top_list {
   __device__ void start(float cm, unsigned* orders)
   {
     orders[threadIdx.x] = order_of(cm);
-    __syncthreads();
+    lds_barrier();
     unsigned order[NT / 64];
 #pragma unroll
     for (int j = 0; j < NT / 64; ++j)
       order[j] = orders[threadIdx.x % 64 + 64 * j];
     raise(floor_of(order, k, k + 8));
-    __syncthreads();
+    lds_barrier();
   }
 
   /** The list's keys, 0 past its end. */
@@ -295,7 +303,7 @@ __device__ inline auto gather_keys(const key64 (&key)[4], int mine, int k, key64
     mine += __popcll(in[j]);
   }
   if (threadIdx.x % 64 == 0) counts[wave] = mine;
-  __syncthreads();
+  lds_barrier();
   int from = 0, n = 0;
   for (int w = 0; w < NT / 64; ++w) {
     from += w < wave ? counts[w] : 0;
@@ -306,7 +314,7 @@ __device__ inline auto gather_keys(const key64 (&key)[4], int mine, int k, key64
     if (key[j] != 0 && key[j] >= p) keys[from + lanes_below(in[j])] = key[j];
     from += __popcll(in[j]);
   }
-  __syncthreads();
+  lds_barrier();
   return n;
 }
 
@@ -574,37 +582,82 @@ __global__ __launch_bounds__(kThreads) void finish_log_probs_kernel(score_rows i
   if constexpr (kTop) write_top(in, out, r, o, keys, gather_keys<kThreads>(key, 256, out.top, keys, counts));
 }
 
-// ---- the teacher's distribution: one wavefront's work, in LDS, a lane taking every 64th entry
+// ---- the teacher's distribution: entry e of a thread is the row's entry threadIdx.x + e * NT
 
-/** A row's list: ids (-1: not listed), teacher / T (-inf where not listed), the student's scores, and shares of its
- * gradient. */
-struct listed_row {
-  int* id;
-  float *z, *x, *w;
+/** Entries a thread: all of a list but for a single wavefront, which takes lists of up to kShortList. */
+constexpr int kShortList = 128;
+template <int NT>
+constexpr int kEntries = (NT == 64 ? kShortList : kMaxListed) / NT;
+
+/** A thread's entries of a row's list: ids (-1: not listed), teacher / T (-inf where not listed) and the student's scores. */
+template <int E>
+struct listed_part {
+  int id[E];
+  float z[E], x[E];
 };
 
-extern __shared__ __align__(16) char row_lds[];  // the kernel's `lists` of k entries
-
-__device__ inline auto listed_at(int k, int list) -> listed_row
+template <int NT, int E>
+__device__ inline void read_list(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, int64_t r,
+                                 listed_part<E>& l)
 {
-  auto* p = reinterpret_cast<float*>(row_lds) + list * 4 * k;
-  return {reinterpret_cast<int*>(p), p + k, p + 2 * k, p + 3 * k};
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int j = static_cast<int>(threadIdx.x) + e * NT;
+    l.id[e]     = -1;
+    l.z[e]      = -INFINITY;
+    if (j < ids.k) {
+      const int64_t id = id_at(ids, r, j);
+      const float z    = load_any(teacher.x, teacher.type, r * teacher.stride + j);
+      const bool in_row = id >= 0 && id < in.n;
+      l.id[e]          = in_row ? static_cast<int>(id) : -1;
+      l.z[e]           = in_row ? z / in.temperature : -INFINITY;
+    }
+  }
 }
 
-constexpr auto listed_bytes(int k, int lists) -> size_t { return size_t{16} * lists * k; }
+template <typename T, int E>
+__device__ inline void read_listed(const T* row, listed_part<E>& l)
+{
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    l.x[e] = l.id[e] >= 0 ? static_cast<float>(row[l.id[e]]) : 0.f;
+}
 
-/** What a teacher's entries need: ln q = z - top - ln_w. */
+/** The sums of the thread's entries, in units of 1: a NaN entry makes them NaN. */
+template <int E>
+__device__ inline auto teacher_run(listed_part<E> const& l) -> run
+{
+  run t = nothing();
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    t.m = fmaxf(t.m, l.z[e]);
+  t.ref = t.m == -INFINITY ? 0.f : t.m;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (l.z[e] != -INFINITY) t.s += expf(l.z[e] - t.ref);
+  return t;
+}
+
+/** ln q of an entry of a list whose sums are t. */
 struct teacher_sums {
   float top, ln_w;
   bool some;  // whether an entry has a probability
 };
 
-__device__ inline auto wave_max(float v) -> float
+__device__ inline auto teacher_of(run const& t) -> teacher_sums { return {t.m, logf(t.s), t.s != 0.f}; }
+
+/** The thread's share of a row's loss. */
+template <int E>
+__device__ inline auto loss_of(score_rows const& in, listed_part<E> const& l, teacher_sums const& t, row_sums const& o) -> float
 {
+  float sum = 0.f;
 #pragma unroll
-  for (int mask = 32; mask > 0; mask >>= 1)
-    v = fmaxf(v, __shfl_xor(v, mask));
-  return v;
+  for (int e = 0; e < E; ++e) {
+    if (l.z[e] == -INFINITY) continue;
+    const float lq = l.z[e] - t.top - t.ln_w, p = expf(lq);
+    if (p != 0.f) sum += p * (lq - log_prob(l.x[e], o, in.temperature));
+  }
+  return sum;
 }
 
 __device__ inline auto wave_sum(float v) -> float
@@ -615,86 +668,69 @@ __device__ inline auto wave_sum(float v) -> float
   return v;
 }
 
-template <typename T>
-__device__ inline auto read_teacher(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, int64_t r,
-                                    listed_row const& l) -> teacher_sums
+/** join_block of a row's sums and of its list's at one barrier; both is LDS, two a wavefront. */
+template <int NT>
+__device__ inline void join_both(run& sums, float c, run& t, run* both)
 {
-  const int lane = threadIdx.x % 64;
-  const T* row   = static_cast<const T*>(in.x) + r * in.stride;
-  float top = -INFINITY, bad = 0.f, w = 0.f;
-  for (int j = lane; j < ids.k; j += 64) {
-    const int64_t id   = id_at(ids, r, j);
-    const float z      = load_any(teacher.x, teacher.type, r * teacher.stride + j) / in.temperature;
-    const bool listed  = id >= 0 && id < in.n;
-    l.id[j]            = listed ? static_cast<int>(id) : -1;
-    l.z[j]             = listed ? z : -INFINITY;
-    l.x[j]             = listed ? static_cast<float>(row[id]) : 0.f;
-    top                = listed ? fmaxf(top, z) : top;
-    if (listed && isnan(z)) bad = z;
+#pragma unroll
+  for (int mask = 32; mask > 0; mask >>= 1)
+    sums = join(sums, shuffle_xor(sums, mask), c);
+  if (__ballot(t.s != 0.f) != 0) {
+#pragma unroll
+    for (int mask = 32; mask > 0; mask >>= 1)
+      t = join(t, shuffle_xor(t, mask), kLog2e);
   }
-  teacher_sums t;
-  t.top  = wave_max(top);
-  t.some = t.top != -INFINITY || __ballot(isnan(bad)) != 0;
-  for (int j = lane; j < ids.k; j += 64)
-    if (l.z[j] != -INFINITY) w += expf(l.z[j] - t.top);
-  t.ln_w = logf(wave_sum(w));
-  return t;
-}
-
-/** The loss of a row whose sums are o: the same in every lane of the wavefront that read its list. */
-__device__ inline auto loss_of(score_rows const& in, int k, teacher_sums const& t, listed_row const& l, row_sums const& o)
-  -> float
-{
-  float sum = 0.f;
-  for (int j = threadIdx.x % 64; j < k; j += 64) {
-    if (l.z[j] == -INFINITY) continue;
-    const float lq = l.z[j] - t.top - t.ln_w, p = expf(lq);
-    if (p != 0.f) sum += p * (lq - log_prob(l.x[j], o, in.temperature));
-  }
-  sum = wave_sum(sum);
-  return t.some ? sum : 0.f;
-}
-
-/** The shares -a q of the list's entries, for the wavefront that read it. */
-__device__ inline void write_shares(teacher_sums const& t, int k, float a, listed_row const& l)
-{
-  for (int j = threadIdx.x % 64; j < k; j += 64)
-    l.w[j] = l.z[j] != -INFINITY ? -a * expf(l.z[j] - t.top - t.ln_w) : 0.f;
-}
-
-/** The last step of row r, for one wavefront. */
-template <typename T>
-__device__ inline void write_loss(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, float* loss,
-                                  float* lse, int64_t r, listed_row const& l, row_sums const& o)
-{
-  const auto t      = read_teacher<T>(in, ids, teacher, r, l);
-  const float value = loss_of(in, ids.k, t, l, o);
   if (threadIdx.x % 64 == 0) {
-    loss[r] = value;
-    lse[r]  = o.lse;
+    both[threadIdx.x / 64 * 2]     = sums;
+    both[threadIdx.x / 64 * 2 + 1] = t;
+  }
+  lds_barrier();
+  sums = both[0];
+  t    = both[1];
+  for (int w = 1; w < NT / 64; ++w) {
+    sums          = join(sums, both[2 * w], c);
+    const run one = both[2 * w + 1];
+    if (one.s != 0.f) t = join(t, one, kLog2e);
   }
 }
 
+/** A pass over rows, a workgroup each, or with kSplit a workgroup a part of a row, which leaves its sums to
+ * finish_distill_kernel. */
 template <typename T, int NT, bool kSplit>
 __global__ __launch_bounds__(NT) void distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
-                                                           float* loss, float* lse, row_split split, part_sums* part,
-                                                           int64_t row0)
+                                                     float* loss, float* lse, row_split split, part_sums* part,
+                                                     int64_t row0)
 {
-  __shared__ run parts[NT / 64];
-  const auto listed = listed_at(ids.k, 0);
+  constexpr int E = kEntries<NT>;
+  __shared__ run both[2 * NT / 64];
+  __shared__ float losses[NT / 64];
   const int64_t b = row0 + blockIdx.x, r = kSplit ? b / split.parts : b;
   const int c0  = kSplit ? static_cast<int>(b - r * split.parts) * split.width : 0;
   const int c1  = kSplit ? min(c0 + split.width, in.n) : in.n;
   const T* row  = static_cast<const T*>(in.x) + r * in.stride;
   const float c = kLog2e / in.temperature;
-  run sums      = nothing();
+  listed_part<E> l;
+  if constexpr (!kSplit) read_list<NT>(in, ids, teacher, r, l);
+  run sums = nothing();
   for_scores<T, NT>(row, c0, c1, [](float) {}, [&](const auto& v, int) { add_scores<false>(sums, v, c); });
-  sums = join_block<NT>(sums, c, parts);
-  if (threadIdx.x >= 64) return;
   if constexpr (kSplit) {
+    sums = join_block<NT>(sums, c, both);
     if (threadIdx.x == 0) part[b] = {sums.m, sums.s, 0.f};
   } else {
-    write_loss<T>(in, ids, teacher, loss, lse, r, listed, finish(sums, in.temperature));
+    read_listed(row, l);
+    run list = teacher_run(l);
+    join_both<NT>(sums, c, list, both);
+    const auto o      = finish(sums, in.temperature);
+    const float share = wave_sum(loss_of(in, l, teacher_of(list), o));
+    if (threadIdx.x % 64 == 0) losses[threadIdx.x / 64] = share;
+    lds_barrier();
+    if (threadIdx.x == 0) {
+      float sum = losses[0];
+      for (int w = 1; w < NT / 64; ++w)
+        sum += losses[w];
+      loss[r] = sum;
+      lse[r]  = o.lse;
+    }
   }
 }
 
@@ -703,10 +739,21 @@ __global__ __launch_bounds__(64) void finish_distill_kernel(score_rows in, liste
                                                             float* loss, float* lse, row_split split,
                                                             const part_sums* part, int64_t row0)
 {
-  const auto listed = listed_at(ids.k, 0);
+  constexpr int E = kMaxListed / 64;
   const int64_t r = row0 + blockIdx.x;
-  write_loss<T>(in, ids, teacher, loss, lse, r, listed,
-                finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature));
+  listed_part<E> l;
+  read_list<64>(in, ids, teacher, r, l);
+  const auto o = finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature);
+  read_listed(static_cast<const T*>(in.x) + r * in.stride, l);
+  run list = teacher_run(l);
+#pragma unroll
+  for (int mask = 32; mask > 0; mask >>= 1)
+    list = join(list, shuffle_xor(list, mask), kLog2e);
+  const float sum = wave_sum(loss_of(in, l, teacher_of(list), o));
+  if (threadIdx.x == 0) {
+    loss[r] = sum;
+    lse[r]  = o.lse;
+  }
 }
 
 // ---- gradients
@@ -726,71 +773,104 @@ __device__ inline auto gradient(float x, gradient_row const& g) -> float
   return p * g.a;
 }
 
-/** Writes the gradients of the listed ids in columns [c0, c1) again, with their shares, after everything else's and a
- * barrier; an id that is listed more than once gets the sum of its shares, in their order. */
-template <typename T, bool kEntropy, int NT>
-__device__ inline void write_listed(T* grad, int c0, int c1, gradient_row const& g, listed_row const& l, int k)
+/** The ids of a row's list (-1: not listed) and their shares of its gradient, k of them in LDS. */
+struct listed_shares {
+  int id[kMaxListed];
+  float w[kMaxListed];
+};
+
+/** The list's entry of a lane's number, id -1 past the end. */
+struct listed_share {
+  int id;
+  float w;
+};
+
+__device__ inline auto share_at(listed_shares const& s, int j, int k) -> listed_share
 {
-  for (int j = threadIdx.x; j < k; j += NT) {
-    const int id = l.id[j];
-    if (id < c0 || id >= c1) continue;
-    bool first = true;
-    float sum  = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < k; ++i) {
-      const bool same = l.id[i] == id;
-      first           = first && (!same || i >= j);
-      sum += same ? l.w[i] : 0.f;
+  return j < k ? listed_share{s.id[j], s.w[j]} : listed_share{-1, 0.f};
+}
+
+/** Adds the shares of the list's ids to the gradients v of columns at + i, in the list's order; the wavefront's columns lie
+ * in [lo, hi).  first is the lane's of the first 64 entries. */
+template <int N>
+__device__ inline void add_shares(float (&v)[N], int at, int lo, int hi, listed_share first, listed_shares const& s, int k)
+{
+  for (int q = 0; q < k; q += 64) {
+    const listed_share mine = q == 0 ? first : share_at(s, q + static_cast<int>(threadIdx.x % 64), k);
+    for (key64 in = __ballot(mine.id >= lo && mine.id < hi); in != 0; in &= in - 1) {
+      const int i = __builtin_ctzll(in), column = __builtin_amdgcn_readlane(mine.id, i) - at;
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine.w), i));
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        v[e] += column == e ? w : 0.f;
     }
-    if (first) grad[id] = static_cast<T>(gradient<kEntropy>(l.x[j], g) + sum);
   }
 }
 
-/** Writes the gradient of columns [c0, c1).  prepare() gives what a row needs, and false in `some` for a gradient of 0; it
- * may hold barriers, and runs while the first scores are on their way. */
-template <typename T, bool kEntropy, typename P>
-__device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, listed_row const& l, int k, P prepare)
+/** The shares -a q of the thread's entries. */
+template <int NT, int E>
+__device__ inline void write_shares(listed_part<E> const& l, teacher_sums const& t, float a, int k, listed_shares& s)
 {
-  constexpr int N = kPer16<T>, kStep = kThreads * N;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int j = static_cast<int>(threadIdx.x) + e * NT;
+    if (j >= k) continue;
+    s.id[j] = l.id[e];
+    s.w[j]  = l.z[e] != -INFINITY ? -a * expf(l.z[e] - t.top - t.ln_w) : 0.f;
+  }
+}
+
+/** Writes the gradient of columns [c0, c1).  prepare() gives what a row needs, its list's shares in LDS and, in `some`,
+ * whether the gradient is other than 0; it may hold barriers, and runs while the first scores are on their way. */
+template <typename T, bool kEntropy, int NT, typename P>
+__device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, listed_shares const& s, int k, P prepare)
+{
+  constexpr int N = kPer16<T>, kStep = NT * N;
   const bool tiny = c1 - c0 < N;
   const int last  = c1 - N;
+  const int wave = c0 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 64 * N;
+  const int mine = static_cast<int>(threadIdx.x % 64) * N;
   uint4 next[kPieces];
-  int at = c0 + static_cast<int>(threadIdx.x) * N;
   if (!tiny) {
 #pragma unroll
     for (int u = 0; u < kPieces; ++u)
-      next[u] = load16(row + min(at + u * kStep, last));
+      next[u] = load16(row + min(wave + u * kStep + mine, last));
   }
   bool some            = true;
   const gradient_row g = prepare(some);
-  float v[N];
+  const listed_share first    = share_at(s, static_cast<int>(threadIdx.x % 64), k);
   if (tiny) {
-    at = c0 + static_cast<int>(threadIdx.x);
-    if (at < c1) grad[at] = static_cast<T>(some ? gradient<kEntropy>(static_cast<float>(row[at]), g) : 0.f);
-  } else {
-    for (; at < c1; at += kPieces * kStep) {
-      uint4 cur[kPieces];
+    const int at = c0 + static_cast<int>(threadIdx.x);
+    float v[1]   = {0.f};
+    if (at < c1 && some) v[0] = gradient<kEntropy>(static_cast<float>(row[at]), g);
+    if (some) add_shares(v, at, c0, c1, first, s, k);
+    if (at < c1) grad[at] = static_cast<T>(v[0]);
+    return;
+  }
+  float v[N];
+  for (int w = wave; w < c1; w += kPieces * kStep) {
+    uint4 cur[kPieces];
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u)
+      cur[u] = next[u];
+    if (w + kPieces * kStep < c1) {
 #pragma unroll
       for (int u = 0; u < kPieces; ++u)
-        cur[u] = next[u];
-      if (at + kPieces * kStep < c1) {
+        next[u] = load16(row + min(w + (kPieces + u) * kStep + mine, last));
+    }
 #pragma unroll
-        for (int u = 0; u < kPieces; ++u)
-          next[u] = load16(row + min(at + (kPieces + u) * kStep, last));
-      }
+    for (int u = 0; u < kPieces; ++u) {
+      const int w0 = w + u * kStep;
+      if (w0 >= c1) break;
+      const int at = min(w0 + mine, last);  // a lane that was moved back writes what its neighbor does
+      unpack16<T>(cur[u], v);
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u) {
-        if (at + u * kStep >= c1) break;
-        unpack16<T>(cur[u], v);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          v[i] = some ? gradient<kEntropy>(v[i], g) : 0.f;
-        store16(grad + min(at + u * kStep, last), pack16<T>(v));  // a lane that was moved back writes what its neighbor does
-      }
+      for (int i = 0; i < N; ++i)
+        v[i] = some ? gradient<kEntropy>(v[i], g) : 0.f;
+      if (some) add_shares(v, at, min(w0, last), min(w0 + 64 * N, c1), first, s, k);
+      if (w0 + mine < c1) store16(grad + at, pack16<T>(v));
     }
   }
-  __syncthreads();
-  if (some) write_listed<T, kEntropy, kThreads>(grad, c0, c1, g, l, k);
 }
 
 /**
@@ -798,7 +878,7 @@ __device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, lis
  * has lost too much of ln s to its rounding (all of it in a row of the type's lowest values), so such a row's sums are made
  * again.  All threads call this; parts [kWaves] is LDS.
  */
-template <typename T>
+template <typename T, int NT>
 __device__ inline auto gradient_base(const T* row, int n, float lse, float temperature, run* parts) -> gradient_row
 {
   gradient_row g{};
@@ -806,71 +886,75 @@ __device__ inline auto gradient_base(const T* row, int n, float lse, float tempe
   g.l2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
   if (fabsf(lse) > kMaxLse && fabsf(lse) != INFINITY) {
     run sums = nothing();
-    for_scores<T, kThreads>(row, 0, n, [](float) {}, [&](const auto& v, int) { add_scores<false>(sums, v, g.c); });
-    sums  = join_block<kThreads>(sums, g.c, parts);
+    for_scores<T, NT>(row, 0, n, [](float) {}, [&](const auto& v, int) { add_scores<false>(sums, v, g.c); });
+    sums  = join_block<NT>(sums, g.c, parts);
     g.ref = sums.ref;
     g.l2  = log2f(sums.s);
   }
   return g;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void log_probs_backward_kernel(score_rows in, listed_ids ids, const float* grad_logp,
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void log_probs_backward_kernel(score_rows in, listed_ids ids, const float* grad_logp,
                                                                       const float* grad_entropy, const float* lse,
                                                                       const float* entropy, T* grad, int64_t gstride,
                                                                       row_split split, int64_t row0)
 {
-  const auto listed = listed_at(ids.k, 0);
-  __shared__ float total;
-  __shared__ run parts[kWaves];
+  constexpr int E = kEntries<NT>;
+  __shared__ listed_shares shares;
+  __shared__ float totals[NT / 64];
+  __shared__ run parts[NT / 64];
   const int64_t b = row0 + blockIdx.x, r = b / split.parts;
   const int c0 = static_cast<int>(b - r * split.parts) * split.width, c1 = min(c0 + split.width, in.n);
   const T* row = static_cast<const T*>(in.x) + r * in.stride;
-  write_gradient<T, true>(row, grad + r * gstride, c0, c1, listed, ids.k, [&](bool&) {
-    if (threadIdx.x < 64) {
-      float sum = 0.f;
-      for (int j = threadIdx.x; j < ids.k; j += 64) {
-        const int64_t id  = id_at(ids, r, j);
-        const bool in_row = id >= 0 && id < in.n;
-        const float gj    = in_row && grad_logp != nullptr ? grad_logp[r * ids.k + j] : 0.f;
-        listed.id[j]      = in_row ? static_cast<int>(id) : -1;
-        listed.x[j]       = in_row ? static_cast<float>(row[id]) : 0.f;
-        listed.w[j]       = gj / in.temperature;
-        sum += gj;
-      }
-      sum = wave_sum(sum);
-      if (threadIdx.x == 0) total = sum;
+  write_gradient<T, true, NT>(row, grad + r * gstride, c0, c1, shares, ids.k, [&](bool&) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = static_cast<int>(threadIdx.x) + e * NT;
+      if (j >= ids.k) continue;
+      const int64_t id  = id_at(ids, r, j);
+      const bool in_row = id >= 0 && id < in.n;
+      const float gj    = in_row && grad_logp != nullptr ? grad_logp[r * ids.k + j] : 0.f;
+      shares.id[j]      = in_row ? static_cast<int>(id) : -1;
+      shares.w[j]       = gj / in.temperature;
+      sum += gj;
     }
-    __syncthreads();
+    sum = wave_sum(sum);
+    if (threadIdx.x % 64 == 0) totals[threadIdx.x / 64] = sum;
+    lds_barrier();
+    float total = totals[0];
+    for (int w = 1; w < NT / 64; ++w)
+      total += totals[w];
     const float h = grad_entropy != nullptr ? grad_entropy[r] : 0.f;
-    auto g        = gradient_base(row, in.n, lse[r], in.temperature, parts);
+    auto g        = gradient_base<T, NT>(row, in.n, lse[r], in.temperature, parts);
     g.a           = -(total + (h != 0.f ? h * entropy[r] : 0.f)) / in.temperature;
     g.b           = -h / in.temperature;
     return g;
   });
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_backward_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                                     const float* grad_loss, const float* lse, T* grad,
                                                                     int64_t gstride, row_split split, int64_t row0)
 {
-  const auto listed = listed_at(ids.k, 0);
-  __shared__ int any;
-  __shared__ run parts[kWaves];
+  constexpr int E = kEntries<NT>;
+  __shared__ listed_shares shares;
+  __shared__ run parts[NT / 64];
   const int64_t b = row0 + blockIdx.x, r = b / split.parts;
   const int c0 = static_cast<int>(b - r * split.parts) * split.width, c1 = min(c0 + split.width, in.n);
   const T* row  = static_cast<const T*>(in.x) + r * in.stride;
   const float a = grad_loss[r] / in.temperature;
-  write_gradient<T, false>(row, grad + r * gstride, c0, c1, listed, ids.k, [&](bool& some) {
-    if (threadIdx.x < 64) {
-      const auto t = read_teacher<T>(in, ids, teacher, r, listed);
-      write_shares(t, ids.k, a, listed);
-      if (threadIdx.x == 0) any = t.some;
-    }
-    __syncthreads();
-    some   = any != 0;
-    auto g = gradient_base(row, in.n, lse[r], in.temperature, parts);
+  listed_part<E> l;
+  read_list<NT>(in, ids, teacher, r, l);
+  write_gradient<T, false, NT>(row, grad + r * gstride, c0, c1, shares, ids.k, [&](bool& some) {
+    const run list = join_block<NT>(teacher_run(l), kLog2e, parts);
+    const auto t   = teacher_of(list);
+    some           = t.some;
+    write_shares<NT>(l, t, a, ids.k, shares);
+    lds_barrier();  // parts has been read
+    auto g = gradient_base<T, NT>(row, in.n, lse[r], in.temperature, parts);
     g.a    = a;
     return g;
   });
@@ -880,26 +964,28 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(score_rows i
  * Both directions of rows that a workgroup holds in registers, H pieces of 16 bytes a thread: each is read once and its
  * gradient written once.  A workgroup takes every gridDim-th row; as a piece of a row's gradient is stored, the same piece
  * of its next row is loaded in its place, and pieces that have arrived enter that row's sums, so that reads, writes and
- * arithmetic go on side by side.  The first wavefront reads the next row's list meanwhile.
+ * arithmetic go on side by side.  The next row's list comes meanwhile, E entries a thread.
  */
 template <typename T, int NT, int H>
 __global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                           const float* grad_loss, float* loss, float* lse, T* grad,
-                                                          int64_t gstride)
+                                                          int64_t gstride, bool by_cache)
 {
-  constexpr int N = kPer16<T>, kStep = NT * N, kLag = H < 8 ? H : 4;  // pieces on their way
-  __shared__ int any[2];
-  __shared__ run parts[NT / 64];
-  const int last = in.n - N;
+  constexpr int N = kPer16<T>, kStep = NT * N, kLag = 4;  // pieces on their way
+  constexpr int E = NT > kMaxListed ? 1 : kEntries<NT>;
+  __shared__ listed_shares shares;
+  __shared__ run both[2 * NT / 64];
+  __shared__ float losses[NT / 64];
+  const int last = in.n - N, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 64 * N;
   int mine       = static_cast<int>(threadIdx.x) * N;
   const float c  = kLog2e / in.temperature;
   uint4 held[H];
-  run sums;
+  run sums = nothing();
   float v[N];
-  const auto load = [&](int64_t r, int h) {
-    held[h] = load16(static_cast<const T*>(in.x) + r * in.stride + min(h * kStep + mine, last));
-  };
-  const auto add = [&](int h) {
+  listed_part<E> l, after;
+  const auto row_at = [&](int64_t r) { return static_cast<const T*>(in.x) + r * in.stride; };
+  const auto load   = [&](int64_t r, int h) { held[h] = load16(row_at(r) + min(h * kStep + mine, last)); };
+  const auto add    = [&](int h) {
     unpack16<T>(held[h], v);
     if (h * kStep + kStep > in.n) {  // columns that another thread holds
       const int at = h * kStep + mine, from = min(at, last);
@@ -909,57 +995,60 @@ __global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_
     }
     add_scores<false>(sums, v, c);
   };
-  teacher_sums t{};
-  const auto read_list = [&](int64_t r, int list) {
-    if (threadIdx.x >= 64) return;
-    const auto l = listed_at(ids.k, list);
-    t            = read_teacher<T>(in, ids, teacher, r, l);
-    write_shares(t, ids.k, grad_loss[r] / in.temperature, l);
-    if (threadIdx.x == 0) any[list] = t.some;
-  };
+  read_list<NT>(in, ids, teacher, blockIdx.x, l);
 #pragma unroll
   for (int h = 0; h < H; ++h)
     if (h * kStep < in.n) load(blockIdx.x, h);
-  read_list(blockIdx.x, 0);
-  sums = nothing();
+  read_listed(row_at(blockIdx.x), l);
 #pragma unroll
   for (int h = 0; h < H; ++h)
     if (h * kStep < in.n) add(h);
-  int list = 0;
-  for (int64_t r = blockIdx.x; r < in.m; r += gridDim.x, list ^= 1) {
+  for (int64_t r = blockIdx.x; r < in.m; r += gridDim.x) {
     asm volatile("" : "+v"(mine));  // the pieces' places are made again for every row: kept, they would take H registers
     const int64_t next = r + gridDim.x;
     const bool more    = next < in.m;
-    const run all      = join_block<NT>(sums, c, parts);
-    const auto l       = listed_at(ids.k, list);
-    if (threadIdx.x < 64) {
-      const auto o      = finish(all, in.temperature);
-      const float value = loss_of(in, ids.k, t, l, o);
-      if (threadIdx.x == 0) {
-        loss[r] = value;
-        lse[r]  = o.lse;
-      }
+    if (more) read_list<NT>(in, ids, teacher, next, after);
+    run list = teacher_run(l);
+    join_both<NT>(sums, c, list, both);
+    const auto t  = teacher_of(list);
+    const auto o  = finish(sums, in.temperature);
+    const float a = grad_loss[r] / in.temperature;
+    write_shares<NT>(l, t, a, ids.k, shares);
+    const float share = wave_sum(loss_of(in, l, t, o));
+    if (threadIdx.x % 64 == 0) losses[threadIdx.x / 64] = share;
+    lds_barrier();
+    if (threadIdx.x == 0) {
+      float sum = losses[0];
+      for (int w = 1; w < NT / 64; ++w)
+        sum += losses[w];
+      loss[r] = sum;
+      lse[r]  = o.lse;
     }
-    const bool some = any[list] != 0;
-    if (more) read_list(next, list ^ 1);
-    const gradient_row g{all.ref, c, all.s > 0.f ? log2f(all.s) : all.s == 0.f ? INFINITY : all.s,
-                         grad_loss[r] / in.temperature, 0.f};
+    const listed_share first = share_at(shares, static_cast<int>(threadIdx.x % 64), ids.k);
+    const gradient_row g{sums.ref, c, sums.s > 0.f ? log2f(sums.s) : sums.s == 0.f ? INFINITY : sums.s, a, 0.f};
     T* out = grad + r * gstride;
     sums   = nothing();
 #pragma unroll
     for (int h = 0; h < H + kLag; ++h) {
       if (h < H && h * kStep < in.n) {
+        const int at = min(h * kStep + mine, last), w0 = h * kStep + wave;
         unpack16<T>(held[h], v);
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          v[i] = some ? gradient<false>(v[i], g) : 0.f;
-        if (h * kStep + mine < in.n) store16(out + min(h * kStep + mine, last), pack16<T>(v));
+          v[i] = t.some ? gradient<false>(v[i], g) : 0.f;
+        if (t.some) add_shares(v, at, min(w0, last), min(w0 + 64 * N, in.n), first, shares, ids.k);
+        if (h * kStep + mine < in.n) {
+          if (by_cache)
+            store16(out + at, pack16<T>(v));
+          else
+            store16_nt(out + at, pack16<T>(v));
+        }
         if (more) load(next, h);
       }
+      if (h == H / 2 && more) read_listed(row_at(next), after);
       if (more && h >= kLag && (h - kLag) * kStep < in.n) add(h - kLag);
     }
-    __syncthreads();
-    if (some) write_listed<T, false, NT>(out, 0, in.n, g, l, ids.k);
+    l = after;
   }
 }
 
@@ -1005,8 +1094,10 @@ auto forward_split_of(int64_t m, int n, int top) -> row_split
   return split_of(m, n, std::min(kMaxParts, 4 * kThreads / std::max(top, 1)));
 }
 
+constexpr int64_t kCachedBytes = int64_t{128} << 20;  // of a gradient that the last-level cache may keep for its reader
+
 /** Rows of few columns take a wavefront each where there are enough of them. */
-auto by_wavefront(int64_t m, int n) -> bool { return m >= 2048 && n <= 4096; }
+auto by_wavefront(int64_t m, int n, int k) -> bool { return m >= 2048 && n <= 4096 && k <= kShortList; }
 
 }  // namespace
 
@@ -1036,7 +1127,7 @@ void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out
       launch(top ? log_probs_kernel<T, kThreads, true, true> : log_probs_kernel<T, kThreads, false, true>, kThreads,
              in.m * split.parts);
       launch(top ? finish_log_probs_kernel<T, true> : finish_log_probs_kernel<T, false>, kThreads, in.m);
-    } else if (by_wavefront(in.m, in.n)) {
+    } else if (by_wavefront(in.m, in.n, 0)) {
       launch(top ? log_probs_kernel<T, 64, true, false> : log_probs_kernel<T, 64, false, false>, 64, in.m);
     } else {
       launch(top ? log_probs_kernel<T, kThreads, true, false> : log_probs_kernel<T, kThreads, false, false>, kThreads, in.m);
@@ -1050,12 +1141,18 @@ void launch_log_probs_backward(score_rows const& in, listed_ids const& ids, cons
 {
   const auto split = split_of(in.m, in.n);
   with_type(in.type, [&](auto e) {
-    using T = decltype(e);
-    for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
-      log_probs_backward_kernel<T><<<count, kThreads, listed_bytes(ids.k, 1), s>>>(in, ids, grad_logp, grad_entropy, lse, entropy,
-                                                              static_cast<T*>(grad), gstride, split, first);
-      OCTEX_HIP(hipGetLastError());
-    });
+    using T           = decltype(e);
+    const auto launch = [&](auto kernel, int threads) {
+      for_grids(in.m * split.parts, threads, [&](int64_t first, unsigned count) {
+        kernel<<<count, threads, 0, s>>>(in, ids, grad_logp, grad_entropy, lse, entropy, static_cast<T*>(grad), gstride, split,
+                                         first);
+        OCTEX_HIP(hipGetLastError());
+      });
+    };
+    if (by_wavefront(in.m, in.n, ids.k))
+      launch(log_probs_backward_kernel<T, 64>, 64);
+    else
+      launch(log_probs_backward_kernel<T, kThreads>, kThreads);
   });
 }
 
@@ -1066,20 +1163,19 @@ void launch_distill(score_rows const& in, listed_ids const& ids, teacher_logits 
   auto* part       = static_cast<part_sums*>(workspace);
   with_type(in.type, [&](auto e) {
     using T = decltype(e);
-    const size_t lds = listed_bytes(ids.k, 1);
-    const auto launch = [&](auto kernel, int threads, int64_t total, size_t bytes) {
+    const auto launch = [&](auto kernel, int threads, int64_t total) {
       for_grids(total, threads, [&](int64_t first, unsigned count) {
-        kernel<<<count, threads, bytes, s>>>(in, ids, teacher, loss, lse, split, part, first);
+        kernel<<<count, threads, 0, s>>>(in, ids, teacher, loss, lse, split, part, first);
         OCTEX_HIP(hipGetLastError());
       });
     };
     if (split.parts > 1) {
-      launch(distill_kernel<T, kThreads, true>, kThreads, in.m * split.parts, 0);
-      launch(finish_distill_kernel<T>, 64, in.m, lds);
-    } else if (by_wavefront(in.m, in.n)) {
-      launch(distill_kernel<T, 64, false>, 64, in.m, lds);
+      launch(distill_kernel<T, kThreads, true>, kThreads, in.m * split.parts);
+      launch(finish_distill_kernel<T>, 64, in.m);
+    } else if (by_wavefront(in.m, in.n, ids.k)) {
+      launch(distill_kernel<T, 64, false>, 64, in.m);
     } else {
-      launch(distill_kernel<T, kThreads, false>, kThreads, in.m, lds);
+      launch(distill_kernel<T, kThreads, false>, kThreads, in.m);
     }
   });
 }
@@ -1089,42 +1185,51 @@ void launch_distill_backward(score_rows const& in, listed_ids const& ids, teache
 {
   const auto split = split_of(in.m, in.n);
   with_type(in.type, [&](auto e) {
-    using T = decltype(e);
-    for_grids(in.m * split.parts, kThreads, [&](int64_t first, unsigned count) {
-      distill_backward_kernel<T><<<count, kThreads, listed_bytes(ids.k, 1), s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride,
-                                                            split, first);
-      OCTEX_HIP(hipGetLastError());
-    });
+    using T           = decltype(e);
+    const auto launch = [&](auto kernel, int threads) {
+      for_grids(in.m * split.parts, threads, [&](int64_t first, unsigned count) {
+        kernel<<<count, threads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride, split, first);
+        OCTEX_HIP(hipGetLastError());
+      });
+    };
+    if (by_wavefront(in.m, in.n, ids.k))
+      launch(distill_backward_kernel<T, 64>, 64);
+    else
+      launch(distill_backward_kernel<T, kThreads>, kThreads);
   });
 }
 
 constexpr int kHeldThreads = 1024, kHeldPieces = 16;  // of the widest row that a workgroup holds
 
-auto distill_step_held(int n, elem type) -> bool
+/** Few wide rows are quicker in parts, by two passes: 1 x 128,000 bfloat16 in 14 us against 27 (but 16 x 32,000 float32 in 13
+ * either way), 333 x 50,021 float32 in 37 against 41, 1000 x 100,003 float16 in 135 against 102. */
+auto distill_step_held(int64_t m, int n, elem type) -> bool
 {
-  const int per = 16 / elem_size(type);
-  return n >= per && n <= kHeldThreads * kHeldPieces * per;
+  const int per = 16 / elem_size(type), pieces = (n + per - 1) / per;
+  if (n < per || pieces > kHeldThreads * kHeldPieces) return false;
+  return pieces <= kHeldThreads * 8 || m >= 512;
 }
 
 void launch_distill_step(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, const float* grad_loss,
                          float* loss, float* lse, void* grad, int64_t gstride, void* workspace, hipStream_t s)
 {
-  if (!distill_step_held(in.n, in.type)) {
+  if (!distill_step_held(in.m, in.n, in.type)) {
     launch_distill(in, ids, teacher, loss, lse, workspace, s);
     launch_distill_backward(in, ids, teacher, grad_loss, lse, grad, gstride, s);
     return;
   }
   with_type(in.type, [&](auto e) {
-    using T           = decltype(e);
-    const auto launch = [&](auto kernel, int threads, int64_t slots) {
-      kernel<<<static_cast<unsigned>(std::min(in.m, slots)), threads, listed_bytes(ids.k, 2), s>>>(
-        in, ids, teacher, grad_loss, loss, lse, static_cast<T*>(grad), gstride);
+    using T             = decltype(e);
+    const bool by_cache = in.m * in.n * static_cast<int64_t>(sizeof(T)) <= kCachedBytes;
+    const auto launch   = [&](auto kernel, int threads, int64_t slots) {
+      kernel<<<static_cast<unsigned>(std::min(in.m, slots)), threads, 0, s>>>(in, ids, teacher, grad_loss, loss, lse,
+                                                                              static_cast<T*>(grad), gstride, by_cache);
       OCTEX_HIP(hipGetLastError());
     };
     const int pieces = (in.n + kPer16<T> - 1) / kPer16<T>;
-    if (pieces <= 256 && in.m >= 2048)
+    if (pieces <= 256 && in.m >= 2048 && ids.k <= kShortList)
       launch(distill_step_kernel<T, 64, 4>, 64, 8192);
-    else if (pieces <= 1024 && in.m >= 2048)
+    else if (pieces <= 1024 && in.m >= 2048 && ids.k <= kShortList)
       launch(distill_step_kernel<T, 64, 16>, 64, 4096);
     else if (pieces <= 1024)
       launch(distill_step_kernel<T, 256, 4>, 256, 2048);

@@ -72,7 +72,7 @@ void launch_distill_backward(score_rows const& in, listed_ids const& ids, teache
                              const float* grad_loss, const float* lse, void* grad, int64_t gstride, hipStream_t s);
 
 /** Whether launch_distill_step holds a row in registers; else it needs launch_distill's workspace. */
-auto distill_step_held(int n, elem type) -> bool;
+auto distill_step_held(int64_t m, int n, elem type) -> bool;
 
 /** Both directions; the logits are read once if a workgroup can hold a row. */
 void launch_distill_step(score_rows const& in, listed_ids const& ids, teacher_logits const& teacher, const float* grad_loss,
