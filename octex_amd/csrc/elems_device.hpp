@@ -12,6 +12,16 @@ namespace cuvs::neighbors::octex::detail {
 using bf16 = __bf16;
 using f16  = _Float16;
 
+__device__ inline void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+/** A barrier for what lies in LDS: the workgroup's loads and stores of other memory stay on their way. */
+__device__ inline void lds_barrier()
+{
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 /** Elements of 16 bytes. */
 template <typename T>
 constexpr int kPer16 = 16 / static_cast<int>(sizeof(T));

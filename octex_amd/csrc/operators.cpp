@@ -154,8 +154,7 @@ extern "C" cuvsError_t octexQuantizeRows(const octexMatrix* x, const octexMatrix
     if (x->rows == 0) return;
     on_gpu gpu;
     gpu.take(x->data, "x"), gpu.take(codes->data, "codes"), gpu.take(scales, "scales");
-    const int k = static_cast<int>(x->cols);
-    launch_quantize_rows(x->data, elem_of(*x), x->rows, k, k, x->stride,
+    launch_quantize_rows(x->data, elem_of(*x), x->rows, static_cast<int>(x->cols), x->stride,
                          static_cast<int8_t*>(codes->data), codes->stride, scales, static_cast<hipStream_t>(stream));
   });
 }

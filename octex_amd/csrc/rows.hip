@@ -30,16 +30,6 @@ constexpr int kFull    = 128;   // keys from which a list is compacted
 
 __device__ inline auto exp2_fast(float v) -> float { return __builtin_amdgcn_exp2f(v); }
 
-__device__ inline void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
-
-/** A barrier for what lies in LDS: the workgroup's loads and stores of other memory stay on their way. */
-__device__ inline void lds_barrier()
-{
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 /** The running sums of a part of a row; ref is m, or 0 while there is no finite score. */
 struct run {
   float m, ref, s, t;
@@ -166,23 +156,24 @@ __device__ inline auto floor_of(const unsigned (&order)[N], int k, int most) -> 
 }
 
 /** The same for distinct keys, which leave at most `most`. */
-__device__ inline auto floor_of(const key64 (&key)[4], int k, int most) -> key64
+template <int N>
+__device__ inline auto floor_of(const key64 (&key)[N], int k, int most) -> key64
 {
-  unsigned order[4];
+  unsigned order[N];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < N; ++j)
     order[j] = static_cast<unsigned>(key[j] >> 32);
   key64 p = key64{floor_of(order, k, most)} << 32;
   if (p == 0) return 0;
   int c = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < N; ++j)
     c += __popcll(__ballot(key[j] >= p));
   for (int bit = 31; bit >= 0 && c > most; --bit) {  // equal values: by column
     const key64 q = p | key64{1} << bit;
     int d         = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < N; ++j)
       d += __popcll(__ballot(key[j] >= q));
     if (d >= k) p = q, c = d;
   }
@@ -318,22 +309,22 @@ __device__ inline auto gather_keys(const key64 (&key)[4], int mine, int k, key64
   return n;
 }
 
-/** Calls f(rank, key) for the k best of n (at most 256) distinct keys in LDS, which it leaves in another order; a key's rank
+/** Calls f(rank, key) for the k best of n (at most 64 * R) distinct keys in LDS, which it leaves in another order; a key's rank
  * is the number of greater ones.  One wavefront's work. */
-template <typename F>
+template <int R, typename F>
 __device__ inline void rank_keys(key64* keys, int n, int k, F f)
 {
   const int lane = threadIdx.x % 64;
   if (n > 64) {
-    key64 key[4];
+    key64 key[R];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < R; ++j)
       key[j] = lane + 64 * j < n ? keys[lane + 64 * j] : 0;
     wave_fence();
     const key64 p = floor_of(key, k, 64);
     n             = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < R; ++j) {
       const bool in  = key[j] != 0 && key[j] >= p;
       const key64 at = __ballot(in);
       if (in) keys[n + lanes_below(at)] = key[j];
@@ -481,6 +472,7 @@ __device__ inline void write_log_probs(score_rows const& in, listed_ids const& i
 }
 
 /** The alternatives of row r: the best of n keys in LDS.  The first wavefront's work. */
+template <int R>
 __device__ inline void write_top(score_rows const& in, log_probs_out const& out, int64_t r, row_sums const& o, key64* keys,
                                  int n)
 {
@@ -488,7 +480,7 @@ __device__ inline void write_top(score_rows const& in, log_probs_out const& out,
   if (lane >= 64) return;
   const bool bad = isnan(o.lse);
   const int have = bad ? 0 : min(n, out.top);
-  rank_keys(keys, bad ? 0 : n, out.top, [&](int rank, key64 key) {
+  rank_keys<R>(keys, bad ? 0 : n, out.top, [&](int rank, key64 key) {
     out.top_logp[r * out.top + rank] = log_prob(value_of(key), o, in.temperature);
     out.top_ids[r * out.top + rank]  = column_of(key);
   });
@@ -536,14 +528,14 @@ __global__ __launch_bounds__(NT) void log_probs_kernel(score_rows in, listed_ids
     if (threadIdx.x == 0) part[b] = {sums.m, sums.s, sums.t};
     if constexpr (kTop) {
       if (threadIdx.x < 64) {
-        rank_keys(keys, n, out.top, [&](int rank, key64 key) { best[b * out.top + rank] = key; });
+        rank_keys<kWavesHere>(keys, n, out.top, [&](int rank, key64 key) { best[b * out.top + rank] = key; });
         if (static_cast<int>(threadIdx.x) >= n && static_cast<int>(threadIdx.x) < out.top) best[b * out.top + threadIdx.x] = 0;
       }
     }
   } else {
     const auto o = finish(sums, in.temperature);
     write_log_probs<T, NT>(in, ids, out, r, o);
-    if constexpr (kTop) write_top(in, out, r, o, keys, n);
+    if constexpr (kTop) write_top<kWavesHere>(in, out, r, o, keys, n);
   }
 }
 
@@ -579,7 +571,7 @@ __global__ __launch_bounds__(kThreads) void finish_log_probs_kernel(score_rows i
   }
   const auto o = finish(join_parts(part, r, split.parts, kLog2e / in.temperature), in.temperature);
   write_log_probs<T, kThreads>(in, ids, out, r, o);
-  if constexpr (kTop) write_top(in, out, r, o, keys, gather_keys<kThreads>(key, 256, out.top, keys, counts));
+  if constexpr (kTop) write_top<kWaves>(in, out, r, o, keys, gather_keys<kThreads>(key, 256, out.top, keys, counts));
 }
 
 // ---- the teacher's distribution: entry e of a thread is the row's entry threadIdx.x + e * NT
@@ -1078,6 +1070,8 @@ constexpr int kMinWidth  = 4096;  // columns of a part
 constexpr int kMaxParts  = 32;    // of a row
 constexpr int kFewRows   = 128;   // rows whose forward pass is split: more fill the GPU well enough to spare the second kernel
 
+constexpr int kMidRows   = 512;   // rows whose top entries take 512 threads (333 x 50,021 float32: 25.7 us, of 256 threads 28.2)
+
 /** Rows are split into parts of whole 16-byte pieces while they are fewer than the workgroups that fill the GPU. */
 auto split_of(int64_t m, int n, int64_t most = kMaxParts) -> row_split
 {
@@ -1129,6 +1123,8 @@ void launch_log_probs(score_rows const& in, listed_ids const& ids, log_probs_out
       launch(top ? finish_log_probs_kernel<T, true> : finish_log_probs_kernel<T, false>, kThreads, in.m);
     } else if (by_wavefront(in.m, in.n, 0)) {
       launch(top ? log_probs_kernel<T, 64, true, false> : log_probs_kernel<T, 64, false, false>, 64, in.m);
+    } else if (top && in.m <= kMidRows) {
+      launch(log_probs_kernel<T, 512, true, false>, 512, in.m);
     } else {
       launch(top ? log_probs_kernel<T, kThreads, true, false> : log_probs_kernel<T, kThreads, false, false>, kThreads, in.m);
     }

@@ -15,8 +15,6 @@ namespace {
 using i32x4  = int __attribute__((ext_vector_type(4)));
 using i32x16 = int __attribute__((ext_vector_type(16)));
 
-__device__ inline void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
-
 // ---- quantization of rows
 
 constexpr int kQuantThreads = 256;
@@ -45,10 +43,67 @@ __device__ inline auto block_max(unsigned top, unsigned* parts) -> unsigned
   for (int mask = 32; mask > 0; mask >>= 1)
     top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), mask)));
   if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = top;
-  __syncthreads();
+  lds_barrier();
   for (int w = 0; w < static_cast<int>(blockDim.x) / 64; ++w)
     top = max(top, parts[w]);
   return top;
+}
+
+struct product {
+  int8_rows q, r;
+  int64_t m, n;
+  int k;
+  const float* bias;
+  void* out;
+  int64_t ostride;
+};
+
+__device__ inline auto score_of(int sum, float qs, product const& p, int64_t j) -> float
+{
+  const float v = static_cast<float>(sum) * qs * p.r.scales[j];
+  return p.bias != nullptr ? v + p.bias[j] : v;
+}
+
+/** 16 values of a row at column at, those from k on 0. */
+__device__ inline auto load_codes(const int8_t* row, int at, int k) -> i32x4
+{
+  i32x4 v = {0, 0, 0, 0};
+  if (at + 16 <= k)
+    __builtin_memcpy(&v, row + at, 16);
+  else if (at < k) {
+    int8_t e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      e[i] = at + i < k ? row[at + i] : int8_t{0};
+    __builtin_memcpy(&v, e, 16);
+  }
+  return v;
+}
+
+// ---- rows laid out anew: 16-byte chunks at aligned places, zeros after the last value
+
+/** Rows x [n, k] that a kernel lays out at out, `pitch` apart; n = 0: none. */
+struct pack_job {
+  const int8_t* x;
+  int64_t stride, n;
+  int k;
+  int8_t* out;
+  int64_t pitch;
+};
+
+constexpr int kPackRows = 4;  // of a workgroup, a wavefront each
+
+__device__ inline void pack_rows(pack_job const& p, int64_t first)
+{
+  const int64_t i = first + threadIdx.x / 64;
+  if (i >= p.n) return;
+  for (int at = static_cast<int>(threadIdx.x % 64) * 16; at < p.k; at += 64 * 16)
+    *reinterpret_cast<i32x4*>(p.out + i * p.pitch + at) = load_codes(p.x + i * p.stride, at, p.k);
+}
+
+__global__ __launch_bounds__(64 * kPackRows) void pack_kernel(pack_job p, int64_t first)
+{
+  pack_rows(p, first + int64_t{blockIdx.x} * kPackRows);
 }
 
 /**
@@ -56,14 +111,20 @@ __device__ inline auto block_max(unsigned top, unsigned* parts) -> unsigned
  * A row of zeros has scale 0 and codes 0; one with a NaN or an infinity has scale NaN and codes 0.
  *
  * A workgroup holds a row of up to kHeld * 256 values in registers between the maximum and the codes, so that it is read
- * once; longer rows are read again.  Columns k .. pad are written as 0.
+ * once; longer rows are read again.  Columns k .. pad are written as 0.  Workgroups past the rows' lay out `job`.
  */
 template <typename T, int kHeld>
 __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T* x, int64_t stride, int k, int pad, int8_t* codes,
-                                                                 int64_t cstride, float* scales, int64_t row0)
+                                                                 int64_t cstride, float* scales, int64_t row0,
+                                                                 unsigned rows, pack_job job)
 {
   constexpr int N = kPer16<T>, kStep = kQuantThreads * N;
+  static_assert(kQuantThreads == 64 * kPackRows);
   __shared__ unsigned parts[kQuantThreads / 64];
+  if (blockIdx.x >= rows) {
+    pack_rows(job, int64_t{blockIdx.x - rows} * kPackRows);
+    return;
+  }
   const int64_t r = row0 + blockIdx.x;
   const T* row    = x + r * stride;
   int8_t* out     = codes + r * cstride;
@@ -107,53 +168,6 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T* x, int
   if (static_cast<int>(threadIdx.x) < pad - k) out[k + threadIdx.x] = 0;
 }
 
-struct product {
-  int8_rows q, r;
-  int64_t m, n;
-  int k;
-  const float* bias;
-  void* out;
-  int64_t ostride;
-};
-
-__device__ inline auto score_of(int sum, float qs, product const& p, int64_t j) -> float
-{
-  const float v = static_cast<float>(sum) * qs * p.r.scales[j];
-  return p.bias != nullptr ? v + p.bias[j] : v;
-}
-
-/** 16 values of a row at column at, those from k on 0. */
-__device__ inline auto load_codes(const int8_t* row, int at, int k) -> i32x4
-{
-  i32x4 v = {0, 0, 0, 0};
-  if (at + 16 <= k)
-    __builtin_memcpy(&v, row + at, 16);
-  else if (at < k) {
-    int8_t e[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      e[i] = at + i < k ? row[at + i] : int8_t{0};
-    __builtin_memcpy(&v, e, 16);
-  }
-  return v;
-}
-
-// ---- rows laid out anew: 16-byte chunks at aligned places, zeros after the last value
-
-constexpr int kPackThreads = 256;
-
-__global__ __launch_bounds__(kPackThreads) void pack_kernel(const int8_t* x, int64_t stride, int64_t n, int k, int8_t* out,
-                                                            int64_t pitch)
-{
-  const int chunks    = (k + 15) / 16;
-  const int64_t total = n * chunks;
-  for (int64_t e = int64_t{blockIdx.x} * kPackThreads + threadIdx.x; e < total; e += int64_t{gridDim.x} * kPackThreads) {
-    const int64_t i = e / chunks;
-    const int c     = static_cast<int>(e - i * chunks);
-    *reinterpret_cast<i32x4*>(out + i * pitch + 16 * c) = load_codes(x + i * stride, 16 * c, k);
-  }
-}
-
 // ---- the product
 
 constexpr int64_t kMaxInt8Stride = int64_t{1} << 22;  // a tile's 256 rows within 32-bit offsets
@@ -176,6 +190,34 @@ __global__ __launch_bounds__(64 * KW) void few_scores_kernel(product p, const Q*
   constexpr int kThreadsHere = 64 * KW;
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, m = static_cast<int>(p.m);
   const int64_t j0 = int64_t{blockIdx.x} * RT * 16;
+  int k0           = wave * kPiece;
+  const int8_t* rows[RT];
+  i32x4 acc[RT] = {}, b[RT][4];
+#pragma unroll
+  for (int y = 0; y < RT; ++y)
+    rows[y] = p.r.x + min(j0 + 16 * y + lane % 16, p.n - 1) * p.r.stride;
+  const auto load_rows = [&](int from) {
+    if (from + kPiece <= p.k) {
+#pragma unroll
+      for (int y = 0; y < RT; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          __builtin_memcpy(&b[y][i], rows[y] + from + 64 * i + 16 * (lane / 16), 16);
+    } else if (from < p.k) {
+#pragma unroll
+      for (int y = 0; y < RT; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          b[y][i] = load_codes(rows[y], from + 64 * i + 16 * (lane / 16), p.k);
+    }
+  };
+  load_rows(k0);  // they are on their way while the queries are quantized
+  const auto load_query = [&](int at) {
+    const int i = min(lane % 16, m - 1);
+    if constexpr (!kFused) return load_codes(p.q.x + i * p.q.stride, at, p.k);
+    // the codes in LDS end with zeros
+    return at < pitch ? *reinterpret_cast<const i32x4*>(few_lds + i * pitch + at) : i32x4{0, 0, 0, 0};
+  };
   if constexpr (kFused) {
     for (int i = 0; i < m; ++i) {
       const Q* row = floats + i * fstride;
@@ -187,64 +229,33 @@ __global__ __launch_bounds__(64 * KW) void few_scores_kernel(product p, const Q*
       for (int at = threadIdx.x; at < pitch; at += kThreadsHere)
         few_lds[i * pitch + at] =
           at < p.k && scale > 0.f ? static_cast<char>(code_of(static_cast<float>(row[at]), scale)) : char{0};
-      __syncthreads();
+      lds_barrier();
     }
   } else {
     for (int i = threadIdx.x; i < m; i += kThreadsHere)
       qscales[i] = p.q.scales[i];
   }
-  i32x4 acc[RT] = {};
-  const int8_t* rows[RT];
+  for (; k0 < p.k; k0 += KW * kPiece) {
+    i32x4 a[4];
 #pragma unroll
-  for (int y = 0; y < RT; ++y)
-    rows[y] = p.r.x + min(j0 + 16 * y + lane % 16, p.n - 1) * p.r.stride;
-  const auto multiply = [&](int k0, auto load_row, auto load_query) {
-    i32x4 a[4], b[RT][4];
+    for (int i = 0; i < 4; ++i)
+      a[i] = load_query(k0 + 64 * i + 16 * (lane / 16));
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int at = k0 + 64 * s + 16 * (lane / 16);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int y = 0; y < RT; ++y)
-        b[y][s] = load_row(rows[y], at);
-      a[s] = load_query(min(lane % 16, m - 1), at);
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int y = 0; y < RT; ++y)
-        acc[y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b[y][s], acc[y], 0, 0, 0);
-  };
-  const auto whole = [](const int8_t* row, int at) {
-    i32x4 v;
-    __builtin_memcpy(&v, row + at, 16);
-    return v;
-  };
-  const auto partial = [&](const int8_t* row, int at) { return load_codes(row, at, p.k); };
-  const auto coded   = [&](int i, int at) {  // the codes in LDS end with zeros
-    return at < pitch ? *reinterpret_cast<const i32x4*>(few_lds + i * pitch + at) : i32x4{0, 0, 0, 0};
-  };
-  for (int k0 = wave * kPiece; k0 < p.k; k0 += KW * kPiece) {
-    if (k0 + kPiece <= p.k) {
-      if constexpr (kFused)
-        multiply(k0, whole, coded);
-      else
-        multiply(k0, whole, [&](int i, int at) { return whole(p.q.x + i * p.q.stride, at); });
-    } else {
-      if constexpr (kFused)
-        multiply(k0, partial, coded);
-      else
-        multiply(k0, partial, [&](int i, int at) { return partial(p.q.x + i * p.q.stride, at); });
-    }
+        acc[y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], b[y][i], acc[y], 0, 0, 0);
+    load_rows(k0 + KW * kPiece);
   }
   auto* sums = reinterpret_cast<int*>(few_lds);  // [KW][16][RT * 16]
   constexpr int kWide = RT * 16, kAll = 16 * kWide;
-  __syncthreads();
+  lds_barrier();
 #pragma unroll
   for (int y = 0; y < RT; ++y)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       sums[wave * kAll + (4 * (lane / 16) + e) * kWide + 16 * y + lane % 16] = acc[y][e];
-  __syncthreads();
+  lds_barrier();
   for (int e = threadIdx.x; e < m * kWide; e += kThreadsHere) {
     const int i = e / kWide;
     const int64_t j = j0 + e % kWide;
@@ -460,17 +471,23 @@ void with_float(elem type, F f)
 
 }  // namespace
 
-void launch_quantize_rows(const void* x, elem type, int64_t m, int k, int pad, int64_t stride, int8_t* codes,
-                          int64_t cstride, float* scales, hipStream_t s)
+namespace {
+
+/** launch_quantize_rows that also lays out `job` beside its first rows. */
+void launch_quantize(const void* x, elem type, int64_t m, int k, int pad, int64_t stride, int8_t* codes, int64_t cstride,
+                     float* scales, pack_job const& job, hipStream_t s)
 {
-  constexpr int64_t kRows = (int64_t{1} << 32) / kQuantThreads - 1;  // less than 2^32 work-items a grid
+  constexpr int64_t kRows = int64_t{1} << 23;  // with a job's, less than 2^32 work-items a grid
   with_float(type, [&](auto e) {
     using T = decltype(e);
     for (int64_t row0 = 0; row0 < m; row0 += kRows) {
-      const auto rows   = static_cast<unsigned>(std::min(kRows, m - row0));
-      constexpr int N   = kPer16<T>;
-      const auto launch = [&](auto kernel) {
-        kernel<<<rows, kQuantThreads, 0, s>>>(static_cast<const T*>(x), stride, k, pad, codes, cstride, scales, row0);
+      const auto rows      = static_cast<unsigned>(std::min(kRows, m - row0));
+      const pack_job part  = row0 == 0 ? job : pack_job{};
+      const auto blocks    = rows + static_cast<unsigned>((part.n + kPackRows - 1) / kPackRows);
+      constexpr int N      = kPer16<T>;
+      const auto launch    = [&](auto kernel) {
+        kernel<<<blocks, kQuantThreads, 0, s>>>(static_cast<const T*>(x), stride, k, pad, codes, cstride, scales, row0, rows,
+                                                part);
       };
       if (k <= kQuantThreads * N)
         launch(quantize_kernel<T, 1>);
@@ -481,6 +498,14 @@ void launch_quantize_rows(const void* x, elem type, int64_t m, int k, int pad, i
       OCTEX_HIP(hipGetLastError());
     }
   });
+}
+
+}  // namespace
+
+void launch_quantize_rows(const void* x, elem type, int64_t m, int k, int64_t stride, int8_t* codes, int64_t cstride,
+                          float* scales, hipStream_t s)
+{
+  launch_quantize(x, type, m, k, k, stride, codes, cstride, scales, {}, s);
 }
 
 namespace {
@@ -516,9 +541,7 @@ void launch_few(product const& p, const Q* floats, int64_t fstride, hipStream_t 
     kernel<<<static_cast<unsigned>(blocks), 64 * KW, lds, s>>>(p, floats, fstride, pitch);
     OCTEX_HIP(hipGetLastError());
   };
-  if (p.n >= 32768)
-    launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-  else if (p.n >= 8192)
+  if (p.n >= 8192)
     launch(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
   else
     launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
@@ -571,11 +594,14 @@ auto chunked(int8_rows const& r, int k) -> bool
   return k % 16 == 0 && r.stride % 16 == 0 && reinterpret_cast<uintptr_t>(r.x) % 16 == 0 && r.stride <= kMaxInt8Stride;
 }
 
-void launch_pack(const int8_t* x, int64_t stride, int64_t n, int k, int8_t* out, int64_t pitch, hipStream_t s)
+void launch_pack(pack_job const& job, hipStream_t s)
 {
-  const int64_t blocks = (n * ((k + 15) / 16) + kPackThreads - 1) / kPackThreads;
-  pack_kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 20)), kPackThreads, 0, s>>>(x, stride, n, k, out, pitch);
-  OCTEX_HIP(hipGetLastError());
+  constexpr int64_t kRows = kMaxItems / (64 * kPackRows) * kPackRows;
+  for (int64_t first = 0; first < job.n; first += kRows) {
+    const int64_t rows = std::min(kRows, job.n - first);
+    pack_kernel<<<static_cast<unsigned>((rows + kPackRows - 1) / kPackRows), 64 * kPackRows, 0, s>>>(job, first);
+    OCTEX_HIP(hipGetLastError());
+  }
 }
 
 constexpr int kFewQueries      = 16;                  // a matrix instruction's
@@ -635,12 +661,16 @@ void launch_int8_scores(int8_query const& q, int64_t m, int8_rows const& r, int6
       return;
     }
     const int chunks = (k + 15) / 16 * 16;
+    const auto pack  = [&](int64_t j0) {  // of the part of the rows that begins at j0
+      return plan.pack_r ? pack_job{r.x + j0 * r.stride, r.stride, std::min(plan.part, n - j0), k, w + plan.rows, plan.pitch}
+                         : pack_job{};
+    };
     if (floats) {
       auto* scales = reinterpret_cast<float*>(w + plan.scales);
-      launch_quantize_rows(q.x, q.type, m, k, chunks, q.stride, w, plan.pitch, scales, s);
+      launch_quantize(q.x, q.type, m, k, chunks, q.stride, w, plan.pitch, scales, pack(0), s);
       p.q = {w, plan.pitch, scales};
     } else if (plan.pack_q) {
-      launch_pack(p.q.x, p.q.stride, m, k, w, plan.pitch, s);
+      launch_pack({p.q.x, p.q.stride, m, k, w, plan.pitch}, s);
       p.q = {w, plan.pitch, q.scales};
     }
     if (plan.few) {
@@ -652,7 +682,7 @@ void launch_int8_scores(int8_query const& q, int64_t m, int8_rows const& r, int6
       p.n = std::min(plan.part, n - j0);
       p.r = {r.x + j0 * r.stride, r.stride, r.scales + j0};
       if (plan.pack_r) {
-        launch_pack(p.r.x, r.stride, p.n, k, w + plan.rows, plan.pitch, s);
+        if (j0 > 0 || !floats) launch_pack(pack(j0), s);
         p.r.x = w + plan.rows, p.r.stride = plan.pitch;
       }
       p.bias = bias != nullptr ? bias + j0 : nullptr;

@@ -10,10 +10,9 @@ namespace cuvs::neighbors::octex::detail {
 // the products of k values of -128 x -128 stay within an int32 sum
 constexpr int kMaxInt8Width = 131071;
 
-/** codes [m, k] (rows cstride apart) and scales [m] of x [m, k] (rows `stride` apart); columns k .. pad (fewer than 256)
- * are written as 0. */
-void launch_quantize_rows(const void* x, elem type, int64_t m, int k, int pad, int64_t stride, int8_t* codes,
-                          int64_t cstride, float* scales, hipStream_t s);
+/** codes [m, k] (rows cstride apart) and scales [m] of x [m, k] (rows `stride` apart). */
+void launch_quantize_rows(const void* x, elem type, int64_t m, int k, int64_t stride, int8_t* codes, int64_t cstride,
+                          float* scales, hipStream_t s);
 
 /** Bytes from row to row of quantized queries of k values: whole 16-byte chunks, and no multiple of 1024, at which the same
  * columns of many rows meet in few channels of the L2 (8192 x 4096 x 16,384: 510 us in place of 581). */

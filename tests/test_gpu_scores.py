@@ -149,6 +149,28 @@ def test_int8_scores_of_floats(O, m, k, n, dtype):
     close(got, prod, (4 * E + rel) * prod.abs() + floor, "scores of floats")
 
 
+@pytest.mark.parametrize("m,k,n,pad", [
+    (600, 1040, 12345, 0), (2050, 4112, 4100, 0), (1000, 512, 30001, 16), (300, 100, 20001, 0), (70, 1001, 140_000, 0),
+    (40, 999, 3000, 1), (2000, 64, 2000, 0), (130, 16, 70_001, 0), (9, 8192, 9000, 0),
+])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_int8_scores_of_every_tiling(O, m, k, n, pad, dtype):
+    """Products large enough for every tiling, ragged at every edge, rows in place and laid out anew in several parts."""
+    g = torch.Generator("cuda").manual_seed(m + n)
+    q = torch.randint(-128, 128, (m, k + pad), generator=g, dtype=torch.int8, device="cuda")[:, :k]
+    r = torch.randint(-128, 128, (n, k + pad), generator=g, dtype=torch.int8, device="cuda")[:, :k]
+    qs, rs = torch.rand(m, generator=g, device="cuda") * 0.01, torch.rand(n, generator=g, device="cuda") * 0.01
+    bias = torch.randn(n, generator=g, device="cuda")
+    got = O.int8_scores(q, r, rs, query_scales=qs, bias=bias, dtype=dtype)
+    rel, floor = HALF[dtype]
+    for a in range(0, m, 256):
+        prod = torch.mm(q[a : a + 256].double(), r.double().t()) * qs[a : a + 256].double()[:, None] * rs.double()
+        want = prod + bias.double()
+        err = (got[a : a + 256].double() - want).abs()
+        tol = 4 * E * (prod.abs() + bias.double().abs()) + rel * want.abs() + floor
+        assert (err <= tol).all(), f"queries {a}: off by {err.max():.3e}"
+
+
 def test_int8_scores_at_the_ends_of_their_sums(O):
     k = 131071  # the widest rows: sums of -128 x -128 just stay under 2^31
     q = torch.full((2, k), -128, dtype=torch.int8)
@@ -250,6 +272,23 @@ def test_log_probs_of_many_rows(O, m):
     r = O.log_probs(x.cuda(), ids[:, 0].int().cuda(), top=7)
     assert r.log_probs.shape == (m,)
     check_log_probs(r, x, ids, 1.0, 7)
+
+
+@pytest.mark.parametrize("m,n,t", [(129, 20_000, 1), (500, 1200, 2), (2500, 700, 130), (2500, 4096, 3), (2048, 5, 1),
+                                   (1025, 4097, 300)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_log_probs_of_every_grouping(O, m, n, t, dtype):
+    """A wavefront, 256 or 512 threads a row: values, alternatives and gradients."""
+    g = gen(m + n)
+    x = (2 * torch.randn((m, n), generator=g)).to(TYPES[dtype])
+    x[m // 2] = float("-inf")
+    ids = torch.randint(-1, n, (m, t), generator=g)
+    r = O.log_probs(x.cuda(), ids.cuda(), top=20, temperature=1.3)
+    check_log_probs(r, x, ids, 1.3, 20)
+    gl, gh = torch.randn((m, t), generator=g), torch.randn(m, generator=g)
+    want, tol = grad64(x, ids, 1.3, gl, gh)
+    got = O.log_probs_backward(gl.cuda(), gh.cuda(), x.cuda(), ids.cuda(), r.lse, r.entropy, temperature=1.3)
+    close(got, want, gradient_tolerance(want, tol, dtype), "gradient")
 
 
 @pytest.mark.parametrize("n", [40, 1000, 9000, 70000])
@@ -476,6 +515,20 @@ def test_distill_lists(O, m, k):
         assert loss[1] == 0 and (grad[1] == 0).all()
 
 
+@pytest.mark.parametrize("m,n,k,dtype", [
+    (9000, 500, 5, "float32"), (2100, 3000, 20, "bfloat16"), (2100, 1000, 200, "bfloat16"), (1100, 9000, 10, "float16"),
+    (200, 9000, 70, "float32"), (300, 40_001, 10, "bfloat16"), (520, 66_003, 70, "bfloat16"), (513, 33_000, 3, "float32"),
+])
+def test_distill_of_every_grouping(O, m, n, k, dtype):
+    """A wavefront to 1,024 threads a row, and several rows one after another in a workgroup; some rows list nothing."""
+    g = gen(m + n)
+    x = (2 * torch.randn((m, n), generator=g)).to(TYPES[dtype])
+    ids = torch.randint(-1, n, (m, k), generator=g)
+    ids[:: 7] = -1
+    teacher = 2 * torch.randn((m, k), generator=g)
+    check_distill(O, x, ids, teacher, 1.0, (0.5 + torch.rand(m, generator=g)) * (1 if dtype == "float32" else 1024), dtype, 3)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [30, 5000, 140000])
 def test_distill_masks_infinities_and_nan(O, dtype, n):
@@ -624,6 +677,19 @@ def test_rows_beyond_32_bit_offsets(O):
     assert grad[0, n - 1].item() < -4000 and grad[m - 1, n - 1].item() < -4000 and grad[m - 2, 0].item() >= 0
     del x, grad
     torch.cuda.empty_cache()
+
+
+def test_the_example_learns(O):
+    """examples/distill_queries.py: search, scores, distillation and log probabilities together."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "distill_queries.py")
+    spec = importlib.util.spec_from_file_location("distill_queries", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    first, last, before, after = example.main(steps=30, n=5000, quiet=True)
+    assert last < 0.7 * first and after > before
 
 
 # --------------------------------------------------------------------------------------------------------------- refusals
