@@ -815,7 +815,8 @@ __device__ inline void write_shares(listed_part<E> const& l, teacher_sums const&
 /** Writes the gradient of columns [c0, c1).  prepare() gives what a row needs, its list's shares in LDS and, in `some`,
  * whether the gradient is other than 0; it may hold barriers, and runs while the first scores are on their way. */
 template <typename T, bool kEntropy, int NT, typename P>
-__device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, listed_shares const& s, int k, P prepare)
+__device__ inline void write_gradient(const T* row, T* grad, bool by_cache, int c0, int c1, listed_shares const& s, int k,
+                                      P prepare)
 {
   constexpr int N = kPer16<T>, kStep = NT * N;
   const bool tiny = c1 - c0 < N;
@@ -860,7 +861,11 @@ __device__ inline void write_gradient(const T* row, T* grad, int c0, int c1, lis
       for (int i = 0; i < N; ++i)
         v[i] = some ? gradient<kEntropy>(v[i], g) : 0.f;
       if (some) add_shares(v, at, min(w0, last), min(w0 + 64 * N, c1), first, s, k);
-      if (w0 + mine < c1) store16(grad + at, pack16<T>(v));
+      if (w0 + mine >= c1) continue;
+      if (by_cache)
+        store16(grad + at, pack16<T>(v));
+      else
+        store16_nt(grad + at, pack16<T>(v));
     }
   }
 }
@@ -890,7 +895,7 @@ template <typename T, int NT>
 __global__ __launch_bounds__(NT) void log_probs_backward_kernel(score_rows in, listed_ids ids, const float* grad_logp,
                                                                       const float* grad_entropy, const float* lse,
                                                                       const float* entropy, T* grad, int64_t gstride,
-                                                                      row_split split, int64_t row0)
+                                                                      bool by_cache, row_split split, int64_t row0)
 {
   constexpr int E = kEntries<NT>;
   __shared__ listed_shares shares;
@@ -899,7 +904,7 @@ __global__ __launch_bounds__(NT) void log_probs_backward_kernel(score_rows in, l
   const int64_t b = row0 + blockIdx.x, r = b / split.parts;
   const int c0 = static_cast<int>(b - r * split.parts) * split.width, c1 = min(c0 + split.width, in.n);
   const T* row = static_cast<const T*>(in.x) + r * in.stride;
-  write_gradient<T, true, NT>(row, grad + r * gstride, c0, c1, shares, ids.k, [&](bool&) {
+  write_gradient<T, true, NT>(row, grad + r * gstride, by_cache, c0, c1, shares, ids.k, [&](bool&) {
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -929,7 +934,7 @@ __global__ __launch_bounds__(NT) void log_probs_backward_kernel(score_rows in, l
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_backward_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                                     const float* grad_loss, const float* lse, T* grad,
-                                                                    int64_t gstride, row_split split, int64_t row0)
+                                                                    int64_t gstride, bool by_cache, row_split split, int64_t row0)
 {
   constexpr int E = kEntries<NT>;
   __shared__ listed_shares shares;
@@ -940,7 +945,7 @@ __global__ __launch_bounds__(NT) void distill_backward_kernel(score_rows in, lis
   const float a = grad_loss[r] / in.temperature;
   listed_part<E> l;
   read_list<NT>(in, ids, teacher, r, l);
-  write_gradient<T, false, NT>(row, grad + r * gstride, c0, c1, shares, ids.k, [&](bool& some) {
+  write_gradient<T, false, NT>(row, grad + r * gstride, by_cache, c0, c1, shares, ids.k, [&](bool& some) {
     const run list = join_block<NT>(teacher_run(l), kLog2e, parts);
     const auto t   = teacher_of(list);
     some           = t.some;
@@ -1088,7 +1093,10 @@ auto forward_split_of(int64_t m, int n, int top) -> row_split
   return split_of(m, n, std::min(kMaxParts, 4 * kThreads / std::max(top, 1)));
 }
 
-constexpr int64_t kCachedBytes = int64_t{128} << 20;  // of a gradient that the last-level cache may keep for its reader
+/** Whether a gradient is stored through the caches: one of up to half of the last-level cache's 256 MB, that its reader may
+ * find there.  A larger one would drive out the logits that a forward pass has left there (4096 x 32,000
+ * bfloat16, both directions of log_probs: 139 us in place of 165). */
+auto passes_cache(score_rows const& in) -> bool { return in.m * in.n * elem_size(in.type) <= int64_t{128} << 20; }
 
 /** Rows of few columns take a wavefront each where there are enough of them. */
 auto by_wavefront(int64_t m, int n, int k) -> bool { return m >= 2048 && n <= 4096 && k <= kShortList; }
@@ -1140,8 +1148,8 @@ void launch_log_probs_backward(score_rows const& in, listed_ids const& ids, cons
     using T           = decltype(e);
     const auto launch = [&](auto kernel, int threads) {
       for_grids(in.m * split.parts, threads, [&](int64_t first, unsigned count) {
-        kernel<<<count, threads, 0, s>>>(in, ids, grad_logp, grad_entropy, lse, entropy, static_cast<T*>(grad), gstride, split,
-                                         first);
+        kernel<<<count, threads, 0, s>>>(in, ids, grad_logp, grad_entropy, lse, entropy, static_cast<T*>(grad), gstride,
+                                         passes_cache(in), split, first);
         OCTEX_HIP(hipGetLastError());
       });
     };
@@ -1184,7 +1192,8 @@ void launch_distill_backward(score_rows const& in, listed_ids const& ids, teache
     using T           = decltype(e);
     const auto launch = [&](auto kernel, int threads) {
       for_grids(in.m * split.parts, threads, [&](int64_t first, unsigned count) {
-        kernel<<<count, threads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride, split, first);
+        kernel<<<count, threads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride, passes_cache(in), split,
+                                         first);
         OCTEX_HIP(hipGetLastError());
       });
     };
@@ -1215,11 +1224,10 @@ void launch_distill_step(score_rows const& in, listed_ids const& ids, teacher_lo
     return;
   }
   with_type(in.type, [&](auto e) {
-    using T             = decltype(e);
-    const bool by_cache = in.m * in.n * static_cast<int64_t>(sizeof(T)) <= kCachedBytes;
-    const auto launch   = [&](auto kernel, int threads, int64_t slots) {
+    using T           = decltype(e);
+    const auto launch = [&](auto kernel, int threads, int64_t slots) {
       kernel<<<static_cast<unsigned>(std::min(in.m, slots)), threads, 0, s>>>(in, ids, teacher, grad_loss, loss, lse,
-                                                                              static_cast<T*>(grad), gstride, by_cache);
+                                                                              static_cast<T*>(grad), gstride, passes_cache(in));
       OCTEX_HIP(hipGetLastError());
     };
     const int pieces = (in.n + kPer16<T> - 1) / kPer16<T>;

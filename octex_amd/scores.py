@@ -224,6 +224,8 @@ def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtyp
         dtype = np.dtype(dtype).name if isinstance(dtype, type) else str(dtype).replace("torch.", "")
     if dtype not in FLOATS:
         raise ValueError(f"octex: scores are of type {', '.join(FLOATS)}, not {dtype}")
+    if dtype == "bfloat16" and c.on_host and not isinstance(queries, c.torch.Tensor):
+        raise TypeError("octex: numpy has no bfloat16 for the scores of its queries")
     out = c.new((m, n), dtype=getattr(c.torch, dtype))
     c.run_sized("octexInt8Scores", c.matrix(q), query_scales.data_ptr() if coded else None, c.matrix(rows),
                 row_scales.data_ptr(), None if bias is None else bias.data_ptr(), c.matrix(out))
