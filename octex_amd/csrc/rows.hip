@@ -25,8 +25,11 @@ constexpr float kLn2   = 0.693147180559945309417f;
 constexpr float kFloor = -200.f;  // an exponent whose power of two is 0; keeps 0 * -inf out of the sums
 constexpr int kThreads = 256;
 constexpr int kWaves   = kThreads / 64;
-constexpr int kList    = 256;   // a wavefront's candidate keys: four a lane
-constexpr int kFull    = 128;   // keys from which a list is compacted
+constexpr int kList    = 256;  // a wavefront's candidate keys: four a lane
+constexpr int kFull    = 128;  // keys from which a list is compacted
+/** New keys of a call that are listed column by column; more of them are quicker one of every lane at a time.  2048 x 128,000
+ * bfloat16, top 20: 117 us (all one a lane: 135); 8000 x 1000 float32: 18 us (all column by column: 20). */
+constexpr int kSparse = 8;
 
 __device__ inline auto exp2_fast(float v) -> float { return __builtin_amdgcn_exp2f(v); }
 
@@ -253,6 +256,22 @@ struct top_list {
   __device__ void add(const float (&v)[N], float cm, int at)
   {
     if (__ballot(cm >= low) == 0) return;
+    key64 reach[N];
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      reach[i] = __ballot(v[i] >= low);
+      count += __popcll(reach[i]);
+    }
+    if (count <= kSparse && n + count <= kFull) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (reach[i] == 0) continue;
+        if (v[i] >= low) list[n + lanes_below(reach[i])] = {static_cast<unsigned>(at + i), v[i]};
+        n += __popcll(reach[i]);
+      }
+      return;
+    }
     unsigned left = 0;  // of this lane's scores
 #pragma unroll
     for (int i = 0; i < N; ++i)
