@@ -8,6 +8,9 @@
 // One pass over a row holds, a thread, the running maximum m, s = sum 2^u and t = sum 2^u u with u = (x - m) log2(e) / T:
 // then l = m / T + ln s and H = ln s - ln 2 t / s, a difference of small numbers.  All sums are fp32, in a fixed order.
 // A row without a finite score has p = 0 everywhere: l = -inf, H = 0, log p = -inf.  A NaN or +inf makes its row NaN.
+//
+// All of it is bound by the logits' bytes: a large copy takes 4.77 TB/s of this GPU, a kernel that only reads up to 5.5.
+// The times below are a launch's among others of its kind; "TB/s" counts the logits, and a gradient, once.
 
 #include "common.hpp"
 #include "elems_device.hpp"
@@ -141,6 +144,10 @@ __device__ inline auto log_prob(float x, row_sums const& o, float temperature) -
 }
 
 // ---- the top entries: a wavefront's list of keys (order of the value, ~column), compacted when it fills
+//
+// A score is compared with a floor that only grows, so that the pass costs one comparison a score and a few entries: the
+// first floor is one that k of the workgroup's threads reach with their first scores, and later ones come from a full list.
+// Floors are found bit by bit from counts of the lanes that reach them, without sorting; only the last 64 keys are ranked.
 
 using key64 = unsigned long long;
 
@@ -212,7 +219,8 @@ struct entry {
 
 __device__ inline auto lanes_below(key64 lanes) -> int
 {
-  return __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(lanes >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(lanes), 0));
+  return __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(lanes >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(lanes), 0));
 }
 
 struct top_list {
@@ -530,8 +538,13 @@ __device__ inline void write_top(score_rows const& in, log_probs_out const& out,
   }
 }
 
-/** A workgroup a row, or with kSplit a workgroup a part of a row, which leaves its sums and its best keys (0: none) to
- * finish_log_probs_kernel. */
+/**
+ * A workgroup a row, or with kSplit a workgroup a part of a row, which leaves its sums and its best keys (0: none) to
+ * finish_log_probs_kernel.  One pass: a thread has 64 bytes on their way while it adds and lists 64 others.
+ *
+ * 4096 x 128,000 bfloat16: 191 us, 5.5 TB/s; with the 20 best 214 us, 4.9 TB/s, the first floors and the lists' ends being
+ * what is not hidden (2048 rows: 98 and 120).  1 x 128,000, in two launches: 6.5 us, with the 20 best 12.
+ */
 template <typename T, int NT, bool kTop, bool kSplit>
 __global__ __launch_bounds__(NT) void log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
                                                              row_split split, part_sums* part, key64* best, int64_t row0)
@@ -705,7 +718,8 @@ __device__ inline void join_both(run& sums, float c, run& t, run* both)
 }
 
 /** A pass over rows, a workgroup each, or with kSplit a workgroup a part of a row, which leaves its sums to
- * finish_distill_kernel. */
+ * finish_distill_kernel.  The list's q needs no pass of its own: its logits are a few registers of the threads, and its sums
+ * are joined at the row's barrier.  4096 x 128,000 bfloat16 with 64 ids a row: 189 us, 5.5 TB/s. */
 template <typename T, int NT, bool kSplit>
 __global__ __launch_bounds__(NT) void distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                      float* loss, float* lse, row_split split, part_sums* part,
@@ -797,19 +811,42 @@ __device__ inline auto share_at(listed_shares const& s, int j, int k) -> listed_
   return j < k ? listed_share{s.id[j], s.w[j]} : listed_share{-1, 0.f};
 }
 
-/** Adds the shares of the list's ids to the gradients v of columns at + i, in the list's order; the wavefront's columns lie
- * in [lo, hi).  first is the lane's of the first 64 entries. */
-template <int N>
-__device__ inline void add_shares(float (&v)[N], int at, int lo, int hi, listed_share first, listed_shares const& s, int k)
+/**
+ * Adds the shares of the list's ids to the gradients v of columns at + i, in the list's order; the wavefront's columns are
+ * the 64 * N from w0 (a multiple of N) on that lie below end, and a lane whose own would pass the end has those from `last`
+ * on.  first is the lane's of the first 64 entries.  So every gradient is stored once, by one thread, with no atomics: an id
+ * that is listed twice gets the same sum in every run.
+ *
+ * A wavefront that has the whole list to itself (kAlone) meets many entries at a time: it takes them by their place among a
+ * lane's columns, which is the same for all lanes but where some were moved back, at one addition each instead of N.
+ * 8000 x 1000 float32 with 64 ids, distill's gradient: 23 us against 26; but 4096 x 128,000 bfloat16 in both directions,
+ * where most pieces meet none, 467 against 455.
+ */
+template <bool kAlone, int N>
+__device__ inline void add_shares(float (&v)[N], int at, int w0, int last, int end, listed_share first, listed_shares const& s,
+                                  int k)
 {
+  const int lane = static_cast<int>(threadIdx.x % 64), lo = min(w0, last), hi = min(w0 + 64 * N, end);
   for (int q = 0; q < k; q += 64) {
-    const listed_share mine = q == 0 ? first : share_at(s, q + static_cast<int>(threadIdx.x % 64), k);
-    for (key64 in = __ballot(mine.id >= lo && mine.id < hi); in != 0; in &= in - 1) {
-      const int i = __builtin_ctzll(in), column = __builtin_amdgcn_readlane(mine.id, i) - at;
-      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine.w), i));
+    const listed_share mine = q == 0 ? first : share_at(s, q + lane, k);
+    const key64 all         = __ballot(mine.id >= lo && mine.id < hi);
+    if (all == 0) continue;
+    if (kAlone && w0 + 64 * N <= end) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        v[e] += column == e ? w : 0.f;
+        for (key64 in = all & __ballot(mine.id % N == e); in != 0; in &= in - 1) {
+          const int i = __builtin_ctzll(in), owner = (__builtin_amdgcn_readlane(mine.id, i) - w0) / N;
+          const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine.w), i));
+          v[e] += lane == owner ? w : 0.f;
+        }
+    } else {
+      for (key64 in = all; in != 0; in &= in - 1) {
+        const int i = __builtin_ctzll(in), column = __builtin_amdgcn_readlane(mine.id, i) - at;
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine.w), i));
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          v[e] += column == e ? w : 0.f;
+      }
     }
   }
 }
@@ -827,8 +864,9 @@ __device__ inline void write_shares(listed_part<E> const& l, teacher_sums const&
   }
 }
 
-/** Writes the gradient of columns [c0, c1).  prepare() gives what a row needs, its list's shares in LDS and, in `some`,
- * whether the gradient is other than 0; it may hold barriers, and runs while the first scores are on their way. */
+/** Writes the gradient of columns [c0, c1), a thread 64 bytes while the next 64 are on their way.  prepare() gives what a
+ * row needs, its list's shares in LDS and, in `some`, whether the gradient is other than 0; it may hold barriers, and runs
+ * while the first scores are on their way. */
 template <typename T, bool kEntropy, int NT, typename P>
 __device__ inline void write_gradient(const T* row, T* grad, bool by_cache, int c0, int c1, listed_shares const& s, int k,
                                       P prepare)
@@ -846,12 +884,12 @@ __device__ inline void write_gradient(const T* row, T* grad, bool by_cache, int 
   }
   bool some            = true;
   const gradient_row g = prepare(some);
-  const listed_share first    = share_at(s, static_cast<int>(threadIdx.x % 64), k);
+  const listed_share first = share_at(s, static_cast<int>(threadIdx.x % 64), k);
   if (tiny) {
     const int at = c0 + static_cast<int>(threadIdx.x);
     float v[1]   = {0.f};
     if (at < c1 && some) v[0] = gradient<kEntropy>(static_cast<float>(row[at]), g);
-    if (some) add_shares(v, at, c0, c1, first, s, k);
+    if (some) add_shares<NT == 64>(v, at, c0, c0, c1, first, s, k);
     if (at < c1) grad[at] = static_cast<T>(v[0]);
     return;
   }
@@ -875,7 +913,7 @@ __device__ inline void write_gradient(const T* row, T* grad, bool by_cache, int 
 #pragma unroll
       for (int i = 0; i < N; ++i)
         v[i] = some ? gradient<kEntropy>(v[i], g) : 0.f;
-      if (some) add_shares(v, at, min(w0, last), min(w0 + 64 * N, c1), first, s, k);
+      if (some) add_shares<NT == 64>(v, at, w0, last, c1, first, s, k);
       if (w0 + mine >= c1) continue;
       if (by_cache)
         store16(grad + at, pack16<T>(v));
@@ -906,6 +944,8 @@ __device__ inline auto gradient_base(const T* row, int n, float lse, float tempe
   return g;
 }
 
+/** A workgroup a row or a part of one: A and B of the row from its list and its saved sums, then one pass.  4096 x 128,000
+ * bfloat16: 418 us, 5.0 TB/s; 4096 x 32,000, its logits still in the last-level cache: 82 us, 6.4 TB/s. */
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void log_probs_backward_kernel(score_rows in, listed_ids ids, const float* grad_logp,
                                                                       const float* grad_entropy, const float* lse,
@@ -946,10 +986,13 @@ __global__ __launch_bounds__(NT) void log_probs_backward_kernel(score_rows in, l
   });
 }
 
+/** The same for distill, whose q are made again from the teacher's logits: 4096 x 128,000 bfloat16 with 64 ids a row 418 us,
+ * 5.0 TB/s. */
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_backward_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                                     const float* grad_loss, const float* lse, T* grad,
-                                                                    int64_t gstride, bool by_cache, row_split split, int64_t row0)
+                                                                    int64_t gstride, bool by_cache, row_split split,
+                                                                    int64_t row0)
 {
   constexpr int E = kEntries<NT>;
   __shared__ listed_shares shares;
@@ -977,6 +1020,9 @@ __global__ __launch_bounds__(NT) void distill_backward_kernel(score_rows in, lis
  * gradient written once.  A workgroup takes every gridDim-th row; as a piece of a row's gradient is stored, the same piece
  * of its next row is loaded in its place, and pieces that have arrived enter that row's sums, so that reads, writes and
  * arithmetic go on side by side.  The next row's list comes meanwhile, E entries a thread.
+ *
+ * 4096 x 128,000 bfloat16 with 64 ids a row: 456 us, 4.6 TB/s, against 607 by two passes; what it lacks to a copy's 440 is
+ * the join between a row's last load and its gradient's first store, when this workgroup has nothing on its way.
  */
 template <typename T, int NT, int H>
 __global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
@@ -1048,7 +1094,7 @@ __global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_
 #pragma unroll
         for (int i = 0; i < N; ++i)
           v[i] = t.some ? gradient<false>(v[i], g) : 0.f;
-        if (t.some) add_shares(v, at, min(w0, last), min(w0 + 64 * N, in.n), first, shares, ids.k);
+        if (t.some) add_shares<NT == 64>(v, at, w0, last, in.n, first, shares, ids.k);
         if (h * kStep + mine < in.n) {
           if (by_cache)
             store16(out + at, pack16<T>(v));
@@ -1085,12 +1131,11 @@ void for_grids(int64_t total, int threads, F f)
     f(first, static_cast<unsigned>(std::min(most, total - first)));
 }
 
-constexpr int kEnough    = 1024;  // workgroups of 256 threads that fill the GPU
-constexpr int kMinWidth  = 4096;  // columns of a part
-constexpr int kMaxParts  = 32;    // of a row
-constexpr int kFewRows   = 128;   // rows whose forward pass is split: more fill the GPU well enough to spare the second kernel
-
-constexpr int kMidRows   = 512;   // rows whose top entries take 512 threads (333 x 50,021 float32: 25.7 us, of 256 threads 28.2)
+constexpr int kEnough   = 1024;  // workgroups of 256 threads that fill the GPU
+constexpr int kMinWidth = 4096;  // columns of a part
+constexpr int kMaxParts = 32;    // of a row
+constexpr int kFewRows  = 128;   // rows whose forward pass is split: more fill the GPU well enough to spare the second kernel
+constexpr int kMidRows  = 512;   // rows whose top entries take 512 threads (333 x 50,021 float32: 25.7 us, by 256 28.2)
 
 /** Rows are split into parts of whole 16-byte pieces while they are fewer than the workgroups that fill the GPU. */
 auto split_of(int64_t m, int n, int64_t most = kMaxParts) -> row_split
@@ -1207,8 +1252,8 @@ void launch_distill_backward(score_rows const& in, listed_ids const& ids, teache
     using T           = decltype(e);
     const auto launch = [&](auto kernel, int threads) {
       for_grids(in.m * split.parts, threads, [&](int64_t first, unsigned count) {
-        kernel<<<count, threads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride, passes_cache(in), split,
-                                         first);
+        kernel<<<count, threads, 0, s>>>(in, ids, teacher, grad_loss, lse, static_cast<T*>(grad), gstride, passes_cache(in),
+                                         split, first);
         OCTEX_HIP(hipGetLastError());
       });
     };
@@ -1221,8 +1266,8 @@ void launch_distill_backward(score_rows const& in, listed_ids const& ids, teache
 
 constexpr int kHeldThreads = 1024, kHeldPieces = 16;  // of the widest row that a workgroup holds
 
-/** Few wide rows are quicker in parts, by two passes: 1 x 128,000 bfloat16 in 14 us against 27 (but 16 x 32,000 float32 in 13
- * either way), 333 x 50,021 float32 in 37 against 41, 1000 x 100,003 float16 in 135 against 102. */
+/** Few wide rows are quicker in parts, by two passes: 1 x 128,000 bfloat16 in 10.7 us against 24, 300 x 100,003 float16 in 42
+ * against 47 (but 16 x 32,000 float32 in 11.5 against 10.6, 768 x 128,000 bfloat16 in 97 against 81). */
 auto distill_step_held(int64_t m, int n, elem type) -> bool
 {
   const int per = 16 / elem_size(type), pieces = (n + per - 1) / per;
