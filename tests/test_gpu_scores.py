@@ -309,6 +309,18 @@ def test_top_of_equal_and_sorted_scores(O, n, dtype):
         check_log_probs(O.log_probs(x.cuda(), ids.cuda(), top=top), x, ids, 1.0, top)
 
 
+@pytest.mark.parametrize("m,n", [(2100, 1000), (2100, 4001), (600, 9000), (300, 9000)])
+def test_top_of_equal_and_sorted_scores_of_every_grouping(O, m, n):
+    g = gen(m + n)
+    x = torch.randint(0, 3, (m, n), generator=g).float()
+    x[::4] = torch.arange(n) / n * 50
+    x[1::4] = -torch.arange(n) / n * 50
+    x[2::8] = 0
+    ids = torch.zeros((m, 1), dtype=torch.int64)
+    for top in (3, 64):
+        check_log_probs(O.log_probs(x.cuda(), ids.cuda(), top=top), x, ids, 1.0, top)
+
+
 @pytest.mark.parametrize("n", [5, 77, 1030, 40000])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_masks_infinities_and_nan(O, n, dtype):
@@ -525,6 +537,19 @@ def test_distill_of_every_grouping(O, m, n, k, dtype):
     x = (2 * torch.randn((m, n), generator=g)).to(TYPES[dtype])
     ids = torch.randint(-1, n, (m, k), generator=g)
     ids[:: 7] = -1
+    teacher = 2 * torch.randn((m, k), generator=g)
+    check_distill(O, x, ids, teacher, 1.0, (0.5 + torch.rand(m, generator=g)) * (1 if dtype == "float32" else 1024), dtype, 3)
+
+
+@pytest.mark.parametrize("m,n,k", [(2100, 1000, 128), (2051, 523, 65), (2048, 4096, 100), (2100, 70, 64), (300, 2000, 512)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_of_dense_lists(O, m, n, k, dtype):
+    """Many listed ids in every piece of a row, most of them more than once."""
+    g = gen(m + n + k)
+    x = (2 * torch.randn((m, n), generator=g)).to(TYPES[dtype])
+    ids = torch.randint(0, min(n, 2 * k), (m, k), generator=g) * torch.tensor(max(1, n // (2 * k)))
+    ids[::5] = torch.randint(n - min(n, 40), n, ids[::5].shape, generator=g)
+    ids[::9, ::3] = -1
     teacher = 2 * torch.randn((m, k), generator=g)
     check_distill(O, x, ids, teacher, 1.0, (0.5 + torch.rand(m, generator=g)) * (1 if dtype == "float32" else 1024), dtype, 3)
 
