@@ -84,7 +84,7 @@ __device__ inline void store16_nt(T* p, uint4 raw)
   __builtin_nontemporal_store(words{raw.x, raw.y, raw.z, raw.w}, reinterpret_cast<words*>(p));
 }
 
-/** Elements [at, at + kPer16) of a row as they lie in memory, those from `end` on -inf. */
+/** Elements [at, at + kPer16) of a row as they lie in memory, those from `end` on 0. */
 template <typename T>
 __device__ inline auto load_row16(const T* row, int at, int end) -> uint4
 {
@@ -92,7 +92,7 @@ __device__ inline auto load_row16(const T* row, int at, int end) -> uint4
   T e[kPer16<T>];
 #pragma unroll
   for (int i = 0; i < kPer16<T>; ++i)
-    e[i] = at + i < end ? row[at + i] : static_cast<T>(-INFINITY);
+    e[i] = at + i < end ? row[at + i] : static_cast<T>(0.f);
   uint4 raw;
   __builtin_memcpy(&raw, e, 16);
   return raw;

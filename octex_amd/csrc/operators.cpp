@@ -77,7 +77,8 @@ auto elem_of(octexMatrix const& m) -> elem { return static_cast<elem>(m.type); }
 void shape(const octexMatrix* m, const char* what, int64_t rows, int64_t cols)
 {
   OCTEX_EXPECTS(m != nullptr, "octex: %s is NULL", what);
-  OCTEX_EXPECTS(m->rows >= 0 && m->cols >= 0 && m->stride >= m->cols, "octex: %s has a negative size or rows that overlap", what);
+  OCTEX_EXPECTS(m->rows >= 0 && m->cols >= 0 && m->stride >= m->cols, "octex: %s has a negative size or rows that overlap",
+                what);
   OCTEX_EXPECTS((rows < 0 || m->rows == rows) && (cols < 0 || m->cols == cols),
                 "octex: %s is [%lld, %lld], expected [%lld, %lld]", what, static_cast<long long>(m->rows),
                 static_cast<long long>(m->cols), static_cast<long long>(rows < 0 ? m->rows : rows),

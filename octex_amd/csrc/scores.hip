@@ -19,29 +19,49 @@ using i32x16 = int __attribute__((ext_vector_type(16)));
 
 constexpr int kQuantThreads = 256;
 
-__device__ inline auto code_of(float v, float scale) -> int
-{
-  return static_cast<int>(fminf(fmaxf(rintf(v / scale), -127.f), 127.f));
-}
-
 /** A magnitude's bits, which order as it does, with infinity and NaN above every finite one. */
 __device__ inline auto magnitude(float v) -> unsigned { return __float_as_uint(v) & 0x7fffffffu; }
 
 __device__ inline auto scale_of(unsigned top) -> float { return top < 0x7f800000u ? __uint_as_float(top) / 127.f : NAN; }
 
+/**
+ * The codes of v: v / scale, rounded to fp32, then to a whole number.  The product with 1 / scale is at most 3 units in the
+ * last place from the quotient, 2.3e-5 where it is below 128, and rounds alike unless it lies as near to the middle of two
+ * whole numbers: then, or if 1 / scale is no finite number, the divisions are made.  8192 x 4096 bfloat16: 23.5 us, with all
+ * divided 29.
+ */
 template <int N>
-__device__ inline void codes_of(const float (&v)[N], float scale, int8_t (&c)[N])
+__device__ inline void codes_of(const float (&v)[N], float scale, float inverse, int8_t (&c)[N])
 {
+  float code[N], far = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float q = v[i] * inverse;
+    code[i]       = rintf(q);
+    far           = fmaxf(far, fabsf(q - code[i]));
+  }
+  if (!(inverse < INFINITY && far < 0.5f - 3e-5f)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      code[i] = scale > 0.f ? fminf(fmaxf(rintf(v[i] / scale), -127.f), 127.f) : 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    c[i] = scale > 0.f ? static_cast<int8_t>(code_of(v[i], scale)) : int8_t{0};
+    c[i] = static_cast<int8_t>(static_cast<int>(code[i]));
+}
+
+template <int W>
+__device__ inline auto max_lanes(unsigned top) -> unsigned
+{
+#pragma unroll
+  for (int mask = W / 2; mask > 0; mask >>= 1)
+    top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), mask)));
+  return top;
 }
 
 __device__ inline auto block_max(unsigned top, unsigned* parts) -> unsigned
 {
-#pragma unroll
-  for (int mask = 32; mask > 0; mask >>= 1)
-    top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), mask)));
+  top = max_lanes<64>(top);
   if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = top;
   lds_barrier();
   for (int w = 0; w < static_cast<int>(blockDim.x) / 64; ++w)
@@ -110,48 +130,54 @@ __global__ __launch_bounds__(64 * kPackRows) void pack_kernel(pack_job p, int64_
  * scale = max |x| / 127; code = the whole number nearest to x / scale (ties to even), the quotient rounded to fp32 first.
  * A row of zeros has scale 0 and codes 0; one with a NaN or an infinity has scale NaN and codes 0.
  *
- * A workgroup holds a row of up to kHeld * 256 values in registers between the maximum and the codes, so that it is read
- * once; longer rows are read again.  Columns k .. pad are written as 0.  Workgroups past the rows' lay out `job`.
+ * kLanes threads hold a row of up to kHeld * kLanes 16-byte pieces in registers between the maximum and the codes, so that it
+ * is read once; longer rows are read again.  Columns k .. pad are written as 0.  Workgroups past the rows' lay out `job`.
+ * Bound by the rows' bytes: 100,000 x 960 float32 takes 86 us, 5.6 TB/s.
  */
-template <typename T, int kHeld>
+template <typename T, int kLanes, int kHeld>
 __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T* x, int64_t stride, int k, int pad, int8_t* codes,
-                                                                 int64_t cstride, float* scales, int64_t row0,
-                                                                 unsigned rows, pack_job job)
+                                                                 int64_t cstride, float* scales, int64_t row0, int64_t rows,
+                                                                 unsigned blocks, pack_job job)
 {
-  constexpr int N = kPer16<T>, kStep = kQuantThreads * N;
+  constexpr int N = kPer16<T>, kStep = kLanes * N;
   static_assert(kQuantThreads == 64 * kPackRows);
   __shared__ unsigned parts[kQuantThreads / 64];
-  if (blockIdx.x >= rows) {
-    pack_rows(job, int64_t{blockIdx.x - rows} * kPackRows);
+  if (blockIdx.x >= blocks) {
+    pack_rows(job, int64_t{blockIdx.x - blocks} * kPackRows);
     return;
   }
-  const int64_t r = row0 + blockIdx.x;
-  const T* row    = x + r * stride;
-  int8_t* out     = codes + r * cstride;
-  const int mine  = threadIdx.x * N;
+  const int64_t r = row0 + int64_t{blockIdx.x} * (kQuantThreads / kLanes) + threadIdx.x / kLanes;
+  const int lane  = threadIdx.x % kLanes, mine = lane * N;
+  if (kLanes <= 64 && r >= row0 + rows) return;
+  const T* row = x + r * stride;
+  int8_t* out  = codes + r * cstride;
   uint4 held[kHeld];
   float v[N];
   unsigned top = 0;
 #pragma unroll
   for (int u = 0; u < kHeld; ++u)
     if (u * kStep + mine < k) held[u] = load_row16(row, u * kStep + mine, k);
-  const auto take = [&](uint4 raw, int at) {
+  const auto take = [&](uint4 raw) {  // 0 past the row
     unpack16<T>(raw, v);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (at + i < k) top = max(top, magnitude(v[i]));
+      top = max(top, magnitude(v[i]));
   };
 #pragma unroll
   for (int u = 0; u < kHeld; ++u)
-    if (u * kStep + mine < k) take(held[u], u * kStep + mine);
+    if (u * kStep + mine < k) take(held[u]);
   for (int at = kHeld * kStep + mine; at < k; at += kStep)
-    take(load_row16(row, at, k), at);
-  const float scale = scale_of(block_max(top, parts));
-  if (threadIdx.x == 0) scales[r] = scale;
+    take(load_row16(row, at, k));
+  if constexpr (kLanes <= 64)
+    top = max_lanes<kLanes>(top);
+  else
+    top = block_max(top, parts);
+  const float scale = scale_of(top), inverse = 1.f / scale;
+  if (lane == 0) scales[r] = scale;
   const auto give = [&](uint4 raw, int at) {
     unpack16<T>(raw, v);
     int8_t c[N];
-    codes_of(v, scale, c);
+    codes_of(v, scale, inverse, c);
     if (at + N <= k) {
       __builtin_memcpy(out + at, c, N);
     } else {
@@ -165,7 +191,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const T* x, int
     if (u * kStep + mine < k) give(held[u], u * kStep + mine);
   for (int at = kHeld * kStep + mine; at < k; at += kStep)
     give(load_row16(row, at, k), at);
-  if (static_cast<int>(threadIdx.x) < pad - k) out[k + threadIdx.x] = 0;
+  if (lane < pad - k) out[k + lane] = 0;
 }
 
 // ---- the product
@@ -180,6 +206,9 @@ constexpr int kPiece = 256;  // bytes of a row that a wavefront multiplies at a 
  * A workgroup scores RT * 16 rows for up to 16 queries; its KW wavefronts share the columns out and their sums meet in
  * LDS.  A matrix instruction takes 64 columns of 16 rows and 16 queries, so a lane loads 16 bytes of a row, and four such
  * loads cover whole 128-byte lines.  With kFused the queries are floats: the workgroup quantizes them into LDS first.
+ *
+ * Bound by the rows' bytes: 1 x 1024 x 32,000 (queries, values, rows) takes 6.9 us, 4.7 TB/s; 16 x 4096 x 100,000 98 us,
+ * 4.2 TB/s.
  */
 template <int RT, int KW, bool kFused, typename Q, typename O>
 __global__ __launch_bounds__(64 * KW) void few_scores_kernel(product p, const Q* floats, int64_t fstride, int pitch)
@@ -224,11 +253,14 @@ __global__ __launch_bounds__(64 * KW) void few_scores_kernel(product p, const Q*
       unsigned top = 0;
       for (int at = threadIdx.x; at < p.k; at += kThreadsHere)
         top = max(top, magnitude(static_cast<float>(row[at])));
-      const float scale = scale_of(block_max(top, parts));
+      const float scale = scale_of(block_max(top, parts)), inverse = 1.f / scale;
       if (threadIdx.x == 0) qscales[i] = scale;
-      for (int at = threadIdx.x; at < pitch; at += kThreadsHere)
-        few_lds[i * pitch + at] =
-          at < p.k && scale > 0.f ? static_cast<char>(code_of(static_cast<float>(row[at]), scale)) : char{0};
+      for (int at = threadIdx.x; at < pitch; at += kThreadsHere) {
+        const float v[1] = {at < p.k ? static_cast<float>(row[at]) : 0.f};
+        int8_t c[1];
+        codes_of(v, scale, inverse, c);
+        few_lds[i * pitch + at] = static_cast<char>(c[0]);
+      }
       lds_barrier();
     }
   } else {
@@ -302,6 +334,18 @@ __device__ inline void wait_loads()
   asm volatile("" ::: "memory");
 }
 
+/**
+ * WM x WN wavefronts score TM x TN parts of 32 x 32 each, kStep values of the rows at a time, with kAhead steps on their way
+ * from memory to LDS, which the loads fill without passing by registers.  Of a step, the next 32 values' operands are read
+ * from LDS while the matrix cores multiply these; the loads are spread over the step, one or two a matrix instruction, and
+ * wait for each other only by count, so that a barrier a step is all that stalls.
+ *
+ * Bound by the matrix cores and the power that they draw: 8192 x 4096 x 16,384 takes 525 us, 2090 TOP/s, with scales,
+ * rounding and all (a library's bare product 498 us; this loop alone, from registers, 3000 to 3300 TOP/s).  A part of 4 x 2
+ * asks LDS for 3/4 of its bandwidth, one of 2 x 2 for all of it: that is why 256 x 128 tiles reach 1920 TOP/s and 256 x 256
+ * ones 2400.  Where few values are summed the results' bytes count as much: 1000 x 960 x 100,000 takes 150 us, 1280 TOP/s
+ * and 1.9 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 22.5 us, 4.6 TB/s.
+ */
 template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
 __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, tile_order order)
 {
@@ -370,7 +414,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, t
         __builtin_amdgcn_s_barrier();
         read(after, 0, a[1 - now], b[1 - now]);
       }
-      constexpr int kMfma = TM * TN, kReads = TM + TN, kEach = (kLoads + kParts - 2) / (kParts - 1);  // the last part loads none
+      constexpr int kMfma = TM * TN, kReads = TM + TN;
+      constexpr int kEach = (kLoads + kParts - 2) / (kParts - 1);  // the last part loads none
       constexpr int kLoadsEach = (kEach + kMfma - 1) / kMfma, kReadsEach = (kReads + kMfma - 1) / kMfma;
 #pragma unroll
       for (int x = 0; x < TM; ++x)
@@ -419,9 +464,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, t
       for (int e4 = 0; e4 < 4; ++e4) {
         const int j     = 32 * y + 8 * e4 + 4 * (lane / 32);
         const float4 rs = *reinterpret_cast<const float4*>(scales + wj + j);
-        float f[4]      = {static_cast<float>(acc[x][y][4 * e4]) * qs * rs.x, static_cast<float>(acc[x][y][4 * e4 + 1]) * qs * rs.y,
-                           static_cast<float>(acc[x][y][4 * e4 + 2]) * qs * rs.z,
-                           static_cast<float>(acc[x][y][4 * e4 + 3]) * qs * rs.w};
+        const auto sum  = [&](int e) { return static_cast<float>(acc[x][y][4 * e4 + e]) * qs; };
+        float f[4]      = {sum(0) * rs.x, sum(1) * rs.y, sum(2) * rs.z, sum(3) * rs.w};
         if (p.bias != nullptr) {
           const float4 bs = *reinterpret_cast<const float4*>(biases + wj + j);
           f[0] += bs.x, f[1] += bs.y, f[2] += bs.z, f[3] += bs.w;
@@ -430,7 +474,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, t
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           v[e] = static_cast<O>(f[e]);
-        __builtin_memcpy(__builtin_assume_aligned(mine + (lane % 32) * kPitch + j * static_cast<int>(sizeof(O)), 8), v, sizeof(v));
+        char* at = mine + (lane % 32) * kPitch + j * static_cast<int>(sizeof(O));
+        __builtin_memcpy(__builtin_assume_aligned(at, 8), v, sizeof(v));
       }
     wave_fence();
     constexpr int kPieces = kWide / N;  // of a row
@@ -481,20 +526,22 @@ void launch_quantize(const void* x, elem type, int64_t m, int k, int pad, int64_
   with_float(type, [&](auto e) {
     using T = decltype(e);
     for (int64_t row0 = 0; row0 < m; row0 += kRows) {
-      const auto rows      = static_cast<unsigned>(std::min(kRows, m - row0));
-      const pack_job part  = row0 == 0 ? job : pack_job{};
-      const auto blocks    = rows + static_cast<unsigned>((part.n + kPackRows - 1) / kPackRows);
-      constexpr int N      = kPer16<T>;
-      const auto launch    = [&](auto kernel) {
-        kernel<<<blocks, kQuantThreads, 0, s>>>(static_cast<const T*>(x), stride, k, pad, codes, cstride, scales, row0, rows,
-                                                part);
+      const auto rows     = std::min(kRows, m - row0);
+      const pack_job part = row0 == 0 ? job : pack_job{};
+      constexpr int N     = kPer16<T>;
+      const auto launch   = [&](auto kernel, int lanes) {
+        const int64_t blocks = (rows * lanes + kQuantThreads - 1) / kQuantThreads;
+        kernel<<<static_cast<unsigned>(blocks + (part.n + kPackRows - 1) / kPackRows), kQuantThreads, 0, s>>>(
+          static_cast<const T*>(x), stride, k, pad, codes, cstride, scales, row0, rows, static_cast<unsigned>(blocks), part);
       };
-      if (k <= kQuantThreads * N)
-        launch(quantize_kernel<T, 1>);
+      if (k <= 2 * 16 * N)  // 100,000 x 128 float32: 14.5 us, by 256 threads a row 82
+        launch(quantize_kernel<T, 16, 2>, 16);
+      else if (k <= 4 * 64 * N)  // 100,000 x 960 float32: 89 us, by 256 threads a row 134
+        launch(quantize_kernel<T, 64, 4>, 64);
       else if (k <= 2 * kQuantThreads * N)
-        launch(quantize_kernel<T, 2>);
+        launch(quantize_kernel<T, kQuantThreads, 2>, kQuantThreads);
       else
-        launch(quantize_kernel<T, 8>);
+        launch(quantize_kernel<T, kQuantThreads, 8>, kQuantThreads);
       OCTEX_HIP(hipGetLastError());
     }
   });
@@ -530,7 +577,7 @@ void launch_tiled(product const& p, hipStream_t s)
 template <typename Q, bool kFused, typename O>
 void launch_few(product const& p, const Q* floats, int64_t fstride, hipStream_t s)
 {
-  const int pitch = (p.k + 15) / 16 * 16 + ((p.k + 15) / 16 % 2 == 0 ? 16 : 0);  // an odd number of chunks: rows on other banks
+  const int chunks = (p.k + 15) / 16, pitch = 16 * (chunks | 1);  // an odd number of chunks: rows on other banks
   const auto launch = [&](auto rt, auto kw) {
     constexpr int RT = decltype(rt)::value, KW = decltype(kw)::value;
     const auto kernel = few_scores_kernel<RT, KW, kFused, Q, O>;
@@ -605,7 +652,7 @@ void launch_pack(pack_job const& job, hipStream_t s)
 }
 
 constexpr int kFewQueries      = 16;                  // a matrix instruction's
-constexpr int64_t kFewRows     = 8192;                // whose tiles would leave half of the GPU idle (1 x 4096 x 5000: 12.2 us, not 7.2)
+constexpr int64_t kFewRows     = 8192;                // tiles leave half of the GPU idle (1 x 4096 x 5000: 12.2 us, not 7.2)
 constexpr int kFewFused        = 8192;                // values up to which each workgroup quantizes all queries itself
 constexpr int64_t kPackedBytes = int64_t{128} << 20;  // of rows laid out anew at a time: they stay in the last-level cache
 
