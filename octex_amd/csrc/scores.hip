@@ -340,11 +340,11 @@ __device__ inline void wait_loads()
  * from LDS while the matrix cores multiply these; the loads are spread over the step, one or two a matrix instruction, and
  * wait for each other only by count, so that a barrier a step is all that stalls.
  *
- * Bound by the matrix cores and the power that they draw: 8192 x 4096 x 16,384 takes 525 us, 2090 TOP/s, with scales,
- * rounding and all (a library's bare product 498 us; this loop alone, from registers, 3000 to 3300 TOP/s).  A part of 4 x 2
- * asks LDS for 3/4 of its bandwidth, one of 2 x 2 for all of it: that is why 256 x 128 tiles reach 1920 TOP/s and 256 x 256
- * ones 2400.  Where few values are summed the results' bytes count as much: 1000 x 960 x 100,000 takes 150 us, 1280 TOP/s
- * and 1.9 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 22.5 us, 4.6 TB/s.
+ * Bound by the matrix cores and the power that they draw: 8192 x 4096 x 16,384 takes 522 us, 2110 TOP/s, with scales,
+ * rounding and all (a library's bare product 498 us; the matrix instructions alone 3000 to 3300 TOP/s).  A part of 4 x 2 asks
+ * LDS for 3/4 of its bandwidth, one of 2 x 2 for all of it, which holds 256 x 128 tiles back.  Where few values are summed
+ * the results' bytes count as much: 1000 x 960 x 100,000 takes 159 us, 1210 TOP/s and 1.9 TB/s.  Few queries are bound by
+ * the rows: 24 x 2048 x 50,000 28 us, 3.7 TB/s.
  */
 template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
 __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, tile_order order)
@@ -595,21 +595,24 @@ void launch_few(product const& p, const Q* floats, int64_t fstride, hipStream_t 
 }
 
 /**
- * The tilings, and what each was measured to take: `a` us a column and c us for one tile by itself; with all of its slots
- * (workgroups on the GPU at a time) busy, `rate` operations a us and e us to store a round's results.  Larger tiles load
- * each operand fewer times and smaller ones fill the GPU with less, so a product takes the tiling whose estimate is least
- * (us, of 256 x 256, 256 x 128, 128 x 128 and 64 x 64):
- *   1000 x 960 x 100,000: 161, 146, 180, 262;  4096 x 4096 x 4096: 66, 78, 90, 117;  2048 x 2048 x 2048: 27, 20, 16, 20;
- *   333 x 1008 x 5003: 19, 12, 11, 8.5;  128 x 4096 x 8192: 50, 29, 22, 15.
+ * The tilings, and what each takes: `a` us a column and c us for one tile by itself; with all of its slots (workgroups on the
+ * GPU at a time) busy, `rate` operations a us and e us to store a round's results.  Larger tiles load each operand fewer
+ * times and smaller ones fill the GPU with less, so a product takes the tiling whose estimate is least.  The numbers are
+ * fitted to the times of 21 products whose rows come from memory, and choose a tiling within 4 % of the best for each (us,
+ * of 256 x 256, 256 x 128, 128 x 128 and 64 x 64):
+ *   1000 x 960 x 100,000: 159, 178, 220, 291;  512 x 512 x 200,000: 127, 105, 136, 186;  4096 x 4096 x 4096: 68, 81, 95, 120;
+ *   2048 x 2048 x 2048: 27, 19, 16, 20;  333 x 1008 x 5003: 20, 12, 11, 9.4;  128 x 4096 x 8192: 43, 28, 22, 14.
+ * 256 x 256 tiles have two steps of 64 on their way: with one of 128 the first of these products takes 171 us, 8192 x 4096 x
+ * 16,384 539 in place of 522 (but 4096 x 4096 x 4096 65 in place of 68); with three of 64 160, 530 and 69.
  */
 struct tiling {
   int bm, bn, slots;
   double c, a, rate, e;
 };
-constexpr tiling kTilings[] = {{256, 256, 256, 8.6, 0.0080, 2.40e9, 10.0},
-                               {256, 128, 512, 6.9, 0.0044, 1.92e9, 5.0},
-                               {128, 128, 512, 6.3, 0.0035, 1.75e9, 5.2},
-                               {64, 64, 768, 3.4, 0.0019, 1.65e9, 4.2}};
+constexpr tiling kTilings[] = {{256, 256, 256, 8.0, 0.0100, 2.24e9, 10.5},
+                               {256, 128, 512, 5.8, 0.0068, 1.48e9, 5.4},
+                               {128, 128, 512, 6.2, 0.0044, 1.50e9, 5.7},
+                               {64, 64, 768, 4.5, 0.0023, 1.07e9, 2.6}};
 
 auto estimate(tiling const& t, product const& p) -> double
 {
@@ -626,7 +629,7 @@ void launch_best(product const& p, hipStream_t s)
   for (int i = 1; i < 4; ++i)
     if (estimate(kTilings[i], p) < estimate(kTilings[best], p)) best = i;
   if (best == 0)
-    launch_tiled<2, 4, 4, 2, 128, 1, O>(p, s);
+    launch_tiled<2, 4, 4, 2, 64, 2, O>(p, s);
   else if (best == 1)
     launch_tiled<4, 2, 2, 2, 64, 2, O>(p, s);
   else if (best == 2)
