@@ -344,7 +344,7 @@ __device__ inline void wait_loads()
  * rounding and all (a library's bare product 498 us; the matrix instructions alone 3000 to 3300 TOP/s).  A part of 4 x 2 asks
  * LDS for 3/4 of its bandwidth, one of 2 x 2 for all of it, which holds 256 x 128 tiles back.  Where few values are summed
  * the results' bytes count as much: 1000 x 960 x 100,000 takes 159 us, 1210 TOP/s and 1.9 TB/s.  Few queries are bound by
- * the rows: 24 x 2048 x 50,000 28 us, 3.7 TB/s.
+ * the rows: 24 x 2048 x 50,000 23.6 us, 4.4 TB/s.
  */
 template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
 __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, tile_order order)
@@ -598,8 +598,8 @@ void launch_few(product const& p, const Q* floats, int64_t fstride, hipStream_t 
  * The tilings, and what each takes: `a` us a column and c us for one tile by itself; with all of its slots (workgroups on the
  * GPU at a time) busy, `rate` operations a us and e us to store a round's results.  Larger tiles load each operand fewer
  * times and smaller ones fill the GPU with less, so a product takes the tiling whose estimate is least.  The numbers are
- * fitted to the times of 21 products whose rows come from memory, and choose a tiling within 4 % of the best for each (us,
- * of 256 x 256, 256 x 128, 128 x 128 and 64 x 64):
+ * fitted to the times of 21 products whose rows come from memory, and choose the best tiling for these and 5 others (us, of
+ * 256 x 256, 256 x 128, 128 x 128 and 64 x 64):
  *   1000 x 960 x 100,000: 159, 178, 220, 291;  512 x 512 x 200,000: 127, 105, 136, 186;  4096 x 4096 x 4096: 68, 81, 95, 120;
  *   2048 x 2048 x 2048: 27, 19, 16, 20;  333 x 1008 x 5003: 20, 12, 11, 9.4;  128 x 4096 x 8192: 43, 28, 22, 14.
  * 256 x 256 tiles have two steps of 64 on their way: with one of 128 the first of these products takes 171 us, 8192 x 4096 x
@@ -614,6 +614,10 @@ constexpr tiling kTilings[] = {{256, 256, 256, 8.0, 0.0100, 2.24e9, 10.5},
                                {128, 128, 512, 6.2, 0.0044, 1.50e9, 5.7},
                                {64, 64, 768, 4.5, 0.0023, 1.07e9, 2.6}};
 
+/** Queries that take tiles of 32 x 128, which hold fewer zeros: 24 x 2048 x 50,000 23.6 us, by 64 x 64 28 (but 32 x 4096 x
+ * 100,000 102 against 98). */
+constexpr int64_t kThinQueries = 32;
+
 auto estimate(tiling const& t, product const& p) -> double
 {
   const double tiles  = static_cast<double>((p.m + t.bm - 1) / t.bm) * static_cast<double>((p.n + t.bn - 1) / t.bn);
@@ -625,6 +629,7 @@ auto estimate(tiling const& t, product const& p) -> double
 template <typename O>
 void launch_best(product const& p, hipStream_t s)
 {
+  if (p.m <= kThinQueries) return launch_tiled<1, 4, 1, 1, 128, 2, O>(p, s);
   int best = 0;
   for (int i = 1; i < 4; ++i)
     if (estimate(kTilings[i], p) < estimate(kTilings[best], p)) best = i;

@@ -83,6 +83,21 @@ def test_quantize_rows(O, dtype, m, k, pad):
     assert torch.equal(codes.cpu(), want) and torch.equal(scales.cpu(), ws)
 
 
+@pytest.mark.parametrize("k", [15, 31, 127, 128, 129, 255, 256, 257, 1023, 1025, 2047, 2048, 2049, 4095, 4097, 8193])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_rows_of_every_width(O, dtype, k):
+    """Rows that 16, 64 or 256 threads hold, and quotients at and beside the middle of two whole numbers."""
+    g = gen(k)
+    x = torch.randn((37, k), generator=g) * torch.logspace(-30, 3, 37)[:, None].clamp(min=1e-3 if dtype == "float16" else 0)
+    x[::3] = torch.randint(-254, 255, x[::3].shape, generator=g) / 2  # halves: a scale of 1 where 127 is among them
+    x[::3, 0] = 127
+    x[5] = 0
+    x = x.to(TYPES[dtype])
+    codes, scales = O.quantize_rows(padded(x, 1))
+    want, ws = codes_of(x)
+    assert torch.equal(codes.cpu(), want) and torch.equal(scales.cpu(), ws)
+
+
 def test_quantize_extremes(O):
     top = torch.finfo(torch.float32).max
     x = torch.zeros((7, 33))
@@ -169,6 +184,12 @@ def test_int8_scores_of_every_tiling(O, m, k, n, pad, dtype):
         err = (got[a : a + 256].double() - want).abs()
         tol = 4 * E * (prod.abs() + bias.double().abs()) + rel * want.abs() + floor
         assert (err <= tol).all(), f"queries {a}: off by {err.max():.3e}"
+
+
+@pytest.mark.parametrize("m,k,n", [(17, 960, 20_001), (32, 128, 8257), (3, 4112, 9001), (16, 64, 70_003), (33, 80, 9000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_int8_scores_of_thin_batches(O, m, k, n, dtype):
+    test_int8_scores_of_every_tiling(O, m, k, n, 0, dtype)
 
 
 def test_int8_scores_at_the_ends_of_their_sums(O):
