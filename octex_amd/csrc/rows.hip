@@ -1134,7 +1134,6 @@ void for_grids(int64_t total, int threads, F f)
 constexpr int kEnough   = 1024;  // workgroups of 256 threads that fill the GPU
 constexpr int kMinWidth = 4096;  // columns of a part
 constexpr int kMaxParts = 32;    // of a row
-constexpr int kFewRows  = 128;   // rows whose forward pass is split: more fill the GPU well enough to spare the second kernel
 constexpr int kMidRows  = 512;   // rows whose top entries take 512 threads (333 x 50,021 float32: 25.7 us, by 256 28.2)
 
 /** Rows are split into parts of whole 16-byte pieces while they are fewer than the workgroups that fill the GPU. */
@@ -1146,10 +1145,16 @@ auto split_of(int64_t m, int n, int64_t most = kMaxParts) -> row_split
   return {(n + width - 1) / width, width};
 }
 
+/** Up to kFewRows rows of kWideRow columns or more are split in a forward pass, at a second launch (and a workspace, 4 us of
+ * a caller's time): 16 x 128,000 bfloat16 in 6.5 us against 16.4 whole, with the 20 best 13.8 against 25; 128 rows in 14
+ * against 17.5, but 256 in 19 either way and with the 20 best in 31 against 27; 16 x 32,000 in 5.7 against 6.3, with the 20
+ * best 13.0 against 11.8. */
+constexpr int kFewRows = 128, kWideRow = 65536;
+
 /** Of a forward pass, whose parts' best entries are at most four a thread of the kernel that joins them. */
 auto forward_split_of(int64_t m, int n, int top) -> row_split
 {
-  if (m > kFewRows) return {1, n};
+  if (m > kFewRows || n < kWideRow) return {1, n};
   return split_of(m, n, std::min(kMaxParts, 4 * kThreads / std::max(top, 1)));
 }
 
