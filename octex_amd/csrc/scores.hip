@@ -338,14 +338,13 @@ __device__ inline void wait_loads()
  * WM x WN wavefronts score TM x TN parts of 32 x 32 each, kStep values of the rows at a time, with kAhead steps on their way
  * from memory to LDS, which the loads fill without passing by registers.  Of a step, the next 32 values' operands are read
  * from LDS while the matrix cores multiply these; the loads are spread over the step, one or two a matrix instruction, and
- * wait for each other only by count, so that a barrier a step is all that stalls.
+ * are waited for by count, at the step's one barrier.
  *
  * Bound by power, as far as it is by one thing: 8192 x 4096 x 16,384 takes 510 us, 2150 TOP/s, with scales, rounding and all
  * (a library's bare product 498 us), the clock falls to 1.7 GHz and the matrix cores are busy for 62 % of its cycles; matrix
  * instructions alone reach 3000 to 3300 TOP/s.  A part of 4 x 2 reads 3/4 of what two of 2 x 2 read from LDS, and 256 x 256
- * tiles load 2/3 of what 256 x 128 ones do.  Where few values are summed
- * the results' bytes count as much: 1000 x 960 x 100,000 takes 159 us, 1210 TOP/s and 1.9 TB/s.  Few queries are bound by
- * the rows: 24 x 2048 x 50,000 23.6 us, 4.4 TB/s.
+ * tiles load 2/3 of what 256 x 128 ones do.  Where few values are summed the results' bytes count as much: 1000 x 960 x
+ * 100,000 takes 159 us, 1210 TOP/s and 1.9 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 23.6 us, 4.4 TB/s.
  */
 template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
 __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, tile_order order)

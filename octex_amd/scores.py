@@ -9,7 +9,8 @@
 Every operator is a hand-written kernel and takes matrices whose rows may lie apart (a slice of a padded vocabulary's
 columns, say).  Operands in GPU memory are read in place: the work is ordered on their stream (torch's current stream, or
 the one their framework names) and not waited for.  Host operands are copied to the GPU and results come back as the
-first operand is.  Types that an operator does not take are converted, as for a search.
+first operand is.  Types that an operator does not take are converted, as for a search.  Results carry no autograd graph:
+the gradients have calls of their own.
 """
 
 import collections
@@ -268,7 +269,7 @@ def log_probs(logits, ids, *, top=0, temperature=1.0):
     t, shape = _ids(c, ids, m)
     logp, entropy, lse, top_logp = c.new(shape, (m,), (m,), (m, top))
     top_ids = c.new((m, top), dtype=c.torch.int64)
-    c.run_sized("octexLogProbs", c.matrix(x), c.matrix(t), temperature, top, logp.data_ptr(), entropy.data_ptr(),
+    c.run_sized("octexLogProbs", c.matrix(x), c.matrix(t), float(temperature), top, logp.data_ptr(), entropy.data_ptr(),
                 lse.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
     return LogProbs(c.give(logp), c.give(entropy), c.give(lse), c.give(top_logp), c.give(top_ids))
 
@@ -287,7 +288,7 @@ def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, 
     gh = None if grad_entropy is None else c.dense(grad_entropy, "grad_entropy", (m,))
     lse, entropy = c.dense(lse, "lse", (m,)), c.dense(entropy, "entropy", (m,))
     grad = c.new(x.shape, dtype=x.dtype)
-    c.run("octexLogProbsBackward", c.matrix(x), c.matrix(t), temperature, None if gl is None else gl.data_ptr(),
+    c.run("octexLogProbsBackward", c.matrix(x), c.matrix(t), float(temperature), None if gl is None else gl.data_ptr(),
           None if gh is None else gh.data_ptr(), lse.data_ptr(), entropy.data_ptr(), c.matrix(grad))
     return c.give(grad)
 
@@ -310,7 +311,8 @@ def distill(logits, ids, teacher, *, temperature=1.0):
     c, x, t, teacher = _teacher(logits, ids, teacher)
     m = x.shape[0]
     loss, lse = c.new((m,), (m,))
-    c.run_sized("octexDistill", c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, loss.data_ptr(), lse.data_ptr())
+    c.run_sized("octexDistill", c.matrix(x), c.matrix(t), c.matrix(teacher), float(temperature), loss.data_ptr(),
+                lse.data_ptr())
     return c.give(loss), c.give(lse)
 
 
@@ -323,8 +325,8 @@ def distill_backward(grad_loss, logits, ids, teacher, lse, *, temperature=1.0):
     m = x.shape[0]
     g, lse = c.dense(grad_loss, "grad_loss", (m,)), c.dense(lse, "lse", (m,))
     grad = c.new(x.shape, dtype=x.dtype)
-    c.run("octexDistillBackward", c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, g.data_ptr(), lse.data_ptr(),
-          c.matrix(grad))
+    c.run("octexDistillBackward", c.matrix(x), c.matrix(t), c.matrix(teacher), float(temperature), g.data_ptr(),
+          lse.data_ptr(), c.matrix(grad))
     return c.give(grad)
 
 
@@ -334,6 +336,6 @@ def distill_step(grad_loss, logits, ids, teacher, *, temperature=1.0):
     m = x.shape[0]
     g = c.dense(grad_loss, "grad_loss", (m,))
     (loss, lse), grad = c.new((m,), (m,)), c.new(x.shape, dtype=x.dtype)
-    c.run_sized("octexDistillStep", c.matrix(x), c.matrix(t), c.matrix(teacher), temperature, g.data_ptr(), loss.data_ptr(),
-                lse.data_ptr(), c.matrix(grad))
+    c.run_sized("octexDistillStep", c.matrix(x), c.matrix(t), c.matrix(teacher), float(temperature), g.data_ptr(),
+                loss.data_ptr(), lse.data_ptr(), c.matrix(grad))
     return c.give(loss), c.give(grad)

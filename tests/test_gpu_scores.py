@@ -641,6 +641,14 @@ def test_operands_of_other_kinds(O):
     assert np.array_equal(y, O.int8_scores(x.cuda(), torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda()).cpu().numpy())
 
 
+def test_scalars_of_any_kind(O):
+    x, ids = torch.randn((3, 50)).cuda(), torch.zeros((3, 1), dtype=torch.int64).cuda()
+    want = O.log_probs(x, ids, top=2, temperature=2.0)
+    for two in (2, np.float32(2), np.int64(2), torch.tensor(2.0)):
+        r = O.log_probs(x, ids, top=np.int32(2), temperature=two)
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 def test_no_rows(O):
     x, ids = torch.zeros((0, 50)).cuda(), torch.zeros((0, 3), dtype=torch.int64).cuda()
     r = O.log_probs(x, ids, top=4)
@@ -721,6 +729,45 @@ def test_rows_beyond_32_bit_offsets(O):
     loss, grad = O.distill_step(torch.full((m,), 4096.0, device="cuda"), x, ids, torch.zeros((m, 1), device="cuda"))
     assert abs(loss[0].item() - (lse - 3)) < 1e-3
     assert grad[0, n - 1].item() < -4000 and grad[m - 1, n - 1].item() < -4000 and grad[m - 2, 0].item() >= 0
+    del x, grad
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("m,k", [(1, 2048), (20, 2048), (300, 2048), (2000, 2048), (20, 2047)])
+def test_scores_beyond_32_bit_offsets(O, m, k):
+    """Rows of more than 2^32 bytes, and (of 2000 queries) more than 2^32 scores."""
+    n = 2_200_000
+    rows = torch.zeros((n, k), dtype=torch.int8, device="cuda")
+    rows[-1], rows[n // 2] = 1, 2
+    rs = torch.ones(n, device="cuda")
+    q = torch.ones((m, k), dtype=torch.int8, device="cuda")
+    q[-1] = 3
+    s = O.int8_scores(q, rows, rs, query_scales=torch.full((m,), 2.0**-8, device="cuda"), dtype="float16")
+    want = torch.zeros(n, dtype=torch.float16, device="cuda")
+    want[-1], want[n // 2] = k / 256, 2 * k / 256
+    assert torch.equal(s[-1], 3 * want)
+    for i in (0, m // 2) if m > 1 else ():
+        assert torch.equal(s[i], want)
+    del rows, s
+    torch.cuda.empty_cache()
+
+
+def test_quantized_rows_and_gradients_beyond_32_bit_offsets(O):
+    x = torch.zeros((2_200_000, 2048), dtype=torch.float16, device="cuda")
+    x[-1, 5], x[-1, 6], x[1_100_000] = 127, -3, 2
+    codes, scales = O.quantize_rows(x)
+    assert codes[-1, 5] == 127 and codes[-1, 6] == -3 and (codes[1_100_000] == 127).all() and scales[-1] == 1
+    assert scales[-2] == 0 and (codes[-2] == 0).all()
+    del x, codes
+    m, n = 36_000, 120_000  # a workgroup holds a row
+    x = torch.zeros((m, n), dtype=torch.float16, device="cuda")
+    ids = torch.full((m, 1), n - 1, device="cuda")
+    loss, grad = O.distill_step(torch.full((m,), 4096.0, device="cuda"), x, ids, torch.zeros((m, 1), device="cuda"))
+    want = torch.full((n,), 4096 / n, device="cuda")
+    want[-1] -= 4096
+    for i in (0, m // 2, m - 1):
+        assert abs(loss[i].item() - math.log(n)) < 1e-3
+        assert torch.allclose(grad[i].float(), want, rtol=2e-3)
     del x, grad
     torch.cuda.empty_cache()
 
