@@ -80,8 +80,7 @@ struct product {
 
 __device__ inline auto score_of(int sum, float qs, product const& p, int64_t j) -> float
 {
-  const float v = static_cast<float>(sum) * qs * p.r.scales[j];
-  return p.bias != nullptr ? v + p.bias[j] : v;
+  return fmaf(static_cast<float>(sum) * qs, p.r.scales[j], p.bias != nullptr ? p.bias[j] : -0.f);
 }
 
 /** 16 values of a row at column at, those from k on 0. */
@@ -347,7 +346,8 @@ __device__ inline void wait_loads()
  * 100,000 takes 159 us, 1210 TOP/s and 1.9 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 23.6 us, 4.4 TB/s.
  */
 template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
-__global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, tile_order order)
+__global__ __launch_bounds__(64 * WM * WN, (160 << 10) / ((kAhead + 1) * (WM * TM + WN * TN) * 32 * kStep) * WM * WN / 4)
+void tiled_scores_kernel(product p, tile_order order)  // registers for as many workgroups as LDS has place for
 {
   constexpr int kWavesHere = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int kChunks    = kStep / 16, kRows = 64 / kChunks;        // of a row; rows that a load of a wavefront covers
@@ -442,51 +442,56 @@ __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, t
   // 32 queries of the wavefront's at a time, so that a row of the output is stored in 16-byte pieces side by side
   constexpr int kThreadsHere = 64 * kWavesHere, kWide = TN * 32, N = kPer16<O>;
   constexpr int kPitch       = kWide * static_cast<int>(sizeof(O)) + 16;
-  auto* scales               = reinterpret_cast<float*>(lds);  // of the tile's rows, then their biases
-  auto* biases               = scales + BN;
+  constexpr int kPieces = kWide / N, kAtOnce = 64 / kPieces;  // of a row; rows that a store of the wavefront covers
+  auto* scales = reinterpret_cast<float*>(lds);  // of the tile's rows, then their biases
+  auto* biases = scales + BN;
   // results of whole 64-byte pieces pass by the caches: the 200 MB of 1,000 x 960 x 100,000 in float16 then take 161 us in
   // place of 177, where pieces at odd places lose (2048 x 512 x 50,000: 110 us against 86)
   const bool by_cache = (reinterpret_cast<uintptr_t>(p.out) | p.ostride * sizeof(O)) % 64 != 0;
-  char* mine                 = lds + 2 * BN * sizeof(float) + wave * 32 * kPitch;
+  char* mine          = lds + 2 * BN * sizeof(float) + wave * 32 * kPitch;
   wait_loads<0, true>();  // the steps past the last, which load zeros
   __syncthreads();
   for (int j = threadIdx.x; j < BN; j += kThreadsHere) {
     scales[j] = j < nj ? p.r.scales[j0 + j] : 0.f;
-    if (p.bias != nullptr) biases[j] = j < nj ? p.bias[j0 + j] : 0.f;
+    biases[j] = j < nj && p.bias != nullptr ? p.bias[j0 + j] : -0.f;
   }
+  float qs[TM];
+#pragma unroll
+  for (int x = 0; x < TM; ++x)
+    qs[x] = p.q.scales[i0 + min(wi + 32 * x + lane % 32, mi - 1)];
   __syncthreads();
+  const auto of_rows = [&](const float* from, int y, int e4) {
+    return *reinterpret_cast<const float4*>(from + wj + 32 * y + 8 * e4 + 4 * (lane / 32));
+  };
+  constexpr bool kHeld = TM > 2;  // where registers are left for them
+  float4 rs[TN][4], bs[TN][4];
+#pragma unroll
+  for (int y = 0; y < TN; ++y)
+#pragma unroll
+    for (int e4 = 0; kHeld && e4 < 4; ++e4)
+      rs[y][e4] = of_rows(scales, y, e4), bs[y][e4] = of_rows(biases, y, e4);
+  const int io = wi + lane / kPieces, jo = wj + lane % kPieces * N, left = nj - jo;
+  O* to        = static_cast<O*>(p.out) + (i0 + io) * p.ostride + j0 + jo;
 #pragma unroll
   for (int x = 0; x < TM; ++x) {
-    const float qs = p.q.scales[i0 + min(wi + 32 * x + lane % 32, mi - 1)];
 #pragma unroll
     for (int y = 0; y < TN; ++y)
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
-        const int j     = 32 * y + 8 * e4 + 4 * (lane / 32);
-        const float4 rs = *reinterpret_cast<const float4*>(scales + wj + j);
-        const auto sum  = [&](int e) { return static_cast<float>(acc[x][y][4 * e4 + e]) * qs; };
-        float f[4]      = {sum(0) * rs.x, sum(1) * rs.y, sum(2) * rs.z, sum(3) * rs.w};
-        if (p.bias != nullptr) {
-          const float4 bs = *reinterpret_cast<const float4*>(biases + wj + j);
-          f[0] += bs.x, f[1] += bs.y, f[2] += bs.z, f[3] += bs.w;
-        }
-        O v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = static_cast<O>(f[e]);
-        char* at = mine + (lane % 32) * kPitch + j * static_cast<int>(sizeof(O));
+        const float4 r = kHeld ? rs[y][e4] : of_rows(scales, y, e4), d = kHeld ? bs[y][e4] : of_rows(biases, y, e4);
+        const auto sum = [&](int e) { return static_cast<float>(acc[x][y][4 * e4 + e]) * qs[x]; };
+        const O v[4]   = {static_cast<O>(fmaf(sum(0), r.x, d.x)), static_cast<O>(fmaf(sum(1), r.y, d.y)),
+                          static_cast<O>(fmaf(sum(2), r.z, d.z)), static_cast<O>(fmaf(sum(3), r.w, d.w))};
+        char* at       = mine + (lane % 32) * kPitch + (32 * y + 8 * e4 + 4 * (lane / 32)) * static_cast<int>(sizeof(O));
         __builtin_memcpy(__builtin_assume_aligned(at, 8), v, sizeof(v));
       }
     wave_fence();
-    constexpr int kPieces = kWide / N;  // of a row
-#pragma unroll 4
-    for (int u = 0; u < 32 * kPieces / 64; ++u) {
-      const int e = u * 64 + lane, row = e / kPieces, piece = e % kPieces;
-      const int io = wi + 32 * x + row, jo = wj + piece * N;
-      uint4 raw = *reinterpret_cast<const uint4*>(mine + row * kPitch + piece * 16);
-      if (io >= mi || jo >= nj) continue;
-      O* at = static_cast<O*>(p.out) + (i0 + io) * p.ostride + j0 + jo;
-      if (jo + N <= nj) {
+#pragma unroll
+    for (int u = 0; u < 32 / kAtOnce; ++u) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(mine + (u * kAtOnce + lane / kPieces) * kPitch + lane % kPieces * 16);
+      if (io + 32 * x + u * kAtOnce >= mi || left <= 0) continue;
+      O* at = to + (32 * x + u * kAtOnce) * p.ostride;
+      if (left >= N) {
         if (by_cache)
           store16(at, raw);
         else
@@ -496,7 +501,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tiled_scores_kernel(product p, t
         __builtin_memcpy(part, &raw, 16);
 #pragma unroll
         for (int q = 0; q < N - 1; ++q)
-          if (q < nj - jo) at[q] = part[q];
+          if (q < left) at[q] = part[q];
       }
     }
     wave_fence();
