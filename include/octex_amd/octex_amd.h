@@ -225,9 +225,9 @@ typedef struct {
   int64_t rows, cols, stride;
 } octexMatrix;
 
-/** codes [m, k] (int8) and scales [m] (float32, dense) of x [m, k] (float32, float16 or bfloat16): scale = max |x| / 127,
- * code = the whole number nearest to x / scale, ties to even, the quotient rounded to float32 first.  A row of zeros has
- * scale 0; one with a NaN or an infinity has scale NaN and codes 0. */
+/** codes [m, k] (int8) and scales [m] (float32, dense) of x [m, k] (float32, float16 or bfloat16): scale = max |x| / 127 (the
+ * float32 product with 1 / 127), code = the whole number nearest to x / scale, ties to even, the quotient rounded to float32
+ * first.  A row of zeros has scale 0; one with a NaN or an infinity has scale NaN and codes 0. */
 cuvsError_t octexQuantizeRows(const octexMatrix* x, const octexMatrix* codes, float* scales, void* stream);
 
 /** out [m, n] (float32, float16 or bfloat16) of queries [m, k] and rows [n, k] (int8), k at most 131071:

@@ -187,7 +187,8 @@ class _Call:
 
 def quantize_rows(x):
     """(codes, scales) of the rows of x [m, k] in 8 bits: scale = max |x| / 127, code = the whole number nearest to
-    x / scale (ties to even), so that x is about codes * scales[:, None].
+    x / scale (ties to even), as torch's x.abs().amax(1) / 127 and division have them on the GPU: x is about
+    codes * scales[:, None].
 
     A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN, which makes all its scores NaN.
     """

@@ -66,7 +66,7 @@ def padded(t, pad, fill=7.0):
 def codes_of(x):
     """The definition: 32-bit scale and quotients, whole numbers by ties to even."""
     x = x.float().numpy()
-    scale = (np.abs(x).max(1) / np.float32(127)).astype(np.float32)
+    scale = np.abs(x).max(1) * (np.float32(1) / np.float32(127))  # as torch's division by a number on the GPU
     safe = np.where(scale > 0, scale, np.float32(1)).astype(np.float32)
     c = np.clip(np.rint((x / safe[:, None]).astype(np.float32)), -127, 127)
     return torch.from_numpy(np.where(scale[:, None] > 0, c, 0).astype(np.int8)), torch.from_numpy(scale)
