@@ -348,7 +348,7 @@ __device__ inline void wait_loads()
  * (a library's bare product 498 us), the clock falls to 1.7 GHz and the matrix cores are busy for 62 % of its cycles; matrix
  * instructions alone reach 3000 to 3300 TOP/s.  A part of 4 x 2 reads 3/4 of what two of 2 x 2 read from LDS, and 256 x 256
  * tiles load 2/3 of what 256 x 128 ones do.  Where few values are summed the results' bytes count as much: 1000 x 960 x
- * 100,000 takes 159 us, 1210 TOP/s and 1.9 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 23.6 us, 4.4 TB/s.
+ * 100,000 takes 154 us, 1250 TOP/s and 1.9 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 23.6 us, 4.4 TB/s.
  */
 template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
 __global__ __launch_bounds__(64 * WM * WN, (160 << 10) / ((kAhead + 1) * (WM * TM + WN * TN) * 32 * kStep) * WM * WN / 4)
