@@ -7,7 +7,7 @@ only features of the query and learns, from the search's neighbors and distances
     loss, g  = octex.distill_step(weights, scores, neighbors, -distances / 2)          # q over the neighbors, p over all rows
     r        = octex.log_probs(scores, ids of the nearest rows, top=5)                 # how sure it is, and of what
 
-    python examples/distill_queries.py [--steps 200]
+    PYTHONPATH=. python examples/distill_queries.py [--steps 200]
 """
 
 import argparse
