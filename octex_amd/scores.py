@@ -160,6 +160,12 @@ class _Call:
             out = [empty(s, dtype=dtype, device=device) for s in shapes]
         return out if len(out) > 1 else out[0]
 
+    def like(self, t):
+        """A new dense result of t's shape and type (quicker than by its shape)."""
+        if self.foreign or not t.is_contiguous():
+            return self.new(t.shape, dtype=t.dtype)
+        return self.torch.empty_like(t)
+
     def run(self, entry, *args):
         if _entry(entry)(*args, self.stream) != _lib.CUVS_SUCCESS:
             raise _lib.OctexError(_lib.lib().cuvsGetLastErrorText().decode())
@@ -268,7 +274,8 @@ def log_probs(logits, ids, *, top=0, temperature=1.0):
     if not 0 <= top <= 64:
         raise ValueError(f"octex: 0 to 64 top entries, not {top}")
     t, shape = _ids(c, ids, m)
-    logp, entropy, lse, top_logp = c.new(shape, (m,), (m,), (m, top))
+    logp, entropy, top_logp = c.new(shape, (m,), (m, top))
+    lse = c.like(entropy)
     top_ids = c.new((m, top), dtype=c.torch.int64)
     c.run_sized("octexLogProbs", c.matrix(x), c.matrix(t), float(temperature), top, logp.data_ptr(), entropy.data_ptr(),
                 lse.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
@@ -288,7 +295,7 @@ def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, 
     gl = None if grad_log_probs is None else c.dense(grad_log_probs, "grad_log_probs", shape)
     gh = None if grad_entropy is None else c.dense(grad_entropy, "grad_entropy", (m,))
     lse, entropy = c.dense(lse, "lse", (m,)), c.dense(entropy, "entropy", (m,))
-    grad = c.new(x.shape, dtype=x.dtype)
+    grad = c.like(x)
     c.run("octexLogProbsBackward", c.matrix(x), c.matrix(t), float(temperature), None if gl is None else gl.data_ptr(),
           None if gh is None else gh.data_ptr(), lse.data_ptr(), entropy.data_ptr(), c.matrix(grad))
     return c.give(grad)
@@ -311,7 +318,8 @@ def distill(logits, ids, teacher, *, temperature=1.0):
     """
     c, x, t, teacher = _teacher(logits, ids, teacher)
     m = x.shape[0]
-    loss, lse = c.new((m,), (m,))
+    loss = c.new((m,))
+    lse = c.like(loss)
     c.run_sized("octexDistill", c.matrix(x), c.matrix(t), c.matrix(teacher), float(temperature), loss.data_ptr(),
                 lse.data_ptr())
     return c.give(loss), c.give(lse)
@@ -325,7 +333,7 @@ def distill_backward(grad_loss, logits, ids, teacher, lse, *, temperature=1.0):
     c, x, t, teacher = _teacher(logits, ids, teacher)
     m = x.shape[0]
     g, lse = c.dense(grad_loss, "grad_loss", (m,)), c.dense(lse, "lse", (m,))
-    grad = c.new(x.shape, dtype=x.dtype)
+    grad = c.like(x)
     c.run("octexDistillBackward", c.matrix(x), c.matrix(t), c.matrix(teacher), float(temperature), g.data_ptr(),
           lse.data_ptr(), c.matrix(grad))
     return c.give(grad)
@@ -336,7 +344,8 @@ def distill_step(grad_loss, logits, ids, teacher, *, temperature=1.0):
     c, x, t, teacher = _teacher(logits, ids, teacher)
     m = x.shape[0]
     g = c.dense(grad_loss, "grad_loss", (m,))
-    (loss, lse), grad = c.new((m,), (m,)), c.new(x.shape, dtype=x.dtype)
+    loss, grad = c.like(g), c.like(x)
+    lse = c.like(loss)
     c.run_sized("octexDistillStep", c.matrix(x), c.matrix(t), c.matrix(teacher), float(temperature), g.data_ptr(),
                 loss.data_ptr(), lse.data_ptr(), c.matrix(grad))
     return c.give(loss), c.give(grad)
