@@ -926,20 +926,21 @@ __device__ inline void write_gradient(const T* row, T* grad, bool by_cache, int 
 /**
  * ref, c and l2 of a row from its saved log-sum-exp; a row with nothing has p = 0 everywhere.  An l of more than kMaxLse
  * has lost too much of ln s to its rounding (all of it in a row of the type's lowest values), so such a row's sums are made
- * again.  All threads call this; parts [kWaves] is LDS.
+ * again.  That is so for infinite l too: a row of lowest values has one at temperatures below 1, as a row of nothing has.
+ * All threads call this; parts [NT / 64] is LDS.
  */
 template <typename T, int NT>
 __device__ inline auto gradient_base(const T* row, int n, float lse, float temperature, run* parts) -> gradient_row
 {
   gradient_row g{};
   g.c  = kLog2e / temperature;
-  g.l2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
-  if (fabsf(lse) > kMaxLse && fabsf(lse) != INFINITY) {
+  g.l2 = lse * kLog2e;
+  if (fabsf(lse) > kMaxLse) {
     run sums = nothing();
     for_scores<T, NT>(row, 0, n, [](float) {}, [&](const auto& v, int) { add_scores<false>(sums, v, g.c); });
     sums  = join_block<NT, false>(sums, g.c, parts);
     g.ref = sums.ref;
-    g.l2  = log2f(sums.s);
+    g.l2  = sums.s == 0.f ? INFINITY : log2f(sums.s);
   }
   return g;
 }

@@ -442,6 +442,33 @@ def test_gradients_of_rows_far_from_zero(O):
     close(loss, -logp.gather(1, ids)[:, 0], sum_error(1000) + 64 * E, "loss far from zero")
 
 
+@pytest.mark.parametrize("m,n", [(2, 5), (2, 1000), (2, 70_001), (2100, 300)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [0.5, 0.75])
+def test_gradients_of_the_lowest_value_below_temperature_one(O, m, n, dtype, T):
+    """A row masked by the type's lowest value is uniform, its log-sum-exp past fp32 or not; a row of -inf has p = 0."""
+    x = torch.full((m, n), torch.finfo(TYPES[dtype]).min).to(TYPES[dtype])
+    x[1::2] = float("-inf")
+    ids = torch.full((m, 1), n - 1)
+    one = torch.ones((m, 1))
+    want = torch.full((m, n), -1 / n, dtype=torch.float64)
+    want[1::2] = 0
+    want[:, n - 1] += 1
+    want /= T
+    # p = 2^(0 - log2 n) by fp32 exponent and power; then a rounding of each term and of their sum
+    tol = gradient_tolerance(want, (2 * sum_error(n) + 32 * E * (1 + math.log2(n))) / n / T + 8 * E * want.abs(), dtype)
+    r = O.log_probs(x.cuda(), ids.cuda(), temperature=T)
+    close(r.log_probs[::2], torch.full(((m + 1) // 2, 1), -math.log(n), dtype=torch.float64), sum_error(n) + 32 * E, "log_probs")
+    got = O.log_probs_backward(one.cuda(), None, x.cuda(), ids.cuda(), r.lse, r.entropy, temperature=T)
+    close(got, want, tol, "gradient")
+    loss, lse = O.distill(x.cuda(), ids.cuda(), one.cuda(), temperature=T)
+    got = O.distill_backward(one[:, 0].cuda(), x.cuda(), ids.cuda(), one.cuda(), lse, temperature=T)
+    close(got, -want, tol, "distillation's gradient")
+    step, got = O.distill_step(one[:, 0].cuda(), x.cuda(), ids.cuda(), one.cuda(), temperature=T)
+    close(got, -want, tol, "distillation step's gradient")
+    assert torch.equal(step, loss)
+
+
 @pytest.mark.parametrize("T", [1.0, 1.5])
 def test_gradients_against_differences(O, T):
     """Central differences of the kernels' own values: of step s they are off by s^2 / T^3 of the third derivative (under 1)
