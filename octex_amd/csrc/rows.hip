@@ -629,7 +629,8 @@ constexpr int kShortList = 128;
 template <int NT>
 constexpr int kEntries = (NT == 64 ? kShortList : kMaxListed) / NT;
 
-/** A thread's entries of a row's list: ids (-1: not listed), teacher / T (-inf where not listed) and the student's scores. */
+/** A thread's entries of a row's list: ids (-1: not listed), the teacher's logits (-inf where not listed; differences of them
+ * are divided by T, as a quotient of the lowest value may pass fp32) and the student's scores. */
 template <int E>
 struct listed_part {
   int id[E];
@@ -650,7 +651,7 @@ __device__ inline void read_list(score_rows const& in, listed_ids const& ids, te
       const float z    = load_any(teacher.x, teacher.type, r * teacher.stride + j);
       const bool in_row = id >= 0 && id < in.n;
       l.id[e]          = in_row ? static_cast<int>(id) : -1;
-      l.z[e]           = in_row ? z / in.temperature : -INFINITY;
+      l.z[e]           = in_row ? z : -INFINITY;
     }
   }
 }
@@ -663,9 +664,9 @@ __device__ inline void read_listed(const T* row, listed_part<E>& l)
     l.x[e] = l.id[e] >= 0 ? static_cast<float>(row[l.id[e]]) : 0.f;
 }
 
-/** The sums of the thread's entries, in units of 1: a NaN entry makes them NaN. */
+/** The sums of the thread's entries: a NaN entry makes them NaN. */
 template <int E>
-__device__ inline auto teacher_run(listed_part<E> const& l) -> run
+__device__ inline auto teacher_run(listed_part<E> const& l, float temperature) -> run
 {
   run t = nothing();
 #pragma unroll
@@ -674,17 +675,22 @@ __device__ inline auto teacher_run(listed_part<E> const& l) -> run
   t.ref = t.m == -INFINITY ? 0.f : t.m;
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    if (l.z[e] != -INFINITY) t.s += expf(l.z[e] - t.ref);
+    if (l.z[e] != -INFINITY) t.s += expf((l.z[e] - t.ref) / temperature);
   return t;
 }
 
-/** ln q of an entry of a list whose sums are t. */
+/** A list's sums, for the ln q of its entries. */
 struct teacher_sums {
-  float top, ln_w;
+  float top, ln_w, temperature;
   bool some;  // whether an entry has a probability
 };
 
-__device__ inline auto teacher_of(run const& t) -> teacher_sums { return {t.m, logf(t.s), t.s != 0.f}; }
+__device__ inline auto teacher_of(run const& t, float temperature) -> teacher_sums
+{
+  return {t.m, logf(t.s), temperature, t.s != 0.f};
+}
+
+__device__ inline auto ln_q(float z, teacher_sums const& t) -> float { return (z - t.top) / t.temperature - t.ln_w; }
 
 /** The thread's share of a row's loss. */
 template <int E>
@@ -694,7 +700,7 @@ __device__ inline auto loss_of(score_rows const& in, listed_part<E> const& l, te
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (l.z[e] == -INFINITY) continue;
-    const float lq = l.z[e] - t.top - t.ln_w, p = expf(lq);
+    const float lq = ln_q(l.z[e], t), p = expf(lq);
     if (p != 0.f) sum += p * (lq - log_prob(l.x[e], o, in.temperature));
   }
   return sum;
@@ -705,7 +711,7 @@ template <int NT>
 __device__ inline void join_both(run& sums, float c, run& t, run* both)
 {
   sums = join_lanes<64, false>(sums, c);
-  if (__ballot(t.s != 0.f) != 0) t = join_lanes<64, false>(t, kLog2e);
+  if (__ballot(t.s != 0.f) != 0) t = join_lanes<64, false>(t, c);
   if (threadIdx.x % 64 == 0) {
     both[threadIdx.x / 64 * 2]     = sums;
     both[threadIdx.x / 64 * 2 + 1] = t;
@@ -714,7 +720,7 @@ __device__ inline void join_both(run& sums, float c, run& t, run* both)
   const int w = threadIdx.x % (NT / 64);
   sums        = join_lanes<NT / 64, false>(both[2 * w], c);
   t           = both[2 * w + 1];
-  if (__ballot(t.s != 0.f) != 0) t = join_lanes<NT / 64, false>(t, kLog2e);
+  if (__ballot(t.s != 0.f) != 0) t = join_lanes<NT / 64, false>(t, c);
 }
 
 /** A pass over rows, a workgroup each, or with kSplit a workgroup a part of a row, which leaves its sums to
@@ -742,10 +748,10 @@ __global__ __launch_bounds__(NT) void distill_kernel(score_rows in, listed_ids i
     if (threadIdx.x == 0) part[b] = {sums.m, sums.s, 0.f};
   } else {
     read_listed(row, l);
-    run list = teacher_run(l);
+    run list = teacher_run(l, in.temperature);
     join_both<NT>(sums, c, list, both);
     const auto o      = finish(sums, in.temperature);
-    const float share = sum_lanes(loss_of(in, l, teacher_of(list), o));
+    const float share = sum_lanes(loss_of(in, l, teacher_of(list, in.temperature), o));
     if (threadIdx.x % 64 == 0) losses[threadIdx.x / 64] = share;
     lds_barrier();
     if (threadIdx.x == 0) {
@@ -769,8 +775,8 @@ __global__ __launch_bounds__(64) void finish_distill_kernel(score_rows in, liste
   read_list<64>(in, ids, teacher, r, l);
   const auto o = finish(join_parts<false>(part, r, split.parts, kLog2e / in.temperature), in.temperature);
   read_listed(static_cast<const T*>(in.x) + r * in.stride, l);
-  const run list  = join_lanes<64, false>(teacher_run(l), kLog2e);
-  const float sum = sum_lanes(loss_of(in, l, teacher_of(list), o));
+  const run list  = join_lanes<64, false>(teacher_run(l, in.temperature), kLog2e / in.temperature);
+  const float sum = sum_lanes(loss_of(in, l, teacher_of(list, in.temperature), o));
   if (threadIdx.x == 0) {
     loss[r] = sum;
     lse[r]  = o.lse;
@@ -860,7 +866,7 @@ __device__ inline void write_shares(listed_part<E> const& l, teacher_sums const&
     const int j = static_cast<int>(threadIdx.x) + e * NT;
     if (j >= k) continue;
     s.id[j] = l.id[e];
-    s.w[j]  = l.z[e] != -INFINITY ? -a * expf(l.z[e] - t.top - t.ln_w) : 0.f;
+    s.w[j]  = l.z[e] != -INFINITY ? -a * expf(ln_q(l.z[e], t)) : 0.f;
   }
 }
 
@@ -1005,8 +1011,8 @@ __global__ __launch_bounds__(NT) void distill_backward_kernel(score_rows in, lis
   listed_part<E> l;
   read_list<NT>(in, ids, teacher, r, l);
   write_gradient<T, false, NT>(row, grad + r * gstride, by_cache, c0, c1, shares, ids.k, [&](bool& some) {
-    const run list = join_block<NT, false>(teacher_run(l), kLog2e, parts);
-    const auto t   = teacher_of(list);
+    const run list = join_block<NT, false>(teacher_run(l, in.temperature), kLog2e / in.temperature, parts);
+    const auto t   = teacher_of(list, in.temperature);
     some           = t.some;
     write_shares<NT>(l, t, a, ids.k, shares);
     lds_barrier();  // parts has been read
@@ -1067,9 +1073,9 @@ __global__ __launch_bounds__(NT) void distill_step_kernel(score_rows in, listed_
     const int64_t next = r + gridDim.x;
     const bool more    = next < in.m;
     if (more) read_list<NT>(in, ids, teacher, next, after);
-    run list = teacher_run(l);
+    run list = teacher_run(l, in.temperature);
     join_both<NT>(sums, c, list, both);
-    const auto t  = teacher_of(list);
+    const auto t  = teacher_of(list, in.temperature);
     const auto o  = finish(sums, in.temperature);
     const float a = grad_loss[r] / in.temperature;
     write_shares<NT>(l, t, a, ids.k, shares);

@@ -602,6 +602,33 @@ def test_distill_of_dense_lists(O, m, n, k, dtype):
     check_distill(O, x, ids, teacher, 1.0, (0.5 + torch.rand(m, generator=g)) * (1 if dtype == "float32" else 1024), dtype, 3)
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 30, 4), (3, 5000, 512), (3, 140_000, 70), (2100, 700, 100)])
+@pytest.mark.parametrize("T", [0.5, 1.0, 2.0])
+def test_teachers_of_extreme_values(O, m, n, k, T):
+    """A teacher's lowest and highest values are values: a list of the lowest is uniform, whatever the temperature."""
+    g = gen(n + k)
+    low = torch.finfo(torch.float32).min
+    x = torch.randn((m, n), generator=g)
+    ids = torch.randint(0, n, (m, k), generator=g)
+    teacher = 2 * torch.randn((m, k), generator=g)
+    teacher[0] = low
+    teacher[1, 1:] = low
+    teacher[2, : k // 2] = -low
+    w = torch.ones(m)
+    # the same q from logits of ordinary size, by which the tolerances go
+    like = teacher.clamp_min(-1e6)
+    like[0] = 0
+    like[2] = torch.where(teacher[2] == -low, 0.0, -1e6)
+    want_loss, want, ltol, gtol = distill64(x, ids, like, T, w)
+    loss, grad = O.distill_step(w.cuda(), x.cuda(), ids.cuda(), teacher.cuda(), temperature=T)
+    close(loss, want_loss, ltol, "loss of a step")
+    close(grad, want, gradient_tolerance(want, gtol, "float32"), "gradient of a step")
+    loss, lse = O.distill(x.cuda(), ids.cuda(), teacher.cuda(), temperature=T)
+    close(loss, want_loss, ltol, "loss")
+    got = O.distill_backward(w.cuda(), x.cuda(), ids.cuda(), teacher.cuda(), lse, temperature=T)
+    close(got, want, gradient_tolerance(want, gtol, "float32"), "gradient")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [30, 5000, 140000])
 def test_distill_masks_infinities_and_nan(O, dtype, n):
