@@ -98,8 +98,8 @@ class _Call:
         """Any array as a torch tensor in the memory where it lies."""
         if _arrays.is_foreign_device(a):
             return self.torch.from_dlpack(a) if hasattr(a, "__dlpack__") else self.torch.as_tensor(a, device="cuda")
-        x = np.asarray(a)
-        return self.torch.from_numpy(x if x.flags.writeable else x.copy())
+        x = np.asarray(a)  # torch takes no views of read-only arrays, nor backward ones
+        return self.torch.from_numpy(x if x.flags.writeable and min(x.strides, default=0) >= 0 else x.copy())
 
     def take(self, a, name, types, ndim=2, shape=None):
         """The operand as a torch tensor on the call's GPU: of one of `types` (else converted to the first), the elements
@@ -183,12 +183,12 @@ class _Call:
         """A result in the framework, and the memory, of the first operand."""
         if not self.on_host and not self.foreign:
             return t
-        if isinstance(self.origin, self.torch.Tensor):
-            return t.cpu()
+        if self.on_host:
+            t = t.cpu()
         if self.foreign:
             conv = getattr(sys.modules.get(_arrays._module_of(self.origin)), "from_dlpack", None)
             return conv(t) if conv is not None else t
-        return t.cpu().numpy()
+        return t if isinstance(self.origin, self.torch.Tensor) else t.numpy()
 
 
 def quantize_rows(x):

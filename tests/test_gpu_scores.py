@@ -695,6 +695,37 @@ def test_operands_of_other_kinds(O):
     assert np.array_equal(y, O.int8_scores(x.cuda(), torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda()).cpu().numpy())
 
 
+class Exported:
+    """An array of another framework, in the memory of a torch tensor."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def __dlpack__(self, **kw):
+        return self.t.__dlpack__()
+
+    def __dlpack_device__(self):
+        return self.t.__dlpack_device__()
+
+
+def test_views_and_other_frameworks_on_either_side(O):
+    """numpy's backward, read-only and broadcast views; arrays of other frameworks are answered where they lie."""
+    g = gen(4)
+    x, ids = torch.randn((4, 300), generator=g), torch.randint(0, 300, (4, 2), generator=g)
+    want = O.log_probs(x.flip(0).flip(1).cuda(), ids.flip(1).cuda(), top=3)
+    got = O.log_probs(x.numpy()[::-1, ::-1], ids.numpy()[:, ::-1], top=3)
+    assert all(np.array_equal(a, b.cpu().numpy()) for a, b in zip(got, want))
+    row = np.broadcast_to(x.numpy()[0], (4, 300))
+    assert np.array_equal(O.log_probs(row, ids.numpy()).lse, O.log_probs(x[:1].repeat(4, 1).cuda(), ids.cuda()).lse.cpu().numpy())
+    want = O.log_probs(x.cuda(), ids.cuda(), top=3)
+    for side in ("cpu", "cuda"):
+        xs = x.to(side)
+        torch.cuda.synchronize()
+        got = O.log_probs(Exported(xs), ids, top=3)
+        torch.cuda.synchronize()
+        assert all(a.device.type == side and torch.equal(a.cpu(), b.cpu()) for a, b in zip(got, want))
+
+
 def test_scalars_of_any_kind(O):
     x, ids = torch.randn((3, 50)).cuda(), torch.zeros((3, 1), dtype=torch.int64).cuda()
     want = O.log_probs(x, ids, top=2, temperature=2.0)
