@@ -39,19 +39,22 @@ def _hip_stream_of_cai(code):
     return {_CAI_LEGACY: _HIP_NULL_STREAM, _CAI_PER_THREAD: _HIP_PER_THREAD_STREAM}.get(code, code)
 
 
-def _foreign_stream(a):
-    """The stream a foreign device array was produced on: the interface's own 'stream' entry, else the current
-    stream of its framework when the framework has that notion (CuPy), else the null stream."""
+def named_stream(a):
+    """The stream that a foreign device array names: the interface's own 'stream' entry, else the current stream of its
+    framework when the framework has that notion (CuPy); None if neither is there."""
     cai = getattr(a, "__cuda_array_interface__", None)
     if cai is not None and "stream" in cai:
-        s = _hip_stream_of_cai(cai["stream"])
-        return _HIP_NULL_STREAM if s is None else s
+        return _hip_stream_of_cai(cai["stream"])
     mod = sys.modules.get(_module_of(a))
     cuda = getattr(mod, "cuda", None)
     get = getattr(cuda, "get_current_stream", None)
-    if callable(get):
-        return int(get().ptr)
-    return _HIP_NULL_STREAM
+    return int(get().ptr) if callable(get) else None
+
+
+def _foreign_stream(a):
+    """The stream a foreign device array was produced on: the one that it names, else the null stream."""
+    s = named_stream(a)
+    return _HIP_NULL_STREAM if s is None else s
 
 
 class Operand:

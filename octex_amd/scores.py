@@ -7,9 +7,9 @@
     loss, grad = octex.distill_step(weights, logits, neighbors, -distances, temperature=2.0)   # ... and the lesson
 
 Every operator is a hand-written kernel and takes matrices whose rows may lie apart (a slice of a padded vocabulary's
-columns, say).  Operands in GPU memory are read in place: the work is ordered on their stream (torch's current stream, or
-the one their framework names) and not waited for.  Host operands are copied to the GPU and results come back as the
-first operand is.  Types that an operator does not take are converted, as for a search.  Results carry no autograd graph:
+columns, say).  Operands in GPU memory are read in place: the work is ordered on the first one's stream (torch's current
+stream, or the one its framework names) and not waited for; operands of other streams precede it, and what those streams do
+next comes after it.  Host operands are copied to the GPU and results come back as the first operand is.  Types that an operator does not take are converted, as for a search.  Results carry no autograd graph:
 the gradients have calls of their own.
 """
 
@@ -72,26 +72,23 @@ _HERE = contextlib.nullcontext()
 
 
 class _Call:
-    """One call's operands and results, all on one GPU, and the stream they are ordered on."""
+    """One call's operands and results, all on one GPU, and the stream that they are ordered on: torch's current one, or
+    (`side`) another that the first operand's framework names.  `others` are the streams of the remaining operands."""
 
-    __slots__ = ("torch", "names", "origin", "device", "stream", "on_host", "foreign", "first", "scratch")
+    __slots__ = ("torch", "names", "origin", "device", "stream", "side", "others", "on_host", "foreign", "first", "scratch")
 
     def __init__(self, first, name, types):
         self.torch, self.names, raw_stream = _torch()
-        self.origin, self.device, self.foreign = first, None, False
-        if isinstance(first, self.torch.Tensor):
-            t = first
-        elif _arrays.is_foreign_device(first):
-            self.foreign = True
-            t = self.view(first)
-        else:
-            t = self.view(first)
+        self.origin, self.side, self.others = first, None, ()
+        self.foreign = not isinstance(first, self.torch.Tensor) and _arrays.is_foreign_device(first)
+        t = first if isinstance(first, self.torch.Tensor) else self.view(first)
         self.on_host = not t.is_cuda
-        if self.on_host:
-            self.device = self.torch.device("cuda", self.torch.cuda.current_device())
-        else:
-            self.device = t.device
-        self.stream = _arrays._foreign_stream(first) if self.foreign and t.is_cuda else raw_stream(self.device.index)
+        self.device = self.torch.device("cuda", self.torch.cuda.current_device()) if self.on_host else t.device
+        self.stream = raw_stream(self.device.index)
+        if self.foreign and t.is_cuda:  # of a framework that names no stream: its export has ordered it on torch's
+            named = _arrays.named_stream(first)
+            if named is not None and named != self.stream:
+                self.stream, self.side = named, self.external(named)
         self.first = self.take(t, name, types)
 
     def view(self, a):
@@ -101,11 +98,39 @@ class _Call:
         x = np.asarray(a)  # torch takes no views of read-only arrays, nor backward ones
         return self.torch.from_numpy(x if x.flags.writeable and min(x.strides, default=0) >= 0 else x.copy())
 
-    def take(self, a, name, types, ndim=2, shape=None):
-        """The operand as a torch tensor on the call's GPU: of one of `types` (else converted to the first), the elements
+    def external(self, handle):
+        cuda = self.torch.cuda
+        return cuda.ExternalStream(handle, device=self.device) if handle else cuda.default_stream(self.device)
+
+    def own_stream(self):
+        return self.side if self.side is not None else self.torch.cuda.current_stream(self.device)
+
+    def join(self, stream):
+        """Orders the call after all that `stream` holds; run orders what the stream does next after the call."""
+        if stream not in self.others:
+            self.own_stream().wait_stream(stream)
+            self.others += (stream,)
+
+    def array(self, a):
+        """An operand behind the first as a torch tensor in the memory where it lies, ordered with the call."""
+        if isinstance(a, self.torch.Tensor):
+            if self.side is not None and a.is_cuda:
+                self.join(self.torch.cuda.current_stream(self.device))
+            return a
+        if not _arrays.is_foreign_device(a):
+            return self.view(a)
+        with self.context():  # DLPack orders its producer on the stream that is current
+            t = self.view(a)
+        if t.is_cuda:  # __cuda_array_interface__ leaves that to its reader
+            named = _arrays.named_stream(a)
+            if named is not None and named != self.stream:
+                self.join(self.external(named))
+        return t
+
+    def take(self, t, name, types, ndim=2, shape=None):
+        """The operand (as array gives it) on the call's GPU: of one of `types` (else converted to the first), the elements
         of a row side by side.  A vector is one row unless ndim is 1."""
         torch = self.torch
-        t = a if isinstance(a, torch.Tensor) else self.view(a)
         if t.device != self.device:
             if t.is_cuda:
                 raise ValueError(f"octex: {name} lies on {t.device}, the other operands on {self.device}")
@@ -134,7 +159,7 @@ class _Call:
 
     def dense(self, a, name, shape):
         """A float32 operand without gaps between its rows."""
-        t = self.take(a, name, ("float32",), len(shape), shape)
+        t = self.take(self.array(a), name, ("float32",), len(shape), shape)
         if t.is_contiguous():
             return t
         with self.context():
@@ -142,9 +167,7 @@ class _Call:
 
     def context(self):
         """For torch's own work (conversions, allocations) on the call's stream."""
-        if not self.foreign:
-            return _HERE
-        return self.torch.cuda.stream(self.torch.cuda.ExternalStream(self.stream, device=self.device))
+        return _HERE if self.side is None else self.torch.cuda.stream(self.side)
 
     def matrix(self, t):
         rows, cols = t.shape
@@ -153,7 +176,7 @@ class _Call:
     def new(self, *shapes, dtype=None):
         """New results: float32, or of a torch type."""
         empty, device, dtype = self.torch.empty, self.device, dtype or self.torch.float32
-        if self.foreign:
+        if self.side is not None:
             with self.context():
                 out = [empty(s, dtype=dtype, device=device) for s in shapes]
         else:
@@ -162,13 +185,15 @@ class _Call:
 
     def like(self, t):
         """A new dense result of t's shape and type (quicker than by its shape)."""
-        if self.foreign or not t.is_contiguous():
+        if self.side is not None or not t.is_contiguous():
             return self.new(t.shape, dtype=t.dtype)
         return self.torch.empty_like(t)
 
     def run(self, entry, *args):
         if _entry(entry)(*args, self.stream) != _lib.CUVS_SUCCESS:
             raise _lib.OctexError(_lib.lib().cuvsGetLastErrorText().decode())
+        for stream in self.others:
+            stream.wait_stream(self.own_stream())
 
     def run_sized(self, entry, *args):
         """run with the workspace that the arguments need; its tensor is kept with the call."""
@@ -187,7 +212,14 @@ class _Call:
             t = t.cpu()
         if self.foreign:
             conv = getattr(sys.modules.get(_arrays._module_of(self.origin)), "from_dlpack", None)
-            return conv(t) if conv is not None else t
+            if conv is not None:
+                with self.context():
+                    return conv(t)
+            if self.side is not None:  # a torch tensor after all, which is read on torch's stream
+                current = self.torch.cuda.current_stream(self.device)
+                current.wait_stream(self.side)
+                t.record_stream(current)
+            return t
         return t if isinstance(self.origin, self.torch.Tensor) else t.numpy()
 
 
@@ -217,7 +249,7 @@ def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtyp
     coded = query_scales is not None
     c = _Call(queries, "queries", ("int8",) if coded else FLOATS)
     q = c.first
-    rows = c.take(rows, "rows", ("int8",))
+    rows = c.take(c.array(rows), "rows", ("int8",))
     (m, k), n = q.shape, rows.shape[0]
     if rows.shape[1] != k:
         raise ValueError(f"octex: queries have {k} values, rows {rows.shape[1]}")
@@ -251,7 +283,7 @@ def _columns(a):
 def _ids(c, ids, m):
     """The ids of m rows as a matrix, and the shape their values come back in."""
     ids, shape = _columns(ids)
-    t = c.take(ids, "ids", INTS)
+    t = c.take(c.array(ids), "ids", INTS)
     if t.shape[0] != m:
         raise ValueError(f"octex: ids of {t.shape[0]} rows, logits of {m}")
     return t, tuple(shape)
@@ -304,7 +336,7 @@ def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, 
 def _teacher(logits, ids, teacher):
     c = _Call(logits, "logits", FLOATS)
     t, _ = _ids(c, ids, c.first.shape[0])
-    return c, c.first, t, c.take(_columns(teacher)[0], "teacher", FLOATS, shape=t.shape)
+    return c, c.first, t, c.take(c.array(_columns(teacher)[0]), "teacher", FLOATS, shape=t.shape)
 
 
 def distill(logits, ids, teacher, *, temperature=1.0):

@@ -1,0 +1,122 @@
+"""The operators on rows of scores on operands of several frameworks, each ordered on a stream of its own.  This module plays
+one of these frameworks: it has a current stream (`cuda`), arrays that export DLPack, and from_dlpack."""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def O():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import octex_amd
+
+    return octex_amd
+
+
+class cuda:
+    stream = None  # the framework's current one
+
+    class _Handle:
+        def __init__(self, ptr):
+            self.ptr = ptr
+
+    @staticmethod
+    def get_current_stream():
+        return cuda._Handle(cuda.stream.cuda_stream)
+
+
+class Array:
+    """An array of this framework; its export orders its reader's stream after its own, as DLPack asks of it."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def __dlpack__(self, *, stream=None, **kw):
+        if stream is not None and stream != cuda.stream.cuda_stream:
+            reader = torch.cuda.ExternalStream(stream) if stream > 2 else torch.cuda.default_stream()
+            reader.wait_stream(cuda.stream)
+        return self.t.__dlpack__()
+
+    def __dlpack_device__(self):
+        return self.t.__dlpack_device__()
+
+
+def from_dlpack(t):
+    return Array(t)
+
+
+class Nameless(Array):
+    """The same of a framework that names no stream."""
+
+
+Nameless.__module__ = "nowhere"
+
+
+class Interface:
+    """An array that has __cuda_array_interface__ alone, with the stream that it is ordered on."""
+
+    def __init__(self, t):
+        self.t = t
+        code = cuda.stream.cuda_stream
+        self.__cuda_array_interface__ = dict(shape=tuple(t.shape), typestr={torch.float32: "<f4", torch.int64: "<i8"}[t.dtype],
+                                             data=(t.data_ptr(), False), version=3, stream=code)
+
+
+Interface.__module__ = "nowhere"
+
+
+def delay():
+    """Some 10 ms of work on the current stream."""
+    a = torch.ones((4096, 4096), device="cuda")
+    for _ in range(8):
+        a = a @ a / 4096
+
+
+KINDS = {"torch": lambda t: t, "array": Array, "nameless": Nameless, "interface": Interface}
+
+
+@pytest.mark.parametrize("logits,ids", [("array", "torch"), ("torch", "array"), ("torch", "interface"), ("interface", "torch"),
+                                        ("nameless", "torch"), ("nameless", "array"), ("array", "interface"),
+                                        ("interface", "array")])
+def test_operands_of_several_frameworks_are_ordered(O, logits, ids):
+    """Each operand changes behind work that is still on its own stream when the call is made, and again after the call, on the
+    same stream: the results are those of its values at the call.  Nothing is synchronized in between.  (What a framework that
+    names no stream does after the call is its own to order.)"""
+    g = torch.Generator().manual_seed(3)
+    m, n, k = 300, 5000, 4
+    right = [torch.randn((m, n), generator=g).cuda(), torch.randint(0, n, (m, k), generator=g).cuda()]
+    weight, teacher = torch.rand(m, generator=g).cuda(), torch.randn((m, k), generator=g).cuda()
+    torch.cuda.synchronize()
+    want = list(O.log_probs(*right, top=3)) + list(O.distill_step(weight, right[0], right[1], teacher))
+    ours, theirs = torch.cuda.Stream(), torch.cuda.Stream()
+    cuda.stream = theirs
+    held = [torch.zeros_like(t) for t in right]
+    streams = [ours if kind == "torch" else theirs for kind in (logits, ids)]
+    for s in (ours, theirs):  # the allocator's first calls are made
+        with torch.cuda.stream(s):
+            delay()
+    torch.cuda.synchronize()
+    for s, t, r in zip(streams, held, right):
+        with torch.cuda.stream(s):
+            delay()
+            t.copy_(r)
+    with torch.cuda.stream(ours):
+        x, i = (KINDS[kind](t) for kind, t in zip((logits, ids), held))
+        r = O.log_probs(x, i, top=3)
+        loss, grad = O.distill_step(weight, x, i, teacher)
+    for kind, s, t in zip((logits, ids), streams, held):
+        if kind != "nameless":
+            with torch.cuda.stream(s):
+                t.zero_()
+    got = list(r) + [loss, grad]
+    # what comes back is ordered on the first operand's stream, or on torch's
+    with torch.cuda.stream(theirs if isinstance(got[0], Array) else ours):
+        got = [(v.t if isinstance(v, Array) else v).clone() for v in got]
+    torch.cuda.synchronize()
+    assert isinstance(r.lse, Array) == (logits == "array")
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
