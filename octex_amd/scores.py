@@ -247,8 +247,10 @@ def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtyp
     ("float32", "float16" or "bfloat16") is that of the scores: the queries' own if they are floats, else float32.
     """
     coded = query_scales is not None
-    c = _Call(queries, "queries", ("int8",) if coded else FLOATS)
+    c = _Call(queries, "queries", ("int8",) if coded else FLOATS + ("int8",))
     q = c.first
+    if not coded and c.names[q.dtype] == "int8":
+        raise TypeError("octex: int8 queries need their query_scales")
     rows = c.take(c.array(rows), "rows", ("int8",))
     (m, k), n = q.shape, rows.shape[0]
     if rows.shape[1] != k:

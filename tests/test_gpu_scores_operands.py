@@ -14,6 +14,7 @@ def O():
         pytest.skip("no GPU")
     import octex_amd
 
+    cuda.stream = torch.cuda.Stream()
     return octex_amd
 
 
@@ -120,3 +121,13 @@ def test_operands_of_several_frameworks_are_ordered(O, logits, ids):
     assert isinstance(r.lse, Array) == (logits == "array")
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_codes_without_their_scales_are_refused(O):
+    """int8 queries are codes: taken for values, they would be quantized once more, as if their scales were 1."""
+    codes, scales = O.quantize_rows(torch.randn((3, 50), generator=torch.Generator().manual_seed(1)).cuda())
+    for queries in (codes, codes.cpu(), codes.cpu().numpy(), codes[0], Nameless(codes)):
+        with pytest.raises(TypeError, match="octex: int8 queries need their query_scales"):
+            O.int8_scores(queries, codes, scales)
+    s = O.int8_scores(codes.int().float(), codes, scales)  # whole numbers in a float type are values
+    assert s.dtype == torch.float32 and s.shape == (3, 3)
