@@ -274,21 +274,19 @@ def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtyp
     return c.give(out)
 
 
-def _columns(a):
-    """A vector, one entry a row, as a matrix of one column; and its shape."""
-    shape = a.shape if hasattr(a, "shape") else _arrays.shape_of(a)
-    if len(shape) != 1:
-        return a, shape
-    return (a if hasattr(a, "ndim") else np.asarray(a))[:, None], shape
+def _columns(c, a):
+    """An operand as array gives it, a vector (one entry a row) as a matrix of one column; and its own shape."""
+    t = c.array(a)
+    return (t[:, None] if t.ndim == 1 else t), tuple(t.shape)
 
 
 def _ids(c, ids, m):
     """The ids of m rows as a matrix, and the shape their values come back in."""
-    ids, shape = _columns(ids)
-    t = c.take(c.array(ids), "ids", INTS)
+    ids, shape = _columns(c, ids)
+    t = c.take(ids, "ids", INTS)
     if t.shape[0] != m:
         raise ValueError(f"octex: ids of {t.shape[0]} rows, logits of {m}")
-    return t, tuple(shape)
+    return t, shape
 
 
 def log_probs(logits, ids, *, top=0, temperature=1.0):
@@ -338,7 +336,7 @@ def log_probs_backward(grad_log_probs, grad_entropy, logits, ids, lse, entropy, 
 def _teacher(logits, ids, teacher):
     c = _Call(logits, "logits", FLOATS)
     t, _ = _ids(c, ids, c.first.shape[0])
-    return c, c.first, t, c.take(c.array(_columns(teacher)[0]), "teacher", FLOATS, shape=t.shape)
+    return c, c.first, t, c.take(_columns(c, teacher)[0], "teacher", FLOATS, shape=t.shape)
 
 
 def distill(logits, ids, teacher, *, temperature=1.0):

@@ -131,3 +131,23 @@ def test_codes_without_their_scales_are_refused(O):
             O.int8_scores(queries, codes, scales)
     s = O.int8_scores(codes.int().float(), codes, scales)  # whole numbers in a float type are values
     assert s.dtype == torch.float32 and s.shape == (3, 3)
+
+
+def test_vectors_and_lists_of_ids(O):
+    """One id a row, and its teacher's logit, as a tensor, numpy's, a list, or an array that has only DLPack."""
+    g = torch.Generator().manual_seed(2)
+    x, ids, teacher = torch.randn((4, 30), generator=g).cuda(), torch.tensor([3, 29, -1, 0]), torch.randn(4, generator=g)
+    want = O.log_probs(x, ids.cuda()[:, None])
+    loss, lse = O.distill(x, ids.cuda()[:, None], teacher.cuda()[:, None])
+    torch.cuda.synchronize()
+    for kind in (lambda t: t.cuda(), lambda t: t, lambda t: t.numpy(), lambda t: t.tolist(), lambda t: Nameless(t.cuda()),
+                 lambda t: Nameless(t)):
+        r = O.log_probs(x, kind(ids))
+        assert r.log_probs.shape == (4,) and torch.equal(r.log_probs, want.log_probs[:, 0])
+        one = kind(torch.ones(4))
+        grad = O.log_probs_backward(one, None, x, kind(ids), r.lse, r.entropy)
+        assert torch.equal(grad, O.log_probs_backward(torch.ones((4, 1)).cuda(), None, x, ids.cuda()[:, None], r.lse, r.entropy))
+        assert torch.equal(O.distill(x, kind(ids), kind(teacher))[0], loss)
+        assert torch.equal(O.distill_step(one, x, kind(ids), kind(teacher))[0], loss)
+    r = O.log_probs(x.tolist(), ids[:, None].tolist())
+    assert torch.equal(torch.as_tensor(r.log_probs), want.log_probs.cpu())
