@@ -262,8 +262,9 @@ def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtyp
         bias = c.dense(bias, "bias", (n,))
     if dtype is None:
         dtype = "float32" if coded else c.names[q.dtype]
-    if dtype not in FLOATS:
-        dtype = np.dtype(dtype).name if isinstance(dtype, type) else str(dtype).replace("torch.", "")
+    if not isinstance(dtype, str):
+        dtype = np.dtype(dtype).name if isinstance(dtype, (type, np.dtype)) else str(dtype)
+    dtype = dtype.replace("torch.", "")
     if dtype not in FLOATS:
         raise ValueError(f"octex: scores are of type {', '.join(FLOATS)}, not {dtype}")
     if dtype == "bfloat16" and c.on_host and not isinstance(queries, c.torch.Tensor):

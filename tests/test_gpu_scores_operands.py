@@ -1,6 +1,7 @@
 """The operators on rows of scores on operands of several frameworks, each ordered on a stream of its own.  This module plays
 one of these frameworks: it has a current stream (`cuda`), arrays that export DLPack, and from_dlpack."""
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -151,3 +152,17 @@ def test_vectors_and_lists_of_ids(O):
         assert torch.equal(O.distill_step(one, x, kind(ids), kind(teacher))[0], loss)
     r = O.log_probs(x.tolist(), ids[:, None].tolist())
     assert torch.equal(torch.as_tensor(r.log_probs), want.log_probs.cpu())
+
+
+def test_types_of_scores_by_any_name(O):
+    x = torch.randn((3, 50), generator=torch.Generator().manual_seed(6)).cuda()
+    codes, scales = O.quantize_rows(x)
+    for name in ("float32", "float16", "bfloat16"):
+        names = [name, getattr(torch, name), f"torch.{name}"]
+        if name != "bfloat16":
+            names += [np.dtype(name), np.dtype(name).type]
+        for dtype in names:
+            assert O.int8_scores(x, codes, scales, dtype=dtype).dtype == getattr(torch, name)
+    for dtype in (np.dtype("int8"), np.int32, torch.float64, "double"):
+        with pytest.raises(ValueError, match="octex: scores are of type"):
+            O.int8_scores(x, codes, scales, dtype=dtype)
