@@ -152,6 +152,9 @@ class _Call:
         s = t.shape
         if shape is not None and s != shape:
             raise ValueError(f"octex: {name} has shape {tuple(s)}, expected {tuple(shape)}")
+        if t.is_neg():  # a view whose sign torch has yet to turn in memory, as of a conjugate's imaginary part
+            with self.context():
+                t = t.resolve_neg()
         if not t.is_contiguous() and (s[-1] > 1 and t.stride(-1) != 1 or (ndim == 2 and s[0] > 1 and t.stride(0) < s[1])):
             with self.context():
                 t = t.contiguous()

@@ -166,3 +166,17 @@ def test_types_of_scores_by_any_name(O):
     for dtype in (np.dtype("int8"), np.int32, torch.float64, "double"):
         with pytest.raises(ValueError, match="octex: scores are of type"):
             O.int8_scores(x, codes, scales, dtype=dtype)
+
+
+def test_views_with_a_lazy_sign(O):
+    """The imaginary part of a conjugate is a view of the values before their sign is turned."""
+    z = torch.randn((4, 60), dtype=torch.complex64, generator=torch.Generator().manual_seed(8)).cuda()
+    ids = torch.zeros((4, 1), dtype=torch.int64).cuda()
+    w = torch._neg_view(torch.ones(4).cuda())
+    x = z.conj().imag
+    assert x.is_neg() and w.is_neg()
+    for a, b in zip(O.log_probs(x, ids, top=2), O.log_probs(-z.imag, ids, top=2)):
+        assert torch.equal(a, b)
+    loss, grad = O.distill_step(w, x, ids, x[:, :1])
+    want = O.distill_step(-torch.ones(4).cuda(), -z.imag, ids, -z.imag[:, :1])
+    assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
