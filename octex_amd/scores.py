@@ -227,9 +227,9 @@ class _Call:
 
 
 def quantize_rows(x):
-    """(codes, scales) of the rows of x [m, k] in 8 bits: scale = max |x| / 127, code = the whole number nearest to
-    x / scale (ties to even), as torch's x.abs().amax(1) / 127 and division have them on the GPU: x is about
-    codes * scales[:, None].
+    """(codes, scales) of the rows of x [m, k] in 8 bits: scale = max |x| / 127, as the float32 product with 1 / 127, code = the
+    whole number nearest to x / scale (ties to even): x is about codes * scales[:, None].  torch's x.abs().amax(1) / 127 is that
+    product on the GPU; on the CPU, as numpy's, it is a quotient, which differs by one unit in some rows.
 
     A row of zeros has scale 0; a row with a NaN or an infinity has scale NaN, which makes all its scores NaN.
     """
