@@ -1,8 +1,9 @@
 """Sums over long rows of scores: their error does not grow with the row.
 
-With e = 2^-24: an exponential is off by 2 e and, its exponent being rounded three times, by 3 e of |z - max| (6 at most here);
-eight are added to each other and a few such sums again (4.5 e each), then to the thread's, which keeps what an addition loses
-(2 e); a row's sums are joined in 14 additions: 45 e of the sum.  A logarithm adds 2 e of its size, and so do lse's and log
+With e = 2^-24: an exponential is off by 2 e and, its exponent being the rounded product of an exact difference with a rounded
+factor, by 2 e of |z - max| (6 at most here); eight are added to each other (4.5 e) and up to 16 such sums again (8.5 e), then to
+the thread's, which keeps what an addition loses (2 e); a row's sums are joined in 14 additions: under 45 e of the sum.
+A logarithm adds 2 e of its size, and so do lse's and log
 p's own additions.  The weighted sum has the same errors and 1 e of its product.  So
   lse, log p:  45 e + 4 e (|lse| + |z|)
   entropy:     45 e + 4 e |ln s| + 100 e of |sum p (z - max)|
