@@ -11,7 +11,8 @@
 // A row without a finite score has p = 0 everywhere: l = -inf, H = 0, log p = -inf.  A NaN or +inf makes its row NaN.
 //
 // All of it is bound by the logits' bytes: a large copy takes 4.77 TB/s of this GPU, a kernel that only reads up to 5.5.
-// The times below are a launch's among others of its kind; "TB/s" counts the logits, and a gradient, once.
+// The times below are a launch's among others of its kind, its inputs changing from launch to launch; "TB/s" counts the logits,
+// and a gradient, once.  Two sides of a choice were timed together, some before later steps made both quicker.
 
 #include "common.hpp"
 #include "elems_device.hpp"
@@ -113,8 +114,8 @@ __device__ inline auto add_scores(run& r, const float (&v)[N], float c) -> float
 }
 
 // Reductions over groups of W lanes without LDS: a lane meets lanes that hold the other halves' results, and as f(a, b) is
-// f(b, a) every lane ends with the same.  (By shuffles through LDS, both directions of distill: 4096 x 128,000 bfloat16 487 us
-// in place of 456, 16 x 32,000 float32 14 in place of 11.3.)
+// f(b, a) every lane ends with the same.  (By shuffles through LDS both directions of distill took 7 % longer for 4096 x
+// 128,000 bfloat16, 24 % for 16 x 32,000 float32.)
 
 template <int kControl>
 __device__ inline auto from_lane(float v) -> float
@@ -596,8 +597,8 @@ __device__ inline void write_top(score_rows const& in, log_probs_out const& out,
  * A workgroup a row, or with kSplit a workgroup a part of a row, which leaves its sums and its best keys (0: none) to
  * finish_log_probs_kernel.  One pass: a thread has 64 bytes on their way while it adds and lists 64 others.
  *
- * 4096 x 128,000 bfloat16: 191 us, 5.5 TB/s; with the 20 best 214 us, 4.9 TB/s, the first floors and the lists' ends being
- * what is not hidden (2048 rows: 98 and 120).  1 x 128,000, in two launches: 6.5 us, with the 20 best 12.
+ * 4096 x 128,000 bfloat16: 186 us, 5.6 TB/s; with the 20 best 207 us, 5.1 TB/s, the first floors and the lists' ends being
+ * what is not hidden (2048 rows: 95 and 115).  1 x 128,000, in two launches: 4.9 us, with the 20 best 11.2.
  */
 template <typename T, int NT, bool kTop, bool kSplit>
 __global__ __launch_bounds__(NT) void log_probs_kernel(score_rows in, listed_ids ids, log_probs_out out,
@@ -780,7 +781,7 @@ __device__ inline void join_both(run& sums, float c, run& t, run* both)
 
 /** A pass over rows, a workgroup each, or with kSplit a workgroup a part of a row, which leaves its sums to
  * finish_distill_kernel.  The list's q needs no pass of its own: its logits are a few registers of the threads, and its sums
- * are joined at the row's barrier.  4096 x 128,000 bfloat16 with 64 ids a row: 189 us, 5.5 TB/s. */
+ * are joined at the row's barrier.  4096 x 128,000 bfloat16 with 64 ids a row: 190 us, 5.5 TB/s. */
 template <typename T, int NT, bool kSplit>
 __global__ __launch_bounds__(NT) void distill_kernel(score_rows in, listed_ids ids, teacher_logits teacher,
                                                      float* loss, float* lse, row_split split, part_sums* part,
@@ -883,7 +884,7 @@ __device__ inline auto share_at(listed_shares const& s, int j, int k) -> listed_
  * A wavefront that has the whole list to itself (kAlone) meets many entries at a time: it takes them by their place among a
  * lane's columns, which is the same for all lanes but where some were moved back, at one addition each instead of N.
  * 8000 x 1000 float32 with 64 ids, distill's gradient: 23 us against 26; but 4096 x 128,000 bfloat16 in both directions,
- * where most pieces meet none, 467 against 455.
+ * where most pieces meet none, takes 3 % longer.
  */
 template <bool kAlone, int N>
 __device__ inline void add_shares(float (&v)[N], int at, int w0, int last, int end, listed_share first, listed_shares const& s,
@@ -989,9 +990,9 @@ __device__ inline void write_gradient(const T* row, T* grad, bool by_cache, int 
 /**
  * ref, c and l2 of a row from its saved log-sum-exp l; a row with nothing has p = 0 everywhere.  With ref = l T the difference
  * x - ref is small where p is not, and p is as near as the fp32 l: 3.8e-6 of it at l = 98 (by x c - l log2(e), whose terms are
- * rounded apart, up to 6.0e-6 more).  An l of more than kMaxLse has lost too much of ln s to its rounding (all of it in a row of the
- * type's lowest values), so such a row's sums are made again.  That is so for infinite l too: a row of lowest values has one
- * at temperatures below 1, as a row of nothing has.  All threads call this; parts [NT / 64] is LDS.
+ * rounded apart, up to 6.0e-6 more).  An l of more than kMaxLse has lost too much of ln s to its rounding (all of it in a row
+ * of the type's lowest values), so such a row's sums are made again.  That is so for infinite l too: a row of lowest values has
+ * one at temperatures below 1, as a row of nothing has.  All threads call this; parts [NT / 64] is LDS.
  */
 template <typename T, int NT>
 __device__ inline auto gradient_base(const T* row, int n, float lse, float temperature, run* parts) -> gradient_row
@@ -1012,7 +1013,7 @@ __device__ inline auto gradient_base(const T* row, int n, float lse, float tempe
 }
 
 /** A workgroup a row or a part of one: A and B of the row from its list and its saved sums, then one pass.  4096 x 128,000
- * bfloat16: 418 us, 5.0 TB/s; 4096 x 32,000, its logits still in the last-level cache: 82 us, 6.4 TB/s. */
+ * bfloat16: 418 us, 5.0 TB/s; 4096 x 32,000, its logits still in the last-level cache: 81 us, 6.5 TB/s. */
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void log_probs_backward_kernel(score_rows in, listed_ids ids, const float* grad_logp,
                                                                       const float* grad_entropy, const float* lse,
@@ -1088,7 +1089,7 @@ __global__ __launch_bounds__(NT) void distill_backward_kernel(score_rows in, lis
  * of its next row is loaded in its place, and pieces that have arrived enter that row's sums, so that reads, writes and
  * arithmetic go on side by side.  The next row's list comes meanwhile, E entries a thread.
  *
- * 4096 x 128,000 bfloat16 with 64 ids a row: 456 us, 4.6 TB/s, against 607 by two passes; what it lacks to a copy's 440 is
+ * 4096 x 128,000 bfloat16 with 64 ids a row: 450 us, 4.7 TB/s, against 609 by two passes; what it lacks to a copy's 440 is
  * the join between a row's last load and its gradient's first store, when this workgroup has nothing on its way.
  */
 template <typename T, int NT, int H>
@@ -1201,7 +1202,7 @@ void for_grids(int64_t total, int threads, F f)
 constexpr int kEnough   = 1024;  // workgroups of 256 threads that fill the GPU
 constexpr int kMinWidth = 4096;  // columns of a part
 constexpr int kMaxParts = 32;    // of a row
-constexpr int kMidRows  = 512;   // rows whose top entries take 512 threads (333 x 50,021 float32: 25.7 us, by 256 28.2)
+constexpr int kMidRows  = 512;   // rows whose top entries take 512 threads (333 x 50,021 float32: 21.2 us, by 256 22.9)
 
 /** Rows are split into parts of whole 16-byte pieces while they are fewer than the workgroups that fill the GPU. */
 auto split_of(int64_t m, int n, int64_t most = kMaxParts) -> row_split
@@ -1213,9 +1214,9 @@ auto split_of(int64_t m, int n, int64_t most = kMaxParts) -> row_split
 }
 
 /** Up to kFewRows rows of kWideRow columns or more are split in a forward pass, at a second launch (and a workspace, 4 us of
- * a caller's time): 16 x 128,000 bfloat16 in 6.5 us against 16.4 whole, with the 20 best 13.8 against 25; 128 rows in 14
- * against 17.5, but 256 in 19 either way and with the 20 best in 31 against 27; 16 x 32,000 in 5.7 against 6.3, with the 20
- * best 13.0 against 11.8. */
+ * a caller's time): 16 x 128,000 bfloat16 in 5.6 us against 16.7 whole, with the 20 best 12.5 against 25; 128 rows in 12.6
+ * against 17.3, but 256 in 17.5 either way and with the 20 best in 30 against 27; 16 x 32,000 in 5.1 against 6.1, with the 20
+ * best 12.8 against 11.1. */
 constexpr int kFewRows = 128, kWideRow = 65536;
 
 /** Of a forward pass, whose parts' best entries are at most four a thread of the kernel that joins them. */
@@ -1227,7 +1228,7 @@ auto forward_split_of(int64_t m, int n, int top) -> row_split
 
 /** Whether a gradient is stored through the caches: one of up to half of the last-level cache's 256 MB, that its reader may
  * find there.  A larger one would drive out the logits that a forward pass has left there (4096 x 32,000
- * bfloat16, both directions of log_probs: 139 us in place of 165). */
+ * bfloat16, both directions of log_probs: 135 us in place of 165). */
 auto passes_cache(score_rows const& in) -> bool { return in.m * in.n * elem_size(in.type) <= int64_t{128} << 20; }
 
 /** Rows of few columns take a wavefront each where there are enough of them. */
@@ -1338,8 +1339,8 @@ void launch_distill_backward(score_rows const& in, listed_ids const& ids, teache
 
 constexpr int kHeldThreads = 1024, kHeldPieces = 16;  // of the widest row that a workgroup holds
 
-/** Few wide rows are quicker in parts, by two passes: 1 x 128,000 bfloat16 in 10.7 us against 24, 300 x 100,003 float16 in 42
- * against 47 (but 16 x 32,000 float32 in 11.5 against 10.6, 768 x 128,000 bfloat16 in 97 against 81). */
+/** Few wide rows are quicker in parts, by two passes: 1 x 128,000 bfloat16 in 9.7 us against 23, 300 x 100,003 float16 in 46
+ * against 52 (but 16 x 32,000 float32 in 10.7 against 9.8, 768 x 128,000 bfloat16 in 112 against 93). */
 auto distill_step_held(int64_t m, int n, elem type) -> bool
 {
   const int per = 16 / elem_size(type), pieces = (n + per - 1) / per;

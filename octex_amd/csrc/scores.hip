@@ -214,8 +214,8 @@ constexpr int kPiece = 256;  // bytes of a row that a wavefront multiplies at a 
  * LDS.  A matrix instruction takes 64 columns of 16 rows and 16 queries, so a lane loads 16 bytes of a row, and four such
  * loads cover whole 128-byte lines.  With kFused the queries are floats: the workgroup quantizes them into LDS first.
  *
- * Bound by the rows' bytes: 1 x 1024 x 32,000 (queries, values, rows) takes 6.9 us, 4.7 TB/s; 16 x 4096 x 100,000 98 us,
- * 4.2 TB/s.
+ * Bound by the rows' bytes: 1 x 1024 x 32,000 (queries, values, rows), quantized on the way, takes 9.1 us, 3.6 TB/s; 16 x 4097 x
+ * 100,000, whose rows lie at odd places, 275 us, 1.5 TB/s.
  */
 template <int RT, int KW, bool kFused, typename Q, typename O>
 __global__ __launch_bounds__(64 * KW) void few_scores_kernel(product p, const Q* floats, int64_t fstride, int pitch)
@@ -347,11 +347,11 @@ __device__ inline void wait_loads()
  * from LDS while the matrix cores multiply these; the loads are spread over the step, one or two a matrix instruction, and
  * are waited for by count, at the step's one barrier.
  *
- * Bound by power, as far as it is by one thing: 8192 x 4096 x 16,384 takes 510 us, 2150 TOP/s, with scales, rounding and all
+ * Bound by power, as far as it is by one thing: 8192 x 4096 x 16,384 takes 500 us, 2200 TOP/s, with scales, rounding and all
  * (a library's bare product 498 us), the clock falls to 1.7 GHz and the matrix cores are busy for 62 % of its cycles; matrix
  * instructions alone reach 3000 to 3300 TOP/s.  A part of 4 x 2 reads 3/4 of what two of 2 x 2 read from LDS, and 256 x 256
  * tiles load 2/3 of what 256 x 128 ones do.  Where few values are summed the results' bytes count as much: 1000 x 960 x
- * 100,000 takes 154 us, 1250 TOP/s and 1.9 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 23.6 us, 4.4 TB/s.
+ * 100,000 takes 141 us, 1360 TOP/s and 2.1 TB/s.  Few queries are bound by the rows: 24 x 2048 x 50,000 20.3 us, 5.2 TB/s.
  */
 template <int WM, int WN, int TM, int TN, int kStep, int kAhead, typename O>
 __global__ __launch_bounds__(64 * WM * WN, (160 << 10) / ((kAhead + 1) * (WM * TM + WN * TN) * 32 * kStep) * WM * WN / 4)
@@ -453,8 +453,8 @@ void tiled_scores_kernel(product p, tile_order order)  // registers for as many 
   constexpr int kPieces = kWide / N, kAtOnce = 64 / kPieces;  // of a row; rows that a store of the wavefront covers
   auto* scales = reinterpret_cast<float*>(lds);  // of the tile's rows, then their biases
   auto* biases = scales + BN;
-  // results of whole 64-byte pieces pass by the caches: the 200 MB of 1,000 x 960 x 100,000 in float16 then take 161 us in
-  // place of 177, where pieces at odd places lose (2048 x 512 x 50,000: 110 us against 86)
+  // results of whole 64-byte pieces pass by the caches: the 200 MB of 1,000 x 960 x 100,000 in float16 then take 138 us in
+  // place of 153, where pieces at odd places lose (2048 x 512 x 50,000: 114 us against 102)
   const bool by_cache = (reinterpret_cast<uintptr_t>(p.out) | p.ostride * sizeof(O)) % 64 != 0;
   char* mine          = lds + 2 * BN * sizeof(float) + wave * 32 * kPitch;
   wait_loads<0, true>();  // the steps past the last, which load zeros
@@ -610,13 +610,14 @@ void launch_few(product const& p, const Q* floats, int64_t fstride, hipStream_t 
 /**
  * The tilings, and what each takes: `a` us a column and c us for one tile by itself; with all of its slots (workgroups on the
  * GPU at a time) busy, `rate` operations a us and e us to store a round's results.  Larger tiles load each operand fewer
- * times and smaller ones fill the GPU with less, so a product takes the tiling whose estimate is least.  The numbers are
- * fitted to the times of 21 products whose rows come from memory, and choose the best tiling for these and 5 others (us, of
- * 256 x 256, 256 x 128, 128 x 128 and 64 x 64):
- *   1000 x 960 x 100,000: 159, 178, 220, 291;  512 x 512 x 200,000: 127, 105, 136, 186;  4096 x 4096 x 4096: 68, 81, 95, 120;
- *   2048 x 2048 x 2048: 27, 19, 16, 20;  333 x 1008 x 5003: 20, 12, 11, 9.4;  128 x 4096 x 8192: 43, 28, 22, 14.
- * 256 x 256 tiles have two steps of 64 on their way: with one of 128 the first of these products takes 171 us, 8192 x 4096 x
- * 16,384 539 in place of 522 (but 4096 x 4096 x 4096 65 in place of 68); with three of 64 160, 530 and 69.
+ * times and smaller ones fill the GPU with less, so a product takes the tiling whose estimate is least.  The numbers were
+ * fitted to the times of 21 products whose rows come from memory; of these six they now choose the best tiling for all but the
+ * second, which takes 256 x 128 (us, of 256 x 256, 256 x 128, 128 x 128 and 64 x 64):
+ *   1000 x 960 x 100,000: 141, 166, 212, 282;  512 x 512 x 200,000: 95, 103, 126, 191;  4096 x 4096 x 4096: 62, 76, 84, 110;
+ *   2048 x 2048 x 2048: 24, 19, 14, 19;  333 x 1008 x 5003: 18, 13, 10, 8.8;  128 x 4096 x 8192: 39, 27, 20, 12.7.
+ * No bytes are in the estimate, so it is blind among tilings of a product that is bound by its rows.  256 x 256 tiles have two
+ * steps of 64 on their way: with one of 128 the first of these products took 8 % longer, 8192 x 4096 x 16,384 3 % (but 4096 x
+ * 4096 x 4096 4 % less); with three of 64 all three took 1 % longer.
  */
 struct tiling {
   int bm, bn, slots;
@@ -627,8 +628,8 @@ constexpr tiling kTilings[] = {{256, 256, 256, 8.0, 0.0100, 2.24e9, 10.5},
                                {128, 128, 512, 6.2, 0.0044, 1.50e9, 5.7},
                                {64, 64, 768, 4.5, 0.0023, 1.07e9, 2.6}};
 
-/** Queries that take tiles of 32 x 128, which hold fewer zeros: 24 x 2048 x 50,000 23.6 us, by 64 x 64 28 (but 32 x 4096 x
- * 100,000 102 against 98). */
+/** Queries that take tiles of 32 x 128, which hold fewer zeros: 24 x 2048 x 50,000 20.3 us, by 64 x 64 26.9 (but 32 x 4096 x
+ * 100,000 89 against 87). */
 constexpr int64_t kThinQueries = 32;
 
 auto estimate(tiling const& t, product const& p) -> double
@@ -673,7 +674,7 @@ void launch_pack(pack_job const& job, hipStream_t s)
 }
 
 constexpr int kFewQueries      = 16;                  // a matrix instruction's
-constexpr int64_t kFewRows     = 8192;                // tiles leave half of the GPU idle (1 x 4096 x 5000: 12.2 us, not 7.2)
+constexpr int64_t kFewRows     = 8192;                // tiles leave half of the GPU idle (1 x 4096 x 5000: 12.8 us, not 7.9)
 constexpr int kFewFused        = 8192;                // values up to which each workgroup quantizes all queries itself
 constexpr int64_t kPackedBytes = int64_t{128} << 20;  // of rows laid out anew at a time: they stay in the last-level cache
 

@@ -9,8 +9,8 @@
 Every operator is a hand-written kernel and takes matrices whose rows may lie apart (a slice of a padded vocabulary's
 columns, say).  Operands in GPU memory are read in place: the work is ordered on the first one's stream (torch's current
 stream, or the one its framework names) and not waited for; operands of other streams precede it, and what those streams do
-next comes after it.  Host operands are copied to the GPU and results come back as the first operand is.  Types that an operator does not take are converted, as for a search.  Results carry no autograd graph:
-the gradients have calls of their own.
+next comes after it.  Host operands are copied to the GPU and results come back as the first operand is.  Types that an
+operator does not take are converted, as for a search.  Results carry no autograd graph: the gradients have calls of their own.
 """
 
 import collections
