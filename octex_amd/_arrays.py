@@ -41,14 +41,17 @@ def _hip_stream_of_cai(code):
 
 def named_stream(a):
     """The stream that a foreign device array names: the interface's own 'stream' entry, else the current stream of its
-    framework when the framework has that notion (CuPy); None if neither is there."""
+    framework when the framework has that notion (CuPy).  None if neither is there and its export (DLPack) orders it; an
+    interface of a version before the entry is ordered on the null stream."""
     cai = getattr(a, "__cuda_array_interface__", None)
     if cai is not None and "stream" in cai:
         return _hip_stream_of_cai(cai["stream"])
     mod = sys.modules.get(_module_of(a))
     cuda = getattr(mod, "cuda", None)
     get = getattr(cuda, "get_current_stream", None)
-    return int(get().ptr) if callable(get) else None
+    if callable(get):
+        return int(get().ptr)
+    return _HIP_NULL_STREAM if cai is not None and not hasattr(a, "__dlpack__") else None
 
 
 def _foreign_stream(a):

@@ -67,6 +67,25 @@ def test_torch_operands_of_a_torch_call(call):
     assert notes[1:] == ["current waits for third", "launch", "third waits for current"]
 
 
+class Older:
+    """An interface of a version that had no stream yet."""
+
+    __cuda_array_interface__ = dict(shape=(2, 2), typestr="<f4", data=(0, False), version=2)
+
+
+class OlderWithExport(Older):
+    def __dlpack__(self, **kw):
+        raise NotImplementedError
+
+
+def test_interfaces_without_a_stream_are_ordered_on_the_null_stream(call):
+    assert _arrays.named_stream(Older()) == 0 and _arrays.named_stream(OlderWithExport()) is None
+    c, notes, _ = call
+    c.array(Older()), c.array(OlderWithExport())
+    c.run("any")
+    assert notes == ["side waits for null", "launch", "null waits for side"]
+
+
 def test_named_streams():
     assert _arrays.named_stream(Interface(1)) == 0 and _arrays.named_stream(Interface(9)) == 9
     assert _arrays.named_stream(Interface(None)) is None and _arrays.named_stream(object()) is None
