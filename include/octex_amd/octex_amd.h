@@ -278,6 +278,72 @@ cuvsError_t octexDistillStep(const octexMatrix* logits, const octexMatrix* ids, 
                              float temperature, const float* grad_loss, float* loss, float* lse, const octexMatrix* grad,
                              void* workspace, int64_t bytes, int64_t* size, void* stream);
 
+/**
+ * A policy's clipped loss on rows of logits x [m, n] (float32, float16 or bfloat16; n at most 2^30), p = softmax(x /
+ * temperature), whose ids [m, 1] (int32 or int64) were sampled with old_log_probs [m] and earned advantages [m]: with
+ * r = exp(log p of the id - old) and d = ref_log_probs - log p of the id,
+ *   loss[i] = -min(r A, clip(r, low, high) A) + kl (exp(d) - 1 - d) - entropy_weight * entropy,  0 <= low <= 1 <= high.
+ * ref_log_probs [m] may be NULL if kl is 0.  log_probs, entropy and lse [m] as octexLogProbs gives them.  A row whose id lies
+ * outside [0, n) is padding: it is not read and has 0 everywhere.  An id whose logit is -inf has r = 0; with a KL term its loss
+ * is inf and its row's gradient not finite.  A NaN or +inf makes its row NaN.  All vectors are float32 and dense; `workspace`
+ * and `size` as for octexInt8Scores.
+ */
+cuvsError_t octexPolicyLoss(const octexMatrix* logits, const octexMatrix* ids, float temperature, const float* old_log_probs,
+                            const float* advantages, const float* ref_log_probs, float low, float high, float kl,
+                            float entropy_weight, float* loss, float* log_probs, float* entropy, float* lse, void* workspace,
+                            int64_t bytes, int64_t* size, void* stream);
+
+/** grad [m, n] (the logits' type) of sum(grad_loss * loss) by the logits; log_probs, entropy and lse as octexPolicyLoss gave
+ * them.  A ratio that passes its bound on the side where the loss is clipped has no gradient, one at the bound has. */
+cuvsError_t octexPolicyLossBackward(const octexMatrix* logits, const octexMatrix* ids, float temperature,
+                                    const float* old_log_probs, const float* advantages, const float* ref_log_probs, float low,
+                                    float high, float kl, float entropy_weight, const float* grad_loss, const float* log_probs,
+                                    const float* entropy, const float* lse, const octexMatrix* grad, void* stream);
+
+/** octexPolicyLoss and octexPolicyLossBackward in one call. */
+cuvsError_t octexPolicyLossStep(const octexMatrix* logits, const octexMatrix* ids, float temperature,
+                                const float* old_log_probs, const float* advantages, const float* ref_log_probs, float low,
+                                float high, float kl, float entropy_weight, const float* grad_loss, float* loss,
+                                float* log_probs, float* entropy, float* lse, const octexMatrix* grad, void* workspace,
+                                int64_t bytes, int64_t* size, void* stream);
+
+/**
+ * The balance of rows over e experts (at most 2048) from their logits x [m, e] (float32, float16 or bfloat16), p = softmax(x),
+ * and the experts that the rows chose, experts [m, k] (int32 or int64; k at most 512; ids outside [0, e) are no choice):
+ *   loss = weight * e * sum_v f_v P_v + z_weight * (sum of lse^2) / rows,
+ * f_v expert v's share of all choices, P_v its mean probability over the rows that count, those with a choice.  counts [e] are
+ * the experts' choices, rows [1] the rows that count, probs [e] = P, lse [m] = ln sum exp(x), 0 of rows that do not count.  A
+ * row of nothing but -inf has p = 0 and lse -inf, which is left out of the loss; a NaN or +inf makes the loss NaN.
+ * With grad [m, e] (the logits' type) not NULL also the gradient of grad_loss * loss by the logits, for which the choices are
+ * constants; grad_loss [1] (NULL: 1) is float32 in GPU memory.  No rows at all have loss 0.  `workspace` and `size` as for
+ * octexInt8Scores.
+ */
+cuvsError_t octexBalanceLoss(const octexMatrix* logits, const octexMatrix* experts, float weight, float z_weight, float* loss,
+                             int64_t* counts, int64_t* rows, float* probs, float* lse, const float* grad_loss,
+                             const octexMatrix* grad, void* workspace, int64_t bytes, int64_t* size, void* stream);
+
+/** The gradient alone, from octexBalanceLoss's counts and rows, or from their sums over the ranks of a job. */
+cuvsError_t octexBalanceLossBackward(const octexMatrix* logits, const octexMatrix* experts, float weight, float z_weight,
+                                     const int64_t* counts, const int64_t* rows, const float* grad_loss,
+                                     const octexMatrix* grad, void* stream);
+
+/**
+ * out [m, d] (float32, float16 or bfloat16) = scale * table[ids], of a table [n, d] (float32, float16 or bfloat16, or int8 with
+ * row_scales [n], which multiply their rows) and ids [m, 1] (int32 or int64).  Ids outside [0, n) give rows of 0.  The products
+ * are float32: scale * row_scales first, then with the value.  m and n below 2^31, d at most 2^24.
+ */
+cuvsError_t octexEmbed(const octexMatrix* table, const float* row_scales, const octexMatrix* ids, float scale,
+                       const octexMatrix* out, void* stream);
+
+/**
+ * The gradient of a table's rows, out [n, d] (float32, float16 or bfloat16): out[v] = scale * the sum of grad[i] over the i with
+ * ids[i] = v, grad [m, d] (float32, float16 or bfloat16), or with `add` not 0 that much more than it held, rows without an id
+ * then staying as they are.  Sums are float32, in an order that the ids alone determine, and rounded once.  Ids outside [0, n)
+ * are left out.  `workspace` and `size` as for octexInt8Scores.
+ */
+cuvsError_t octexEmbedBackward(const octexMatrix* grad, const octexMatrix* ids, float scale, int32_t add,
+                               const octexMatrix* out, void* workspace, int64_t bytes, int64_t* size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

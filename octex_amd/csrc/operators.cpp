@@ -1,13 +1,17 @@
 // C entries of the operators on rows of scores (octex_amd/octex_amd.h): arguments checked, the operands' GPU made current,
 // the kernels launched on the caller's stream.  No call waits or allocates.
 
+#include "balance.hpp"
 #include "common.hpp"
+#include "policy.hpp"
 #include "rows.hpp"
 #include "scores.hpp"
+#include "table.hpp"
 
 #include <cuvs/core/c_api.h>
 #include <octex_amd/octex_amd.h>
 
+#include <algorithm>
 #include <cmath>
 #include <exception>
 
@@ -288,5 +292,227 @@ extern "C" cuvsError_t octexDistillStep(const octexMatrix* logits, const octexMa
     if (id.k > 0) gpu.take(id.ids, "ids"), gpu.take(t.x, "teacher");
     launch_distill_step(in, id, t, grad_loss, loss, lse, grad->data, grad->stride, workspace,
                         static_cast<hipStream_t>(stream));
+  });
+}
+
+namespace {
+
+/** The ids of a policy's rows: one a row. */
+auto row_ids_of(const octexMatrix* ids, int64_t m) -> listed_ids
+{
+  shape(ids, "ids", m, 1);
+  return ids_of(ids, m);
+}
+
+auto terms_of(const float* sampled, const float* advantages, const float* reference, float low, float high, float kl,
+              float entropy) -> policy_terms
+{
+  OCTEX_EXPECTS(low >= 0.f && low <= 1.f && high >= 1.f, "octex: a ratio is clipped to bounds from 0 to 1 and from 1 on");
+  OCTEX_EXPECTS(std::isfinite(kl) && std::isfinite(entropy), "octex: the weights of the KL and entropy terms must be finite");
+  OCTEX_EXPECTS(kl == 0.f || reference != nullptr, "octex: the KL term needs ref_log_probs");
+  return {sampled, advantages, kl != 0.f ? reference : nullptr, low, high, kl, entropy};
+}
+
+void take_terms(on_gpu& gpu, score_rows const& in, listed_ids const& ids, policy_terms const& t)
+{
+  gpu.take(in.x, "logits"), gpu.take(ids.ids, "ids"), gpu.take(t.sampled, "old_log_probs");
+  gpu.take(t.advantages, "advantages");
+  if (t.reference != nullptr) gpu.take(t.reference, "ref_log_probs");
+}
+
+void take_results(on_gpu& gpu, policy_out const& out)
+{
+  gpu.take(out.loss, "loss"), gpu.take(out.logp, "log_probs"), gpu.take(out.entropy, "entropy"), gpu.take(out.lse, "lse");
+}
+
+/** Logits over experts and the rows' choices of them. */
+auto experts_of(const octexMatrix* logits, const octexMatrix* experts, score_rows& in) -> listed_ids
+{
+  in = logits_of(logits, 1.f);
+  OCTEX_EXPECTS(in.n <= kMaxExperts, "octex: at most %d experts, not %d", kMaxExperts, in.n);
+  shape(experts, "experts", in.m, -1);
+  OCTEX_EXPECTS(experts->type == OCTEX_INT32 || experts->type == OCTEX_INT64, "octex: experts must be int32 or int64");
+  OCTEX_EXPECTS(experts->cols <= kMaxListed, "octex: at most %d experts a row, not %lld", kMaxListed,
+                static_cast<long long>(experts->cols));
+  OCTEX_EXPECTS(in.m * std::max<int64_t>(experts->cols, 1) <= INT32_MAX, "octex: at most 2^31 - 1 choices");
+  return {experts->data, experts->type == OCTEX_INT64, experts->stride, static_cast<int>(experts->cols)};
+}
+
+auto weights_of(float balance, float z) -> balance_weights
+{
+  OCTEX_EXPECTS(std::isfinite(balance) && std::isfinite(z), "octex: the balance's weights must be finite");
+  return {balance, z};
+}
+
+auto table_ids(const octexMatrix* ids, int64_t m) -> row_ids
+{
+  shape(ids, "ids", m, 1);
+  OCTEX_EXPECTS(ids->type == OCTEX_INT32 || ids->type == OCTEX_INT64, "octex: ids must be int32 or int64");
+  return {ids->data, ids->type == OCTEX_INT64, ids->stride, ids->rows};
+}
+
+void table_size(int64_t m, int64_t n, int64_t d)
+{
+  OCTEX_EXPECTS(m <= INT32_MAX && n <= INT32_MAX, "octex: at most 2^31 - 1 ids and rows");
+  OCTEX_EXPECTS(d <= kMaxRowWidth, "octex: rows of at most %lld values, not %lld", static_cast<long long>(kMaxRowWidth),
+                static_cast<long long>(d));
+}
+
+}  // namespace
+
+extern "C" cuvsError_t octexPolicyLoss(const octexMatrix* logits, const octexMatrix* ids, float temperature,
+                                       const float* old_log_probs, const float* advantages, const float* ref_log_probs,
+                                       float low, float high, float kl, float entropy_weight, float* loss, float* log_probs,
+                                       float* entropy, float* lse, void* workspace, int64_t bytes, int64_t* size, void* stream)
+{
+  return run([&] {
+    const auto in = logits_of(logits, temperature);
+    const auto id = row_ids_of(ids, in.m);
+    const auto t  = terms_of(old_log_probs, advantages, ref_log_probs, low, high, kl, entropy_weight);
+    const int64_t need = in.m == 0 ? 0 : policy_workspace(in.m, in.n);
+    if (asked_size(need, bytes, size)) return;
+    if (in.m == 0) return;
+    const policy_out out{loss, log_probs, entropy, lse};
+    on_gpu gpu;
+    take_workspace(gpu, workspace, need);
+    take_terms(gpu, in, id, t), take_results(gpu, out);
+    launch_policy(in, id, t, out, workspace, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" cuvsError_t octexPolicyLossBackward(const octexMatrix* logits, const octexMatrix* ids, float temperature,
+                                               const float* old_log_probs, const float* advantages,
+                                               const float* ref_log_probs, float low, float high, float kl,
+                                               float entropy_weight, const float* grad_loss, const float* log_probs,
+                                               const float* entropy, const float* lse, const octexMatrix* grad, void* stream)
+{
+  return run([&] {
+    const auto in = logits_of(logits, temperature);
+    const auto id = row_ids_of(ids, in.m);
+    const auto t  = terms_of(old_log_probs, advantages, ref_log_probs, low, high, kl, entropy_weight);
+    grad_of(grad, logits);
+    if (in.m == 0) return;
+    on_gpu gpu;
+    take_terms(gpu, in, id, t);
+    gpu.take(grad_loss, "grad_loss"), gpu.take(log_probs, "log_probs"), gpu.take(entropy, "entropy"), gpu.take(lse, "lse");
+    gpu.take(grad->data, "grad");
+    // what a forward pass gave is read only
+    const policy_out saved{nullptr, const_cast<float*>(log_probs), const_cast<float*>(entropy), const_cast<float*>(lse)};
+    launch_policy_backward(in, id, t, saved, grad_loss, grad->data, grad->stride, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" cuvsError_t octexPolicyLossStep(const octexMatrix* logits, const octexMatrix* ids, float temperature,
+                                           const float* old_log_probs, const float* advantages, const float* ref_log_probs,
+                                           float low, float high, float kl, float entropy_weight, const float* grad_loss,
+                                           float* loss, float* log_probs, float* entropy, float* lse, const octexMatrix* grad,
+                                           void* workspace, int64_t bytes, int64_t* size, void* stream)
+{
+  return run([&] {
+    const auto in = logits_of(logits, temperature);
+    const auto id = row_ids_of(ids, in.m);
+    const auto t  = terms_of(old_log_probs, advantages, ref_log_probs, low, high, kl, entropy_weight);
+    grad_of(grad, logits);
+    const int64_t need = in.m == 0 || policy_step_held(in.m, in.n, in.type) ? 0 : policy_workspace(in.m, in.n);
+    if (asked_size(need, bytes, size)) return;
+    if (in.m == 0) return;
+    const policy_out out{loss, log_probs, entropy, lse};
+    on_gpu gpu;
+    take_workspace(gpu, workspace, need);
+    take_terms(gpu, in, id, t), take_results(gpu, out);
+    gpu.take(grad_loss, "grad_loss"), gpu.take(grad->data, "grad");
+    launch_policy_step(in, id, t, grad_loss, out, grad->data, grad->stride, workspace, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" cuvsError_t octexBalanceLoss(const octexMatrix* logits, const octexMatrix* experts, float weight, float z_weight,
+                                        float* loss, int64_t* counts, int64_t* rows, float* probs, float* lse,
+                                        const float* grad_loss, const octexMatrix* grad, void* workspace, int64_t bytes,
+                                        int64_t* size, void* stream)
+{
+  return run([&] {
+    score_rows in{};
+    const auto id = experts_of(logits, experts, in);
+    const auto w  = weights_of(weight, z_weight);
+    if (grad != nullptr) grad_of(grad, logits);
+    const int64_t need = balance_workspace(in.m, in.n, id.k, in.type);
+    if (asked_size(need, bytes, size)) return;
+    on_gpu gpu;
+    gpu.take(loss, "loss"), gpu.take(counts, "counts"), gpu.take(rows, "rows"), gpu.take(probs, "probs");
+    take_workspace(gpu, workspace, need);
+    if (in.m > 0) {
+      gpu.take(in.x, "logits"), gpu.take(lse, "lse");
+      if (id.k > 0) gpu.take(id.ids, "experts");
+      if (grad != nullptr) gpu.take(grad->data, "grad");
+    }
+    if (grad_loss != nullptr) gpu.take(grad_loss, "grad_loss");
+    launch_balance(in, id, w, {loss, counts, rows, probs, lse}, grad_loss, grad != nullptr ? grad->data : nullptr,
+                   grad != nullptr ? grad->stride : 0, workspace, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" cuvsError_t octexBalanceLossBackward(const octexMatrix* logits, const octexMatrix* experts, float weight,
+                                                float z_weight, const int64_t* counts, const int64_t* rows,
+                                                const float* grad_loss, const octexMatrix* grad, void* stream)
+{
+  return run([&] {
+    score_rows in{};
+    const auto id = experts_of(logits, experts, in);
+    const auto w  = weights_of(weight, z_weight);
+    grad_of(grad, logits);
+    if (in.m == 0) return;
+    on_gpu gpu;
+    gpu.take(in.x, "logits"), gpu.take(counts, "counts"), gpu.take(rows, "rows"), gpu.take(grad->data, "grad");
+    if (id.k > 0) gpu.take(id.ids, "experts");
+    if (grad_loss != nullptr) gpu.take(grad_loss, "grad_loss");
+    launch_balance_backward(in, id, w, counts, rows, grad_loss, grad->data, grad->stride, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" cuvsError_t octexEmbed(const octexMatrix* table, const float* row_scales, const octexMatrix* ids, float scale,
+                                  const octexMatrix* out, void* stream)
+{
+  return run([&] {
+    shape(table, "table", -1, -1);
+    const bool coded = table->type == OCTEX_INT8;
+    OCTEX_EXPECTS(coded || is_float(*table), "octex: the table must be int8, float32, float16 or bfloat16");
+    OCTEX_EXPECTS(coded || row_scales == nullptr, "octex: only int8 rows have row_scales");
+    const auto id = table_ids(ids, -1);
+    shape(out, "out", id.m, table->cols);
+    float_type(*out, "out");
+    table_size(id.m, table->rows, table->cols);
+    if (id.m == 0 || table->cols == 0) return;
+    on_gpu gpu;
+    gpu.take(id.ids, "ids"), gpu.take(out->data, "out");
+    if (table->rows > 0) {
+      gpu.take(table->data, "table");
+      if (coded) gpu.take(row_scales, "row_scales");
+    }
+    launch_embed({table->data, elem_of(*table), table->rows, table->stride, row_scales}, id, table->cols, scale,
+                 {out->data, elem_of(*out), out->stride}, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" cuvsError_t octexEmbedBackward(const octexMatrix* grad, const octexMatrix* ids, float scale, int32_t add,
+                                          const octexMatrix* out, void* workspace, int64_t bytes, int64_t* size, void* stream)
+{
+  return run([&] {
+    shape(grad, "grad", -1, -1);
+    float_type(*grad, "grad");
+    const auto id = table_ids(ids, grad->rows);
+    shape(out, "out", -1, grad->cols);
+    float_type(*out, "out");
+    const int64_t n = out->rows, d = grad->cols;
+    table_size(id.m, n, d);
+    const bool none    = n == 0 || d == 0 || (add != 0 && id.m == 0);
+    const int64_t need = none ? 0 : embed_backward_workspace(id.m, n, d);
+    if (asked_size(need, bytes, size)) return;
+    if (none) return;
+    on_gpu gpu;
+    gpu.take(out->data, "out");
+    take_workspace(gpu, workspace, need);
+    if (id.m > 0) gpu.take(grad->data, "grad"), gpu.take(id.ids, "ids");
+    launch_embed_backward({grad->data, elem_of(*grad), grad->stride}, id, n, d, scale, add != 0,
+                          {out->data, elem_of(*out), out->stride}, workspace, static_cast<hipStream_t>(stream));
   });
 }

@@ -1,0 +1,43 @@
+// Launchers of rows of a table by ids, and of the table's gradient (table.hip).  Shapes, types and pointers are checked by the
+// callers (operators.cpp).
+#pragma once
+
+#include "rows.hpp"
+
+namespace cuvs::neighbors::octex::detail {
+
+constexpr int64_t kMaxRowWidth = int64_t{1} << 24;  // values of a row: its slices are a grid's second dimension
+
+/** A table [n, d], rows `stride` apart; scales [n] of int8 rows, else null. */
+struct table_rows {
+  const void* x;
+  elem type;
+  int64_t n, stride;
+  const float* scales;
+};
+
+/** m ids, `stride` apart; ids outside [0, n) are padding. */
+struct row_ids {
+  const void* ids;
+  bool wide;  // int64, else int32
+  int64_t stride, m;
+};
+
+/** A matrix of rows of d values that is read or written. */
+struct value_rows {
+  void* x;
+  elem type;
+  int64_t stride;
+};
+
+/** out[i] = scale * table[ids[i]], padding 0. */
+void launch_embed(table_rows const& table, row_ids const& ids, int64_t d, float scale, value_rows const& out, hipStream_t s);
+
+/** The bytes of workspace (at a multiple of 256) that launch_embed_backward needs. */
+auto embed_backward_workspace(int64_t m, int64_t n, int64_t d) -> int64_t;
+
+/** out[v] = scale * the sum of grad[i] with ids[i] = v, of n rows; with `add` that much more than it held. */
+void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n, int64_t d, float scale, bool add,
+                           value_rows const& out, void* workspace, hipStream_t s);
+
+}  // namespace cuvs::neighbors::octex::detail

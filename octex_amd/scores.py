@@ -5,6 +5,8 @@
     r = octex.log_probs(logits, ids, top=10)                         # log p of given ids, entropy, alternatives
     distances, neighbors = index.search(queries, k=10)               # a teacher: its nearest rows ...
     loss, grad = octex.distill_step(weights, logits, neighbors, -distances, temperature=2.0)   # ... and the lesson
+    r, grad = octex.policy_step(weights, logits, ids, old, advantages)   # or one from rewards: a policy's clipped loss
+    r, grad = octex.balance_step(None, router, experts, weight=0.01)     # rows spread evenly over experts or shards
 
 Every operator is a hand-written kernel and takes matrices whose rows may lie apart (a slice of a padded vocabulary's
 columns, say).  Operands in GPU memory are read in place: the work is ordered on the first one's stream (torch's current
@@ -28,6 +30,8 @@ INTS = ("int64", "int32")
 _TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3, "int32": 4, "int64": 5}
 
 LogProbs = collections.namedtuple("LogProbs", "log_probs entropy lse top_log_probs top_ids")
+PolicyLoss = collections.namedtuple("PolicyLoss", "loss log_probs entropy lse")
+BalanceLoss = collections.namedtuple("BalanceLoss", "loss counts rows probs lse")
 
 
 class _Matrix(ct.Structure):
@@ -40,6 +44,7 @@ class _Matrix(ct.Structure):
 _P, _I32, _I64, _F = ct.c_void_p, ct.c_int32, ct.c_int64, ct.c_float
 _M = ct.POINTER(_Matrix)
 _SIZED = [_P, _I64, _P]  # workspace, bytes, size
+_POLICY = [_M, _M, _F, _P, _P, _P, _F, _F, _F, _F]  # logits, ids, temperature, a row's terms, bounds and weights
 _ENTRIES = {
     "octexQuantizeRows": [_M, _M, _P],
     "octexInt8Scores": [_M, _P, _M, _P, _P, _M] + _SIZED,
@@ -48,6 +53,13 @@ _ENTRIES = {
     "octexDistill": [_M, _M, _M, _F, _P, _P] + _SIZED,
     "octexDistillBackward": [_M, _M, _M, _F, _P, _P, _M],
     "octexDistillStep": [_M, _M, _M, _F, _P, _P, _P, _M] + _SIZED,
+    "octexPolicyLoss": _POLICY + [_P, _P, _P, _P] + _SIZED,
+    "octexPolicyLossBackward": _POLICY + [_P, _P, _P, _P, _M],
+    "octexPolicyLossStep": _POLICY + [_P, _P, _P, _P, _P, _M] + _SIZED,
+    "octexBalanceLoss": [_M, _M, _F, _F, _P, _P, _P, _P, _P, _P, _M] + _SIZED,
+    "octexBalanceLossBackward": [_M, _M, _F, _F, _P, _P, _P, _M],
+    "octexEmbed": [_M, _P, _M, _F, _M],
+    "octexEmbedBackward": [_M, _M, _F, _I32, _M] + _SIZED,
 }
 
 
@@ -77,7 +89,7 @@ class _Call:
 
     __slots__ = ("torch", "names", "origin", "device", "stream", "side", "others", "on_host", "foreign", "first", "scratch")
 
-    def __init__(self, first, name, types):
+    def __init__(self, first, name, types, flat=False):
         self.torch, self.names, raw_stream = _torch()
         self.origin, self.side, self.others = first, None, ()
         self.foreign = not isinstance(first, self.torch.Tensor) and _arrays.is_foreign_device(first)
@@ -89,6 +101,9 @@ class _Call:
             named = _arrays.named_stream(first)
             if named is not None and named != self.stream:
                 self.stream, self.side = named, self.external(named)
+        if flat and t.ndim > 2:  # all but the last dimension are one
+            with self.context():
+                t = t.reshape(-1, t.shape[-1])
         self.first = self.take(t, name, types)
 
     def view(self, a):
@@ -139,7 +154,7 @@ class _Call:
             with self.context():
                 t = t.to(self.device)
         if self.names.get(t.dtype) not in types:
-            if types == ("int8",) or (types is INTS and t.is_floating_point()):
+            if types in (("int8",), ("int64",)) or (types is INTS and t.is_floating_point()):
                 raise TypeError(f"octex: {name} must be {' or '.join(types)}, not {str(t.dtype).replace('torch.', '')}")
             with self.context():
                 t = t.to(getattr(torch, types[0]))
@@ -240,6 +255,18 @@ def quantize_rows(x):
     return c.give(codes), c.give(scales)
 
 
+def _float_type(c, dtype, what, of):
+    """The torch type that `dtype` (a name, numpy's or torch's type) asks for."""
+    if not isinstance(dtype, str):
+        dtype = np.dtype(dtype).name if isinstance(dtype, (type, np.dtype)) else str(dtype)
+    dtype = dtype.replace("torch.", "")
+    if dtype not in FLOATS:
+        raise ValueError(f"octex: {what} are of type {', '.join(FLOATS)}, not {dtype}")
+    if dtype == "bfloat16" and c.on_host and not isinstance(c.origin, c.torch.Tensor):
+        raise TypeError(f"octex: numpy has no bfloat16 for the {what} of its {of}")
+    return getattr(c.torch, dtype)
+
+
 def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtype=None):
     """The scores [m, n] of every query against every row, a product in 8-bit integers:
     scores[i, j] = query_scales[i] * row_scales[j] * sum(queries[i] * rows[j]) + bias[j].
@@ -265,14 +292,7 @@ def int8_scores(queries, rows, row_scales, *, query_scales=None, bias=None, dtyp
         bias = c.dense(bias, "bias", (n,))
     if dtype is None:
         dtype = "float32" if coded else c.names[q.dtype]
-    if not isinstance(dtype, str):
-        dtype = np.dtype(dtype).name if isinstance(dtype, (type, np.dtype)) else str(dtype)
-    dtype = dtype.replace("torch.", "")
-    if dtype not in FLOATS:
-        raise ValueError(f"octex: scores are of type {', '.join(FLOATS)}, not {dtype}")
-    if dtype == "bfloat16" and c.on_host and not isinstance(queries, c.torch.Tensor):
-        raise TypeError("octex: numpy has no bfloat16 for the scores of its queries")
-    out = c.new((m, n), dtype=getattr(c.torch, dtype))
+    out = c.new((m, n), dtype=_float_type(c, dtype, "scores", "queries"))
     c.run_sized("octexInt8Scores", c.matrix(q), query_scales.data_ptr() if coded else None, c.matrix(rows),
                 row_scales.data_ptr(), None if bias is None else bias.data_ptr(), c.matrix(out))
     return c.give(out)
@@ -385,3 +405,128 @@ def distill_step(grad_loss, logits, ids, teacher, *, temperature=1.0):
     c.run_sized("octexDistillStep", c.matrix(x), c.matrix(t), c.matrix(teacher), float(temperature), g.data_ptr(),
                 loss.data_ptr(), lse.data_ptr(), c.matrix(grad))
     return c.give(loss), c.give(grad)
+
+
+def _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, entropy, temperature):
+    """A call on a policy's rows: its operands, and the arguments that all of its entries begin with."""
+    c = _Call(logits, "logits", FLOATS)
+    x = c.first
+    m = x.shape[0]
+    t = c.take(_columns(c, ids)[0], "ids", INTS, shape=(m, 1))
+    terms = [c.dense(old_log_probs, "old_log_probs", (m,)), c.dense(advantages, "advantages", (m,))]
+    if kl != 0 and ref_log_probs is not None:
+        terms.append(c.dense(ref_log_probs, "ref_log_probs", (m,)))
+    low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    args = (c.matrix(x), c.matrix(t), float(temperature), terms[0].data_ptr(), terms[1].data_ptr(),
+            terms[2].data_ptr() if len(terms) > 2 else None, 1.0 - low, 1.0 + high, float(kl), float(entropy))
+    return c, x, (t, terms), args
+
+
+def policy_loss(logits, ids, old_log_probs, advantages, *, ref_log_probs=None, clip=0.2, kl=0.0, entropy=0.0, temperature=1.0):
+    """A policy's clipped loss on rows of logits [m, n]: of the id that each row sampled, ids [m], its log probability then,
+    old_log_probs [m], and its advantage A [m]; with p = softmax(logits / temperature), r = p of the id / exp(old) and
+    d = ref_log_probs - ln p of the id,
+
+        loss = -min(r A, clip(r, 1 - low, 1 + high) A) + kl (exp(d) - 1 - d) - entropy H(p).
+
+    `clip` is (low, high), or one number for both.  The KL term holds the policy to a reference model, whose log probabilities
+    [m] it needs; at kl = 0 they are not read.  Returns PolicyLoss(loss, log_probs, entropy, lse), float32 [m] each.
+
+    A row whose id lies outside [0, n), a prompt's token say, is padding: it is not read and has 0 everywhere.  An id whose
+    logit is -inf has r = 0; with a KL term its loss is inf and its row's gradient not finite.  A row with a NaN or +inf is NaN.
+    """
+    c, x, keep, args = _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, entropy, temperature)
+    r = PolicyLoss(*c.new(*[(x.shape[0],)] * 4))
+    c.run_sized("octexPolicyLoss", *args, *[v.data_ptr() for v in r])
+    return PolicyLoss(*map(c.give, r))
+
+
+def policy_loss_backward(grad_loss, logits, ids, old_log_probs, advantages, result, *, ref_log_probs=None, clip=0.2, kl=0.0,
+                         entropy=0.0, temperature=1.0):
+    """The gradient by the logits of sum(grad_loss * loss), in the logits' type; `result` is policy_loss's of the same operands.
+
+    A ratio beyond its bound, on the side where the loss is clipped, has no gradient; one at the bound has.
+    """
+    c, x, keep, args = _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, entropy, temperature)
+    shape = (x.shape[0],)
+    g = c.dense(grad_loss, "grad_loss", shape)
+    saved = [c.dense(getattr(result, name), name, shape) for name in ("log_probs", "entropy", "lse")]
+    grad = c.like(x)
+    c.run("octexPolicyLossBackward", *args, g.data_ptr(), *[v.data_ptr() for v in saved], c.matrix(grad))
+    return c.give(grad)
+
+
+def policy_step(grad_loss, logits, ids, old_log_probs, advantages, *, ref_log_probs=None, clip=0.2, kl=0.0, entropy=0.0,
+                temperature=1.0):
+    """(PolicyLoss, grad): policy_loss and policy_loss_backward in one call, which reads the logits less often."""
+    c, x, keep, args = _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, entropy, temperature)
+    g = c.dense(grad_loss, "grad_loss", (x.shape[0],))
+    r, grad = PolicyLoss(*[c.like(g) for _ in range(4)]), c.like(x)
+    c.run_sized("octexPolicyLossStep", *args, g.data_ptr(), *[v.data_ptr() for v in r], c.matrix(grad))
+    return PolicyLoss(*map(c.give, r)), c.give(grad)
+
+
+def _balance(logits, experts):
+    c = _Call(logits, "logits", FLOATS)
+    t = c.take(_columns(c, experts)[0], "experts", INTS)
+    if t.shape[0] != c.first.shape[0]:
+        raise ValueError(f"octex: experts of {t.shape[0]} rows, logits of {c.first.shape[0]}")
+    return c, c.first, t
+
+
+def _one(c, a, name, types):
+    """One number, as an array of no dimension or one."""
+    return c.take(c.array(a).reshape(-1), name, types, 1, (1,))
+
+
+def _balance_results(c, x):
+    m, e = x.shape
+    counts, rows = c.new((e,), (), dtype=c.torch.int64)
+    loss, probs, lse = c.new((), (e,), (m,))
+    return BalanceLoss(loss, counts, rows, probs, lse)
+
+
+def balance_loss(logits, experts, *, weight=1.0, z_weight=0.0):
+    """How evenly rows are spread over experts (parts of a model, or shards of an index), from their logits [m, e] (e at most
+    2048) and the experts that they chose, [m] or [m, k], log_probs' top_ids say:
+
+        loss = weight e sum(f P) + z_weight mean(lse^2),
+
+    f the experts' shares of all choices, P their mean probabilities under softmax(logits).  Returns BalanceLoss(loss, counts,
+    rows, probs, lse): the loss and the number of rows that count as arrays of no dimension, the experts' choices [e] (int64),
+    P [e], and the rows' log-sum-exp [m].
+
+    Ids outside [0, e) are no choice (one that found its expert full); a row without a choice (a batch's padding) does not
+    count: its lse is 0.  Logits of -inf have probability 0; a row of nothing else adds nothing to P or the loss.  A NaN or
+    +inf makes the loss NaN.
+    """
+    c, x, t = _balance(logits, experts)
+    r = _balance_results(c, x)
+    c.run_sized("octexBalanceLoss", c.matrix(x), c.matrix(t), float(weight), float(z_weight), *[v.data_ptr() for v in r], None, None)
+    return BalanceLoss(*map(c.give, r))
+
+
+def balance_loss_backward(grad_loss, logits, experts, result, *, weight=1.0, z_weight=0.0):
+    """The gradient by the logits of grad_loss * loss, in the logits' type; the choices are constants.
+
+    grad_loss is one number, as an array (None: 1).  `result` is balance_loss's of the same operands; one whose counts and rows
+    were added up over the ranks of a job gives the gradient of the job's balance.
+    """
+    c, x, t = _balance(logits, experts)
+    g = None if grad_loss is None else _one(c, grad_loss, "grad_loss", ("float32",))
+    counts = c.take(c.array(result.counts), "counts", ("int64",), 1, (x.shape[1],))
+    rows = _one(c, result.rows, "rows", ("int64",))
+    grad = c.like(x)
+    c.run("octexBalanceLossBackward", c.matrix(x), c.matrix(t), float(weight), float(z_weight), counts.data_ptr(),
+          rows.data_ptr(), None if g is None else g.data_ptr(), c.matrix(grad))
+    return c.give(grad)
+
+
+def balance_step(grad_loss, logits, experts, *, weight=1.0, z_weight=0.0):
+    """(BalanceLoss, grad): balance_loss and balance_loss_backward in one call, which reads the logits once."""
+    c, x, t = _balance(logits, experts)
+    g = None if grad_loss is None else _one(c, grad_loss, "grad_loss", ("float32",))
+    r, grad = _balance_results(c, x), c.like(x)
+    c.run_sized("octexBalanceLoss", c.matrix(x), c.matrix(t), float(weight), float(z_weight), *[v.data_ptr() for v in r],
+                None if g is None else g.data_ptr(), c.matrix(grad))
+    return BalanceLoss(*map(c.give, r)), c.give(grad)
