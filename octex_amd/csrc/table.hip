@@ -28,20 +28,20 @@ struct unit {
   unsigned w[kWords];
 };
 
-/** The values of a row from `from` on; of a row of d < kUnit all of them, and 0 behind its end. */
-template <typename T>
+/** The values of a row from `from` on; of a row of d < kUnit (kShort) all of them, and 0 behind its end. */
+template <bool kShort, typename T>
 __device__ inline auto load_unit(const T* row, int from, int d) -> unit<T>
 {
   unit<T> u;
-  if (d >= kUnit) {
-    __builtin_memcpy(u.w, row + from, sizeof(u.w));
-    return u;
-  }
-  T e[kUnit];
+  if constexpr (kShort) {
+    T e[kUnit];
 #pragma unroll
-  for (int i = 0; i < kUnit; ++i)
-    e[i] = i < d ? row[i] : T{};
-  __builtin_memcpy(u.w, e, sizeof(u.w));
+    for (int i = 0; i < kUnit; ++i)
+      e[i] = i < d ? row[i] : T{};
+    __builtin_memcpy(u.w, e, sizeof(u.w));
+  } else {
+    __builtin_memcpy(u.w, row + from, sizeof(u.w));
+  }
   return u;
 }
 
@@ -65,45 +65,55 @@ __device__ inline void unpack_unit(unit<T> const& u, float (&v)[kUnit])
   }
 }
 
-/** The columns of the unit at `at` (a multiple of kUnit): where the row ends inside, the unit's values are those of the row's
- * last columns, of which the ones before `at` are another lane's. */
+/** Where a lane finds its unit at the column `at` (a multiple of kUnit): one that would pass the row's end is moved back to it, so
+ * that columns before `at` are another lane's too. */
 __device__ inline auto unit_start(int at, int d) -> int { return max(min(at, d - kUnit), 0); }
 
-template <typename T>
-__device__ inline void store_unit(T* row, const float (&v)[kUnit], int at, int d, bool by_cache)
+/** Stores a unit; lanes that have a column twice store it alike. */
+template <bool kShort, typename T>
+__device__ inline void store_unit(T* row, const float (&v)[kUnit], int from, int d, bool by_cache)
 {
   constexpr int N = kPer16<T>;
-  if (at + kUnit > d) {
+  if constexpr (kShort) {
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) {
-      const int column = unit_start(at, d) + i;
-      if (column >= at && column < d) row[column] = static_cast<T>(v[i]);
+    for (int i = 0; i < kUnit; ++i)
+      if (i < d) row[i] = static_cast<T>(v[i]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kUnit / N; ++j) {
+      float e[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        e[i] = v[j * N + i];
+      if (by_cache)
+        store16(row + from + j * N, pack16<T>(e));
+      else
+        store16_nt(row + from + j * N, pack16<T>(e));
     }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < kUnit / N; ++j) {
-    float e[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      e[i] = v[j * N + i];
-    if (by_cache)
-      store16(row + at + j * N, pack16<T>(e));
-    else
-      store16_nt(row + at + j * N, pack16<T>(e));
   }
 }
 
-__device__ inline auto id_of(row_ids const& ids, int64_t i) -> int64_t
+/** The ids at places i0 + q * step, clamped to the last one: all of them on their way at once. */
+template <int N>
+__device__ inline void read_ids(row_ids const& ids, int64_t i0, int64_t step, int64_t (&id)[N])
 {
-  return ids.wide ? static_cast<const int64_t*>(ids.ids)[i * ids.stride] : static_cast<const int32_t*>(ids.ids)[i * ids.stride];
+  if (ids.wide) {
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      id[q] = static_cast<const int64_t*>(ids.ids)[min(i0 + q * step, ids.m - 1) * ids.stride];
+  } else {
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      id[q] = static_cast<const int32_t*>(ids.ids)[min(i0 + q * step, ids.m - 1) * ids.stride];
+  }
 }
 
 constexpr int kRowsAhead = 4;  // rows that a team has on their way
 
 /**
- * Teams of W lanes take kRowsAhead rows each, a unit a lane (of the slice blockIdx.y of their columns): all ids first, then
- * all rows, then the results.
+ * Teams of W lanes (1: of rows shorter than a unit) take kRowsAhead rows each, a unit a lane (of the slice blockIdx.y of their
+ * columns): all ids first, then all rows, then the results.  No load waits for a condition: padding takes the table's first row
+ * and drops it.
  */
 template <typename T, typename O, int W>
 __global__ __launch_bounds__(kThreads) void embed_kernel(table_rows table, row_ids ids, int d, float scale, O* out,
@@ -112,39 +122,36 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(table_rows table, row_i
   constexpr int kTeams = kThreads / W;
   const int at         = (static_cast<int>(blockIdx.y) * W + static_cast<int>(threadIdx.x) % W) * kUnit;
   const int64_t i0     = ((block0 + blockIdx.x) * kTeams + threadIdx.x / W) * kRowsAhead;
-  if (at >= d) return;
+  if (at >= d || i0 >= ids.m) return;
   const int from = unit_start(at, d);
   int64_t id[kRowsAhead];
   float s[kRowsAhead];
-  unit<T> u[kRowsAhead];
+  unit<T> u[kRowsAhead] = {};
+  read_ids(ids, i0, 1, id);
+  if (table.n > 0) {
 #pragma unroll
-  for (int q = 0; q < kRowsAhead; ++q) {
-    id[q] = i0 + q < ids.m ? id_of(ids, i0 + q) : -1;
-    if (id[q] >= table.n) id[q] = -1;
-  }
-#pragma unroll
-  for (int q = 0; q < kRowsAhead; ++q) {
-    if (id[q] < 0) continue;
-    u[q] = load_unit(static_cast<const T*>(table.x) + id[q] * table.stride, from, d);
-    s[q] = sizeof(T) == 1 ? scale * table.scales[id[q]] : scale;
+    for (int q = 0; q < kRowsAhead; ++q) {
+      const int64_t v = id[q] < 0 || id[q] >= table.n ? 0 : id[q];
+      u[q]            = load_unit<W == 1>(static_cast<const T*>(table.x) + v * table.stride, from, d);
+      s[q]            = sizeof(T) == 1 ? scale * table.scales[v] : scale;
+    }
   }
 #pragma unroll
   for (int q = 0; q < kRowsAhead; ++q) {
     if (i0 + q >= ids.m) break;
+    const bool listed = id[q] >= 0 && id[q] < table.n;
     float v[kUnit];
-    if (id[q] >= 0) unpack_unit(u[q], v);
+    unpack_unit(u[q], v);
 #pragma unroll
     for (int i = 0; i < kUnit; ++i)
-      v[i] = id[q] >= 0 ? v[i] * s[q] : 0.f;
-    store_unit(out + (i0 + q) * ostride, v, at, d, by_cache);
+      v[i] = listed ? v[i] * s[q] : 0.f;
+    store_unit<W == 1>(out + (i0 + q) * ostride, v, from, d, by_cache);
   }
 }
 
 // ---- tokens sorted by id
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kSortTile    = 4096;  // tokens of a workgroup
-constexpr int kSortPer     = kSortTile / kSortThreads;
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 
 /** A token: its row of the table (n: padding) and its place. */
@@ -153,29 +160,49 @@ struct token {
   int place;
 };
 
-__device__ inline auto token_of(row_ids const& ids, int64_t n, int64_t i) -> token
+__device__ inline auto row_of(int64_t id, unsigned n) -> unsigned { return id < 0 || id >= n ? n : static_cast<unsigned>(id); }
+
+/** A thread's tokens of the tile of kSortThreads * P places from `first` on: those at wave's first + 64 q + lane, so that ranks
+ * by wavefront, q and lane are ranks by place.  Past the end their place is -1. */
+template <int P>
+__device__ inline auto my_place(int64_t first) -> int64_t
 {
-  const int64_t id = id_of(ids, i);
-  return {static_cast<unsigned>(id < 0 || id >= n ? n : id), static_cast<int>(i)};
+  return first + threadIdx.x / 64 * (64 * P) + threadIdx.x % 64;
 }
 
-/** Tokens [wave's first + 64 q + lane] of a tile, row ~0 past the end. */
-template <typename F>
-__device__ inline void read_tile(int64_t first, int64_t m, token (&t)[kSortPer], F read)
+template <int P>
+__device__ inline void read_tile(row_ids const& ids, unsigned n, const token* in, int64_t first, token (&t)[P])
 {
-  const int64_t mine = first + threadIdx.x / 64 * (64 * kSortPer) + threadIdx.x % 64;
+  const int64_t mine = my_place<P>(first);
+  if (in != nullptr) {
 #pragma unroll
-  for (int q = 0; q < kSortPer; ++q)
-    t[q] = mine + 64 * q < m ? read(mine + 64 * q) : token{~0u, -1};
+    for (int q = 0; q < P; ++q)
+      t[q] = in[min(mine + 64 * q, ids.m - 1)];
+  } else {  // a first pass
+    int64_t id[P];
+    read_ids(ids, mine, 64, id);
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+      t[q] = {row_of(id[q], n), static_cast<int>(mine + 64 * q)};
+  }
+#pragma unroll
+  for (int q = 0; q < P; ++q)
+    if (mine + 64 * q >= ids.m) t[q].place = -1;
 }
+
+/** A digit of a token's row: `bits` (at most kDigitBits) from `shift` on. */
+struct digit {
+  int shift, bits;
+
+  __device__ auto of(token const& t) const -> unsigned { return t.row >> shift & ((1u << bits) - 1); }
+};
 
 /** The lanes of the wavefront that have a token of the same digit. */
-__device__ inline auto same_digit(unsigned digit, bool has) -> unsigned long long
+__device__ inline auto same_digit(unsigned value, int bits, bool has) -> unsigned long long
 {
   unsigned long long same = __ballot(has);
-#pragma unroll
-  for (int b = 0; b < kDigitBits; ++b) {
-    const bool one                = digit >> b & 1;
+  for (int b = 0; b < bits; ++b) {
+    const bool one                = value >> b & 1;
     const unsigned long long ones = __ballot(one);
     same &= one ? ones : ~ones;
   }
@@ -190,18 +217,20 @@ __device__ inline auto lanes_below(unsigned long long lanes) -> int
 
 /** The ranks of a tile's tokens among those of the same digit and wavefront, whose numbers they leave in counts (LDS, 0
  * before). */
-__device__ inline void rank_tile(const token (&t)[kSortPer], int shift, int (*counts)[kDigits], int (&rank)[kSortPer])
+template <int P>
+__device__ inline void rank_tile(const token (&t)[P], digit d, int (*counts)[kDigits], int (&rank)[P])
 {
   int* mine = counts[threadIdx.x / 64];
 #pragma unroll
-  for (int q = 0; q < kSortPer; ++q) {
-    const unsigned digit = t[q].row >> shift & (kDigits - 1);
-    const bool has       = t[q].place >= 0;
-    const auto same      = same_digit(digit, has);
+  for (int q = 0; q < P; ++q) {
+    const bool has = t[q].place >= 0;
+    if (__ballot(has) == 0) break;
+    const unsigned value = d.of(t[q]);
+    const auto same      = same_digit(value, d.bits, has);
     const int below      = lanes_below(same);
-    const int before     = has ? mine[digit] : 0;
+    const int before     = has ? mine[value] : 0;
     wave_fence();
-    if (has && below == 0) mine[digit] = before + __popcll(same);
+    if (has && below == 0) mine[value] = before + __popcll(same);
     wave_fence();
     rank[q] = before + below;
   }
@@ -232,102 +261,139 @@ __device__ inline auto scan_digits(int v, int* sums) -> int
   return before + sum - v;
 }
 
-/** Turns the wavefronts' counts into the places at which their tokens of a digit start; base: of the tile's, a thread's digit. */
-__device__ inline void start_waves(int (*counts)[kDigits], int base)
+/** The wavefronts' counts of a thread's digit, and their sum. */
+__device__ inline auto wave_counts(int (*counts)[kDigits], int (&c)[kSortWaves]) -> int
 {
-  if (threadIdx.x < kDigits) {
-    for (int w = 0; w < kSortWaves; ++w) {
-      const int c            = counts[w][threadIdx.x];
-      counts[w][threadIdx.x] = base;
-      base += c;
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w)
+    sum += c[w] = threadIdx.x < kDigits ? counts[w][threadIdx.x] : 0;
+  return sum;
+}
+
+/** Turns them into the places at which the wavefronts' tokens of the digit start. */
+__device__ inline void start_waves(int (*counts)[kDigits], const int (&c)[kSortWaves], int base)
+{
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) {
+    if (threadIdx.x < kDigits) counts[w][threadIdx.x] = base;
+    base += c[w];
+  }
+}
+
+/** A share of the table's gradient that is set to 0 beside a step of the sort: [first, first + bytes) of dense rows, by `blocks`
+ * workgroups. */
+struct fill_share {
+  char* first;
+  int64_t bytes;
+  unsigned blocks;
+};
+
+constexpr int kFillBytes = 64 << 10;  // that a workgroup fills at a time
+
+/** A workgroup's part of the share: whole 16-byte pieces but for the ends. */
+__device__ inline void fill(fill_share const& f, unsigned block)
+{
+  const auto lead = static_cast<int64_t>(reinterpret_cast<uintptr_t>(f.first) % 16);
+  for (int64_t base = int64_t{block} * kFillBytes - lead; base < f.bytes; base += int64_t{f.blocks} * kFillBytes) {
+#pragma unroll
+    for (int q = 0; q < kFillBytes / 16 / kSortThreads; ++q) {
+      const int64_t at = base + (q * kSortThreads + static_cast<int>(threadIdx.x)) * 16;
+      if (at >= 0 && at + 16 <= f.bytes) {
+        store16(f.first + at, uint4{0, 0, 0, 0});
+      } else {
+        for (int64_t j = max(at, int64_t{0}); j < min(at + 16, f.bytes); j += 2)
+          *reinterpret_cast<uint16_t*>(f.first + j) = 0;
+      }
     }
   }
 }
 
-__device__ inline auto wave_total(int (*counts)[kDigits]) -> int
+/** Up to kSortThreads * P tokens by the first workgroup, all of their `bits` in `passes`; the others fill. */
+template <int P>
+__global__ __launch_bounds__(kSortThreads) void sort_alone_kernel(row_ids ids, unsigned n, int passes, int bits, token* out,
+                                                                  fill_share share)
 {
-  int sum = 0;
-  if (threadIdx.x < kDigits)
-    for (int w = 0; w < kSortWaves; ++w)
-      sum += counts[w][threadIdx.x];
-  return sum;
-}
-
-/** Up to kSortTile tokens by one workgroup, all digits. */
-__global__ __launch_bounds__(kSortThreads) void sort_alone_kernel(row_ids ids, int64_t n, int passes, token* out)
-{
+  if (blockIdx.x > 0) return fill(share, blockIdx.x - 1);
   __shared__ int counts[kSortWaves][kDigits];
-  __shared__ token tokens[kSortTile];
+  __shared__ token tokens[kSortThreads * P];
   __shared__ int sums[kDigits / 64];
-  token t[kSortPer];
-  int rank[kSortPer];
-  read_tile(0, ids.m, t, [&](int64_t i) { return token_of(ids, n, i); });
+  token t[P];
+  int rank[P], c[kSortWaves];
+  read_tile<P>(ids, n, nullptr, 0, t);
   for (int p = 0; p < passes; ++p) {
-    const int shift = p * kDigitBits;
+    const digit d{p * bits, bits};
     clear_counts(counts);
     lds_barrier();
-    rank_tile(t, shift, counts, rank);
+    rank_tile<P>(t, d, counts, rank);
     lds_barrier();
-    start_waves(counts, scan_digits(wave_total(counts), sums));
+    start_waves(counts, c, scan_digits(wave_counts(counts, c), sums));
+    lds_barrier();
+    token* const to = p + 1 < passes ? tokens : out;
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+      if (t[q].place >= 0) to[counts[threadIdx.x / 64][d.of(t[q])] + rank[q]] = t[q];
+    if (p + 1 == passes) return;
     lds_barrier();
 #pragma unroll
-    for (int q = 0; q < kSortPer; ++q)
-      if (t[q].place >= 0) tokens[counts[threadIdx.x / 64][t[q].row >> shift & (kDigits - 1)] + rank[q]] = t[q];
-    lds_barrier();
-    read_tile(0, ids.m, t, [&](int64_t i) { return tokens[i]; });
+    for (int q = 0; q < P; ++q) {
+      const int64_t mine = my_place<P>(0) + 64 * q;
+      t[q]               = tokens[mine];
+      if (mine >= ids.m) t[q].place = -1;
+    }
     lds_barrier();
   }
-  const int64_t mine = threadIdx.x / 64 * (64 * kSortPer) + threadIdx.x % 64;
-#pragma unroll
-  for (int q = 0; q < kSortPer; ++q)
-    if (t[q].place >= 0) out[mine + 64 * q] = t[q];
 }
 
-/** The numbers of a tile's tokens of each digit: tiles [gridDim, kDigits]. */
-__global__ __launch_bounds__(kSortThreads) void count_digits_kernel(row_ids ids, int64_t n, const token* in, int shift,
-                                                                    int* tiles)
+/** The numbers of a tile's tokens of each digit: tiles [n_tiles, kDigits]; workgroups behind those fill. */
+template <int P>
+__global__ __launch_bounds__(kSortThreads) void count_digits_kernel(row_ids ids, unsigned n, const token* in, digit d,
+                                                                    int* tiles, unsigned n_tiles, fill_share share)
 {
+  if (blockIdx.x >= n_tiles) return fill(share, blockIdx.x - n_tiles);
   __shared__ int counts[kDigits];
   if (threadIdx.x < kDigits) counts[threadIdx.x] = 0;
   lds_barrier();
-  token t[kSortPer];
-  read_tile(int64_t{blockIdx.x} * kSortTile, ids.m, t,
-            [&](int64_t i) { return in != nullptr ? in[i] : token_of(ids, n, i); });
+  token t[P];
+  read_tile<P>(ids, n, in, int64_t{blockIdx.x} * (kSortThreads * P), t);
 #pragma unroll
-  for (int q = 0; q < kSortPer; ++q)
-    if (t[q].place >= 0) atomicAdd(counts + (t[q].row >> shift & (kDigits - 1)), 1);
+  for (int q = 0; q < P; ++q)
+    if (t[q].place >= 0) atomicAdd(counts + d.of(t[q]), 1);
   lds_barrier();
   if (threadIdx.x < kDigits) tiles[int64_t{blockIdx.x} * kDigits + threadIdx.x] = counts[threadIdx.x];
 }
 
 /** Moves a tile's tokens to their places by one digit; every workgroup adds up the tiles' counts itself. */
-__global__ __launch_bounds__(kSortThreads) void move_tokens_kernel(row_ids ids, int64_t n, const token* in, int shift,
-                                                                   const int* tiles, token* out)
+template <int P>
+__global__ __launch_bounds__(kSortThreads) void move_tokens_kernel(row_ids ids, unsigned n, const token* in, digit d,
+                                                                   const int* tiles, token* out, unsigned n_tiles,
+                                                                   fill_share share)
 {
+  if (blockIdx.x >= n_tiles) return fill(share, blockIdx.x - n_tiles);
   __shared__ int counts[kSortWaves][kDigits];
   __shared__ int sums[kDigits / 64];
-  token t[kSortPer];
-  int rank[kSortPer];
-  read_tile(int64_t{blockIdx.x} * kSortTile, ids.m, t,
-            [&](int64_t i) { return in != nullptr ? in[i] : token_of(ids, n, i); });
+  token t[P];
+  int rank[P], c[kSortWaves];
+  read_tile<P>(ids, n, in, int64_t{blockIdx.x} * (kSortThreads * P), t);
   clear_counts(counts);
   int before = 0, all = 0;
   if (threadIdx.x < kDigits) {
-#pragma unroll 8
-    for (unsigned b = 0; b < gridDim.x; ++b) {
-      const int c = tiles[int64_t{b} * kDigits + threadIdx.x];
-      all += c;
-      before += b < blockIdx.x ? c : 0;
+#pragma unroll 16
+    for (unsigned b = 0; b < n_tiles; ++b) {
+      const int count = tiles[int64_t{b} * kDigits + threadIdx.x];
+      all += count;
+      before += b < blockIdx.x ? count : 0;
     }
   }
   const int base = scan_digits(all, sums) + before;
-  rank_tile(t, shift, counts, rank);
+  rank_tile<P>(t, d, counts, rank);
   lds_barrier();
-  start_waves(counts, base);
+  (void)wave_counts(counts, c);
+  start_waves(counts, c, base);
   lds_barrier();
 #pragma unroll
-  for (int q = 0; q < kSortPer; ++q)
-    if (t[q].place >= 0) out[counts[threadIdx.x / 64][t[q].row >> shift & (kDigits - 1)] + rank[q]] = t[q];
+  for (int q = 0; q < P; ++q)
+    if (t[q].place >= 0) out[counts[threadIdx.x / 64][d.of(t[q])] + rank[q]] = t[q];
 }
 
 // ---- the sums of sorted tokens
@@ -337,199 +403,352 @@ __global__ __launch_bounds__(kSortThreads) void move_tokens_kernel(row_ids ids, 
  * run that came from before at 0, of one that begins here at 1. */
 struct sorted_tokens {
   const token* t;
-  int64_t m, n;
+  int64_t m;
+  unsigned n;
   int width;
   float* cut;
 
-  __device__ auto row(int64_t i) const -> int64_t { return t[i].row; }
-  /** Whether the run at the last place before the border b goes on behind it. */
-  __device__ auto crosses(int64_t b) const -> bool { return b < m && row(b) == row(b - 1); }
-  /** Whether the run of `row`, which begins in the chunk before the border b and crosses it, is cut. */
-  __device__ auto is_cut(int64_t b, int64_t of) const -> bool { return b + width < m && row(b + width) == of; }
+  /** The row of a token, of the first or last one for places that there are not. */
+  __device__ auto row(int64_t i) const -> unsigned { return t[max(min(i, m - 1), int64_t{0})].row; }
+};
+
+/** What a chunk [b, e) has to do with the runs at its borders. */
+struct chunk_runs {
+  int64_t b, e;
+  unsigned first, last;  // rows of its first and last token
+  bool before;           // the first run came from the chunk before
+  bool head;             // and is cut
+  bool tail;             // the last run begins here and is cut
+  bool goes_on;          // the last run begins here and ends in the next chunk
+
+  __device__ chunk_runs(sorted_tokens const& s, int64_t chunk)
+  {
+    b = chunk * s.width, e = min(b + s.width, s.m);
+    first = s.row(b), last = s.row(e - 1);
+    const unsigned back = s.row(b - 1), far_back = s.row(b - s.width - 1), ahead = s.row(e), far_ahead = s.row(e + s.width);
+    before             = b > 0 && back == first && first < s.n;
+    const bool crosses = e < s.m && ahead == last && last < s.n;
+    const bool through = before && crosses && first == last;  // the whole chunk is a cut run's
+    head               = before && (through || (b > s.width && far_back == first));
+    tail               = crosses && !through && e + s.width < s.m && far_ahead == last;
+    goes_on            = crosses && !through && !tail;
+  }
 };
 
 constexpr int kTokensAhead = 8;  // whose gradients a team has on their way
 
-template <typename O>
-__device__ inline void write_sum(const float (&sum)[kUnit], float scale, bool add, O* row, int at, int d, bool by_cache)
+/** The same in every lane: of teams of 64 lanes, in a scalar register. */
+template <int W, typename V>
+__device__ inline auto of_team(V v) -> V
 {
+  if constexpr (W == 64) return static_cast<V>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+  return v;
+}
+
+/** Tokens [p, p + kTokensAhead), the last one again past the end. */
+template <int W>
+__device__ inline void read_tokens(sorted_tokens const& s, int64_t p, token (&t)[kTokensAhead])
+{
+#pragma unroll
+  for (int q = 0; q < kTokensAhead; ++q)
+    t[q] = s.t[min(p + q, s.m - 1)];
+}
+
+/** The end of the run of `row` that holds place p, or `end`; a team's lanes look side by side. */
+template <int W>
+__device__ inline auto run_end(sorted_tokens const& s, int64_t p, int64_t end, unsigned row) -> int64_t
+{
+  const int lane = threadIdx.x % 64, sub = lane % W;
+  for (;; p += W) {
+    const unsigned long long in = __ballot(p + sub < end && s.row(p + sub) == row) >> (lane - sub);
+    const int n                 = __builtin_ctzll(~in | (W < 64 ? 1ull << (W % 64) : 0));
+    if (W == 64 ? in != ~0ull : n < W) return p + n;
+  }
+}
+
+/** Stores scale * sum, or what the row holds and that.  A column that two lanes have is added to by the one that has it first. */
+template <bool kShort, typename O>
+__device__ inline void write_sum(const float (&sum)[kUnit], float scale, bool add, O* row, int at, int d)
+{
+  if (at >= d) return;
+  const int from = unit_start(at, d);
   float v[kUnit];
 #pragma unroll
   for (int i = 0; i < kUnit; ++i)
     v[i] = sum[i] * scale;
-  if (add) {
-    float old[kUnit];
-    unpack_unit(load_unit(row, unit_start(at, d), d), old);
+  if (!add) return store_unit<kShort>(row, v, from, d, true);
+  float old[kUnit];
+  unpack_unit(load_unit<kShort>(row, from, d), old);
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i)
-      v[i] += old[i];
-  }
-  store_unit(row, v, at, d, by_cache);
+  for (int i = 0; i < kUnit; ++i)
+    v[i] += old[i];
+  if (from == at) return store_unit<kShort>(row, v, from, d, true);
+  for (int i = 0; i < kUnit; ++i)
+    if (from + i >= at) row[from + i] = static_cast<O>(v[i]);
 }
 
-/** Sets the rows [v0, v0 + rows) that have no token to 0; a thread looks for each. */
+/** Sets the elements [j0, j1) of d-wide dense rows to 0 whose row is not used; the first of them is in row r, at col. */
 template <typename O>
-__device__ inline void clear_rows(sorted_tokens const& s, int64_t v0, int rows, int d, O* out, int64_t ostride, bool by_cache)
+__device__ inline void clear_elements(const bool* used, O* x, int j0, int j1, int r, int col, int d)
+{
+  for (int j = j0; j < j1; ++j) {
+    for (; col >= d; col -= d)
+      ++r;
+    if (!used[r]) x[j] = static_cast<O>(0.f);
+    ++col;
+  }
+}
+
+/**
+ * Sets the rows [v0, v0 + rows) that are not used (LDS, in v0's order) to 0.  Dense rows are one stretch of memory, in which a
+ * wavefront's pieces of 16 bytes fill whole lines wherever rows begin; rows that lie apart are taken one by one.
+ */
+template <typename O>
+__device__ inline void clear_rows(const bool* used, int64_t v0, int rows, int d, O* out, int64_t ostride)
 {
   constexpr int N = kPer16<O>;
-  __shared__ bool used[kThreads];
-  if (static_cast<int>(threadIdx.x) < rows) {
-    const int64_t v = v0 + threadIdx.x;
-    int64_t lo = 0, hi = s.m;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (s.row(mid) < v)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    used[threadIdx.x] = lo < s.m && s.row(lo) == v;
+  O* const base   = out + v0 * ostride;
+  if (ostride != d) {
+    for (int r = 0; r < rows; ++r)
+      for (int j = threadIdx.x; !used[r] && j < d; j += kThreads)
+        base[r * ostride + j] = static_cast<O>(0.f);
+    return;
   }
-  lds_barrier();
-  const int pieces = (d + N - 1) / N;
-  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
-    const int r = i / pieces, at = (i - r * pieces) * N;
-    if (used[r]) continue;
-    O* row = out + (v0 + r) * ostride;
-    if (d < N) {
-      for (int j = 0; j < d; ++j)
-        row[j] = static_cast<O>(0.f);
-    } else if (by_cache) {
-      store16(row + min(at, d - N), uint4{0, 0, 0, 0});
-    } else {
-      store16_nt(row + min(at, d - N), uint4{0, 0, 0, 0});
+  const int total = rows * d, before = static_cast<int>(reinterpret_cast<uintptr_t>(base) % 1024 / sizeof(O));
+  const int step_rows = kThreads * N / d, step_cols = kThreads * N - step_rows * d;
+  int x = static_cast<int>(threadIdx.x) * N - before;
+  if (x + N <= 0) x += kThreads * N;
+  int r = max(x, 0) / d, col = x - r * d;  // below 0 where the first row begins inside the piece
+  for (; x < total; x += kThreads * N) {
+    const bool inside = x >= 0 && x + N <= total;
+    if (inside && (col + N <= d ? !used[r] : N <= d && !used[r] && !used[r + 1])) {
+      store16(base + x, uint4{0, 0, 0, 0});
+    } else if (!inside || col + N > d) {
+      const int j0 = max(-x, 0);
+      clear_elements(used, base + x, j0, min(N, total - x), r, col + j0, d);
     }
+    r += step_rows;
+    col += step_cols;
+    if (col >= d) col -= d, ++r;
+    for (; col < 0; col += d)
+      --r;
   }
 }
 
 /**
  * The sums of the runs of a chunk each, by teams of W lanes, a unit a lane (of one of `slices` slices of their columns), the
- * gradients of kTokensAhead tokens on their way at a time.  Workgroups from `sum_blocks` on clear `clear` rows each.
+ * gradients of kTokensAhead tokens on their way at a time.
  */
 template <typename T, typename O, int W>
 __global__ __launch_bounds__(kThreads) void sum_runs_kernel(sorted_tokens s, const T* grad, int64_t gstride, int d, float scale,
-                                                            bool add, O* out, int64_t ostride, bool by_cache,
-                                                            unsigned slices, unsigned sum_blocks, int clear)
+                                                            bool add, O* out, int64_t ostride, unsigned slices)
 {
-  if (blockIdx.x >= sum_blocks) {
-    const int64_t v0 = int64_t{blockIdx.x - sum_blocks} * clear;
-    return clear_rows(s, v0, static_cast<int>(min(s.n - v0, int64_t{clear})), d, out, ostride, by_cache);
-  }
   constexpr int kTeams = kThreads / W;
-  const int64_t chunk  = int64_t{blockIdx.x / slices} * kTeams + threadIdx.x / W;
-  const int at         = (static_cast<int>(blockIdx.x % slices) * W + static_cast<int>(threadIdx.x) % W) * kUnit;
-  const int64_t b = chunk * s.width, e = min(b + s.width, s.m);
-  if (b >= s.m || at >= d) return;
-  const int64_t first = s.row(b), last = s.row(e - 1);
-  if (first >= s.n) return;  // padding, to the end
-  const int from        = unit_start(at, d);
-  const bool before     = b > 0 && s.row(b - 1) == first;
-  const bool crosses    = last < s.n && s.crosses(e);
-  const bool through    = before && crosses && first == last;  // the whole chunk is a cut run's
-  const bool tail       = crosses && !through && s.is_cut(e, last);
-  const bool goes_on    = crosses && !through && !tail;  // the last run ends in the next chunk
-  bool head             = before && (through || (b > s.width && s.row(b - s.width - 1) == first));
-  int64_t p             = b;
-  if (before && !head)  // the chunk before has it
-    while (p < e && s.row(p) == first)
-      ++p;
-  float* cut      = s.cut + chunk * 2 * d;
-  int64_t current = -1;
+  const int64_t team   = int64_t{blockIdx.x} * kTeams + of_team<W>(static_cast<int>(threadIdx.x) / W);
+  const int64_t chunk  = team / slices;  // a workgroup's teams take slices side by side
+  const int at         = (static_cast<int>(team - chunk * slices) * W + static_cast<int>(threadIdx.x) % W) * kUnit;
+  if (chunk * s.width >= s.m) return;  // a team's lanes without a column go along, and write nothing
+  const chunk_runs c(s, chunk);
+  if (c.first >= s.n) return;  // padding, to the end
+  const int from = unit_start(at, d);
+  float* cut     = s.cut + chunk * 2 * d;
   float sum[kUnit];
-  // the place of the sum's run: what came from before, what is cut behind, or the row itself
-  const auto flush = [&](bool at_end) {
-    if (current < 0) return;
-    if (head)
-      write_sum(sum, 1.f, false, cut, at, d, true);
-    else if (at_end && tail)
-      write_sum(sum, 1.f, false, cut + d, at, d, true);
-    else
-      write_sum(sum, scale, add, out + current * ostride, at, d, by_cache);
-    head = false;
-  };
-  const auto token_at = [&](int64_t i) {
-    token t = i < s.m ? s.t[i] : token{~0u, 0};
-    if (t.row >= s.n || (i >= e && !(goes_on && t.row == last))) t.row = ~0u;
-    return t;
-  };
-  token next[kTokensAhead];
-#pragma unroll
-  for (int q = 0; q < kTokensAhead; ++q)
-    next[q] = token_at(p + q);
-  while (next[0].row != ~0u) {
-    token t[kTokensAhead];
-    unit<T> u[kTokensAhead];
-#pragma unroll
-    for (int q = 0; q < kTokensAhead; ++q) {
-      t[q] = next[q];
-      if (t[q].row != ~0u) u[q] = load_unit(grad + t[q].place * gstride, from, d);
-    }
-    p += kTokensAhead;
+  unit<T> u[kTokensAhead];
+  token t[kTokensAhead];
+  // the gradients of the tokens in hand; of those that are not taken the first one's again
+  const auto load = [&](const bool (&taken)[kTokensAhead]) {
 #pragma unroll
     for (int q = 0; q < kTokensAhead; ++q)
-      next[q] = token_at(p + q);
+      u[q] = load_unit<W == 1>(grad + of_team<W>(taken[q] ? t[q].place : t[0].place) * gstride, from, d);
+  };
+  // the part of a cut run that lies in this chunk from p on; returns its end
+  const auto sum_part = [&](int64_t p, unsigned row, float* to) {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+      sum[i] = 0.f;
+    for (bool more = true; more; p += kTokensAhead) {
+      read_tokens<W>(s, p, t);
+      bool taken[kTokensAhead];
+#pragma unroll
+      for (int q = 0; q < kTokensAhead; ++q)
+        taken[q] = p + q < c.e && t[q].row == row;
+      load(taken);
+#pragma unroll
+      for (int q = 0; q < kTokensAhead; ++q) {
+        float v[kUnit];
+        unpack_unit(u[q], v);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i)
+          sum[i] += taken[q] ? v[i] : 0.f;
+      }
+      more = taken[kTokensAhead - 1];
+    }
+    write_sum<W == 1>(sum, 1.f, false, to, at, d);
+  };
+  int64_t p = c.b;
+  if (c.head) sum_part(p, c.first, cut);
+  if (c.before) p = run_end<W>(s, p, c.e, c.first);  // of a run that is not cut the chunk before has all
+  const auto taken_at = [&](int64_t i, unsigned row) {
+    return row < s.n && (i < c.e ? !(c.tail && row == c.last) : i < s.m && c.goes_on && row == c.last);
+  };
+  token next[kTokensAhead];
+  read_tokens<W>(s, p, next);
+  unsigned current = ~0u;
+  bool full         = true;  // so far
+  while (full && taken_at(p, next[0].row)) {
+    bool taken[kTokensAhead];
 #pragma unroll
     for (int q = 0; q < kTokensAhead; ++q) {
-      if (t[q].row == ~0u) break;
+      t[q]     = {of_team<W>(next[q].row), of_team<W>(next[q].place)};
+      taken[q] = taken_at(p + q, t[q].row);
+    }
+    load(taken);
+    read_tokens<W>(s, p + kTokensAhead, next);
+#pragma unroll
+    for (int q = 0; q < kTokensAhead; ++q) {
+      if (!taken[q]) break;
+      ++p;
       float v[kUnit];
       unpack_unit(u[q], v);
-      if (t[q].row != current) {
-        flush(false);
-        current = t[q].row;
+      const bool same = t[q].row == current;
+      if (!same && current != ~0u) write_sum<W == 1>(sum, scale, add, out + current * ostride, at, d);
+      current = t[q].row;
 #pragma unroll
-        for (int i = 0; i < kUnit; ++i)
-          sum[i] = v[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i)
-          sum[i] += v[i];
-      }
+      for (int i = 0; i < kUnit; ++i)
+        sum[i] = same ? sum[i] + v[i] : v[i];
     }
+    full = taken[kTokensAhead - 1];
   }
-  flush(true);
+  if (current != ~0u) write_sum<W == 1>(sum, scale, add, out + current * ostride, at, d);
+  if (c.tail) sum_part(p, c.last, cut + d);
 }
 
 constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
 
-/** Joins the sums of the run that begins in a chunk and is cut, if one is; 64 units of its columns a workgroup. */
-template <typename O>
+/** Joins the sums of the runs that begin in the chunks of a workgroup, one a wavefront to look at, and are cut; 64 units of their
+ * columns a workgroup. */
+template <typename O, bool kShort>
 __global__ __launch_bounds__(kJoinThreads) void join_runs_kernel(sorted_tokens s, int d, float scale, bool add, O* out,
-                                                                 int64_t ostride, bool by_cache, int64_t chunk0)
+                                                                 int64_t ostride, int64_t chunks, int64_t block0)
 {
   __shared__ float sums[kJoinWaves][64][kUnit];
-  const int64_t chunk = chunk0 + blockIdx.x, b = chunk * s.width, e = b + s.width;
-  if (e >= s.m) return;
-  const int64_t last = s.row(e - 1);
-  if (last >= s.n || !s.crosses(e) || !s.is_cut(e, last)) return;
-  if (s.row(b) == last && b > 0 && s.row(b - 1) == last) return;  // it came from before
+  __shared__ unsigned rows[kJoinWaves];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int at = (static_cast<int>(blockIdx.y) * 64 + lane) * kUnit, from = unit_start(at, d);
+  const int at = (static_cast<int>(blockIdx.y) * 64 + lane) * kUnit;
+  const int64_t chunk0 = (block0 + blockIdx.x) * kJoinWaves;
+  if (lane == 0) {
+    rows[wave] = ~0u;
+    if (chunk0 + wave < chunks) {
+      const chunk_runs c(s, chunk0 + wave);
+      if (c.tail) rows[wave] = c.last;
+    }
+  }
+  lds_barrier();
+  for (int j = 0; j < kJoinWaves; ++j) {
+    const unsigned row = rows[j];
+    if (row == ~0u) continue;
+    const int64_t chunk = chunk0 + j;
+    float sum[kUnit];
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+      sum[i] = 0.f;
+    const auto take = [&](const float* part) {
+      float v[kUnit];
+      unpack_unit(load_unit<kShort>(part, unit_start(at, d), d), v);
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i)
+        sum[i] += v[i];
+    };
+    if (wave == 0) take(s.cut + (chunk * 2 + 1) * d);
+    for (int64_t part = chunk + 1 + wave; part * s.width < s.m && s.row(part * s.width) == row; part += kJoinWaves)
+      take(s.cut + part * 2 * d);
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+      sums[wave][lane][i] = sum[i];
+    lds_barrier();
+    if (wave == 0) {
+      for (int w = 1; w < kJoinWaves; ++w)
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i)
+          sum[i] += sums[w][lane][i];
+      write_sum<kShort>(sum, scale, add, out + row * ostride, at, d);
+    }
+    lds_barrier();
+  }
+}
+
+constexpr int kFewTokens = 1024;
+
+/**
+ * The same for up to kFewTokens tokens without sorting them: a team a token looks through all of them, and the first one of a
+ * row lists the places of the others and adds up their gradients.  Workgroups from `sum_blocks` on clear rows.
+ */
+template <typename T, typename O, int W, bool kShort>
+__global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned n, const T* grad, int64_t gstride, int d,
+                                                           float scale, bool add, O* out, int64_t ostride, unsigned slices, unsigned sum_blocks, int clear)
+{
+  constexpr int kTeams = kThreads / W, kPer = kFewTokens / kThreads;
+  __shared__ unsigned rows[kFewTokens];
+  __shared__ unsigned short places[kTeams][kFewTokens];
+  const int m = static_cast<int>(ids.m);
+  int64_t id[kPer];
+#pragma unroll
+  for (int q = 0; q < kPer; ++q)
+    id[q] = -1;
+  if (m > 0) read_ids(ids, threadIdx.x, kThreads, id);
+  if (blockIdx.x >= sum_blocks) {
+    bool* used       = reinterpret_cast<bool*>(rows);
+    const int64_t v0 = int64_t{blockIdx.x - sum_blocks} * clear;
+    const int mine   = static_cast<int>(min(int64_t{n} - v0, int64_t{clear}));
+    used[threadIdx.x] = false;
+    lds_barrier();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q)
+      if (id[q] >= v0 && id[q] < v0 + mine) used[id[q] - v0] = true;
+    lds_barrier();
+    return clear_rows(used, v0, mine, d, out, ostride);
+  }
+#pragma unroll
+  for (int q = 0; q < kPer; ++q)
+    rows[threadIdx.x + q * kThreads] = static_cast<int>(threadIdx.x) + q * kThreads < m ? row_of(id[q], n) : ~0u;
+  lds_barrier();
+  const int team = static_cast<int>(threadIdx.x) / W, lane = threadIdx.x % 64, sub = lane % W;
+  const unsigned all = blockIdx.x * kTeams + team;
+  const int token    = static_cast<int>(all / slices), at = (static_cast<int>(all % slices) * W + sub) * kUnit;
+  if (token >= m) return;
+  const unsigned row = rows[token];
+  if (row >= n) return;
+  int count        = 0;
+  const auto above = [&](unsigned long long lanes) { return W == 64 ? lanes : lanes >> (lane - sub) & ((1ull << (W % 64)) - 1); };
+  for (int i = 0; i < m; i += W) {
+    const bool in   = rows[i + sub] == row;
+    const auto same = above(__ballot(in));
+    if (same == 0) continue;
+    if (i + __builtin_ctzll(same) < token) return;  // an earlier token has the row
+    if (in) places[team][count + __popcll(same & ((1ull << sub) - 1))] = static_cast<unsigned short>(i + sub);
+    count += __popcll(same);
+  }
+  wave_fence();
+  const int from = unit_start(at, d);
   float sum[kUnit];
 #pragma unroll
   for (int i = 0; i < kUnit; ++i)
     sum[i] = 0.f;
-  const auto take = [&](const float* part) {
-    float v[kUnit];
-    unpack_unit(load_unit(part, from, d), v);
+  for (int j = 0; j < count; j += kTokensAhead) {
+    unit<T> u[kTokensAhead];
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i)
-      sum[i] += v[i];
-  };
-  if (at < d) {
-    if (wave == 0) take(s.cut + (chunk * 2 + 1) * d);
-    for (int64_t c = chunk + 1 + wave; c * s.width < s.m && s.row(c * s.width) == last; c += kJoinWaves)
-      take(s.cut + c * 2 * d);
+    for (int q = 0; q < kTokensAhead; ++q)
+      u[q] = load_unit<kShort>(grad + of_team<W>(static_cast<int>(places[team][min(j + q, count - 1)])) * gstride, from, d);
+#pragma unroll
+    for (int q = 0; q < kTokensAhead; ++q) {
+      float v[kUnit];
+      unpack_unit(u[q], v);
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i)
+        sum[i] += j + q < count ? v[i] : 0.f;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < kUnit; ++i)
-    sums[wave][lane][i] = sum[i];
-  lds_barrier();
-  if (wave > 0 || at >= d) return;
-  for (int w = 1; w < kJoinWaves; ++w)
-#pragma unroll
-    for (int i = 0; i < kUnit; ++i)
-      sum[i] += sums[w][lane][i];
-  write_sum(sum, scale, add, out + last * ostride, at, d, by_cache);
+  write_sum<kShort>(sum, scale, add, out + row * ostride, at, d);
 }
 
 /** Calls f with a value of the element type. */
@@ -544,12 +763,14 @@ void with_type(elem type, F f)
     f(bf16{});
 }
 
-/** Calls f with the lanes of a row's team: its units, or 64 of them a slice. */
+/** Calls f with the lanes of a row's team: its units, or 64 of them a slice; one for rows shorter than a unit. */
 template <typename F>
 void with_team(int64_t d, F f)
 {
   const int64_t units = (d + kUnit - 1) / kUnit;
-  if (units <= 8)
+  if (d < kUnit)
+    f(std::integral_constant<int, 1>{});
+  else if (units <= 8)
     f(std::integral_constant<int, 8>{});
   else if (units <= 16)
     f(std::integral_constant<int, 16>{});
@@ -579,7 +800,7 @@ auto chunk_width(int64_t m, int64_t d) -> int
 
 /** How the workspace is laid out, from place to place in bytes. */
 struct sort_layout {
-  int passes;
+  int passes, bits, per;  // of a digit; tokens of a thread
   int64_t tiles, chunks, second, counts, cut, end;
 };
 
@@ -587,18 +808,63 @@ auto layout_of(int64_t m, int64_t n, int64_t d) -> sort_layout
 {
   const auto up = [](int64_t v) { return ceil_div(v, 256) * 256; };
   sort_layout l{};
+  if (m <= kFewTokens) return l;
   int bits = 1;
   while (n >> bits != 0)
     ++bits;
   l.passes        = static_cast<int>(ceil_div(bits, kDigitBits));
-  l.tiles         = ceil_div(m, kSortTile);
+  l.bits          = static_cast<int>(ceil_div(bits, l.passes));
+  l.per           = m <= 2 * kSortThreads ? 2 : m <= 4 * kSortThreads ? 4 : m <= 8 * kSortThreads ? 8 : m <= 65536 ? 2 : 8;
+  l.tiles         = ceil_div(m, l.per * kSortThreads);
   const int width = chunk_width(m, d);
   l.chunks        = ceil_div(m, width);
   l.second        = up(m * static_cast<int64_t>(sizeof(token)));
   l.counts        = l.tiles > 1 ? 2 * l.second : l.second;
   l.cut           = l.counts + (l.tiles > 1 ? up(l.tiles * kDigits * 4) : 0);
-  l.end           = l.cut + (m > width ? l.chunks * 2 * d * 4 : 0);
+  l.end           = l.cut + l.chunks * 2 * d * 4;
   return l;
+}
+
+/** Sorts the tokens, and fills [out, out + bytes) meanwhile: as the sort takes few of the GPU's CUs, this costs what is left of
+ * the longer one. */
+template <int P>
+void sort_tiles(row_ids const& ids, unsigned n, sort_layout const& l, token* tokens, token* second, int* counts, char* out,
+                int64_t bytes, hipStream_t s)
+{
+  const auto tiles = static_cast<unsigned>(l.tiles);
+  const int steps  = tiles == 1 ? 1 : 2 * l.passes;
+  const int64_t per_step = ceil_div(ceil_div(bytes, steps), kFillBytes) * kFillBytes;
+  const auto share = [&](int step) {
+    const int64_t first = std::min(step * per_step, bytes), own = std::min(per_step, bytes - first);
+    // where a share begins inside a piece it takes one more
+    return fill_share{out + first, own,
+                      own > 0 ? static_cast<unsigned>(std::min<int64_t>(ceil_div(own + 16, kFillBytes), 1 << 20)) : 0u};
+  };
+  if (tiles == 1) {
+    const auto f = share(0);
+    sort_alone_kernel<P><<<1 + f.blocks, kSortThreads, 0, s>>>(ids, n, l.passes, l.bits, tokens, f);
+    OCTEX_HIP(hipGetLastError());
+    return;
+  }
+  for (int p = 0; p < l.passes; ++p) {
+    const bool to_first = (l.passes - 1 - p) % 2 == 0;
+    const token* in     = p == 0 ? nullptr : to_first ? second : tokens;
+    const digit of{p * l.bits, l.bits};
+    const auto f = share(2 * p), g = share(2 * p + 1);
+    count_digits_kernel<P><<<tiles + f.blocks, kSortThreads, 0, s>>>(ids, n, in, of, counts, tiles, f);
+    OCTEX_HIP(hipGetLastError());
+    move_tokens_kernel<P><<<tiles + g.blocks, kSortThreads, 0, s>>>(ids, n, in, of, counts, to_first ? tokens : second, tiles, g);
+    OCTEX_HIP(hipGetLastError());
+  }
+}
+
+/** Sets rows that lie apart to 0. */
+template <typename O>
+__global__ __launch_bounds__(kThreads) void clear_apart_kernel(O* out, int64_t n, int d, int64_t ostride)
+{
+  for (int64_t v = blockIdx.x; v < n; v += gridDim.x)
+    for (int j = threadIdx.x; j < d; j += kThreads)
+      out[v * ostride + j] = static_cast<O>(0.f);
 }
 
 }  // namespace
@@ -628,55 +894,57 @@ void launch_embed(table_rows const& table, row_ids const& ids, int64_t d, float 
     with_type(table.type, run);
 }
 
-auto embed_backward_workspace(int64_t m, int64_t n, int64_t d) -> int64_t { return m == 0 ? 0 : layout_of(m, n, d).end; }
+auto embed_backward_workspace(int64_t m, int64_t n, int64_t d) -> int64_t { return layout_of(m, n, d).end; }
 
 void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n, int64_t d, float scale, bool add,
                            value_rows const& out, void* workspace, hipStream_t s)
 {
-  const auto l    = layout_of(ids.m, n, d);
-  auto* base      = static_cast<char*>(workspace);
-  auto* tokens    = reinterpret_cast<token*>(base);
-  auto* second    = reinterpret_cast<token*>(base + l.second);
-  auto* counts    = reinterpret_cast<int*>(base + l.counts);
-  if (l.tiles == 1) {
-    sort_alone_kernel<<<1, kSortThreads, 0, s>>>(ids, n, l.passes, tokens);
-    OCTEX_HIP(hipGetLastError());
-  }
-  for (int p = 0; l.tiles > 1 && p < l.passes; ++p) {
-    const bool to_first = (l.passes - 1 - p) % 2 == 0;
-    const token* in     = p == 0 ? nullptr : to_first ? second : tokens;
-    const int shift     = p * kDigitBits;
-    count_digits_kernel<<<static_cast<unsigned>(l.tiles), kSortThreads, 0, s>>>(ids, n, in, shift, counts);
-    OCTEX_HIP(hipGetLastError());
-    move_tokens_kernel<<<static_cast<unsigned>(l.tiles), kSortThreads, 0, s>>>(ids, n, in, shift, counts,
-                                                                               to_first ? tokens : second);
-    OCTEX_HIP(hipGetLastError());
-  }
-  const sorted_tokens sorted{tokens, ids.m, n, chunk_width(ids.m, d), reinterpret_cast<float*>(base + l.cut)};
-  const bool by_cache = add || passes_cache(n, d, out.type);
-  // rows that a workgroup clears: 256 KB of them, for each of which a thread looks
-  const int clear = static_cast<int>(std::clamp<int64_t>((256 << 10) / (d * elem_size(out.type)), 16, kThreads));
+  const auto rows  = static_cast<unsigned>(n);
+  const auto width = static_cast<int>(d);
+  const bool few   = ids.m <= kFewTokens;
+  // of few tokens: rows that a workgroup clears, 16 KB of them
+  const int clear   = static_cast<int>(std::clamp<int64_t>((16 << 10) / (d * elem_size(out.type)), 1, kThreads));
+  const auto clears = add || !few ? 0u : static_cast<unsigned>(ceil_div(n, clear));
+  const auto l      = layout_of(ids.m, n, d);
+  auto* base        = static_cast<char*>(workspace);
+  const sorted_tokens sorted{reinterpret_cast<token*>(base), ids.m, rows, chunk_width(ids.m, d),
+                             reinterpret_cast<float*>(base + l.cut)};
   with_type(out.type, [&](auto o) {
     using O = decltype(o);
+    O* to   = static_cast<O*>(out.x);
+    if (!few) {
+      const bool apart = !add && out.stride != d;
+      if (apart) {
+        clear_apart_kernel<<<static_cast<unsigned>(std::min<int64_t>(n, 4096)), kThreads, 0, s>>>(to, n, width, out.stride);
+        OCTEX_HIP(hipGetLastError());
+      }
+      const auto sort = l.per == 2 ? sort_tiles<2> : l.per == 4 ? sort_tiles<4> : sort_tiles<8>;
+      sort(ids, rows, l, reinterpret_cast<token*>(base), reinterpret_cast<token*>(base + l.second),
+           reinterpret_cast<int*>(base + l.counts), static_cast<char*>(out.x),
+           add || apart ? 0 : n * d * static_cast<int64_t>(sizeof(O)), s);
+    }
     with_type(grad.type, [&](auto t) {
-      using T = decltype(t);
+      using T       = decltype(t);
+      const T* from = static_cast<const T*>(grad.x);
       with_team(d, [&](auto lanes) {
         constexpr int W   = lanes();
-        const auto slices = static_cast<unsigned>(ceil_div(d, W * kUnit));
-        const auto sums   = static_cast<unsigned>(ceil_div(l.chunks, kThreads / W)) * slices;
-        const auto clears = add ? 0u : static_cast<unsigned>(ceil_div(n, clear));
-        sum_runs_kernel<T, O, W><<<sums + clears, kThreads, 0, s>>>(sorted, static_cast<const T*>(grad.x), grad.stride,
-                                                                    static_cast<int>(d), scale, add, static_cast<O*>(out.x),
-                                                                    out.stride, by_cache, slices, sums, clear);
+        constexpr int F   = std::max(W, 8);
+        const auto slices = static_cast<unsigned>(ceil_div(d, W == 1 ? kUnit : W * kUnit));
+        const auto sums   = static_cast<unsigned>(ceil_div((few ? ids.m : l.chunks) * slices, kThreads / (few ? F : W)));
+        if (few)
+          sum_few_kernel<T, O, F, W == 1><<<sums + clears, kThreads, 0, s>>>(ids, rows, from, grad.stride, width, scale, add,
+                                                                             to, out.stride, slices, sums, clear);
+        else
+          sum_runs_kernel<T, O, W><<<sums, kThreads, 0, s>>>(sorted, from, grad.stride, width, scale, add, to, out.stride, slices);
         OCTEX_HIP(hipGetLastError());
       });
     });
-    // a cut run reaches into a third chunk
-    for (int64_t first = 0; l.chunks > 2 && first < l.chunks; first += kMaxGrid) {
-      const dim3 grid(static_cast<unsigned>(std::min(kMaxGrid, l.chunks - first)),
+    const int64_t joins = ceil_div(l.chunks, kJoinWaves);
+    for (int64_t first = 0; first < joins; first += kMaxGrid) {
+      const dim3 grid(static_cast<unsigned>(std::min(kMaxGrid, joins - first)),
                       static_cast<unsigned>(ceil_div(d, 64 * kUnit)));
-      join_runs_kernel<O><<<grid, kJoinThreads, 0, s>>>(sorted, static_cast<int>(d), scale, add, static_cast<O*>(out.x),
-                                                        out.stride, by_cache, first);
+      const auto join = d < kUnit ? join_runs_kernel<O, true> : join_runs_kernel<O, false>;
+      join<<<grid, kJoinThreads, 0, s>>>(sorted, width, scale, add, to, out.stride, l.chunks, first);
       OCTEX_HIP(hipGetLastError());
     }
   });
