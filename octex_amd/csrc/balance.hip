@@ -31,17 +31,31 @@ __device__ inline auto sum_apart(V v) -> V
   return v;
 }
 
+constexpr int kIdsAhead = 8;  // of a row, that a thread has on their way
+
 /** Adds the choices of rows [r0, r1) to counts[0, e), and the rows that count to counts[e]; LDS. */
 __device__ inline void count_rows(listed_ids const& experts, int e, int64_t r0, int64_t r1, int* counts)
 {
   int rows = 0;
   for (int64_t r = r0 + threadIdx.x; r < r1; r += blockDim.x) {
     bool some = false;
-    for (int j = 0; j < experts.k; ++j) {
-      const int64_t id = id_at(experts, r, j);
-      if (id < 0 || id >= e) continue;
-      some = true;
-      atomicAdd(counts + id, 1);
+    for (int j = 0; j < experts.k; j += kIdsAhead) {
+      int64_t id[kIdsAhead];
+      if (experts.wide) {
+#pragma unroll
+        for (int q = 0; q < kIdsAhead; ++q)
+          id[q] = static_cast<const int64_t*>(experts.ids)[r * experts.stride + min(j + q, experts.k - 1)];
+      } else {
+#pragma unroll
+        for (int q = 0; q < kIdsAhead; ++q)
+          id[q] = static_cast<const int32_t*>(experts.ids)[r * experts.stride + min(j + q, experts.k - 1)];
+      }
+#pragma unroll
+      for (int q = 0; q < kIdsAhead; ++q) {
+        if (j + q >= experts.k || id[q] < 0 || id[q] >= e) continue;
+        some = true;
+        atomicAdd(counts + id[q], 1);
+      }
     }
     rows += some;
   }
@@ -64,17 +78,23 @@ __global__ __launch_bounds__(kCountThreads) void count_choices_kernel(listed_ids
     parts[static_cast<int64_t>(blockIdx.x) * (e + 1) + i] = counts[i];
 }
 
-/** Adds n parts up to counts [e + 1] (LDS). */
+/** Adds n parts up to counts [e + 1] (LDS), as many threads a count as there are. */
 template <int NT>
 __device__ inline void add_parts(const int* parts, int n, int e, int* counts)
 {
-  for (int i = threadIdx.x; i <= e; i += NT) {
+  for (int i = threadIdx.x; i <= e; i += NT)
+    counts[i] = 0;
+  lds_barrier();
+  const int columns = e + 1, groups = max(NT / columns, 1);
+  for (int i = threadIdx.x; i < columns * groups; i += NT) {
+    const int group = i / columns, column = i - group * columns;
     int sum = 0;
-#pragma unroll 8
-    for (int p = 0; p < n; ++p)
-      sum += parts[static_cast<int64_t>(p) * (e + 1) + i];
-    counts[i] = sum;
+#pragma unroll 16
+    for (int p = group; p < n; p += groups)
+      sum += parts[static_cast<int64_t>(p) * columns + column];
+    if (sum > 0) atomicAdd(counts + column, sum);
   }
+  lds_barrier();
 }
 
 /** The sum of all threads' v; sums [NT / 64] is LDS. */
@@ -91,32 +111,6 @@ __device__ inline auto sum_block(V v, V* sums) -> V
   return v;
 }
 
-/** The last step of a forward pass, of one workgroup: counts [e + 1] (LDS), the rows that count last, and p(i), the sum of the
- * rows' p_i, of l^2 for i = e. */
-template <int NT, typename P>
-__device__ inline void write_balance(balance_out const& out, balance_weights const& w, int e, const int* counts, P p,
-                                     double* sums)
-{
-  double choices = 0.;
-  for (int i = threadIdx.x; i < e; i += NT)
-    choices += counts[i];
-  choices           = fmax(sum_block<NT>(choices, sums), 1.);
-  const double rows = max(counts[e], 1);
-  double sum        = 0.;
-  for (int i = threadIdx.x; i < e; i += NT) {
-    const double mean = p(i) / rows;
-    out.probs[i]      = static_cast<float>(mean);
-    out.counts[i]     = counts[i];
-    sum += mean * (counts[i] / choices);
-  }
-  sum = sum_block<NT>(sum, sums);
-  if (threadIdx.x != 0) return;
-  double loss = double{w.balance} * e * sum;
-  if (w.z != 0.f) loss += w.z * (p(e) / rows);
-  *out.loss = static_cast<float>(loss);
-  *out.rows = counts[e];
-}
-
 /** Where a pass takes the choices from: `n` parts; a forward pass's outputs; or (alone) the ids themselves, which its only
  * workgroup counts. */
 struct count_source {
@@ -126,77 +120,93 @@ struct count_source {
   bool alone;
 };
 
+/** Columns that a pass leaves in its parts beside the experts' sums of p: the sums of l^2, and of the rows' sum_v f_v p_v. */
+constexpr int kMoreSums = 2;
+
+__device__ inline auto loss_of(balance_weights const& w, int e, double rows, double squares, double inner) -> float
+{
+  double loss = w.balance != 0.f ? double{w.balance} * e * (inner / rows) : 0.;
+  if (w.z != 0.f) loss += w.z * (squares / rows);
+  return static_cast<float>(loss);
+}
+
 /**
  * Rows by W lanes each, H pieces of 16 bytes a lane, the next row's on their way meanwhile.  A lane keeps the sums of its
- * columns' p in registers over all of its rows; a workgroup's meet in LDS and go to p_parts [gridDim, e + 1] (l^2 last), or,
- * of a workgroup that is alone, to the outputs.
+ * columns' p in registers over all of its rows; a workgroup's meet in LDS and go to p_parts [gridDim, e + kMoreSums], or, of a
+ * workgroup that is alone, to the outputs.  kWhole: rows are whole pieces; else a piece that would pass the row's end is moved
+ * back to it, and columns that it shares with its neighbor are masked.
  */
-template <typename T, int NT, int W, int H>
+template <typename T, int NT, int W, int H, bool kWhole>
 __global__ __launch_bounds__(NT) void balance_kernel(score_rows in, listed_ids experts, balance_weights w, balance_out out,
                                                      const float* grad_loss, T* grad, int64_t gstride, bool by_cache,
                                                      count_source from, float* p_parts)
 {
   constexpr int N = kPer16<T>, kTeams = NT / W, kWavesHere = NT / 64, kPerRound = kWavesHere / kRounds;
   __shared__ int counts[kMaxExperts + 1];
-  __shared__ float p_sums[kPerRound][W * H * N + 1];
+  __shared__ float p_sums[kPerRound][W * H * N + kMoreSums];
   __shared__ double sums[kWavesHere];
+  __shared__ float shares[kMaxExperts];
   const int e = in.n, sub = static_cast<int>(threadIdx.x) % W;
   const bool forward = from.counts == nullptr;
+  // a lane's columns, and where their piece lies
+  const auto at_of    = [&](int h) { return (h * W + sub) * N; };
+  const auto place_of = [&](int h) { return kWhole ? at_of(h) : max(min(at_of(h), e - N), 0); };
+  const auto own      = [&](int h, int i) { return kWhole || (place_of(h) + i >= at_of(h) && place_of(h) + i < e); };
+  const auto row_at   = [&](int64_t r) { return static_cast<const T*>(in.x) + r * in.stride; };
+  uint4 next[H];
+  int64_t first_id = -1;  // the lane's first choice of the row
+  {
+    float nothing_here[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      nothing_here[i] = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      next[h] = pack16<T>(nothing_here);
+  }
+  const auto load = [&](int64_t r) {
+    first_id = sub < experts.k ? id_at(experts, r, sub) : -1;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      if (kWhole ? at_of(h) >= e : h * W * N >= e) continue;
+      next[h] = kWhole || e >= N ? load16(row_at(r) + place_of(h)) : load_row16(row_at(r), 0, e);
+    }
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTeams;
+  // a wavefront's teams go on together: those past the last row take that again, without a result
+  const int64_t leader = static_cast<int64_t>(blockIdx.x) * kTeams + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * (64 / W);
+  const int team       = static_cast<int>(threadIdx.x) % 64 / W;
+  if (leader < in.m) load(min(leader + team, in.m - 1));
   if (from.alone) {
     for (int i = threadIdx.x; i <= e; i += NT)
       counts[i] = 0;
     lds_barrier();
     count_rows(experts, e, 0, in.m, counts);
     lds_barrier();
-  } else if (from.parts != nullptr) {
+  } else if (forward) {
     add_parts<NT>(from.parts, from.n, e, counts);
-    lds_barrier();
   }
-  int at[H];  // a lane's columns; a piece that would pass the row's end is moved back to it
-  float f[H][N], p_sum[H][N], z_sum = 0.f, c_balance = 0.f, c_z = 0.f;
+  const auto count_of = [&](int i) { return forward ? static_cast<double>(counts[i]) : static_cast<double>(from.counts[i]); };
+  double choices      = 0.;
+  for (int i = threadIdx.x; i < e; i += NT)
+    choices += count_of(i);
+  choices = fmax(sum_block<NT>(choices, sums), 1.);
+  for (int i = threadIdx.x; i < e; i += NT)
+    shares[i] = static_cast<float>(count_of(i) / choices);
+  lds_barrier();
+  const double rows = fmax(forward ? static_cast<double>(counts[e]) : static_cast<double>(*from.rows), 1.);
+  const float g = grad_loss != nullptr ? *grad_loss : 1.f, per_row = static_cast<float>(1. / rows);
+  const float c_balance = g * (w.balance * static_cast<float>(e) * per_row), c_z = g * (2.f * w.z * per_row);
+  float f[H][N], p_sum[H][N], z_sum = 0.f, inner_sum = 0.f;
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    at[h] = (h * W + sub) * N;
+  for (int h = 0; h < H; ++h)
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      f[h][i] = p_sum[h][i] = 0.f;
-  }
-  if (grad != nullptr) {
-    double choices = 0.;
-    for (int i = threadIdx.x; i < e; i += NT)
-      choices += forward ? static_cast<double>(counts[i]) : static_cast<double>(from.counts[i]);
-    choices          = fmax(sum_block<NT>(choices, sums), 1.);
-    const double all = forward ? static_cast<double>(counts[e]) : static_cast<double>(*from.rows);
-    const float g    = grad_loss != nullptr ? *grad_loss : 1.f, per_row = static_cast<float>(1. / fmax(all, 1.));
-    c_balance = g * (w.balance * static_cast<float>(e) * per_row);
-    c_z       = g * (2.f * w.z * per_row);
-#pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int column = max(min(at[h], e - N), 0) + i;
-        if (column >= at[h] && column < e)
-          f[h][i] = static_cast<float>((forward ? static_cast<double>(counts[column]) : static_cast<double>(from.counts[column])) /
-                                       choices);
-      }
-  }
-  const auto row_at = [&](int64_t r) { return static_cast<const T*>(in.x) + r * in.stride; };
-  uint4 next[H];
-  int64_t first_id = -1;  // the lane's first choice of the row
-  const auto load  = [&](int64_t r) {
-    first_id = sub < experts.k ? id_at(experts, r, sub) : -1;
-#pragma unroll
-    for (int h = 0; h < H; ++h)
-      if (h == 0 || at[h] < e || h * W * N < e)
-        next[h] = e >= N ? load16(row_at(r) + min(at[h], e - N)) : load_row16(row_at(r), 0, e);
-  };
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kTeams;
-  const int64_t mine = static_cast<int64_t>(blockIdx.x) * kTeams + threadIdx.x / W;
-  // a wavefront's teams go on together: those past the last row take it again, without a result
-  const int64_t leader = static_cast<int64_t>(blockIdx.x) * kTeams + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * (64 / W);
-  if (leader < in.m) load(min(mine, in.m - 1));
+    for (int i = 0; i < N; ++i) {
+      p_sum[h][i] = 0.f;
+      f[h][i]     = own(h, i) && at_of(h) < e ? shares[place_of(h) + i] : 0.f;
+    }
   for (int64_t r0 = leader; r0 < in.m; r0 += step) {
-    const int64_t r = r0 + (mine - leader);
+    const int64_t r = r0 + team;
     const bool here = r < in.m;
     bool some       = first_id >= 0 && first_id < e;
     uint4 cur[H];
@@ -213,11 +223,11 @@ __global__ __launch_bounds__(NT) void balance_kernel(score_rows in, listed_ids e
     float v[H][N], top = -INFINITY;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      unpack16<T>(cur[h], v[h]);
+      // rows that do not count are read as zeros, whatever they hold
+      unpack16<T>(counted ? cur[h] : uint4{0, 0, 0, 0}, v[h]);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int column = max(min(at[h], e - N), 0) + i;
-        if (column < at[h] || column >= e) v[h][i] = -INFINITY;
+        if (!own(h, i)) v[h][i] = -INFINITY;
         top = fmaxf(top, v[h][i]);
       }
     }
@@ -233,51 +243,50 @@ __global__ __launch_bounds__(NT) void balance_kernel(score_rows in, listed_ids e
       }
     s                 = sum_lanes<W>(s);
     const float lse   = s > 0.f ? ref + logf(s) : s + top;  // nothing: 0 - inf; a NaN stays one
-    const float per_s = s > 0.f ? 1.f / s : s;
-    const float l     = s == 0.f ? 0.f : lse;
+    const float per_s = !counted ? 0.f : s > 0.f ? 1.f / s : s;
+    const float l     = counted && s != 0.f ? lse : 0.f;
     float inner       = 0.f;
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         v[h][i] *= per_s;
-        p_sum[h][i] += counted ? v[h][i] : 0.f;
+        p_sum[h][i] += v[h][i];
         inner = fmaf(f[h][i], v[h][i], inner);
       }
-    if (forward && sub == 0) {
-      z_sum += counted ? l * l : 0.f;
-      if (here) out.lse[r] = counted ? lse : 0.f;
-    }
+    inner = sum_lanes<W>(inner);
+    z_sum += l * l;
+    inner_sum += inner;
+    if (forward && sub == 0 && here) out.lse[r] = counted ? lse : 0.f;
     if (grad == nullptr) continue;
-    inner          = sum_lanes<W>(inner);
     const float cz = c_z * l;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        v[h][i] = counted ? v[h][i] * fmaf(c_balance, f[h][i] - inner, cz) : 0.f;
+        v[h][i] *= fmaf(c_balance, f[h][i] - inner, cz);
     }
     if (!here) continue;
     T* to = grad + r * gstride;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      if (at[h] >= e) continue;
-      if (at[h] + N <= e) {
+      if (at_of(h) >= e) continue;
+      if (kWhole || at_of(h) + N <= e) {
         if (by_cache)
-          store16(to + at[h], pack16<T>(v[h]));
+          store16(to + at_of(h), pack16<T>(v[h]));
         else
-          store16_nt(to + at[h], pack16<T>(v[h]));
+          store16_nt(to + at_of(h), pack16<T>(v[h]));
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int column = max(e - N, 0) + i;
-          if (column >= at[h] && column < e) to[column] = static_cast<T>(v[h][i]);
-        }
+        for (int i = 0; i < N; ++i)
+          if (own(h, i)) to[place_of(h) + i] = static_cast<T>(v[h][i]);
       }
     }
   }
   if (!forward) return;
-  z_sum = sum_apart<1>(z_sum);
+  // every lane of a team has its z_sum and inner_sum
+  z_sum     = sum_apart<W>(z_sum);
+  inner_sum = sum_apart<W>(inner_sum);
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -287,15 +296,13 @@ __global__ __launch_bounds__(NT) void balance_kernel(score_rows in, listed_ids e
   for (int round = 0; round < kRounds; ++round) {
     if (wave / kPerRound == round && threadIdx.x % 64 < W) {
       float* to       = p_sums[wave % kPerRound];
-      const auto join = [&](int i, float v) { to[i] = round == 0 ? v : to[i] + v; };
+      const auto join = [&](int i, float x) { to[i] = round == 0 ? x : to[i] + x; };
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int column = max(min(at[h], e - N), 0) + i;
-          if (column >= at[h] && column < e) join(column, p_sum[h][i]);
-        }
-      if (sub == 0) join(e, z_sum);
+        for (int i = 0; i < N; ++i)
+          if (own(h, i) && at_of(h) < e) join(place_of(h) + i, p_sum[h][i]);
+      if (sub == 0) join(e, z_sum), join(e + 1, inner_sum);
     }
     lds_barrier();
   }
@@ -305,87 +312,126 @@ __global__ __launch_bounds__(NT) void balance_kernel(score_rows in, listed_ids e
       sum += p_sums[q][i];
     return sum;
   };
-  if (from.alone) return write_balance<NT>(out, w, e, counts, total, sums);
-  for (int i = threadIdx.x; i <= e; i += NT)
-    p_parts[static_cast<int64_t>(blockIdx.x) * (e + 1) + i] = total(i);
+  if (!from.alone) {
+    for (int i = threadIdx.x; i < e + kMoreSums; i += NT)
+      p_parts[static_cast<int64_t>(blockIdx.x) * (e + kMoreSums) + i] = total(i);
+    return;
+  }
+  for (int i = threadIdx.x; i < e; i += NT) {
+    out.probs[i]  = static_cast<float>(total(i) / rows);
+    out.counts[i] = counts[i];
+  }
+  if (threadIdx.x != 0) return;
+  *out.loss = loss_of(w, e, rows, total(e), total(e + 1));
+  *out.rows = counts[e];
 }
 
-constexpr int kFinishThreads = 1024;
+constexpr int kFinishThreads = 1024, kFinishWaves = kFinishThreads / 64;
 
-/** Joins the parts of the choices and of p. */
+/** Joins the parts of p, 64 columns a workgroup; one more joins those of the choices and gives the loss. */
 __global__ __launch_bounds__(kFinishThreads) void finish_balance_kernel(balance_weights w, balance_out out, int e,
                                                                         const int* parts, int n, const float* p_parts, int np)
 {
+  __shared__ double sums[kFinishWaves][64];
   __shared__ int counts[kMaxExperts + 1];
-  __shared__ double p[kMaxExperts + 1];
-  __shared__ double sums[kFinishThreads / 64];
-  add_parts<kFinishThreads>(parts, n, e, counts);
-  for (int i = threadIdx.x; i <= e; i += kFinishThreads) {
-    double sum = 0.;
-#pragma unroll 8
-    for (int q = 0; q < np; ++q)
-      sum += p_parts[static_cast<int64_t>(q) * (e + 1) + i];
-    p[i] = sum;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const bool last  = blockIdx.x + 1 == gridDim.x;
+  const int column = last ? e + min(lane, kMoreSums - 1) : min(static_cast<int>(blockIdx.x) * 64 + lane, e - 1);
+  const int rows   = sum_apart<1>(lane < n ? parts[lane * (e + 1) + e] : 0);
+  double sum       = 0.;
+#pragma unroll 16
+  for (int q = wave; q < np; q += kFinishWaves)
+    sum += p_parts[static_cast<int64_t>(q) * (e + kMoreSums) + column];
+  sums[wave][lane] = sum;
+  if (last) {
+    add_parts<kFinishThreads>(parts, n, e, counts);
+    for (int i = threadIdx.x; i < e; i += kFinishThreads)
+      out.counts[i] = counts[i];
+    if (threadIdx.x == 0) *out.rows = counts[e];
   }
   lds_barrier();
-  write_balance<kFinishThreads>(out, w, e, counts, [&](int i) { return p[i]; }, sums);
+  if (wave > 0) return;
+  const double rows_here = max(rows, 1);
+  for (int q = 1; q < kFinishWaves; ++q)
+    sum += sums[q][lane];
+  if (!last) {
+    if (static_cast<int>(blockIdx.x) * 64 + lane < e) out.probs[column] = static_cast<float>(sum / rows_here);
+    return;
+  }
+  const double inner = __shfl(sum, 1);
+  if (lane == 0) *out.loss = loss_of(w, e, rows_here, sum, inner);
 }
 
 constexpr int kMaxCountParts = 64, kMaxWorkgroups = 512;
 
+auto pieces_of(int e, elem type) -> int { return (e * elem_size(type) + 15) / 16; }
+
+constexpr int kManyRows = 32768;
+
+/** Calls f with the threads of a workgroup, the lanes of a row and the pieces of a lane.  Many rows take 16 values a lane: what
+ * a row's lanes exchange, and a lane's steps beside its pieces, are fewer then (131,072 x 256 bfloat16: 34 us; 8 values 51, 32
+ * values 46, whose registers leave a CU half of the wavefronts).  Few rows take as many lanes as they have pieces. */
+template <typename T, typename F>
+void with_team(int64_t m, int pieces, F f)
+{
+  using std::integral_constant;
+  constexpr auto one         = integral_constant<int, 1>{};
+  constexpr auto many        = integral_constant<int, sizeof(T) == 4 ? 4 : 2>{};
+  constexpr auto most        = integral_constant<int, sizeof(T) == 4 ? 8 : 4>{};
+  constexpr auto wide        = integral_constant<int, 64>{};
+  constexpr auto small_group = integral_constant<int, 512>{};
+  constexpr auto group       = integral_constant<int, 1024>{};
+  if (pieces > 64 * many()) return f(small_group, wide, most);
+  if (m >= kManyRows || pieces > 64) {
+    if (pieces <= many()) return f(small_group, one, many);
+    if (pieces <= 2 * many()) return f(small_group, integral_constant<int, 2>{}, many);
+    if (pieces <= 4 * many()) return f(small_group, integral_constant<int, 4>{}, many);
+    if (pieces <= 8 * many()) return f(small_group, integral_constant<int, 8>{}, many);
+    if (pieces <= 16 * many()) return f(small_group, integral_constant<int, 16>{}, many);
+    if (pieces <= 32 * many()) return f(small_group, integral_constant<int, 32>{}, many);
+    return f(small_group, wide, many);
+  }
+  if (pieces <= 1) return f(group, one, one);
+  if (pieces <= 2) return f(group, integral_constant<int, 2>{}, one);
+  if (pieces <= 4) return f(group, integral_constant<int, 4>{}, one);
+  if (pieces <= 8) return f(group, integral_constant<int, 8>{}, one);
+  if (pieces <= 16) return f(group, integral_constant<int, 16>{}, one);
+  if (pieces <= 32) return f(group, integral_constant<int, 32>{}, one);
+  f(group, wide, one);
+}
+
 /** How a pass is shared out. */
 struct balance_plan {
   bool alone;
-  int count_parts, workgroups, teams;
+  int count_parts, workgroups;
   int64_t width;  // rows of a part
 };
-
-auto per_row(int e, elem type) -> int { return (e * elem_size(type) + 15) / 16; }
 
 auto plan_of(int64_t m, int e, int k, elem type) -> balance_plan
 {
   balance_plan p{};
-  const int pieces = per_row(e, type);
-  int lanes        = 1;
-  while (lanes < 64 && lanes < pieces)
-    lanes *= 2;
-  const int threads = pieces > 64 ? 512 : 1024;
-  p.teams           = threads / lanes;
-  p.alone           = m * e <= 32768 && m * k <= 8192;
-  p.workgroups      = p.alone ? 1 : static_cast<int>(std::min<int64_t>((m + p.teams - 1) / p.teams, kMaxWorkgroups));
-  p.count_parts     = static_cast<int>(std::clamp<int64_t>(m / kCountThreads, 1, kMaxCountParts));
-  p.width           = (m + p.count_parts - 1) / p.count_parts;
+  int teams = 1;
+  with_type(type, [&](auto x) { with_team<decltype(x)>(m, pieces_of(e, type), [&](auto nt, auto w, auto) { teams = nt() / w(); }); });
+  p.alone       = m * e <= 32768 && m * k <= 8192;
+  p.workgroups  = p.alone ? 1 : static_cast<int>(std::min<int64_t>((m + teams - 1) / teams, kMaxWorkgroups));
+  p.count_parts = static_cast<int>(std::clamp<int64_t>(m / kCountThreads, 1, kMaxCountParts));
+  p.width       = (m + p.count_parts - 1) / p.count_parts;
   return p;
 }
 
-template <typename T, typename F>
-void with_team(int pieces, F f)
-{
-  const auto call = [&](auto nt, auto w, auto h) { f(nt, w, h); };
-  constexpr auto kSmall = std::integral_constant<int, 1024>{};
-  constexpr auto kLarge = std::integral_constant<int, 512>{};
-  constexpr auto one    = std::integral_constant<int, 1>{};
-  if (pieces <= 1) return call(kSmall, one, one);
-  if (pieces <= 2) return call(kSmall, std::integral_constant<int, 2>{}, one);
-  if (pieces <= 4) return call(kSmall, std::integral_constant<int, 4>{}, one);
-  if (pieces <= 8) return call(kSmall, std::integral_constant<int, 8>{}, one);
-  if (pieces <= 16) return call(kSmall, std::integral_constant<int, 16>{}, one);
-  if (pieces <= 32) return call(kSmall, std::integral_constant<int, 32>{}, one);
-  if (pieces <= 64) return call(kSmall, std::integral_constant<int, 64>{}, one);
-  if (pieces <= 128) return call(kLarge, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-  if (sizeof(T) == 2 || pieces <= 256) return call(kLarge, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-  if constexpr (sizeof(T) == 4) call(kLarge, std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
-}
-
-template <typename T>
 void run_balance(score_rows const& in, listed_ids const& experts, balance_weights const& w, balance_out const& out,
                  const float* grad_loss, void* grad, int64_t gstride, count_source const& from, float* p_parts, int workgroups,
                  hipStream_t s)
 {
-  with_team<T>(per_row(in.n, in.type), [&](auto nt, auto lanes, auto h) {
-    balance_kernel<T, nt(), lanes(), h()><<<workgroups, nt(), 0, s>>>(in, experts, w, out, grad_loss, static_cast<T*>(grad),
-                                                                       gstride, passes_cache(in), from, p_parts);
-    OCTEX_HIP(hipGetLastError());
+  with_type(in.type, [&](auto x) {
+    using T = decltype(x);
+    with_team<T>(in.m, pieces_of(in.n, in.type), [&](auto nt, auto lanes, auto h) {
+      const auto kernel = in.n % kPer16<T> == 0 ? balance_kernel<T, nt(), lanes(), h(), true>
+                                                : balance_kernel<T, nt(), lanes(), h(), false>;
+      kernel<<<workgroups, nt(), 0, s>>>(in, experts, w, out, grad_loss, static_cast<T*>(grad), gstride, passes_cache(in), from,
+                                         p_parts);
+      OCTEX_HIP(hipGetLastError());
+    });
   });
 }
 
@@ -394,7 +440,7 @@ void run_balance(score_rows const& in, listed_ids const& experts, balance_weight
 auto balance_workspace(int64_t m, int e, int k, elem type) -> int64_t
 {
   const auto p = plan_of(m, e, k, type);
-  return p.alone ? 0 : int64_t{4} * (p.count_parts + p.workgroups) * (e + 1);
+  return p.alone ? 0 : int64_t{4} * (int64_t{p.count_parts} * (e + 1) + int64_t{p.workgroups} * (e + kMoreSums));
 }
 
 void launch_balance(score_rows const& in, listed_ids const& experts, balance_weights const& w, balance_out const& out,
@@ -407,12 +453,10 @@ void launch_balance(score_rows const& in, listed_ids const& experts, balance_wei
     count_choices_kernel<<<p.count_parts, kCountThreads, 0, s>>>(experts, in.n, in.m, p.width, parts);
     OCTEX_HIP(hipGetLastError());
   }
-  const count_source from{p.alone || grad == nullptr ? nullptr : parts, p.count_parts, nullptr, nullptr, p.alone};
-  with_type(in.type, [&](auto e) {
-    run_balance<decltype(e)>(in, experts, w, out, grad_loss, grad, gstride, from, p_parts, p.workgroups, s);
-  });
+  run_balance(in, experts, w, out, grad_loss, grad, gstride, {parts, p.count_parts, nullptr, nullptr, p.alone}, p_parts,
+              p.workgroups, s);
   if (!p.alone) {
-    finish_balance_kernel<<<1, kFinishThreads, 0, s>>>(w, out, in.n, parts, p.count_parts, p_parts, p.workgroups);
+    finish_balance_kernel<<<(in.n + 63) / 64 + 1, kFinishThreads, 0, s>>>(w, out, in.n, parts, p.count_parts, p_parts, p.workgroups);
     OCTEX_HIP(hipGetLastError());
   }
 }
@@ -420,12 +464,9 @@ void launch_balance(score_rows const& in, listed_ids const& experts, balance_wei
 void launch_balance_backward(score_rows const& in, listed_ids const& experts, balance_weights const& w, const int64_t* counts,
                              const int64_t* rows, const float* grad_loss, void* grad, int64_t gstride, hipStream_t s)
 {
-  const auto p = plan_of(in.m, in.n, experts.k, in.type);
-  const int workgroups = static_cast<int>(std::min<int64_t>((in.m + p.teams - 1) / p.teams, kMaxWorkgroups));
-  const count_source from{nullptr, 0, counts, rows, false};
-  with_type(in.type, [&](auto e) {
-    run_balance<decltype(e)>(in, experts, w, {}, grad_loss, grad, gstride, from, nullptr, workgroups, s);
-  });
+  auto p = plan_of(in.m, in.n, experts.k, in.type);
+  if (p.alone) p.workgroups = 1;
+  run_balance(in, experts, w, {}, grad_loss, grad, gstride, {nullptr, 0, counts, rows, false}, nullptr, p.workgroups, s);
 }
 
 }  // namespace cuvs::neighbors::octex::detail

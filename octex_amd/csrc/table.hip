@@ -111,17 +111,18 @@ __device__ inline void read_ids(row_ids const& ids, int64_t i0, int64_t step, in
 constexpr int kRowsAhead = 4;  // rows that a team has on their way
 
 /**
- * Teams of W lanes (1: of rows shorter than a unit) take kRowsAhead rows each, a unit a lane (of the slice blockIdx.y of their
- * columns): all ids first, then all rows, then the results.  No load waits for a condition: padding takes the table's first row
+ * Teams of W lanes (1: of rows shorter than a unit) take kRowsAhead rows each, a unit a lane (of one of `slices` slices of their
+ * columns, side by side in a workgroup): all ids first, then all rows, then the results.  No load waits for a condition: padding takes the table's first row
  * and drops it.
  */
 template <typename T, typename O, int W>
 __global__ __launch_bounds__(kThreads) void embed_kernel(table_rows table, row_ids ids, int d, float scale, O* out,
-                                                         int64_t ostride, bool by_cache, int64_t block0)
+                                                         int64_t ostride, bool by_cache, unsigned slices, int64_t block0)
 {
   constexpr int kTeams = kThreads / W;
-  const int at         = (static_cast<int>(blockIdx.y) * W + static_cast<int>(threadIdx.x) % W) * kUnit;
-  const int64_t i0     = ((block0 + blockIdx.x) * kTeams + threadIdx.x / W) * kRowsAhead;
+  const int64_t team   = (block0 + blockIdx.x) * kTeams + threadIdx.x / W;
+  const int64_t i0     = team / slices * kRowsAhead;
+  const int at         = (static_cast<int>(team % slices) * W + static_cast<int>(threadIdx.x) % W) * kUnit;
   if (at >= d || i0 >= ids.m) return;
   const int from = unit_start(at, d);
   int64_t id[kRowsAhead];
@@ -877,12 +878,12 @@ void launch_embed(table_rows const& table, row_ids const& ids, int64_t d, float 
       using O = decltype(o);
       with_team(d, [&](auto lanes) {
         constexpr int W      = lanes();
-        const int64_t blocks = ceil_div(ids.m, int64_t{kThreads / W} * kRowsAhead);
-        const auto slices    = static_cast<unsigned>(ceil_div(d, W * kUnit));
+        const auto slices    = static_cast<unsigned>(ceil_div(d, W == 1 ? kUnit : W * kUnit));
+        const int64_t blocks = ceil_div(ceil_div(ids.m, kRowsAhead) * slices, kThreads / W);
         for (int64_t first = 0; first < blocks; first += kMaxGrid) {
-          const dim3 grid(static_cast<unsigned>(std::min(kMaxGrid, blocks - first)), slices);
-          embed_kernel<T, O, W><<<grid, kThreads, 0, s>>>(table, ids, static_cast<int>(d), scale, static_cast<O*>(out.x),
-                                                          out.stride, passes_cache(ids.m, d, out.type), first);
+          embed_kernel<T, O, W><<<static_cast<unsigned>(std::min(kMaxGrid, blocks - first)), kThreads, 0, s>>>(
+            table, ids, static_cast<int>(d), scale, static_cast<O*>(out.x), out.stride, passes_cache(ids.m, d, out.type), slices,
+            first);
           OCTEX_HIP(hipGetLastError());
         }
       });
