@@ -81,6 +81,7 @@ def _torch():
 
 
 _HERE = contextlib.nullcontext()
+_WORKSPACES = {}  # bytes, by entry and sizes
 
 
 class _Call:
@@ -213,14 +214,22 @@ class _Call:
         for stream in self.others:
             stream.wait_stream(self.own_stream())
 
-    def run_sized(self, entry, *args):
-        """run with the workspace that the arguments need; its tensor is kept with the call."""
-        size = _I64(0)
-        self.run(entry, *args, None, 0, ct.addressof(size))
-        if size.value == 0:
+    def run_sized(self, entry, *args, sizes=None):
+        """run with the workspace that the arguments need; its tensor is kept with the call.  Where `sizes` (the entry and all
+        that its workspace depends on: sizes and types) is given, the answer is asked for once."""
+        need = _WORKSPACES.get(sizes)
+        if need is None:
+            size = _I64(0)
+            self.run(entry, *args, None, 0, ct.addressof(size))
+            need = size.value
+            if sizes is not None:
+                if len(_WORKSPACES) >= 4096:
+                    _WORKSPACES.clear()
+                _WORKSPACES[sizes] = need
+        if need == 0:
             return self.run(entry, *args, None, 0, None)
-        self.scratch = self.new((size.value,), dtype=self.torch.int8)
-        return self.run(entry, *args, self.scratch.data_ptr(), size.value, None)
+        self.scratch = self.new((need,), dtype=self.torch.int8)
+        return self.run(entry, *args, self.scratch.data_ptr(), need, None)
 
     def give(self, t):
         """A result in the framework, and the memory, of the first operand."""
@@ -412,12 +421,18 @@ def _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, ent
     c = _Call(logits, "logits", FLOATS)
     x = c.first
     m = x.shape[0]
-    t = c.take(_columns(c, ids)[0], "ids", INTS, shape=(m, 1))
+    t = c.array(ids)
+    if t.ndim == 1:  # a column of m rows
+        t = c.take(t, "ids", INTS, 1, (m,))
+        column = _Matrix(t.data_ptr(), _TYPES[c.names[t.dtype]], m, 1, 1)
+    else:
+        t = c.take(t, "ids", INTS, shape=(m, 1))
+        column = c.matrix(t)
     terms = [c.dense(old_log_probs, "old_log_probs", (m,)), c.dense(advantages, "advantages", (m,))]
     if kl != 0 and ref_log_probs is not None:
         terms.append(c.dense(ref_log_probs, "ref_log_probs", (m,)))
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
-    args = (c.matrix(x), c.matrix(t), float(temperature), terms[0].data_ptr(), terms[1].data_ptr(),
+    args = (c.matrix(x), column, float(temperature), terms[0].data_ptr(), terms[1].data_ptr(),
             terms[2].data_ptr() if len(terms) > 2 else None, 1.0 - low, 1.0 + high, float(kl), float(entropy))
     return c, x, (t, terms), args
 
@@ -437,7 +452,7 @@ def policy_loss(logits, ids, old_log_probs, advantages, *, ref_log_probs=None, c
     """
     c, x, keep, args = _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, entropy, temperature)
     r = PolicyLoss(*c.new(*[(x.shape[0],)] * 4))
-    c.run_sized("octexPolicyLoss", *args, *[v.data_ptr() for v in r])
+    c.run_sized("octexPolicyLoss", *args, *[v.data_ptr() for v in r], sizes=("octexPolicyLoss", x.shape))
     return PolicyLoss(*map(c.give, r))
 
 
@@ -462,7 +477,8 @@ def policy_step(grad_loss, logits, ids, old_log_probs, advantages, *, ref_log_pr
     c, x, keep, args = _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, entropy, temperature)
     g = c.dense(grad_loss, "grad_loss", (x.shape[0],))
     r, grad = PolicyLoss(*[c.like(g) for _ in range(4)]), c.like(x)
-    c.run_sized("octexPolicyLossStep", *args, g.data_ptr(), *[v.data_ptr() for v in r], c.matrix(grad))
+    c.run_sized("octexPolicyLossStep", *args, g.data_ptr(), *[v.data_ptr() for v in r], c.matrix(grad),
+                sizes=("octexPolicyLossStep", x.shape, x.dtype))
     return PolicyLoss(*map(c.give, r)), c.give(grad)
 
 
@@ -476,7 +492,10 @@ def _balance(logits, experts):
 
 def _one(c, a, name, types):
     """One number, as an array of no dimension or one."""
-    return c.take(c.array(a).reshape(-1), name, types, 1, (1,))
+    t = c.array(a)
+    if t.ndim != 1:
+        t = t.reshape(-1)
+    return c.take(t, name, types, 1, (1,))
 
 
 def _balance_results(c, x):
@@ -502,7 +521,8 @@ def balance_loss(logits, experts, *, weight=1.0, z_weight=0.0):
     """
     c, x, t = _balance(logits, experts)
     r = _balance_results(c, x)
-    c.run_sized("octexBalanceLoss", c.matrix(x), c.matrix(t), float(weight), float(z_weight), *[v.data_ptr() for v in r], None, None)
+    c.run_sized("octexBalanceLoss", c.matrix(x), c.matrix(t), float(weight), float(z_weight), *[v.data_ptr() for v in r], None,
+                None, sizes=("octexBalanceLoss", x.shape, t.shape, x.dtype))
     return BalanceLoss(*map(c.give, r))
 
 
@@ -528,5 +548,5 @@ def balance_step(grad_loss, logits, experts, *, weight=1.0, z_weight=0.0):
     g = None if grad_loss is None else _one(c, grad_loss, "grad_loss", ("float32",))
     r, grad = _balance_results(c, x), c.like(x)
     c.run_sized("octexBalanceLoss", c.matrix(x), c.matrix(t), float(weight), float(z_weight), *[v.data_ptr() for v in r],
-                None if g is None else g.data_ptr(), c.matrix(grad))
+                None if g is None else g.data_ptr(), c.matrix(grad), sizes=("octexBalanceLoss", x.shape, t.shape, x.dtype))
     return BalanceLoss(*map(c.give, r)), c.give(grad)

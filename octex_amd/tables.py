@@ -13,13 +13,14 @@ from .scores import FLOATS, INTS
 
 
 def _flat_ids(c, ids):
-    """Ids of any shape as one column, and their shape."""
+    """Ids of any shape as a vector, that as a matrix of one column, and their shape."""
     t = c.array(ids)
-    shape = tuple(t.shape)
+    shape = t.shape
     if t.ndim != 1:
         with c.context():
             t = t.reshape(-1)
-    return c.take(t[:, None], "ids", INTS), shape
+    t = c.take(t, "ids", INTS, 1)
+    return t, _rows(c, t, t.shape[0], 1), shape
 
 
 def _rows(c, t, rows, cols):
@@ -40,13 +41,13 @@ def embed(table, ids, *, row_scales=None, scale=1.0, dtype=None):
     if not coded and c.names[x.dtype] == "int8":
         raise TypeError("octex: an int8 table needs its row_scales")
     n, d = x.shape
-    t, shape = _flat_ids(c, ids)
+    t, flat, shape = _flat_ids(c, ids)
     if coded:
         row_scales = c.dense(row_scales, "row_scales", (n,))
     if dtype is None:
         dtype = "float32" if coded else c.names[x.dtype]
     out = c.new((*shape, d), dtype=scores._float_type(c, dtype, "rows", "table"))
-    c.run("octexEmbed", c.matrix(x), row_scales.data_ptr() if coded else None, c.matrix(t), float(scale),
+    c.run("octexEmbed", c.matrix(x), row_scales.data_ptr() if coded else None, flat, float(scale),
           _rows(c, out, t.shape[0], d))
     return c.give(out)
 
@@ -61,10 +62,10 @@ def embed_backward(grad, ids, rows=None, *, scale=1.0, dtype=None, add_to=None):
     """
     c = scores._Call(grad, "grad", FLOATS, flat=True)
     g = c.first
-    t, shape = _flat_ids(c, ids)
+    t, flat, shape = _flat_ids(c, ids)
     m, d = g.shape
     if _arrays.shape_of(grad)[:-1] != shape:
-        raise ValueError(f"octex: grad has shape {tuple(_arrays.shape_of(grad))}, ids {shape}")
+        raise ValueError(f"octex: grad has shape {_arrays.shape_of(grad)}, ids {tuple(shape)}")
     if add_to is None:
         if rows is None:
             raise TypeError("octex: the table's number of rows, or add_to, must be given")
@@ -72,7 +73,8 @@ def embed_backward(grad, ids, rows=None, *, scale=1.0, dtype=None, add_to=None):
         if rows < 0:
             raise ValueError(f"octex: a table of {rows} rows")
         out = c.new((rows, d), dtype=scores._float_type(c, c.names[g.dtype] if dtype is None else dtype, "gradients", "grad"))
-        c.run_sized("octexEmbedBackward", c.matrix(g), c.matrix(t), float(scale), 0, _rows(c, out, rows, d))
+        c.run_sized("octexEmbedBackward", c.matrix(g), flat, float(scale), 0, _rows(c, out, rows, d),
+                    sizes=("octexEmbedBackward", m, rows, d, 0))
         return c.give(out)
     out = add_to
     if not isinstance(out, c.torch.Tensor) or out.device != c.device or c.on_host:
@@ -85,6 +87,7 @@ def embed_backward(grad, ids, rows=None, *, scale=1.0, dtype=None, add_to=None):
     if out.is_neg() or (d > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < d):
         raise ValueError("octex: add_to's rows must lie apart, their values side by side")
     c.array(out)  # ordered with the call
-    c.run_sized("octexEmbedBackward", c.matrix(g), c.matrix(t), float(scale), 1, c.matrix(out))
+    c.run_sized("octexEmbedBackward", c.matrix(g), flat, float(scale), 1, c.matrix(out),
+                sizes=("octexEmbedBackward", m, out.shape[0], d, 1))
     c.torch.autograd.graph.increment_version(out)
     return out
