@@ -112,8 +112,8 @@ constexpr int kRowsAhead = 4;  // rows that a team has on their way
 
 /**
  * Teams of W lanes (1: of rows shorter than a unit) take kRowsAhead rows each, a unit a lane (of one of `slices` slices of their
- * columns, side by side in a workgroup): all ids first, then all rows, then the results.  No load waits for a condition: padding takes the table's first row
- * and drops it.
+ * columns, side by side in a workgroup): all ids first, then all rows, then the results.  No load waits for a condition: padding
+ * takes the table's first row and drops it.
  */
 template <typename T, typename O, int W>
 __global__ __launch_bounds__(kThreads) void embed_kernel(table_rows table, row_ids ids, int d, float scale, O* out,
@@ -282,8 +282,8 @@ __device__ inline void start_waves(int (*counts)[kDigits], const int (&c)[kSortW
   }
 }
 
-/** A share of the table's gradient that is set to 0 beside a step of the sort: [first, first + bytes) of dense rows, by `blocks`
- * workgroups. */
+/** A share of the table's gradient that is set to 0 beside a step of the sort, whichever rows have tokens: [first, first + bytes)
+ * of dense rows, by `blocks` workgroups. */
 struct fill_share {
   char* first;
   int64_t bytes;
@@ -536,15 +536,85 @@ __device__ inline void clear_rows(const bool* used, int64_t v0, int rows, int d,
   }
 }
 
+constexpr int kClearRows = 4096;  // of a workgroup, at most
+
+/** Rows [first, n), `rows` a workgroup from `block0` on, that are set to 0 beside the sums where no token has them. */
+struct clear_share {
+  unsigned block0;
+  int64_t first;
+  int rows;
+};
+
+/** The first of the sorted tokens whose row is `row` or behind it; the lanes of a wavefront look at 64 places at a time. */
+__device__ inline auto first_at_least(sorted_tokens const& s, int64_t row) -> int64_t
+{
+  int64_t lo = 0, hi = s.m;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) / 64, at = lo + threadIdx.x % 64 * step;
+    const int before   = __popcll(__ballot(at < hi && s.t[min(at, s.m - 1)].row < row));
+    if (before == 0) break;
+    hi = min(lo + before * step, hi);
+    lo += (before - 1) * step + 1;
+  }
+  return lo;
+}
+
+/** Whether one of the tokens [lo, hi) has the row. */
+__device__ inline auto has_row(sorted_tokens const& s, int64_t lo, int64_t hi, unsigned row) -> bool
+{
+  const int64_t end = hi;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (s.t[mid].row < row)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo < end && s.t[lo].row == row;
+}
+
+/** Sets the rows of a workgroup's share that no token has to 0.  It marks its tokens' rows, or, where they are many more than its
+ * rows (a common token's), looks for each row among them. */
+template <typename O>
+__device__ inline void clear_unlisted(sorted_tokens const& s, clear_share const& c, int d, O* out, int64_t ostride, bool* used,
+                                      int64_t* range)
+{
+  const int64_t v0 = c.first + int64_t{blockIdx.x - c.block0} * c.rows;
+  const int rows   = static_cast<int>(min(int64_t{s.n} - v0, int64_t{c.rows}));
+  const int wave   = static_cast<int>(threadIdx.x) / 64;
+  for (int r = threadIdx.x; r < rows; r += kThreads)
+    used[r] = false;
+  if (wave < 2) {
+    const int64_t at = first_at_least(s, v0 + (wave == 0 ? 0 : rows));
+    if (threadIdx.x % 64 == 0) range[wave] = at;
+  }
+  lds_barrier();
+  const int64_t lo = range[0], hi = range[1];
+  if (hi - lo <= int64_t{16} * kThreads * ((rows + kThreads - 1) / kThreads)) {
+    for (int64_t p = lo + threadIdx.x; p < hi; p += kThreads)
+      used[s.t[p].row - v0] = true;
+  } else {
+    for (int r = threadIdx.x; r < rows; r += kThreads)
+      used[r] = has_row(s, lo, hi, static_cast<unsigned>(v0 + r));
+  }
+  lds_barrier();
+  clear_rows(used, v0, rows, d, out, ostride);
+}
+
 /**
  * The sums of the runs of a chunk each, by teams of W lanes, a unit a lane (of one of `slices` slices of their columns), the
- * gradients of kTokensAhead tokens on their way at a time.
+ * gradients of kTokensAhead tokens on their way at a time.  Workgroups behind those clear rows.
  */
 template <typename T, typename O, int W>
 __global__ __launch_bounds__(kThreads) void sum_runs_kernel(sorted_tokens s, const T* grad, int64_t gstride, int d, float scale,
-                                                            bool add, O* out, int64_t ostride, unsigned slices)
+                                                            bool add, O* out, int64_t ostride, unsigned slices, clear_share clear)
 {
   constexpr int kTeams = kThreads / W;
+  if (blockIdx.x >= clear.block0) {
+    __shared__ bool used[kClearRows];
+    __shared__ int64_t range[2];
+    return clear_unlisted(s, clear, d, out, ostride, used, range);
+  }
   const int64_t team   = int64_t{blockIdx.x} * kTeams + of_team<W>(static_cast<int>(threadIdx.x) / W);
   const int64_t chunk  = team / slices;  // a workgroup's teams take slices side by side
   const int at         = (static_cast<int>(team - chunk * slices) * W + static_cast<int>(threadIdx.x) % W) * kUnit;
@@ -686,7 +756,8 @@ constexpr int kFewTokens = 1024;
  */
 template <typename T, typename O, int W, bool kShort>
 __global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned n, const T* grad, int64_t gstride, int d,
-                                                           float scale, bool add, O* out, int64_t ostride, unsigned slices, unsigned sum_blocks, int clear)
+                                                           float scale, bool add, O* out, int64_t ostride, unsigned slices, unsigned sum_blocks,
+                                                           int clear)
 {
   constexpr int kTeams = kThreads / W, kPer = kFewTokens / kThreads;
   __shared__ unsigned rows[kFewTokens];
@@ -826,8 +897,7 @@ auto layout_of(int64_t m, int64_t n, int64_t d) -> sort_layout
   return l;
 }
 
-/** Sorts the tokens, and fills [out, out + bytes) meanwhile: as the sort takes few of the GPU's CUs, this costs what is left of
- * the longer one. */
+/** Sorts the tokens, and fills [out, out + bytes) meanwhile. */
 template <int P>
 void sort_tiles(row_ids const& ids, unsigned n, sort_layout const& l, token* tokens, token* second, int* counts, char* out,
                 int64_t bytes, hipStream_t s)
@@ -859,13 +929,13 @@ void sort_tiles(row_ids const& ids, unsigned n, sort_layout const& l, token* tok
   }
 }
 
-/** Sets rows that lie apart to 0. */
-template <typename O>
-__global__ __launch_bounds__(kThreads) void clear_apart_kernel(O* out, int64_t n, int d, int64_t ostride)
+/** The bytes that are filled while the tokens are sorted, in about the time that this takes on few CUs: 4.6 us and 6.7 to count and
+ * to move tiles of 2048 tokens, 8 to 18 for 2 to 8 tokens a thread of a single workgroup.  128,000 x 4096 bfloat16 from 32,768
+ * tokens: 276 us, 303 if all of the table is filled there, and the tokens' rows are written twice (64 MB a pass: 278, 160 MB:
+ * 278). */
+auto fill_bytes(sort_layout const& l) -> int64_t
 {
-  for (int64_t v = blockIdx.x; v < n; v += gridDim.x)
-    for (int j = threadIdx.x; j < d; j += kThreads)
-      out[v * ostride + j] = static_cast<O>(0.f);
+  return l.tiles == 1 ? (int64_t{l.per} + 4) * (14 << 20) : int64_t{l.passes} * (96 << 20);
 }
 
 }  // namespace
@@ -904,25 +974,27 @@ void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n
   const auto width = static_cast<int>(d);
   const bool few   = ids.m <= kFewTokens;
   // of few tokens: rows that a workgroup clears, 16 KB of them
-  const int clear   = static_cast<int>(std::clamp<int64_t>((16 << 10) / (d * elem_size(out.type)), 1, kThreads));
+  const int clear = static_cast<int>(
+    std::clamp<int64_t>(std::max((16 << 10) / (d * elem_size(out.type)), ceil_div(n, 1 << 22)), 1, kThreads));
   const auto clears = add || !few ? 0u : static_cast<unsigned>(ceil_div(n, clear));
   const auto l      = layout_of(ids.m, n, d);
   auto* base        = static_cast<char*>(workspace);
   const sorted_tokens sorted{reinterpret_cast<token*>(base), ids.m, rows, chunk_width(ids.m, d),
                              reinterpret_cast<float*>(base + l.cut)};
+  // of many: rows that are filled beside the sort, wherever tokens are, and those a workgroup that are cleared after it, up to
+  // 32 KB (1 MB: 288 us for what takes 276) in 2048 workgroups or more
+  const int64_t row_bytes = d * elem_size(out.type);
+  const int64_t filled    = add || few || out.stride != d ? 0 : std::min(n, fill_bytes(l) / row_bytes);
+  const int64_t left      = add || few ? 0 : n - filled;
+  const int64_t per_group = std::clamp<int64_t>(std::min((int64_t{32} << 10) / row_bytes, ceil_div(left, 2048)), 1, kClearRows);
   with_type(out.type, [&](auto o) {
     using O = decltype(o);
     O* to   = static_cast<O*>(out.x);
     if (!few) {
-      const bool apart = !add && out.stride != d;
-      if (apart) {
-        clear_apart_kernel<<<static_cast<unsigned>(std::min<int64_t>(n, 4096)), kThreads, 0, s>>>(to, n, width, out.stride);
-        OCTEX_HIP(hipGetLastError());
-      }
       const auto sort = l.per == 2 ? sort_tiles<2> : l.per == 4 ? sort_tiles<4> : sort_tiles<8>;
       sort(ids, rows, l, reinterpret_cast<token*>(base), reinterpret_cast<token*>(base + l.second),
            reinterpret_cast<int*>(base + l.counts), static_cast<char*>(out.x),
-           add || apart ? 0 : n * d * static_cast<int64_t>(sizeof(O)), s);
+           filled * row_bytes, s);
     }
     with_type(grad.type, [&](auto t) {
       using T       = decltype(t);
@@ -936,7 +1008,8 @@ void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n
           sum_few_kernel<T, O, F, W == 1><<<sums + clears, kThreads, 0, s>>>(ids, rows, from, grad.stride, width, scale, add,
                                                                              to, out.stride, slices, sums, clear);
         else
-          sum_runs_kernel<T, O, W><<<sums, kThreads, 0, s>>>(sorted, from, grad.stride, width, scale, add, to, out.stride, slices);
+          sum_runs_kernel<T, O, W><<<sums + static_cast<unsigned>(ceil_div(left, per_group)), kThreads, 0, s>>>(
+            sorted, from, grad.stride, width, scale, add, to, out.stride, slices, {sums, filled, static_cast<int>(per_group)});
         OCTEX_HIP(hipGetLastError());
       });
     });

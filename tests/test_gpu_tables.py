@@ -191,6 +191,28 @@ def test_gradient_of_tables_of_any_length(O, n, m):
     close(got, want, rounded(m * E * 4 * max(1.0, m / n), want, "float16"), "gradient")
 
 
+@pytest.mark.parametrize("m", [700, 1500, 30_000])
+@pytest.mark.parametrize("kind", ["one", "few", "common", "any", "padding"])
+@pytest.mark.parametrize("n,d,apart", [(45_000, 1001, 0), (9000, 7, 1), (5000, 64, 5), (301, 513, 1), (40, 300_000, 0), (150_000, 512, 0)])
+def test_every_row_without_an_id_is_cleared(O, m, kind, n, d, apart):
+    """Tables larger than what is filled beside the sort, and rows that lie apart; whatever the memory held."""
+    from octex_amd import scores
+
+    if m * d > 40_000_000:
+        m = 40_000_000 // d
+    g = gen(m)
+    ids = ids_of(g, m, n, kind)
+    grad = torch.randint(-4, 5, (m, d), generator=g, device="cuda").bfloat16()
+    wide = torch.full((n, d + apart), float("nan"), device="cuda")
+    out, column = wide[:, :d], ids[:, None]
+    c = scores._Call(grad, "grad", scores.FLOATS)
+    c.run_sized("octexEmbedBackward", c.matrix(grad), c.matrix(column), 1.0, 0, c.matrix(out))
+    at = torch.where((ids >= 0) & (ids < n), ids, n)
+    want = torch.zeros((n + 1, d), device="cuda").index_add_(0, at, grad.float())[:n]  # whole numbers: exact in any order
+    assert torch.equal(out, want)
+    assert wide[:, d:].isnan().all()
+
+
 @pytest.mark.parametrize("given", TYPES)
 @pytest.mark.parametrize("result", TYPES)
 def test_gradient_types(O, given, result):
