@@ -364,7 +364,40 @@ __global__ __launch_bounds__(kSortThreads) void count_digits_kernel(row_ids ids,
   if (threadIdx.x < kDigits) tiles[int64_t{blockIdx.x} * kDigits + threadIdx.x] = counts[threadIdx.x];
 }
 
-/** Moves a tile's tokens to their places by one digit; every workgroup adds up the tiles' counts itself. */
+constexpr int kFewTiles = 64;  // whose counts every workgroup adds up itself
+constexpr int kScanDigits = 16, kScanGroups = kSortThreads / kScanDigits;
+
+/** Turns the counts of tiles into those of all tiles before each, and their sums into one more row; kScanDigits digits a
+ * workgroup, a share of the tiles each of its groups of threads. */
+__global__ __launch_bounds__(kSortThreads) void scan_tiles_kernel(int* tiles, unsigned n_tiles)
+{
+  __shared__ int sums[kScanGroups][kScanDigits];
+  const int group = static_cast<int>(threadIdx.x) / kScanDigits, mine = static_cast<int>(threadIdx.x) % kScanDigits;
+  int* const column   = tiles + blockIdx.x * kScanDigits + mine;
+  const int64_t width = (int64_t{n_tiles} + kScanGroups - 1) / kScanGroups;
+  const int64_t b0 = min(group * width, int64_t{n_tiles}), b1 = min(b0 + width, int64_t{n_tiles});
+  int sum = 0;
+#pragma unroll 8
+  for (int64_t b = b0; b < b1; ++b)
+    sum += column[b * kDigits];
+  sums[group][mine] = sum;
+  lds_barrier();
+  int before = 0, all = 0;
+  for (int g = 0; g < kScanGroups; ++g) {
+    before += g < group ? sums[g][mine] : 0;
+    all += sums[g][mine];
+  }
+#pragma unroll 8
+  for (int64_t b = b0; b < b1; ++b) {
+    const int count     = column[b * kDigits];
+    column[b * kDigits] = before;
+    before += count;
+  }
+  if (group == 0) column[int64_t{n_tiles} * kDigits] = all;
+}
+
+/** Moves a tile's tokens to their places by one digit; of up to kFewTiles tiles every workgroup adds up the counts itself, else
+ * scan_tiles_kernel has. */
 template <int P>
 __global__ __launch_bounds__(kSortThreads) void move_tokens_kernel(row_ids ids, unsigned n, const token* in, digit d,
                                                                    const int* tiles, token* out, unsigned n_tiles,
@@ -378,7 +411,10 @@ __global__ __launch_bounds__(kSortThreads) void move_tokens_kernel(row_ids ids, 
   read_tile<P>(ids, n, in, int64_t{blockIdx.x} * (kSortThreads * P), t);
   clear_counts(counts);
   int before = 0, all = 0;
-  if (threadIdx.x < kDigits) {
+  if (threadIdx.x < kDigits && n_tiles > kFewTiles) {
+    before = tiles[int64_t{blockIdx.x} * kDigits + threadIdx.x];
+    all    = tiles[int64_t{n_tiles} * kDigits + threadIdx.x];
+  } else if (threadIdx.x < kDigits) {
 #pragma unroll 16
     for (unsigned b = 0; b < n_tiles; ++b) {
       const int count = tiles[int64_t{b} * kDigits + threadIdx.x];
@@ -892,7 +928,7 @@ auto layout_of(int64_t m, int64_t n, int64_t d) -> sort_layout
   l.chunks        = ceil_div(m, width);
   l.second        = up(m * static_cast<int64_t>(sizeof(token)));
   l.counts        = l.tiles > 1 ? 2 * l.second : l.second;
-  l.cut           = l.counts + (l.tiles > 1 ? up(l.tiles * kDigits * 4) : 0);
+  l.cut           = l.counts + (l.tiles > 1 ? up((l.tiles + 1) * kDigits * 4) : 0);
   l.end           = l.cut + l.chunks * 2 * d * 4;
   return l;
 }
@@ -924,6 +960,10 @@ void sort_tiles(row_ids const& ids, unsigned n, sort_layout const& l, token* tok
     const auto f = share(2 * p), g = share(2 * p + 1);
     count_digits_kernel<P><<<tiles + f.blocks, kSortThreads, 0, s>>>(ids, n, in, of, counts, tiles, f);
     OCTEX_HIP(hipGetLastError());
+    if (tiles > kFewTiles) {
+      scan_tiles_kernel<<<kDigits / kScanDigits, kSortThreads, 0, s>>>(counts, tiles);
+      OCTEX_HIP(hipGetLastError());
+    }
     move_tokens_kernel<P><<<tiles + g.blocks, kSortThreads, 0, s>>>(ids, n, in, of, counts, to_first ? tokens : second, tiles, g);
     OCTEX_HIP(hipGetLastError());
   }

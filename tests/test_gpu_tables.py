@@ -176,6 +176,19 @@ def test_gradient_of_wide_chunks(O, m, n, d, kind):
     check_gradient(O, randn(g, m, d).bfloat16(), ids_of(g, m, n, kind), n)
 
 
+@pytest.mark.parametrize("m", [524_288, 524_289, 3_000_017])
+@pytest.mark.parametrize("kind", ["few", "common", "any"])
+def test_gradient_of_many_tokens(O, m, kind):
+    """More tiles than a workgroup adds up; whole numbers, whose sums are exact in any order."""
+    g = gen(m)
+    n, d = 70_000, 4
+    ids = ids_of(g, m, n, kind)
+    grad = torch.randint(-2, 3, (m, d), generator=g, device="cuda").half()
+    at = torch.where((ids >= 0) & (ids < n), ids, n)
+    want = torch.zeros((n + 1, d), dtype=torch.float64, device="cuda").index_add_(0, at, grad.double())[:n]
+    assert torch.equal(O.embed_backward(grad, ids, n, dtype="float32").double(), want)
+
+
 @pytest.mark.parametrize("n", [1, 2, 511, 512, 513, 300_000, 5_000_000, 140_000_000])
 @pytest.mark.parametrize("m", [100, 9000])
 def test_gradient_of_tables_of_any_length(O, n, m):
