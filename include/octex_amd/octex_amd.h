@@ -6,7 +6,8 @@
  *   - the stage entry points: one HIP kernel each, on caller-provided device buffers, so that the
  *     parity tests call every kernel of the search path with controlled inputs (as the reference's
  *     cpp/tests/test_search.cu launches its kernels directly);
- *   - operators on rows of scores: products in 8-bit integers, log probabilities, distillation.
+ *   - operators on rows of scores: products in 8-bit integers, log probabilities, distillation, a policy's clipped loss, the
+ *     balance of rows over experts; rows of a table by ids and the table's gradient.
  * All return CUVS_SUCCESS / CUVS_ERROR with cuvsGetLastErrorText() set; `stream` is a hipStream_t
  * (NULL: the null stream); the stage calls wait for their kernel before returning.
  */
