@@ -784,20 +784,23 @@ __global__ __launch_bounds__(kJoinThreads) void join_runs_kernel(sorted_tokens s
   }
 }
 
-constexpr int kFewTokens = 1024;
+constexpr int kFewTokens = 1024, kSomeTokens = 4096;
+constexpr int kLongRun = 4 * kTokensAhead;  // by one team 120 equal tokens of 1024 took 13.7 us, by all 9.4
 
 /**
- * The same for up to kFewTokens tokens without sorting them: a team a token looks through all of them, and the first one of a
- * row lists the places of the others and adds up their gradients.  Workgroups from `sum_blocks` on clear rows.
+ * The same for up to M tokens without sorting them: a team a token looks through all of them, W at a time, and the first one of a
+ * row lists the places of the others and adds up their gradients; those of more than kLongRun (a common token's) all teams of the
+ * workgroup add up.  Workgroups from `sum_blocks` on clear rows, `clear` (at most M) each.
  */
-template <typename T, typename O, int W, bool kShort>
+template <typename T, typename O, int W, bool kShort, int M>
 __global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned n, const T* grad, int64_t gstride, int d,
-                                                           float scale, bool add, O* out, int64_t ostride, unsigned slices, unsigned sum_blocks,
-                                                           int clear)
+                                                           float scale, bool add, O* out, int64_t ostride, unsigned slices,
+                                                           unsigned sum_blocks, int clear)
 {
-  constexpr int kTeams = kThreads / W, kPer = kFewTokens / kThreads;
-  __shared__ unsigned rows[kFewTokens];
-  __shared__ unsigned short places[kTeams][kFewTokens];
+  constexpr int kTeams = kThreads / W, kPer = M / kThreads, kLooks = M / kFewTokens;
+  __shared__ unsigned rows[std::max(M, kUnit * kThreads)];
+  __shared__ unsigned short places[kTeams][M];
+  __shared__ int counts[kTeams];
   const int m = static_cast<int>(ids.m);
   int64_t id[kPer];
 #pragma unroll
@@ -808,7 +811,8 @@ __global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned
     bool* used       = reinterpret_cast<bool*>(rows);
     const int64_t v0 = int64_t{blockIdx.x - sum_blocks} * clear;
     const int mine   = static_cast<int>(min(int64_t{n} - v0, int64_t{clear}));
-    used[threadIdx.x] = false;
+    for (int r = threadIdx.x; r < mine; r += kThreads)
+      used[r] = false;
     lds_barrier();
 #pragma unroll
     for (int q = 0; q < kPer; ++q)
@@ -823,40 +827,73 @@ __global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned
   const int team = static_cast<int>(threadIdx.x) / W, lane = threadIdx.x % 64, sub = lane % W;
   const unsigned all = blockIdx.x * kTeams + team;
   const int token    = static_cast<int>(all / slices), at = (static_cast<int>(all % slices) * W + sub) * kUnit;
-  if (token >= m) return;
-  const unsigned row = rows[token];
-  if (row >= n) return;
-  int count        = 0;
+  const unsigned row = token < m ? rows[token] : n;
   const auto above = [&](unsigned long long lanes) { return W == 64 ? lanes : lanes >> (lane - sub) & ((1ull << (W % 64)) - 1); };
-  for (int i = 0; i < m; i += W) {
-    const bool in   = rows[i + sub] == row;
-    const auto same = above(__ballot(in));
-    if (same == 0) continue;
-    if (i + __builtin_ctzll(same) < token) return;  // an earlier token has the row
-    if (in) places[team][count + __popcll(same & ((1ull << sub) - 1))] = static_cast<unsigned short>(i + sub);
-    count += __popcll(same);
-  }
-  wave_fence();
-  const int from = unit_start(at, d);
-  float sum[kUnit];
+  int count = 0;
+  for (int i = 0; i < m && row < n; i += W * kLooks) {
+    bool in[kLooks], earlier = false;
 #pragma unroll
-  for (int i = 0; i < kUnit; ++i)
-    sum[i] = 0.f;
-  for (int j = 0; j < count; j += kTokensAhead) {
-    unit<T> u[kTokensAhead];
+    for (int q = 0; q < kLooks; ++q)
+      in[q] = rows[i + q * W + sub] == row;
 #pragma unroll
-    for (int q = 0; q < kTokensAhead; ++q)
-      u[q] = load_unit<kShort>(grad + of_team<W>(static_cast<int>(places[team][min(j + q, count - 1)])) * gstride, from, d);
-#pragma unroll
-    for (int q = 0; q < kTokensAhead; ++q) {
-      float v[kUnit];
-      unpack_unit(u[q], v);
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i)
-        sum[i] += j + q < count ? v[i] : 0.f;
+    for (int q = 0; q < kLooks; ++q) {
+      const auto same = above(__ballot(in[q]));
+      if (same == 0) continue;
+      earlier = earlier || i + q * W + __builtin_ctzll(same) < token;
+      if (in[q]) places[team][count + __popcll(same & ((1ull << sub) - 1))] = static_cast<unsigned short>(i + q * W + sub);
+      count += __popcll(same);
+    }
+    if (earlier) {  // that token's team has the row
+      count = 0;
+      break;
     }
   }
-  write_sum<kShort>(sum, scale, add, out + row * ostride, at, d);
+  if (sub == 0) counts[team] = count;
+  float sum[kUnit];
+  // the gradients of kTokensAhead of every `step` listed places, from `first` on
+  const auto add_up = [&](const unsigned short* list, int length, int first, int step, int from) {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+      sum[i] = 0.f;
+    for (int j = first; j < length; j += step) {
+      unit<T> u[kTokensAhead];
+#pragma unroll
+      for (int q = 0; q < kTokensAhead; ++q)
+        u[q] = load_unit<kShort>(grad + of_team<W>(static_cast<int>(list[min(j + q, length - 1)])) * gstride, from, d);
+#pragma unroll
+      for (int q = 0; q < kTokensAhead; ++q) {
+        float v[kUnit];
+        unpack_unit(u[q], v);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i)
+          sum[i] += j + q < length ? v[i] : 0.f;
+      }
+    }
+  };
+  wave_fence();
+  if (count > 0 && count <= kLongRun) {
+    add_up(places[team], count, 0, kTokensAhead, unit_start(at, d));
+    write_sum<kShort>(sum, scale, add, out + row * ostride, at, d);
+  }
+  lds_barrier();
+  auto* const parts = reinterpret_cast<float(*)[kThreads]>(rows);  // the rows of tokens make room
+  for (int t = 0; t < kTeams; ++t) {
+    if (counts[t] <= kLongRun) continue;
+    const int its_at = (static_cast<int>((blockIdx.x * kTeams + t) % slices) * W + sub) * kUnit;
+    add_up(places[t], counts[t], team * kTokensAhead, kTeams * kTokensAhead, unit_start(its_at, d));
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+      parts[i][threadIdx.x] = sum[i];
+    lds_barrier();
+    if (team == t) {
+      for (int other = 0; other < kTeams; ++other)
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i)
+          sum[i] = (other == 0 ? 0.f : sum[i]) + parts[i][other * W + sub];
+      write_sum<kShort>(sum, scale, add, out + row * ostride, at, d);
+    }
+    lds_barrier();
+  }
 }
 
 /** Calls f with a value of the element type. */
@@ -906,6 +943,14 @@ auto chunk_width(int64_t m, int64_t d) -> int
   return width;
 }
 
+/** Whether a gradient's tokens are looked through, by every slice of every token, and not sorted: one launch in place of three to
+ * six.  8000 x 512 bfloat16 from 4096 tokens, the i-th commonest as 1 / i: 19 us, sorted 28; 2000 x 64 from 2000: 11 and 25; 8000
+ * x 1024 from 3000, at the rule's other side, 34 and 28. */
+auto takes_few(int64_t m, int64_t d) -> bool
+{
+  return m <= kFewTokens || (m <= kSomeTokens && m * m * ceil_div(d, 64 * kUnit) <= int64_t{1} << 24);
+}
+
 /** How the workspace is laid out, from place to place in bytes. */
 struct sort_layout {
   int passes, bits, per;  // of a digit; tokens of a thread
@@ -916,7 +961,7 @@ auto layout_of(int64_t m, int64_t n, int64_t d) -> sort_layout
 {
   const auto up = [](int64_t v) { return ceil_div(v, 256) * 256; };
   sort_layout l{};
-  if (m <= kFewTokens) return l;
+  if (takes_few(m, d)) return l;
   int bits = 1;
   while (n >> bits != 0)
     ++bits;
@@ -1012,10 +1057,11 @@ void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n
 {
   const auto rows  = static_cast<unsigned>(n);
   const auto width = static_cast<int>(d);
-  const bool few   = ids.m <= kFewTokens;
-  // of few tokens: rows that a workgroup clears, 16 KB of them
-  const int clear = static_cast<int>(
-    std::clamp<int64_t>(std::max((16 << 10) / (d * elem_size(out.type)), ceil_div(n, 1 << 22)), 1, kThreads));
+  const bool few = takes_few(ids.m, d), fewer = ids.m <= kFewTokens;
+  // of few tokens: rows that a workgroup clears, 16 KB of them, or 64 KB where it reads more ids for that
+  const int64_t least = (fewer ? 16 << 10 : 64 << 10) / (d * elem_size(out.type));
+  const int clear     = static_cast<int>(
+    std::clamp<int64_t>(std::max(least, ceil_div(n, 1 << 22)), 1, fewer ? kFewTokens : kSomeTokens));
   const auto clears = add || !few ? 0u : static_cast<unsigned>(ceil_div(n, clear));
   const auto l      = layout_of(ids.m, n, d);
   auto* base        = static_cast<char*>(workspace);
@@ -1043,10 +1089,18 @@ void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n
         constexpr int W   = lanes();
         constexpr int F   = std::max(W, 8);
         const auto slices = static_cast<unsigned>(ceil_div(d, W == 1 ? kUnit : W * kUnit));
-        const auto sums   = static_cast<unsigned>(ceil_div((few ? ids.m : l.chunks) * slices, kThreads / (few ? F : W)));
-        if (few)
-          sum_few_kernel<T, O, F, W == 1><<<sums + clears, kThreads, 0, s>>>(ids, rows, from, grad.stride, width, scale, add,
-                                                                             to, out.stride, slices, sums, clear);
+        const int team    = !few ? W : fewer ? F : 64;
+        const auto sums   = static_cast<unsigned>(ceil_div((few ? ids.m : l.chunks) * slices, kThreads / team));
+        const auto launch_few = [&](auto kernel) {
+          kernel<<<sums + clears, kThreads, 0, s>>>(ids, rows, from, grad.stride, width, scale, add, to, out.stride, slices, sums,
+                                                    clear);
+        };
+        if (fewer)
+          launch_few(sum_few_kernel<T, O, F, W == 1, kFewTokens>);
+        else if (few && ids.m <= kSomeTokens / 2)
+          launch_few(sum_few_kernel<T, O, 64, W == 1, kSomeTokens / 2>);
+        else if (few)
+          launch_few(sum_few_kernel<T, O, 64, W == 1, kSomeTokens>);
         else
           sum_runs_kernel<T, O, W><<<sums + static_cast<unsigned>(ceil_div(left, per_group)), kThreads, 0, s>>>(
             sorted, from, grad.stride, width, scale, add, to, out.stride, slices, {sums, filled, static_cast<int>(per_group)});

@@ -176,6 +176,16 @@ def test_gradient_of_wide_chunks(O, m, n, d, kind):
     check_gradient(O, randn(g, m, d).bfloat16(), ids_of(g, m, n, kind), n)
 
 
+@pytest.mark.parametrize("m,widths", [(1024, (8, 100, 600)), (1025, (5, 24, 600)), (2048, (3, 64, 1001)), (2049, (7, 130, 520)),
+                                      (2896, (9, 513)), (4095, (1, 65, 512)), (4096, (8, 256, 511))])
+@pytest.mark.parametrize("kind", ["one", "few", "common", "any", "padding"])
+def test_gradient_of_unsorted_tokens(O, m, widths, kind):
+    """Up to 4096 tokens, which are looked through; runs that a workgroup adds up."""
+    for d in widths:
+        g = gen(m + d)
+        check_gradient(O, randn(g, m, d), ids_of(g, m, 700, kind), 700)
+
+
 @pytest.mark.parametrize("m", [524_288, 524_289, 3_000_017])
 @pytest.mark.parametrize("kind", ["few", "common", "any"])
 def test_gradient_of_many_tokens(O, m, kind):
