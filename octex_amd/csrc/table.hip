@@ -945,10 +945,10 @@ auto chunk_width(int64_t m, int64_t d) -> int
 
 /** Whether a gradient's tokens are looked through, by every slice of every token, and not sorted: one launch in place of three to
  * six.  8000 x 512 bfloat16 from 4096 tokens, the i-th commonest as 1 / i: 19 us, sorted 28; 2000 x 64 from 2000: 11 and 25; 8000
- * x 1024 from 3000, at the rule's other side, 34 and 28. */
+ * x 1024 from 3000: 22 and 29; near the bound 8000 x 1000 from 4096 28 and 30, 8000 x 2000 from 2500 32 and 30. */
 auto takes_few(int64_t m, int64_t d) -> bool
 {
-  return m <= kFewTokens || (m <= kSomeTokens && m * m * ceil_div(d, 64 * kUnit) <= int64_t{1} << 24);
+  return m <= kFewTokens || (m <= kSomeTokens && m * m * ceil_div(d, 64 * kUnit) <= int64_t{1} << 25);
 }
 
 /** How the workspace is laid out, from place to place in bytes. */
