@@ -339,8 +339,8 @@ cuvsError_t octexEmbed(const octexMatrix* table, const float* row_scales, const 
 /**
  * The gradient of a table's rows, out [n, d] (float32, float16 or bfloat16): out[v] = scale * the sum of grad[i] over the i with
  * ids[i] = v, grad [m, d] (float32, float16 or bfloat16), or with `add` not 0 that much more than it held, rows without an id
- * then staying as they are.  Sums are float32, in an order that the ids alone determine, and rounded once.  Ids outside [0, n)
- * are left out.  `workspace` and `size` as for octexInt8Scores.
+ * then staying as they are.  Sums are float32, in an order that the ids and sizes alone determine, and rounded once.  Ids outside
+ * [0, n) are left out.  `workspace` and `size` as for octexInt8Scores.
  */
 cuvsError_t octexEmbedBackward(const octexMatrix* grad, const octexMatrix* ids, float scale, int32_t add,
                                const octexMatrix* out, void* workspace, int64_t bytes, int64_t* size, void* stream);

@@ -56,9 +56,9 @@ def embed_backward(grad, ids, rows=None, *, scale=1.0, dtype=None, add_to=None):
     """The gradient [rows, d] of a table of `rows` rows, given that of embed's result, grad [..., d], and its ids [...]: row v is
     scale times the sum of grad over the places where ids is v.
 
-    Sums are float32, in an order that the ids alone determine, and rounded once to `dtype` (grad's own type).  Ids outside
-    [0, rows) are left out.  With `add_to`, a torch matrix [rows, d] of floats on grad's GPU, the gradient is added to it in
-    place, and it is returned; rows without an id are not touched.
+    Sums are float32, in an order that the ids and sizes alone determine, and rounded once to `dtype` (grad's own type).  Ids
+    outside [0, rows) are left out.  With `add_to`, a torch matrix [rows, d] of floats on grad's GPU that shares no memory with
+    grad, the gradient is added to it in place, and it is returned; rows without an id are not touched.
     """
     c = scores._Call(grad, "grad", FLOATS, flat=True)
     g = c.first

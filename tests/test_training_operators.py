@@ -138,3 +138,34 @@ def test_embed_sizes_and_no_work():
     accepted("octexEmbed", matrix(9, 16), None, none[1], 1.0, none[0])
     accepted("octexEmbedBackward", *none, 1.0, 1, matrix(9, 16), None, 0, None)
     accepted("octexEmbedBackward", *none, 1.0, 0, none[0], None, 0, None)
+
+
+def test_a_workspace_is_asked_for_once_for_its_sizes(monkeypatch):
+    import torch
+
+    asked, ran = [], []
+
+    def entry(name):
+        def call(rows, workspace, size, at, stream):
+            if at is None:
+                ran.append((rows, size, workspace is not None))
+            else:
+                asked.append(rows)
+                ct.c_int64.from_address(at).value = 100 * rows
+            return _lib.CUVS_SUCCESS
+
+        return call
+
+    monkeypatch.setattr(S, "_entry", entry)
+    monkeypatch.setattr(S, "_WORKSPACES", {})
+    c = S._Call.__new__(S._Call)
+    c.torch, c.device, c.stream, c.side, c.others = torch, torch.device("cpu"), None, None, ()
+    for rows in (3, 3, 0, 4, 3, 0):
+        c.run_sized("any", rows, sizes=("any", rows))
+    assert asked == [3, 0, 4]
+    assert ran == [(3, 300, True), (3, 300, True), (0, 0, False), (4, 400, True), (3, 300, True), (0, 0, False)]
+    c.run_sized("any", 5), c.run_sized("any", 5)
+    assert asked == [3, 0, 4, 5, 5]
+    S._WORKSPACES.update((("full", i), 0) for i in range(4096))  # as many as are kept
+    c.run_sized("any", 6, sizes=("any", 6))
+    assert S._WORKSPACES == {("any", 6): 600}
