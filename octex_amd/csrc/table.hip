@@ -21,22 +21,22 @@ namespace {
 constexpr int kUnit    = 8;  // values that a lane takes at a time
 constexpr int kThreads = 256;
 
-/** kUnit values as they lie in memory. */
-template <typename T>
+/** U values as they lie in memory. */
+template <typename T, int U = kUnit>
 struct unit {
-  static constexpr int kWords = kUnit * static_cast<int>(sizeof(T)) / 4;
+  static constexpr int kWords = U * static_cast<int>(sizeof(T)) / 4;
   unsigned w[kWords];
 };
 
-/** The values of a row from `from` on; of a row of d < kUnit (kShort) all of them, and 0 behind its end. */
-template <bool kShort, typename T>
-__device__ inline auto load_unit(const T* row, int from, int d) -> unit<T>
+/** The values of a row from `from` on; of a row of d < U (kShort) all of them, and 0 behind its end. */
+template <bool kShort, int U = kUnit, typename T>
+__device__ inline auto load_unit(const T* row, int from, int d) -> unit<T, U>
 {
-  unit<T> u;
+  unit<T, U> u;
   if constexpr (kShort) {
-    T e[kUnit];
+    T e[U];
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i)
+    for (int i = 0; i < U; ++i)
       e[i] = i < d ? row[i] : T{};
     __builtin_memcpy(u.w, e, sizeof(u.w));
   } else {
@@ -45,42 +45,42 @@ __device__ inline auto load_unit(const T* row, int from, int d) -> unit<T>
   return u;
 }
 
-template <typename T>
-__device__ inline void unpack_unit(unit<T> const& u, float (&v)[kUnit])
+template <typename T, int U>
+__device__ inline void unpack_unit(unit<T, U> const& u, float (&v)[U])
 {
-  if constexpr (sizeof(T) == 1) {
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i)
+  for (int i = 0; i < U; ++i) {
+    if constexpr (sizeof(T) == 1)
       v[i] = static_cast<float>(static_cast<int>(u.w[i / 4] << (24 - 8 * (i % 4))) >> 24);
-  } else {
-    constexpr int N = kPer16<T>;
-#pragma unroll
-    for (int j = 0; j < kUnit / N; ++j) {
-      float e[N];
-      unpack16<T>(uint4{u.w[4 * j], u.w[4 * j + 1], u.w[4 * j + 2], u.w[4 * j + 3]}, e);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        v[j * N + i] = e[i];
-    }
+    else if constexpr (sizeof(T) == 4)
+      v[i] = __uint_as_float(u.w[i]);
+    else if constexpr (std::is_same_v<T, bf16>)
+      v[i] = __uint_as_float(i % 2 == 0 ? u.w[i / 2] << 16 : u.w[i / 2] & 0xffff0000u);
+    else
+      v[i] = static_cast<float>(__builtin_bit_cast(f16, static_cast<unsigned short>(u.w[i / 2] >> 16 * (i % 2))));
   }
 }
 
-/** Where a lane finds its unit at the column `at` (a multiple of kUnit): one that would pass the row's end is moved back to it, so
+/** Where a lane finds its unit at the column `at` (a multiple of U): one that would pass the row's end is moved back to it, so
  * that columns before `at` are another lane's too. */
-__device__ inline auto unit_start(int at, int d) -> int { return max(min(at, d - kUnit), 0); }
+template <int U = kUnit>
+__device__ inline auto unit_start(int at, int d) -> int
+{
+  return max(min(at, d - U), 0);
+}
 
 /** Stores a unit; lanes that have a column twice store it alike. */
-template <bool kShort, typename T>
-__device__ inline void store_unit(T* row, const float (&v)[kUnit], int from, int d, bool by_cache)
+template <bool kShort, typename T, int U>
+__device__ inline void store_unit(T* row, const float (&v)[U], int from, int d, bool by_cache)
 {
   constexpr int N = kPer16<T>;
   if constexpr (kShort) {
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i)
+    for (int i = 0; i < U; ++i)
       if (i < d) row[i] = static_cast<T>(v[i]);
   } else {
 #pragma unroll
-    for (int j = 0; j < kUnit / N; ++j) {
+    for (int j = 0; j < U / N; ++j) {
       float e[N];
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -110,30 +110,35 @@ __device__ inline void read_ids(row_ids const& ids, int64_t i0, int64_t step, in
 
 constexpr int kRowsAhead = 4;  // rows that a team has on their way
 
+/** Values of a result's 16 bytes, which a lane has: past the caches, pieces that do not lie side by side leave their lines in parts
+ * (8 values of float32 a lane, in two pieces: 17,235 x 2752 of a table in 92 us). */
+template <typename O>
+constexpr int kResultUnit = kPer16<O>;
+
 /**
- * Teams of W lanes (1: of rows shorter than a unit) take kRowsAhead rows each, a unit a lane (of one of `slices` slices of their
- * columns, side by side in a workgroup): all ids first, then all rows, then the results.  No load waits for a condition: padding
- * takes the table's first row and drops it.
+ * Teams of W lanes (1: of rows shorter than a unit) take kRowsAhead rows each, kResultUnit values a lane (of one of `slices`
+ * slices of their columns, side by side in a workgroup): all ids first, then all rows, then the results.  No load waits for a
+ * condition: padding takes the table's first row and drops it.
  */
 template <typename T, typename O, int W>
 __global__ __launch_bounds__(kThreads) void embed_kernel(table_rows table, row_ids ids, int d, float scale, O* out,
                                                          int64_t ostride, bool by_cache, unsigned slices, int64_t block0)
 {
-  constexpr int kTeams = kThreads / W;
+  constexpr int kTeams = kThreads / W, U = kResultUnit<O>;
   const int64_t team   = (block0 + blockIdx.x) * kTeams + threadIdx.x / W;
   const int64_t i0     = team / slices * kRowsAhead;
-  const int at         = (static_cast<int>(team % slices) * W + static_cast<int>(threadIdx.x) % W) * kUnit;
+  const int at         = (static_cast<int>(team % slices) * W + static_cast<int>(threadIdx.x) % W) * U;
   if (at >= d || i0 >= ids.m) return;
-  const int from = unit_start(at, d);
+  const int from = unit_start<U>(at, d);
   int64_t id[kRowsAhead];
   float s[kRowsAhead];
-  unit<T> u[kRowsAhead] = {};
+  unit<T, U> u[kRowsAhead] = {};
   read_ids(ids, i0, 1, id);
   if (table.n > 0) {
 #pragma unroll
     for (int q = 0; q < kRowsAhead; ++q) {
       const int64_t v = id[q] < 0 || id[q] >= table.n ? 0 : id[q];
-      u[q]            = load_unit<W == 1>(static_cast<const T*>(table.x) + v * table.stride, from, d);
+      u[q]            = load_unit<W == 1, U>(static_cast<const T*>(table.x) + v * table.stride, from, d);
       s[q]            = sizeof(T) == 1 ? scale * table.scales[v] : scale;
     }
   }
@@ -141,10 +146,10 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(table_rows table, row_i
   for (int q = 0; q < kRowsAhead; ++q) {
     if (i0 + q >= ids.m) break;
     const bool listed = id[q] >= 0 && id[q] < table.n;
-    float v[kUnit];
+    float v[U];
     unpack_unit(u[q], v);
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i)
+    for (int i = 0; i < U; ++i)
       v[i] = listed ? v[i] * s[q] : 0.f;
     store_unit<W == 1>(out + (i0 + q) * ostride, v, from, d, by_cache);
   }
@@ -909,11 +914,11 @@ void with_type(elem type, F f)
 }
 
 /** Calls f with the lanes of a row's team: its units, or 64 of them a slice; one for rows shorter than a unit. */
-template <typename F>
+template <int U = kUnit, typename F>
 void with_team(int64_t d, F f)
 {
-  const int64_t units = (d + kUnit - 1) / kUnit;
-  if (d < kUnit)
+  const int64_t units = (d + U - 1) / U;
+  if (d < U)
     f(std::integral_constant<int, 1>{});
   else if (units <= 8)
     f(std::integral_constant<int, 8>{});
@@ -1031,9 +1036,9 @@ void launch_embed(table_rows const& table, row_ids const& ids, int64_t d, float 
     using T = decltype(t);
     with_type(out.type, [&](auto o) {
       using O = decltype(o);
-      with_team(d, [&](auto lanes) {
+      with_team<kResultUnit<O>>(d, [&](auto lanes) {
         constexpr int W      = lanes();
-        const auto slices    = static_cast<unsigned>(ceil_div(d, W == 1 ? kUnit : W * kUnit));
+        const auto slices    = static_cast<unsigned>(ceil_div(d, W * kResultUnit<O>));
         const int64_t blocks = ceil_div(ceil_div(ids.m, kRowsAhead) * slices, kThreads / W);
         for (int64_t first = 0; first < blocks; first += kMaxGrid) {
           embed_kernel<T, O, W><<<static_cast<unsigned>(std::min(kMaxGrid, blocks - first)), kThreads, 0, s>>>(
