@@ -9,7 +9,8 @@
 // A row's sums are those of log_probs (rows_device.hpp), and its gradient p (a + b ln p) with one share w at the id:
 // a = g / T (entropy H - c), b = g / T entropy, w = g / T c.  A row whose id is padding (a prompt's token) is not read.
 //
-// Bound by the logits' bytes: a large copy takes 5.06 TB/s of this GPU.
+// Bound by the logits' bytes: a large copy takes 5.06 TB/s of this GPU.  Both directions of 4096 x 128,000 bfloat16 take 456 us,
+// 4.6 TB/s; 333 x 50,021 float16 10 and 13; 16 x 32,000 float32 10, where a row is one CU's and its exponentials bound it.
 
 #include "policy.hpp"
 #include "rows_device.hpp"
