@@ -363,7 +363,9 @@ __global__ __launch_bounds__(kFinishThreads) void finish_balance_kernel(balance_
   if (lane == 0) *out.loss = loss_of(w, e, rows_here, sum, inner);
 }
 
-constexpr int kMaxCountParts = 64, kMaxWorkgroups = 512;
+constexpr int kMaxCountParts = 64;
+/** Threads of a pass: two workgroups of 512 a CU, or one of 1024 (30,000 x 128 bfloat16: 20 us; two 28). */
+constexpr int kMaxThreads = 1 << 18;
 
 auto pieces_of(int e, elem type) -> int { return (e * elem_size(type) + 15) / 16; }
 
@@ -411,10 +413,12 @@ struct balance_plan {
 auto plan_of(int64_t m, int e, int k, elem type) -> balance_plan
 {
   balance_plan p{};
-  int teams = 1;
-  with_type(type, [&](auto x) { with_team<decltype(x)>(m, pieces_of(e, type), [&](auto nt, auto w, auto) { teams = nt() / w(); }); });
+  int threads = 1, teams = 1;
+  with_type(type, [&](auto x) {
+    with_team<decltype(x)>(m, pieces_of(e, type), [&](auto nt, auto w, auto) { threads = nt(), teams = nt() / w(); });
+  });
   p.alone       = m * e <= 32768 && m * k <= 8192;
-  p.workgroups  = p.alone ? 1 : static_cast<int>(std::min<int64_t>((m + teams - 1) / teams, kMaxWorkgroups));
+  p.workgroups  = p.alone ? 1 : static_cast<int>(std::min<int64_t>((m + teams - 1) / teams, kMaxThreads / threads));
   p.count_parts = static_cast<int>(std::clamp<int64_t>(m / kCountThreads, 1, kMaxCountParts));
   p.width       = (m + p.count_parts - 1) / p.count_parts;
   return p;
