@@ -737,53 +737,71 @@ __global__ __launch_bounds__(kThreads) void sum_runs_kernel(sorted_tokens s, con
 }
 
 constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
+constexpr int kJoinLanes = 32, kJoinTeams = kJoinThreads / kJoinLanes;
+constexpr int kPartsAhead = 4;
 
-/** Joins the sums of the runs that begin in the chunks of a workgroup, one a wavefront to look at, and are cut; 64 units of their
- * columns a workgroup. */
+/**
+ * Joins the sums of the runs that begin in the chunks of a workgroup, one a wavefront to look at, and are cut; kJoinLanes units of
+ * their columns (one of `slices` slices) a workgroup, whose teams take parts in turn, kPartsAhead of them on their way.  A common
+ * token's run, or that of a batch's padding where it is a row of the table, has many: 65,536 tokens of 512 bfloat16 values, half of
+ * them equal, take 67 us, and 222 where a workgroup of wavefronts for 512 columns each goes from part to part.
+ */
 template <typename O, bool kShort>
 __global__ __launch_bounds__(kJoinThreads) void join_runs_kernel(sorted_tokens s, int d, float scale, bool add, O* out,
-                                                                 int64_t ostride, int64_t chunks, int64_t block0)
+                                                                 int64_t ostride, int64_t chunks, unsigned slices, int64_t block0)
 {
-  __shared__ float sums[kJoinWaves][64][kUnit];
+  __shared__ float sums[kJoinWaves][kUnit][kJoinLanes];
   __shared__ unsigned rows[kJoinWaves];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int at = (static_cast<int>(blockIdx.y) * 64 + lane) * kUnit;
-  const int64_t chunk0 = (block0 + blockIdx.x) * kJoinWaves;
-  if (lane == 0) {
-    rows[wave] = ~0u;
-    if (chunk0 + wave < chunks) {
-      const chunk_runs c(s, chunk0 + wave);
-      if (c.tail) rows[wave] = c.last;
+  __shared__ int64_t lasts[kJoinWaves];  // the chunks that the runs end in
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, sub = lane % kJoinLanes;
+  const int64_t group = (block0 + blockIdx.x) / slices, chunk0 = group * kJoinWaves;
+  const int at = (static_cast<int>(block0 + blockIdx.x - group * slices) * kJoinLanes + sub) * kUnit;
+  unsigned mine = ~0u;
+  if (chunk0 + wave < chunks) {
+    const chunk_runs c(s, chunk0 + wave);
+    if (c.tail) {
+      mine               = c.last;
+      const int64_t last = (first_at_least(s, int64_t{c.last} + 1) - 1) / s.width;
+      if (lane == 0) lasts[wave] = last;
     }
   }
+  if (lane == 0) rows[wave] = mine;
   lds_barrier();
   for (int j = 0; j < kJoinWaves; ++j) {
     const unsigned row = rows[j];
     if (row == ~0u) continue;
-    const int64_t chunk = chunk0 + j;
+    const int64_t chunk = chunk0 + j, last = lasts[j];
     float sum[kUnit];
 #pragma unroll
     for (int i = 0; i < kUnit; ++i)
       sum[i] = 0.f;
-    const auto take = [&](const float* part) {
-      float v[kUnit];
-      unpack_unit(load_unit<kShort>(part, unit_start(at, d), d), v);
+    for (int64_t p = chunk + threadIdx.x / kJoinLanes; p <= last; p += kJoinTeams * kPartsAhead) {
+      unit<float> u[kPartsAhead];
 #pragma unroll
-      for (int i = 0; i < kUnit; ++i)
-        sum[i] += v[i];
-    };
-    if (wave == 0) take(s.cut + (chunk * 2 + 1) * d);
-    for (int64_t part = chunk + 1 + wave; part * s.width < s.m && s.row(part * s.width) == row; part += kJoinWaves)
-      take(s.cut + part * 2 * d);
+      for (int q = 0; q < kPartsAhead; ++q) {
+        const int64_t part = min(p + q * kJoinTeams, last);
+        u[q] = load_unit<kShort>(s.cut + (part * 2 + (part == chunk ? 1 : 0)) * d, unit_start(at, d), d);
+      }
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i)
-      sums[wave][lane][i] = sum[i];
+      for (int q = 0; q < kPartsAhead; ++q) {
+        float v[kUnit];
+        unpack_unit(u[q], v);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i)
+          sum[i] += p + q * kJoinTeams <= last ? v[i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) {
+      sum[i] += __shfl_xor(sum[i], kJoinLanes);
+      if (lane < kJoinLanes) sums[wave][i][lane] = sum[i];
+    }
     lds_barrier();
-    if (wave == 0) {
+    if (threadIdx.x < kJoinLanes) {
       for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
         for (int i = 0; i < kUnit; ++i)
-          sum[i] += sums[w][lane][i];
+          sum[i] += sums[w][i][lane];
       write_sum<kShort>(sum, scale, add, out + row * ostride, at, d);
     }
     lds_barrier();
@@ -1113,12 +1131,12 @@ void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n
         OCTEX_HIP(hipGetLastError());
       });
     });
-    const int64_t joins = ceil_div(l.chunks, kJoinWaves);
+    const auto slices   = static_cast<unsigned>(ceil_div(d, kJoinLanes * kUnit));
+    const int64_t joins = ceil_div(l.chunks, kJoinWaves) * slices;
     for (int64_t first = 0; first < joins; first += kMaxGrid) {
-      const dim3 grid(static_cast<unsigned>(std::min(kMaxGrid, joins - first)),
-                      static_cast<unsigned>(ceil_div(d, 64 * kUnit)));
       const auto join = d < kUnit ? join_runs_kernel<O, true> : join_runs_kernel<O, false>;
-      join<<<grid, kJoinThreads, 0, s>>>(sorted, width, scale, add, to, out.stride, l.chunks, first);
+      join<<<static_cast<unsigned>(std::min(kMaxGrid, joins - first)), kJoinThreads, 0, s>>>(sorted, width, scale, add, to,
+                                                                                             out.stride, l.chunks, slices, first);
       OCTEX_HIP(hipGetLastError());
     }
   });

@@ -6,7 +6,7 @@
 
 namespace cuvs::neighbors::octex::detail {
 
-constexpr int64_t kMaxRowWidth = int64_t{1} << 24;  // values of a row: its slices are a grid's second dimension
+constexpr int64_t kMaxRowWidth = int64_t{1} << 24;  // values of a row
 
 /** A table [n, d], rows `stride` apart; scales [n] of int8 rows, else null. */
 struct table_rows {

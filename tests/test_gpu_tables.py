@@ -186,6 +186,19 @@ def test_gradient_of_unsorted_tokens(O, m, widths, kind):
         check_gradient(O, randn(g, m, d), ids_of(g, m, 700, kind), 700)
 
 
+@pytest.mark.parametrize("d", [5, 130, 520])
+@pytest.mark.parametrize("share", [0.5, 1.0])
+def test_gradient_of_a_batch_that_is_padded_with_a_row(O, d, share):
+    """A run of thousands of chunks; whole numbers, whose sums are exact in any order."""
+    m, n = 66_000, 800
+    g = gen(d)
+    ids = torch.randint(0, n, (m,), generator=g, device="cuda")
+    ids[torch.rand(m, generator=g, device="cuda") < share] = 300
+    grad = torch.randint(-2, 3, (m, d), generator=g, device="cuda").bfloat16()
+    want = torch.zeros((n, d), dtype=torch.float64, device="cuda").index_add_(0, ids, grad.double())
+    assert torch.equal(O.embed_backward(grad, ids, n, dtype="float32").double(), want)
+
+
 @pytest.mark.parametrize("m", [524_288, 524_289, 3_000_017])
 @pytest.mark.parametrize("kind", ["few", "common", "any"])
 def test_gradient_of_many_tokens(O, m, kind):
