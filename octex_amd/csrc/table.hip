@@ -4,8 +4,9 @@
 //   backward   G_v = scale (sum of g_i over i with ids_i = v)  [+ what G_v held]
 //
 // The gradient's tokens are sorted by id, equal ones by place (a stable sort, digit by digit; up to 4096 of them are looked
-// through instead), so that a row's gradients are added in a fixed order in fp32 and rounded once.  A sorted chunk is one team's; a row's tokens that reach into the chunk
-// behind theirs are still their own team's, and longer runs (a common token's) leave a sum a chunk, which are joined after.
+// through instead), so that a row's gradients are added in a fixed order in fp32 and rounded once.  A sorted chunk is one team's; a
+// row's tokens that reach into the chunk behind theirs are still their own team's, and longer runs (a common token's) leave a sum a
+// chunk, which are joined after.
 // Both are bound by the bytes of the rows; a large copy takes 5.06 TB/s of this GPU, writing alone 6.85.  32,768 rows of 4096
 // bfloat16 take 78 us (152 MB read, 268 written: 5.4 TB/s), the gradient of a table of 128,000 such rows 275 (1.3 GB: 4.8).
 
