@@ -2,7 +2,11 @@
 
 Bounds, derived before the first run: a row's value rounds its scale once (int8 rows their product of scales once more) and the
 product once, 3 E of it; a sum of c gradients rounds at most c times, by E of the sum of sizes so far each, then its product with
-the scale and, added to what the table held, their sum: (c + 3) E of the sum of sizes and E of the result."""
+the scale and, added to what the table held, their sum: (c + 3) E of the sum of sizes and E of the result.
+
+Which tokens are sorted: none of up to 1024, and of up to 4096 only those of wide rows (m^2 ceil(d / 512) beyond 2^25), so that tests
+of fewer tokens look them through.  The sort by one workgroup (2, 4 or 8 tokens a thread; one to four digits) and by many is
+reached by test_gradient_on_both_sides_of_the_sort and what follows it."""
 
 import numpy as np
 import pytest
@@ -387,3 +391,49 @@ def test_refusals(O):
     ]:
         with pytest.raises(error, match=text):
             call()
+
+
+def check_whole_numbers(O, m, n, d, kind):
+    """Gradients of whole numbers, whose sums in 32 bits are exact in any order; the ends of the table have tokens, and places
+    outside it."""
+    g = gen(m + n + d)
+    ids = ids_of(g, m, n, kind)
+    if m >= 8:
+        ids[1], ids[m // 2], ids[m - 2], ids[m - 1] = 0, n - 1, n, -(2**40)
+    grad = torch.randint(-2, 3, (m, d), generator=g, device="cuda").half()
+    inside = (ids >= 0) & (ids < n)
+    want = torch.zeros((n, d), device="cuda").index_add_(0, ids[inside], grad[inside].float())
+    assert torch.equal(O.embed_backward(grad, ids, n, dtype="float32"), want)
+    sums = torch.ones((n, d), device="cuda")
+    O.embed_backward(grad, ids, add_to=sums)
+    assert torch.equal(sums, want + 1)
+
+
+# Up to 1024 tokens are looked through, up to 4096 while m^2 ceil(d / 512) is at most 2^25, others are sorted: both sides.  A
+# single workgroup sorts 2 tokens a thread up to 2048, 4 up to 4096, 8 up to 8192
+@pytest.mark.parametrize("m,d", [(1024, 16_000), (1025, 15_872), (1025, 15_873), (2000, 4104), (2048, 4096), (2048, 4097),
+                                 (2049, 3585), (2896, 2048), (2896, 2049), (3000, 2056), (4096, 1024), (4096, 1025), (4097, 8)])
+@pytest.mark.parametrize("kind", ["one", "few", "common", "any", "padding"])
+def test_gradient_on_both_sides_of_the_sort(O, m, d, kind):
+    check_whole_numbers(O, m, 700, d, kind)
+
+
+# of one to four digits, by 2, 4 and 8 tokens a thread
+@pytest.mark.parametrize("m,d", [(2048, 4104), (4096, 1032), (5000, 8), (8192, 1)])
+@pytest.mark.parametrize("n", [1, 2, 511, 512, 513, 262_143, 262_144, 300_000])
+@pytest.mark.parametrize("kind", ["common", "any"])
+def test_digits_that_a_workgroup_sorts_alone(O, m, d, n, kind):
+    check_whole_numbers(O, m, n, d, kind)
+
+
+@pytest.mark.parametrize("m", [100, 4097, 8192, 9000, 66_000, 524_289])
+@pytest.mark.parametrize("n", [1, 2, 3, 134_217_727, 134_217_728, 140_000_000])
+def test_shortest_and_longest_tables(O, m, n):
+    check_whole_numbers(O, m, n, 1, "any")
+
+
+# of more tiles than a workgroup adds up, and of fewer
+@pytest.mark.parametrize("m", [66_000, 524_288, 524_289, 600_001])
+@pytest.mark.parametrize("kind", ["one", "common", "any", "padding"])
+def test_three_digits_of_many_tiles(O, m, kind):
+    check_whole_numbers(O, m, 300_000, 4, kind)
