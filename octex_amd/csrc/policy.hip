@@ -33,6 +33,22 @@ __device__ inline auto row_of(score_rows const& in, listed_ids const& ids, polic
           t.reference != nullptr ? t.reference[r] : 0.f, grad_loss != nullptr ? grad_loss[r] : 0.f};
 }
 
+/** exp(d) - 1 - d, given e = exp(d) - 1.  Near 0 that difference would keep few of its digits (1e-4 of it lost at d = 1e-3) or
+ * fall below 0; there it is d^2 (1/2 + d/6 + d^2/24 ...), whose next term is 2^-28 of it at |d| = 1/2. */
+__device__ inline auto kl_of(float d, float e) -> float
+{
+  if (!(fabsf(d) < 0.5f)) return e == INFINITY ? e : e - d;
+  float s = 1.f / 362880.f;
+  s       = fmaf(s, d, 1.f / 40320.f);
+  s       = fmaf(s, d, 1.f / 5040.f);
+  s       = fmaf(s, d, 1.f / 720.f);
+  s       = fmaf(s, d, 1.f / 120.f);
+  s       = fmaf(s, d, 1.f / 24.f);
+  s       = fmaf(s, d, 1.f / 6.f);
+  s       = fmaf(s, d, 0.5f);
+  return d * d * s;
+}
+
 /** A row's loss but for the entropy's term, and its slope by the log probability. */
 struct policy_loss {
   float loss, slope;
@@ -46,7 +62,7 @@ __device__ inline auto loss_of(float logp, policy_row const& p, policy_terms con
   policy_loss l{-p.advantage * (clipped ? bound : r), clipped ? 0.f : -p.advantage * r};
   if (t.reference != nullptr) {
     const float d = p.reference - logp, e = expm1f(d);
-    l.loss += t.kl * (e == INFINITY ? e : e - d);
+    l.loss += t.kl * kl_of(d, e);
     l.slope -= t.kl * e;
   }
   return l;

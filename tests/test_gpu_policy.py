@@ -327,3 +327,23 @@ def test_refusals(O):
     ]:
         with pytest.raises(error, match=text):
             step(**change)
+
+
+@pytest.mark.parametrize("m,n", [(800, 2), (800, 3000), (60, 140_000)])
+def test_kl_of_near_policies_keeps_its_digits(O, m, n):
+    """exp(d) - 1 - d where d is given exactly (the id's ln p is 0), from 1e-17 to 80 of both signs; kl 1, A 0: the loss itself.
+
+    Bound: up to 1/2 by its series, d * d (E) times a sum (2 E, whose coefficients add E) rounds once more (E); from there on by
+    expm1, whose unit in the last place (2 E |e|) weighs |e| / k <= 4.4 times, and a difference (E): 10 E."""
+    size = torch.logspace(-17, np.log10(80.0), m // 2, dtype=torch.float64, device="cuda").float()
+    ref = torch.cat([size, -size])
+    x = torch.full((m, n), -1000.0, device="cuda")
+    x[:, 0] = 0
+    ids, none = torch.zeros(m, dtype=torch.int64, device="cuda"), torch.zeros(m, device="cuda")
+    d = ref.double()
+    series = sum(d**j / float(np.prod(np.arange(1.0, j + 3))) for j in range(12)) * d * d
+    want = torch.where(d.abs() < 0.2, series, torch.expm1(d) - d)
+    for r in (O.policy_loss(x, ids, none, none, ref_log_probs=ref, kl=1.0),
+              O.policy_step(none, x, ids, none, none, ref_log_probs=ref, kl=1.0)[0]):
+        assert (r.log_probs == 0).all() and (r.loss >= 0).all()
+        close(r.loss, want, 10 * E * want, "KL term")
