@@ -260,12 +260,13 @@ __global__ __launch_bounds__(NT) void balance_kernel(score_rows in, listed_ids e
     inner_sum += inner;
     if (forward && sub == 0 && here) out.lse[r] = counted ? lse : 0.f;
     if (grad == nullptr) continue;
-    const float cz = c_z * l;
+    // a row that does not count has none, also where the loss weighs infinitely much
+    const float cb = counted ? c_balance : 0.f, cz = counted ? c_z * l : 0.f;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        v[h][i] *= fmaf(c_balance, f[h][i] - inner, cz);
+        v[h][i] *= fmaf(cb, f[h][i] - inner, cz);
     }
     if (!here) continue;
     T* to = grad + r * gstride;

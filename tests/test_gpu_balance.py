@@ -268,3 +268,17 @@ def test_refusals(O):
         O.balance_loss_backward(None, r.x, r.experts, res._replace(counts=res.counts[:3]))
     with pytest.raises(TypeError, match="counts must be int64"):
         O.balance_loss_backward(None, r.x, r.experts, res._replace(counts=res.counts.float()))
+
+
+@pytest.mark.parametrize("m,e", [(9, 6), (40, 700), (5000, 6), (5000, 100), (900, 1300), (40_000, 60), (40_000, 500)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_do_not_count_have_no_gradient(O, m, e, dtype):
+    """Whatever the loss weighs: an overflowed loss scale leaves a batch's padding at 0."""
+    r = Rows(m, e, 2, dtype, padding=0.4)
+    r.experts[0], r.experts[1] = 0, -1
+    use = ((r.experts >= 0) & (r.experts < e)).any(1)
+    res = O.balance_loss(r.x, r.experts, **r.how)
+    for size in (float("inf"), float("-inf"), float("nan")):
+        g = torch.tensor(size, device="cuda")
+        for grad in (O.balance_loss_backward(g, r.x, r.experts, res, **r.how), O.balance_step(g, r.x, r.experts, **r.how)[1]):
+            assert (grad[~use] == 0).all() and not torch.isfinite(grad[0]).any()
