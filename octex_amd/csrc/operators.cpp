@@ -334,7 +334,7 @@ auto experts_of(const octexMatrix* logits, const octexMatrix* experts, score_row
   OCTEX_EXPECTS(experts->type == OCTEX_INT32 || experts->type == OCTEX_INT64, "octex: experts must be int32 or int64");
   OCTEX_EXPECTS(experts->cols <= kMaxListed, "octex: at most %d experts a row, not %lld", kMaxListed,
                 static_cast<long long>(experts->cols));
-  OCTEX_EXPECTS(in.m * std::max<int64_t>(experts->cols, 1) <= INT32_MAX, "octex: at most 2^31 - 1 choices");
+  OCTEX_EXPECTS(in.m <= INT32_MAX / std::max<int64_t>(experts->cols, 1), "octex: at most 2^31 - 1 choices");
   return {experts->data, experts->type == OCTEX_INT64, experts->stride, static_cast<int>(experts->cols)};
 }
 

@@ -169,3 +169,13 @@ def test_a_workspace_is_asked_for_once_for_its_sizes(monkeypatch):
     S._WORKSPACES.update((("full", i), 0) for i in range(4096))  # as many as are kept
     c.run_sized("any", 6, sizes=("any", 6))
     assert S._WORKSPACES == {("any", 6): 600}
+
+
+def test_balance_of_more_choices_than_64_bits_count():
+    """A product of rows and choices that passes 64 bits is refused like any that passes 31."""
+    size = ct.c_int64(-1)
+    for rows, k in ((1 << 62, 4), (1 << 55, 512), (1 << 31, 1), (1 << 32, 0)):
+        x, experts = matrix(rows, 8), matrix(rows, k, INT64)
+        assert "choices" in refused("octexBalanceLoss", x, experts, 1.0, 0.0, *[HOST] * 5, None, None, None, 0, ct.addressof(size))
+        assert "choices" in refused("octexBalanceLossBackward", x, experts, 1.0, 0.0, HOST, HOST, None, x)
+    assert size.value == -1
