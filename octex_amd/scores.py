@@ -104,7 +104,7 @@ class _Call:
                 self.stream, self.side = named, self.external(named)
         if flat and t.ndim > 2:  # all but the last dimension are one
             with self.context():
-                t = t.reshape(-1, t.shape[-1])
+                t = t.flatten(0, -2)
         self.first = self.take(t, name, types)
 
     def view(self, a):

@@ -393,6 +393,16 @@ def test_refusals(O):
             call()
 
 
+
+@pytest.mark.parametrize("shape", [(2, 3), (0, 3), (2, 1, 4)])
+def test_gradients_of_no_width(O, shape):
+    ids = torch.zeros(shape, dtype=torch.int64, device="cuda")
+    grad = torch.zeros((*shape, 0), device="cuda")
+    assert O.embed_backward(grad, ids, 4).shape == (4, 0)
+    sums = torch.zeros((4, 0), device="cuda")
+    assert O.embed_backward(grad, ids, add_to=sums) is sums
+
+
 def check_whole_numbers(O, m, n, d, kind):
     """Gradients of whole numbers, whose sums in 32 bits are exact in any order; the ends of the table have tokens, and places
     outside it."""
