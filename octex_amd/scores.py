@@ -88,7 +88,8 @@ class _Call:
     """One call's operands and results, all on one GPU, and the stream that they are ordered on: torch's current one, or
     (`side`) another that the first operand's framework names.  `others` are the streams of the remaining operands."""
 
-    __slots__ = ("torch", "names", "origin", "device", "stream", "side", "others", "on_host", "foreign", "first", "scratch")
+    __slots__ = ("torch", "names", "origin", "device", "stream", "side", "others", "on_host", "foreign", "first", "lead",
+                 "scratch")
 
     def __init__(self, first, name, types, flat=False):
         self.torch, self.names, raw_stream = _torch()
@@ -102,9 +103,11 @@ class _Call:
             named = _arrays.named_stream(first)
             if named is not None and named != self.stream:
                 self.stream, self.side = named, self.external(named)
-        if flat and t.ndim > 2:  # all but the last dimension are one
-            with self.context():
-                t = t.flatten(0, -2)
+        if flat:
+            self.lead = t.shape[:-1]
+            if t.ndim > 2:  # all but the last dimension are one
+                with self.context():
+                    t = t.flatten(0, -2)
         self.first = self.take(t, name, types)
 
     def view(self, a):

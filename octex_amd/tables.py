@@ -8,7 +8,7 @@ of a search's neighbors.
 Operands, streams, results and errors are as octex_amd/scores.py has them.
 """
 
-from . import _arrays, scores
+from . import scores
 from .scores import FLOATS, INTS
 
 
@@ -64,8 +64,8 @@ def embed_backward(grad, ids, rows=None, *, scale=1.0, dtype=None, add_to=None):
     g = c.first
     t, flat, shape = _flat_ids(c, ids)
     m, d = g.shape
-    if _arrays.shape_of(grad)[:-1] != shape:
-        raise ValueError(f"octex: grad has shape {_arrays.shape_of(grad)}, ids {tuple(shape)}")
+    if c.lead != shape:
+        raise ValueError(f"octex: grad has shape {(*c.lead, d)}, ids {tuple(shape)}")
     if add_to is None:
         if rows is None:
             raise TypeError("octex: the table's number of rows, or add_to, must be given")

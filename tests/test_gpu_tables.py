@@ -393,6 +393,14 @@ def test_refusals(O):
             call()
 
 
+def test_gradients_as_lists(O):
+    got = O.embed_backward([[1.0, 2.0], [3.0, 4.0]], [1, 1], 3)
+    assert isinstance(got, np.ndarray) and np.array_equal(got, [[0, 0], [4, 6], [0, 0]])
+    got = O.embed_backward([[[1.0, 2.0]], [[3.0, 4.0]]], [[0], [2]], 3)
+    assert np.array_equal(got, [[1, 2], [0, 0], [3, 4]])
+    with pytest.raises(ValueError, match="ids"):
+        O.embed_backward([[1.0, 2.0], [3.0, 4.0]], [1], 3)
+
 
 @pytest.mark.parametrize("shape", [(2, 3), (0, 3), (2, 1, 4)])
 def test_gradients_of_no_width(O, shape):
