@@ -579,8 +579,6 @@ __device__ inline void clear_rows(const bool* used, int64_t v0, int rows, int d,
   }
 }
 
-constexpr int kClearRows = 4096;  // of a workgroup, at most
-
 /** Rows [first, n), `rows` a workgroup from `block0` on, that are set to 0 beside the sums where no token has them. */
 struct clear_share {
   unsigned block0;
@@ -1092,12 +1090,11 @@ void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n
   auto* base        = static_cast<char*>(workspace);
   const sorted_tokens sorted{reinterpret_cast<token*>(base), ids.m, rows, chunk_width(ids.m, d),
                              reinterpret_cast<float*>(base + l.cut)};
-  // of many: rows that are filled beside the sort, wherever tokens are, and those a workgroup that are cleared after it, up to
-  // 32 KB (1 MB: 288 us for what takes 276) in 2048 workgroups or more
+  // of many: rows that are filled beside the sort, wherever tokens are, and those that are cleared after it
   const int64_t row_bytes = d * elem_size(out.type);
   const int64_t filled    = add || few || out.stride != d ? 0 : std::min(n, fill_bytes(l) / row_bytes);
   const int64_t left      = add || few ? 0 : n - filled;
-  const int64_t per_group = std::clamp<int64_t>(std::min((int64_t{32} << 10) / row_bytes, ceil_div(left, 2048)), 1, kClearRows);
+  const int64_t per_group = rows_to_clear(left, row_bytes);
   with_type(out.type, [&](auto o) {
     using O = decltype(o);
     O* to   = static_cast<O*>(out.x);

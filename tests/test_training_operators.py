@@ -2,9 +2,12 @@
 values and memory before anything is launched, and the workspace's size is answered."""
 
 import ctypes as ct
+import os
+import subprocess
 
 import numpy as np
 import pytest
+from conftest import ROOT
 
 from octex_amd import _lib
 from octex_amd import scores as S
@@ -179,3 +182,13 @@ def test_balance_of_more_choices_than_64_bits_count():
         assert "choices" in refused("octexBalanceLoss", x, experts, 1.0, 0.0, *[HOST] * 5, None, None, None, 0, ct.addressof(size))
         assert "choices" in refused("octexBalanceLossBackward", x, experts, 1.0, 0.0, HOST, HOST, None, x)
     assert size.value == -1
+
+
+def test_tables_of_any_size_are_cleared_in_one_launch(tmp_path):
+    """A table as large as the GPU's memory, of rows of just over 16 KB, has more of them than a launch has workgroups."""
+    exe = str(tmp_path / "table_clears")
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(rocm, "include"),
+                    os.path.join(ROOT, "tests", "c", "table_clears.cpp"), "-o", exe], check=True)
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and run.stdout == "ok\n", run.stdout
