@@ -848,8 +848,9 @@ __global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned
     rows[threadIdx.x + q * kThreads] = static_cast<int>(threadIdx.x) + q * kThreads < m ? row_of(id[q], n) : ~0u;
   lds_barrier();
   const int team = static_cast<int>(threadIdx.x) / W, lane = threadIdx.x % 64, sub = lane % W;
-  const unsigned all = blockIdx.x * kTeams + team;
-  const int token    = static_cast<int>(all / slices), at = (static_cast<int>(all % slices) * W + sub) * kUnit;
+  // a workgroup's teams have one slice, so that a long run's slices are different workgroups'
+  const int token    = static_cast<int>(blockIdx.x / slices) * kTeams + team;
+  const int at       = (static_cast<int>(blockIdx.x % slices) * W + sub) * kUnit;
   const unsigned row = token < m ? rows[token] : n;
   const auto above = [&](unsigned long long lanes) { return W == 64 ? lanes : lanes >> (lane - sub) & ((1ull << (W % 64)) - 1); };
   int count = 0;
@@ -902,8 +903,7 @@ __global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned
   auto* const parts = reinterpret_cast<float(*)[kThreads]>(rows);  // the rows of tokens make room
   for (int t = 0; t < kTeams; ++t) {
     if (counts[t] <= kLongRun) continue;
-    const int its_at = (static_cast<int>((blockIdx.x * kTeams + t) % slices) * W + sub) * kUnit;
-    add_up(places[t], counts[t], team * kTokensAhead, kTeams * kTokensAhead, unit_start(its_at, d));
+    add_up(places[t], counts[t], team * kTokensAhead, kTeams * kTokensAhead, unit_start(at, d));
 #pragma unroll
     for (int i = 0; i < kUnit; ++i)
       parts[i][threadIdx.x] = sum[i];
@@ -967,8 +967,10 @@ auto chunk_width(int64_t m, int64_t d) -> int
 }
 
 /** Whether a gradient's tokens are looked through, by every slice of every token, and not sorted: one launch in place of three to
- * six.  8000 x 512 bfloat16 from 4096 tokens, the i-th commonest as 1 / i: 19 us, sorted 28; 2000 x 64 from 2000: 11 and 25; 8000
- * x 1024 from 3000: 22 and 29; near the bound 8000 x 1000 from 4096 28 and 30, 8000 x 2000 from 2500 32 and 30. */
+ * six.  Even ids, those of text (the i-th commonest as 1 / i), and half or all of them equal (a padded batch's), sorted in brackets:
+ * 32,000 x 512 bfloat16 from 3000 tokens 16, 16, 48, 83 us (27, 33, 30, 26), 8000 x 512 from 4096 15, 19, 55, 101 (25, 31, 30, 25),
+ * 8000 x 2000 from 2896, near the bound, 30, 29, 47, 83 (27, 32, 32, 26).  Which ids they are is not known here: batches of one
+ * token pay for the others, and still take less than torch's additions by atomics (126, 134, 127 where all are equal). */
 auto takes_few(int64_t m, int64_t d) -> bool
 {
   return m <= kFewTokens || (m <= kSomeTokens && m * m * ceil_div(d, 64 * kUnit) <= int64_t{1} << 25);
@@ -1112,7 +1114,8 @@ void launch_embed_backward(value_rows const& grad, row_ids const& ids, int64_t n
         constexpr int F   = std::max(W, 8);
         const auto slices = static_cast<unsigned>(ceil_div(d, W == 1 ? kUnit : W * kUnit));
         const int team    = !few ? W : fewer ? F : 64;
-        const auto sums   = static_cast<unsigned>(ceil_div((few ? ids.m : l.chunks) * slices, kThreads / team));
+        const int teams   = kThreads / team;
+        const auto sums   = static_cast<unsigned>(few ? ceil_div(ids.m, teams) * slices : ceil_div(l.chunks * slices, teams));
         const auto launch_few = [&](auto kernel) {
           kernel<<<sums + clears, kThreads, 0, s>>>(ids, rows, from, grad.stride, width, scale, add, to, out.stride, slices, sums,
                                                     clear);

@@ -436,6 +436,20 @@ def test_gradient_on_both_sides_of_the_sort(O, m, d, kind):
     check_whole_numbers(O, m, 700, d, kind)
 
 
+@pytest.mark.parametrize("m,d", [(300, 1600), (1024, 4100), (2896, 2000), (4096, 1024)])
+@pytest.mark.parametrize("share", [0.3, 1.0])
+def test_long_runs_of_wide_rows(O, m, d, share):
+    """A slice's sums are those of its columns alone, bit for bit, whoever adds them up."""
+    g = gen(m + d)
+    ids = torch.randint(0, 500, (m,), generator=g, device="cuda")
+    ids[torch.rand(m, generator=g, device="cuda") < share] = 77
+    grad = randn(g, m, d)
+    got = O.embed_backward(grad, ids, 500)
+    for at in range(0, d - 511, 512):
+        assert torch.equal(got[:, at : at + 512], O.embed_backward(grad[:, at : at + 512], ids, 500))
+    check_gradient(O, grad, ids, 500)
+
+
 # of one to four digits, by 2, 4 and 8 tokens a thread
 @pytest.mark.parametrize("m,d", [(2048, 4104), (4096, 1032), (5000, 8), (8192, 1)])
 @pytest.mark.parametrize("n", [1, 2, 511, 512, 513, 262_143, 262_144, 300_000])
