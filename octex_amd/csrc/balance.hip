@@ -9,8 +9,9 @@
 //
 // The gradient needs all choices first, which come from the ids alone: one kernel counts them by parts, the next adds the
 // parts up, takes the logits once, writes the gradient and adds up p, a third joins those sums.  Every sum has a fixed order;
-// p's are fp32 within a workgroup and fp64 over them.  Bound by the logits' bytes, or by the launches:
-// 131,072 x 256 bfloat16 with 8 choices in both directions take 46 us (7.7 + 31.9, at 4.2 TB/s, + 6.5), 64 x 8 float32 5.9.
+// p's are fp32 within a workgroup and fp64 over several (up to 32,768 logits are one's alone).  Bound by the logits' bytes, or by
+// the launches: 131,072 x 256 bfloat16 with 8 choices in both directions take 46 us (7.7 + 31.9, at 4.2 TB/s, + 6.5), 64 x 8
+// float32 5.8.
 
 #include "balance.hpp"
 #include "rows_device.hpp"

@@ -10,7 +10,8 @@
 // a = g / T (entropy H - c), b = g / T entropy, w = g / T c.  A row whose id is padding (a prompt's token) is not read.
 //
 // Bound by the logits' bytes: a large copy takes 5.06 TB/s of this GPU.  Both directions of 4096 x 128,000 bfloat16 take 456 us,
-// 4.6 TB/s; 333 x 50,021 float16 10 and 13; 16 x 32,000 float32 10, where a row is one CU's and its exponentials bound it.
+// 4.6 TB/s; 333 x 50,021 float16 11 and 13; 16 x 32,000 float32 10, where a row is one CU's and its exponentials bound it.  Rows
+// that no workgroup holds are read twice, by a kernel a direction: 4096 x 150,000 bfloat16 756 us, 2048 x 128,000 float32 592.
 
 #include "policy.hpp"
 #include "rows_device.hpp"
@@ -299,6 +300,8 @@ void launch_policy(score_rows const& in, listed_ids const& ids, policy_terms con
         OCTEX_HIP(hipGetLastError());
       });
     };
+    // by a wavefront a row, by 256 threads: 8192 x 1000 float32 11.5 us, 15.5; 8192 x 4000 bfloat16 18.4, 21.5; of 1500 rows 8.2,
+    // 7.8.  512 or 1024 threads gain nothing: 333 x 50,021 float16 14.6, 15.1, 15.0, of 250 rows 11.3, 10.6, 11.1
     if (split.parts > 1) {
       launch(policy_kernel<T, kThreads, true>, kThreads, in.m * split.parts);
       launch(finish_policy_kernel<T>, 64, in.m);
@@ -323,6 +326,7 @@ void launch_policy_backward(score_rows const& in, listed_ids const& ids, policy_
         OCTEX_HIP(hipGetLastError());
       });
     };
+    // 2048 x 1000 float32 7.1 us, by 256 threads 8.5; 8192 x 4000 bfloat16 27.7, 28.1; of 1500 rows 10.3, 9.6
     if (by_wavefront(in.m, in.n, 1))
       launch(policy_backward_kernel<T, 64>, 64);
     else
@@ -347,6 +351,15 @@ void launch_policy_step(score_rows const& in, listed_ids const& ids, policy_term
                                                                               static_cast<T*>(grad), gstride, passes_cache(in));
       OCTEX_HIP(hipGetLastError());
     };
+    // How a row is held, measured on both sides (us):
+    // - a wavefront, 4 pieces a lane: 8192 x 1000 float32 17.6, of 16 pieces 20.6, by 256 threads 27.8; 2048 rows 8.7, 9.9, 10.9;
+    //   500 x 2000 bfloat16 6.7 by a wavefront, 6.1 by 256 threads
+    // - a wavefront, 16 pieces: 8192 x 4000 float32 57.9, by 256 threads 60.5; but 2048 rows 19.7, 17.1
+    // - 256 threads, 4 pieces: 300 x 8000 bfloat16 8.2, by a wavefront 13.4, by 1024 threads 11.7
+    // - 256 threads, 16 pieces: 4096 x 32,000 bfloat16 123, by 1024 threads 139; 512 rows 22.7, 22.2
+    // - 1024 threads, 4 pieces, of no more rows than CUs: 256 x 16,000 float32 12.2, by 256 threads 15.7
+    // - 1024 threads, 8 pieces: 16 x 32,000 float32 11.2, of 16 pieces 12.4; 2048 rows 118, 123
+    // - 1024 threads, 16 pieces: 4096 x 128,000 bfloat16 460, in two kernels 597
     const int pieces = (in.n + kPer16<T> - 1) / kPer16<T>;
     if (pieces <= 256 && in.m >= 2048)
       launch(policy_step_kernel<T, 64, 4>, 64, 8192);

@@ -30,7 +30,8 @@ void launch_policy(score_rows const& in, listed_ids const& ids, policy_terms con
 void launch_policy_backward(score_rows const& in, listed_ids const& ids, policy_terms const& terms, policy_out const& saved,
                             const float* grad_loss, void* grad, int64_t gstride, hipStream_t s);
 
-/** Whether launch_policy_step holds a row in registers; else it needs launch_policy's workspace. */
+/** Whether launch_policy_step holds a row in registers (up to 256 KB of one, 128 KB of fewer than 512 rows); else it needs
+ * launch_policy's workspace. */
 auto policy_step_held(int64_t m, int n, elem type) -> bool;
 
 /** Both directions; the logits are read once if a workgroup can hold a row. */

@@ -1,6 +1,6 @@
-// Device code that the operators on rows of scores share (rows.hip, policy.hip): the sums of a row's exponentials, their joins
-// over lanes and workgroups, one pass over a row, one that writes a gradient, and how rows are shared out.  Every file that
-// includes it has its own.
+// Device code that the operators on rows of scores share (rows.hip, policy.hip; balance.hip takes its reductions over lanes):
+// the sums of a row's exponentials, their joins over lanes and workgroups, one pass over a row, one that writes a gradient, and
+// how rows are shared out.  Every file that includes it has its own.
 #pragma once
 
 #include "common.hpp"

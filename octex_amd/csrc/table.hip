@@ -3,12 +3,12 @@
 //   embed      out_i = scale r_v T_v,  v = ids_i  (r: the scales of int8 rows);  ids outside the table: 0
 //   backward   G_v = scale (sum of g_i over i with ids_i = v)  [+ what G_v held]
 //
-// The gradient's tokens are sorted by id, equal ones by place (a stable sort, digit by digit; up to 4096 of them are looked
-// through instead), so that a row's gradients are added in a fixed order in fp32 and rounded once.  A sorted chunk is one team's; a
-// row's tokens that reach into the chunk behind theirs are still their own team's, and longer runs (a common token's) leave a sum a
-// chunk, which are joined after.
+// The gradient's tokens are sorted by id, equal ones by place (a stable sort, digit by digit; up to 1024 of them, and of short rows
+// up to 4096, are looked through instead), so that a row's gradients are added in a fixed order in fp32 and rounded once.  A sorted
+// chunk is one team's; a row's tokens that reach into the chunk behind theirs are still their own team's, and longer runs (a common
+// token's) leave a sum a chunk, which are joined after.
 // Both are bound by the bytes of the rows; a large copy takes 5.06 TB/s of this GPU, writing alone 6.85.  32,768 rows of 4096
-// bfloat16 take 78 us (152 MB read, 268 written: 5.4 TB/s), the gradient of a table of 128,000 such rows 275 (1.3 GB: 4.8).
+// bfloat16 take 78 us (152 MB read, 268 written: 5.4 TB/s), the gradient of a table of 128,000 such rows 276 (1.3 GB: 4.8).
 
 #include "common.hpp"
 #include "elems_device.hpp"
@@ -813,7 +813,8 @@ constexpr int kLongRun = 4 * kTokensAhead;  // by one team 120 equal tokens of 1
 /**
  * The same for up to M tokens without sorting them: a team a token looks through all of them, W at a time, and the first one of a
  * row lists the places of the others and adds up their gradients; those of more than kLongRun (a common token's) all teams of the
- * workgroup add up.  Workgroups from `sum_blocks` on clear rows, `clear` (at most M) each.
+ * workgroup add up.  Workgroups from `sum_blocks` on clear rows, `clear` each, whose flags (a byte a row) fit in the words of
+ * `rows`.
  */
 template <typename T, typename O, int W, bool kShort, int M>
 __global__ __launch_bounds__(kThreads) void sum_few_kernel(row_ids ids, unsigned n, const T* grad, int64_t gstride, int d,
@@ -967,10 +968,11 @@ auto chunk_width(int64_t m, int64_t d) -> int
 }
 
 /** Whether a gradient's tokens are looked through, by every slice of every token, and not sorted: one launch in place of three to
- * six.  Even ids, those of text (the i-th commonest as 1 / i), and half or all of them equal (a padded batch's), sorted in brackets:
- * 32,000 x 512 bfloat16 from 3000 tokens 16, 16, 48, 83 us (27, 33, 30, 26), 8000 x 512 from 4096 15, 19, 55, 101 (25, 31, 30, 25),
- * 8000 x 2000 from 2896, near the bound, 30, 29, 47, 83 (27, 32, 32, 26).  Which ids they are is not known here: batches of one
- * token pay for the others, and still take less than torch's additions by atomics (126, 134, 127 where all are equal). */
+ * six.  Of even ids, of those of text (the i-th commonest as 1 / i), and with half or all of them equal (a padded batch's), sorted
+ * in brackets: 32,000 x 512 bfloat16 from 3000 tokens 16, 16, 48, 83 us (27, 33, 30, 26), 8000 x 512 from 4096 15, 19, 55, 101 (25,
+ * 31, 30, 25), 8000 x 2000 from 2896, near the bound, 30, 29, 47, 83 (27, 32, 32, 26).  Which ids they are is not known here:
+ * batches of one token pay for the others, and still take less than torch's additions by atomics (126, 134, 127 where all are
+ * equal). */
 auto takes_few(int64_t m, int64_t d) -> bool
 {
   return m <= kFewTokens || (m <= kSomeTokens && m * m * ceil_div(d, 64 * kUnit) <= int64_t{1} << 25);
@@ -1040,9 +1042,9 @@ void sort_tiles(row_ids const& ids, unsigned n, sort_layout const& l, token* tok
 }
 
 /** The bytes that are filled while the tokens are sorted, in about the time that this takes on few CUs: 4.6 us and 6.7 to count and
- * to move tiles of 2048 tokens, 8 to 18 for 2 to 8 tokens a thread of a single workgroup.  128,000 x 4096 bfloat16 from 32,768
- * tokens: 276 us, 303 if all of the table is filled there, and the tokens' rows are written twice (64 MB a pass: 278, 160 MB:
- * 278). */
+ * to move tiles of 2048 tokens that all run at once (more tiles take longer, and fill the same), 8 to 18 for 2 to 8 tokens a thread
+ * of a single workgroup.  128,000 x 4096 bfloat16 from 32,768 tokens: 276 us, 303 if all of the table is filled there, and the
+ * tokens' rows are written twice (64 MB a pass: 278, 160 MB: 278). */
 auto fill_bytes(sort_layout const& l) -> int64_t
 {
   return l.tiles == 1 ? (int64_t{l.per} + 4) * (14 << 20) : int64_t{l.passes} * (96 << 20);

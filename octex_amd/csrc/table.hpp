@@ -41,8 +41,8 @@ auto embed_backward_workspace(int64_t m, int64_t n, int64_t d) -> int64_t;
 constexpr int kClearRows = 4096;  // of a workgroup, at most
 
 /** Rows that a workgroup clears of the `left` ones that a gradient's sort has not: up to 32 KB (1 MB: 288 us for what takes 276),
- * in 2048 workgroups or more.  At most 2^23 of them, whatever the table's size: with those that sum, fewer than 2^21, a launch stays
- * below 2^32 work-items. */
+ * in 2048 workgroups or more.  At most 2^23 of them, whatever the table's size: with those that sum, fewer than 2^21, a launch
+ * stays below 2^32 work-items. */
 inline auto rows_to_clear(int64_t left, int64_t row_bytes) -> int64_t
 {
   const int64_t enough = std::min((int64_t{32} << 10) / row_bytes, (left + 2047) / 2048);

@@ -476,7 +476,8 @@ def policy_loss_backward(grad_loss, logits, ids, old_log_probs, advantages, resu
 
 def policy_step(grad_loss, logits, ids, old_log_probs, advantages, *, ref_log_probs=None, clip=0.2, kl=0.0, entropy=0.0,
                 temperature=1.0):
-    """(PolicyLoss, grad): policy_loss and policy_loss_backward in one call, which reads the logits less often."""
+    """(PolicyLoss, grad): policy_loss and policy_loss_backward in one call, which reads rows of up to 256 KB (131,072 16-bit logits;
+    half of that of fewer than 512 rows) once, and longer ones as often as the two calls do."""
     c, x, keep, args = _policy(logits, ids, old_log_probs, advantages, ref_log_probs, clip, kl, entropy, temperature)
     g = c.dense(grad_loss, "grad_loss", (x.shape[0],))
     r, grad = PolicyLoss(*[c.like(g) for _ in range(4)]), c.like(x)
